@@ -28,8 +28,9 @@ CSRC = os.path.join(_HERE, "csrc")
 HOST_PATH = os.path.join(_HERE, "_host.so")
 HOST_ABI_PATH = HOST_PATH + ".abi"
 LOCK_PATH = os.path.join(_HERE, ".build.lock")
-SOURCES = ["api.cu"]
+SOURCES = ["api.cu", "fp8_cache.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
+              "--threads", "2",
               "--shared", "-Xcompiler", "-fPIC", "-Xlinker", "-soname=libfa4_nvfp4.so"]
 
 ERROR_NAMES = {1: "null pointer", 2: "unsupported shape", 3: "bad stride", 4: "misaligned pointer",
@@ -293,6 +294,8 @@ EXPORTS = ["fa4_nvfp4_fwd", "fa4_nvfp4_sf_linear_to_tiled", "fa4_nvfp4_query",
            "fa4_nvfp4_decode_is_balanced", "fa4_nvfp4_fwd_splitkv",
            "fa4_nvfp4_fwd_ex", "fa4_nvfp4_sf_tile_jobs", "fa4_nvfp4_quantize_jobs_bf16", "fa4_nvfp4_fwd_device_scales",
            "fa4_nvfp4_fwd_decode_linear_sf"]
+# (the 8-bit KV cache: called by the host extension alone)
+EXPORTS_FP8 = ["fa4_fp8_cache_append", "fa4_fp8_cache_fwd", "fa4_fp8_cache_fwd_workspace_bytes"]
 
 
 def check(rc: int, what: str) -> None:

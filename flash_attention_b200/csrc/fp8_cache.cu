@@ -1,0 +1,172 @@
+// C ABI of the 8-bit KV cache (see include/fa4_nvfp4.h): argument validation and launches of the append and
+// of the attention over it.  Host code only; the kernels live in the .cuh files.
+#include "fp8_attn.cuh"
+#include "launch.cuh"
+
+#include <algorithm>
+
+namespace {
+
+using namespace fa4;
+
+// Shape, strides and alignment of a cache.  Touches no CUDA API.
+int validate_cache(const fa4_fp8_cache* c) {
+  if (c == nullptr) return -FA4_E_NULL;
+  if (c->struct_size != sizeof(fa4_fp8_cache)) return -FA4_E_STRUCT;
+  if (!c->k || !c->v || !c->k_scale || !c->v_scale) return -FA4_E_NULL;
+  if (c->block != 16 && c->block != 32 && c->block != 64 && c->block != 128) return -FA4_E_SHAPE;
+  if (c->num_pages <= 0 || c->page_size <= 0 || c->page_size % c->block != 0 || c->Hkv <= 0) return -FA4_E_SHAPE;
+  if (c->D != 64 && c->D != 128) return -FA4_E_SHAPE;
+  if (c->pages_per_seq <= 0 || (c->page_table == nullptr && c->pages_per_seq != 1)) return -FA4_E_SHAPE;
+  // positions are 32-bit
+  if ((int64_t)c->pages_per_seq * c->page_size > 0x7ffffc00ll) return -FA4_E_TOO_LARGE;
+  const int64_t strides[] = {c->k_stride_page, c->k_stride_token, c->k_stride_head,
+                             c->v_stride_page, c->v_stride_token, c->v_stride_head};
+  for (int64_t s : strides)
+    if (s <= 0 || (s & 15) != 0) return -FA4_E_STRIDE;
+  if (!aligned16(c->k) || !aligned16(c->v)) return -FA4_E_ALIGN;
+  return 0;
+}
+
+int log2_of(int n) {
+  int l = 0;
+  while ((1 << l) < n) ++l;
+  return l;
+}
+
+}  // namespace
+
+extern "C" int fa4_fp8_cache_append(const fa4_fp8_cache* c, const fa4_fp8_append* a, void* cuda_stream) {
+  if (int e = validate_cache(c)) return e;
+  if (a == nullptr) return -FA4_E_NULL;
+  if (a->struct_size != sizeof(fa4_fp8_append)) return -FA4_E_STRUCT;
+  if (!a->k || !a->v || !a->seqlens) return -FA4_E_NULL;
+  if (a->B <= 0 || a->S <= 0 || (c->page_table == nullptr && a->B > c->num_pages)) return -FA4_E_SHAPE;
+  const bool rotate = a->cos != nullptr;
+  if ((a->sin != nullptr) != rotate) return -FA4_E_NULL;
+  if (rotate && (a->rotary_dim <= 0 || a->rotary_dim % 16 != 0 || a->rotary_dim > c->D || a->rotary_rows <= 0)) return -FA4_E_SHAPE;
+  if (rotate && (!aligned16(a->cos) || !aligned16(a->sin))) return -FA4_E_ALIGN;
+  const bool with_q = a->q != nullptr;
+  if (with_q && (!rotate || a->q_out == nullptr)) return -FA4_E_NULL;
+  if (with_q && (a->Hq <= 0 || a->Hq > 0xffff)) return -FA4_E_SHAPE;
+  const int64_t strides[] = {a->k_stride_b, a->k_stride_s, a->k_stride_h, a->v_stride_b, a->v_stride_s, a->v_stride_h,
+                             with_q ? a->q_stride_b : 0, with_q ? a->q_stride_s : 0, with_q ? a->q_stride_h : 0};
+  for (int64_t s : strides)
+    if ((s & 7) != 0) return -FA4_E_STRIDE;
+  if (!aligned16(a->k) || !aligned16(a->v) || (with_q && (!aligned16(a->q) || !aligned16(a->q_out)))) return -FA4_E_ALIGN;
+  const int64_t blocks = ((int64_t)a->S + c->block - 2) / c->block + 1, units = blocks * a->B * c->Hkv * 2;
+  if (units > 0x3fffffffll || (int64_t)a->B * a->S * (with_q ? a->Hq : 1) > 0x0fffffffll) return -FA4_E_TOO_LARGE;
+
+  AppendParams p = {};
+  p.k = static_cast<const __nv_bfloat16*>(a->k);
+  p.v = static_cast<const __nv_bfloat16*>(a->v);
+  p.q = static_cast<const __nv_bfloat16*>(a->q);
+  p.q_out = static_cast<__nv_bfloat16*>(a->q_out);
+  p.k_b = a->k_stride_b; p.k_s = a->k_stride_s; p.k_h = a->k_stride_h;
+  p.v_b = a->v_stride_b; p.v_s = a->v_stride_s; p.v_h = a->v_stride_h;
+  p.q_b = a->q_stride_b; p.q_s = a->q_stride_s; p.q_h = a->q_stride_h;
+  p.kc = static_cast<uint8_t*>(c->k);
+  p.vc = static_cast<uint8_t*>(c->v);
+  p.kc_page = c->k_stride_page; p.kc_tok = c->k_stride_token; p.kc_head = c->k_stride_head;
+  p.vc_page = c->v_stride_page; p.vc_tok = c->v_stride_token; p.vc_head = c->v_stride_head;
+  p.k_scale = c->k_scale;
+  p.v_scale = c->v_scale;
+  p.seqlens = a->seqlens;
+  p.fresh = a->seqused_new;
+  p.table = c->page_table;
+  p.cos = a->cos;
+  p.sin = a->sin;
+  p.rotary_dim = rotate ? a->rotary_dim : 0;
+  p.rotary_rows = a->rotary_rows;
+  p.rotary_bf16 = a->rotary_bf16;
+  p.interleaved = a->interleaved;
+  p.B = a->B; p.S = a->S; p.Hq = a->Hq; p.Hkv = c->Hkv; p.D = c->D;
+  p.log_block = log2_of(c->block);
+  p.num_pages = c->num_pages; p.page_size = c->page_size; p.pages_per_seq = c->pages_per_seq;
+  p.blocks = (int)blocks;
+  p.div_blocks = make_fastdiv((uint32_t)blocks);
+  p.div_hkv2 = make_fastdiv((uint32_t)c->Hkv * 2u);
+  p.div_page = make_fastdiv((uint32_t)c->page_size);
+  p.div_s = make_fastdiv((uint32_t)a->S);
+  p.status = a->status;
+  p.epoch = next_launch_epoch();
+  // q: four heads of a row to a thread, which share the angles, where that leaves threads enough
+  const int64_t chunks = c->D / 16, q_items = with_q ? (int64_t)a->B * a->S * a->Hq * chunks : 0;
+  p.q_heads = q_items >= 4 * kSms * 2048 ? 4 : 1;
+  p.q_head_groups = with_q ? (a->Hq + p.q_heads - 1) / p.q_heads : 1;
+  p.div_groups = make_fastdiv((uint32_t)p.q_head_groups);
+  const int64_t q_threads = with_q ? (int64_t)a->B * a->S * p.q_head_groups * chunks : 0;
+  auto launch = [&](auto kernel, int threads, int64_t ctas) -> int {
+    p.kv_ctas = (int)ctas;
+    const int64_t grid = ctas + (q_threads + threads - 1) / threads;
+    return launch_pdl(kernel, dim3((unsigned)grid), (unsigned)threads, 0, static_cast<cudaStream_t>(cuda_stream), p);
+  };
+  // pieces of 16 elements that a unit may have
+  const int64_t pieces = std::min<int64_t>(a->S, c->block) * chunks;
+  if (pieces <= 32) return launch(fp8_append_kernel<32, 1>, 128, (units + 3) / 4);
+  if (pieces <= 64) return launch(fp8_append_kernel<64, 1>, 64, units);
+  if (pieces <= 128) return launch(fp8_append_kernel<128, 1>, 128, units);
+  if (pieces <= 256) return launch(fp8_append_kernel<256, 1>, 256, units);
+  if (pieces <= 512) return launch(fp8_append_kernel<256, 2>, 256, units);
+  return launch(fp8_append_kernel<256, 4>, 256, units);
+}
+
+namespace {
+
+int validate_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f) {
+  if (int e = validate_cache(c)) return e;
+  if (f == nullptr) return -FA4_E_NULL;
+  if (f->struct_size != sizeof(fa4_fp8_fwd)) return -FA4_E_STRUCT;
+  if (!f->q || !f->out || !f->seqused_k) return -FA4_E_NULL;
+  if (f->B <= 0 || f->Sq <= 0 || f->Hq <= 0 || f->Hq % c->Hkv != 0) return -FA4_E_SHAPE;
+  if (c->page_table == nullptr && f->B > c->num_pages) return -FA4_E_SHAPE;
+  if (!(f->softmax_scale > 0.f) || !(f->softcap >= 0.f) || f->num_splits < 0 || f->num_splits > 128) return -FA4_E_SHAPE;
+  if ((int64_t)f->B * f->Sq * f->Hq > 0x0fffffffll || f->B > 65535) return -FA4_E_TOO_LARGE;
+  const int64_t strides[] = {f->q_stride_b, f->q_stride_s, f->q_stride_h, f->o_stride_b, f->o_stride_s, f->o_stride_h};
+  for (int64_t s : strides)
+    if ((s & 7) != 0) return -FA4_E_STRIDE;
+  if (!aligned16(f->q) || !aligned16(f->out)) return -FA4_E_ALIGN;
+  return 0;
+}
+
+}  // namespace
+
+extern "C" int64_t fa4_fp8_cache_fwd_workspace_bytes(const fa4_fp8_cache* c, const fa4_fp8_fwd* f) {
+  if (int e = validate_fwd(c, f)) return e;
+  return 0;
+}
+
+extern "C" int fa4_fp8_cache_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, void* cuda_stream) {
+  if (int e = validate_fwd(c, f)) return e;
+  Fp8Params p = {};
+  p.q = static_cast<const __nv_bfloat16*>(f->q);
+  p.out = static_cast<__nv_bfloat16*>(f->out);
+  p.lse = f->lse;
+  p.q_b = f->q_stride_b; p.q_s = f->q_stride_s; p.q_h = f->q_stride_h;
+  p.o_b = f->o_stride_b; p.o_s = f->o_stride_s; p.o_h = f->o_stride_h;
+  p.kc = static_cast<const uint8_t*>(c->k);
+  p.vc = static_cast<const uint8_t*>(c->v);
+  p.kc_page = c->k_stride_page; p.kc_tok = c->k_stride_token; p.kc_head = c->k_stride_head;
+  p.vc_page = c->v_stride_page; p.vc_tok = c->v_stride_token; p.vc_head = c->v_stride_head;
+  p.k_scale = c->k_scale;
+  p.v_scale = c->v_scale;
+  p.used = f->seqused_k;
+  p.fresh = f->seqused_q;
+  p.table = c->page_table;
+  p.sink = f->sink;
+  p.B = f->B; p.Sq = f->Sq; p.Hq = f->Hq; p.Hkv = c->Hkv; p.group = f->Hq / c->Hkv; p.D = c->D;
+  p.log_block = log2_of(c->block);
+  p.num_pages = c->num_pages; p.page_size = c->page_size; p.pages_per_seq = c->pages_per_seq;
+  p.capacity = c->pages_per_seq * c->page_size;
+  p.div_page = make_fastdiv((uint32_t)c->page_size);
+  p.div_group = make_fastdiv((uint32_t)p.group);
+  p.scale = f->softmax_scale;
+  p.softcap = f->softcap;
+  p.win_left = f->window_left;
+  p.win_right = f->causal && f->window_right < 0 ? 0 : f->window_right;
+  p.status = f->status;
+  p.epoch = next_launch_epoch();
+  p.budget_ns = f->wait_budget_ns ? f->wait_budget_ns : kDefaultBudgetNs;
+  return launch_pdl(fp8_attn_rows_kernel, dim3((unsigned)(f->Sq * f->Hq), (unsigned)f->B), 128, 0,
+                    static_cast<cudaStream_t>(cuda_stream), p);
+}

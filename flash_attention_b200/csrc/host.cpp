@@ -974,6 +974,266 @@ PyObject* host_pieces(PyObject* const* a) {
   Py_RETURN_NONE;
 }
 
+// ---- the 8-bit KV cache -----------------------------------------------------------------------------
+// What both calls get of a cache: k v k_scale v_scale page_table
+struct Fp8Cache {
+  at::Tensor k, v, k_scale, v_scale, table;
+  fa4_fp8_cache c = {};
+};
+
+// The last dimension contiguous, 16-byte pieces aligned: as it is, or a copy.
+at::Tensor in_pieces(const at::Tensor& t) {
+  bool ok = t.stride(-1) == 1 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0;
+  for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && t.stride(i) % 8 == 0;
+  return ok ? t : t.contiguous();
+}
+
+at::Tensor counts_of(const at::Tensor& t, const char* name, int64_t B, const at::Device& device) {
+  if (!t.defined()) return {};
+  FA4_ASSERT(t.dim() == 1 && t.size(0) == B && t.scalar_type() == at::kInt && t.device() == device,
+             "%s must be a (%lld,) int32 tensor on %s", name, (long long)B, device.str().c_str());
+  return t.contiguous();
+}
+
+void describe_cache(Fp8Cache& f, int64_t B) {
+  const at::Tensor &k = f.k, &v = f.v;
+  FA4_ASSERT(k.is_cuda(), "the cache must be on CUDA");
+  FA4_ASSERT(k.dim() == 4 && k.sizes() == v.sizes(), "k and v of the cache must be (num_pages, page_size, heads, head_dim) both, got %s and %s",
+             dims_of(k.sizes()).c_str(), dims_of(v.sizes()).c_str());
+  const int64_t pages = k.size(0), size = k.size(1), H = k.size(2), D = k.size(3);
+  const at::Device device = k.device();
+  FA4_ASSERT(v.device() == device, "v of the cache is on %s, k on %s", v.device().str().c_str(), device.str().c_str());
+  if (D != 64 && D != 128)
+    fail(PyExc_NotImplementedError, "head dim %lld is not built for the 8-bit cache; supported: 64 and 128", (long long)D);
+  FA4_ASSERT(pages > 0 && size > 0 && H > 0, "the cache is empty");
+  const int64_t blocks = f.k_scale.dim() == 3 ? f.k_scale.size(1) : 0;
+  FA4_ASSERT(blocks > 0 && size % blocks == 0 && (size / blocks == 16 || size / blocks == 32 || size / blocks == 64 || size / blocks == 128),
+             "k_scale must be (num_pages, page_size / block, heads) for blocks of 16, 32, 64 or 128 tokens, got %s", dims_of(f.k_scale.sizes()).c_str());
+  validate(f.k_scale, "k_scale", {pages, blocks, H}, at::kFloat, device);
+  validate(f.v_scale, "v_scale", {pages, blocks, H}, at::kFloat, device);
+  FA4_ASSERT(f.k_scale.is_contiguous() && f.v_scale.is_contiguous(), "the scales of the cache must be contiguous");
+  fa4_fp8_cache& c = f.c;
+  // (the stride of a dimension of one is never used, and may be anything)
+  auto strides = [&](const at::Tensor& t, const char* name, int64_t& page, int64_t& token, int64_t& head) {
+    FA4_ASSERT(t.stride(3) == 1 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0,
+               "%s of the cache must be 16-byte aligned, its last dimension contiguous", name);
+    int64_t s[3];
+    for (int i = 0; i < 3; ++i) {
+      s[i] = t.size(i) == 1 ? D : t.stride(i);
+      FA4_ASSERT(s[i] > 0 && s[i] % 16 == 0, "%s of the cache: strides must be positive multiples of 16 bytes", name);
+    }
+    page = s[0]; token = s[1]; head = s[2];
+  };
+  strides(k, "k", c.k_stride_page, c.k_stride_token, c.k_stride_head);
+  strides(v, "v", c.v_stride_page, c.v_stride_token, c.v_stride_head);
+  c.struct_size = sizeof c;
+  c.num_pages = (int32_t)pages; c.page_size = (int32_t)size; c.block = (int32_t)(size / blocks);
+  c.Hkv = (int32_t)H; c.D = (int32_t)D;
+  c.k = k.data_ptr(); c.v = v.data_ptr();
+  c.k_scale = f.k_scale.data_ptr<float>(); c.v_scale = f.v_scale.data_ptr<float>();
+  c.pages_per_seq = 1;
+  if (f.table.defined()) {
+    FA4_ASSERT(f.table.dim() == 2 && f.table.size(0) == B && f.table.size(1) > 0 && f.table.scalar_type() == at::kInt && f.table.device() == device,
+               "page_table must be a (B, pages_per_seq) int32 tensor on the cache's device");
+    f.table = f.table.contiguous();
+    c.page_table = f.table.data_ptr<int32_t>();
+    c.pages_per_seq = (int32_t)f.table.size(1);
+  } else {
+    FA4_ASSERT(pages >= B, "a cache without a page table has a page for every sequence: %lld for %lld", (long long)pages, (long long)B);
+  }
+}
+
+Fp8Cache cache_of(PyObject* const* a) {
+  Fp8Cache f;
+  f.k = as_u8(a[0], "k of the cache");
+  f.v = as_u8(a[1], "v of the cache");
+  f.k_scale = tensor_of(a[2], "k_scale");
+  f.v_scale = tensor_of(a[3], "v_scale");
+  f.table = optional_tensor(a[4], "page_table");
+  return f;
+}
+
+// k_cache v_cache k_scale v_scale page_table k v cache_seqlens seqused_new rotary_cos rotary_sin rotary_interleaved q
+struct AppendCall {
+  Fp8Cache f;
+  at::Tensor k, v, held, fresh, cos, sin, q, q_out;
+  bool interleaved = false;
+  uint32_t* status = nullptr;
+};
+
+void run_append(AppendCall& c) {
+  FA4_ASSERT(c.k.dim() == 4 && c.v.dim() == 4 && c.k.sizes() == c.v.sizes(), "k and v must be (B, S, heads, head_dim) both, got %s and %s",
+             dims_of(c.k.sizes()).c_str(), dims_of(c.v.sizes()).c_str());
+  const int64_t B = c.k.size(0), S = c.k.size(1), H = c.k.size(2), D = c.k.size(3);
+  describe_cache(c.f, B);
+  const at::Device device = c.f.k.device();
+  validate(c.k, "k", {B, S, c.f.c.Hkv, c.f.c.D}, at::kBFloat16, device);
+  validate(c.v, "v", {B, S, H, D}, at::kBFloat16, device);
+  const at::Tensor held = counts_of(c.held, "cache_seqlens", B, device), fresh = counts_of(c.fresh, "seqused_new", B, device);
+  FA4_ASSERT(c.cos.defined() == c.sin.defined(), "rotary_cos and rotary_sin come together");
+  FA4_ASSERT(!c.q.defined() || c.cos.defined(), "q is for the rotation: pass rotary_cos and rotary_sin too");
+  at::Tensor cos = c.cos, sin = c.sin;
+  if (cos.defined()) {
+    FA4_ASSERT(cos.dim() == 2 && cos.sizes() == sin.sizes() && cos.size(0) > 0, "rotary_cos and rotary_sin must be (positions, rotary_dim / 2) both");
+    FA4_ASSERT(cos.size(1) > 0 && cos.size(1) % 8 == 0 && 2 * cos.size(1) <= D, "rotary_dim must be a multiple of 16 and at most the head dim");
+    FA4_ASSERT((cos.scalar_type() == at::kFloat || cos.scalar_type() == at::kBFloat16) && cos.scalar_type() == sin.scalar_type(),
+               "rotary_cos and rotary_sin must be fp32 or bf16");
+    FA4_ASSERT(cos.device() == device && sin.device() == device, "rotary_cos and rotary_sin must be on the cache's device");
+    FA4_ASSERT(cos.size(0) <= 0x7fffffff, "rotary_cos has too many rows");
+  }
+  if (c.q.defined()) {
+    FA4_ASSERT(c.q.dim() == 4, "q must be (B, S, heads, head_dim)");
+    validate(c.q, "q", {B, S, c.q.size(2), D}, at::kBFloat16, device);
+  }
+  c10::cuda::OptionalCUDAGuard guard;
+  if (device.index() != c10::cuda::current_device()) guard.set_device(device);
+  void* stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
+  if (c.q.defined()) c.q_out = new_tensor(c.q.sizes(), at::kBFloat16, device);
+  if (B == 0 || S == 0) return;
+  const at::Tensor k = in_pieces(c.k), v = in_pieces(c.v), q = c.q.defined() && c.q.numel() > 0 ? in_pieces(c.q) : at::Tensor();
+  fa4_fp8_append a = {};
+  a.struct_size = sizeof a;
+  a.B = (int32_t)B; a.S = (int32_t)S;
+  a.k = k.data_ptr(); a.v = v.data_ptr();
+  a.k_stride_b = k.stride(0); a.k_stride_s = k.stride(1); a.k_stride_h = k.stride(2);
+  a.v_stride_b = v.stride(0); a.v_stride_s = v.stride(1); a.v_stride_h = v.stride(2);
+  if (q.defined()) {
+    a.Hq = (int32_t)q.size(2);
+    a.q = q.data_ptr(); a.q_out = c.q_out.data_ptr();
+    a.q_stride_b = q.stride(0); a.q_stride_s = q.stride(1); a.q_stride_h = q.stride(2);
+  }
+  a.seqlens = held.data_ptr<int32_t>();
+  a.seqused_new = fresh.defined() ? fresh.data_ptr<int32_t>() : nullptr;
+  if (cos.defined()) {
+    auto rows = [](const at::Tensor& t) { return t.is_contiguous() && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0 ? t : t.clone(at::MemoryFormat::Contiguous); };
+    cos = rows(cos);
+    sin = rows(sin);
+    a.cos = cos.data_ptr(); a.sin = sin.data_ptr();
+    a.rotary_dim = (int32_t)(2 * cos.size(1)); a.rotary_rows = (int32_t)cos.size(0);
+    a.rotary_bf16 = cos.scalar_type() == at::kBFloat16;
+  }
+  a.interleaved = c.interleaved;
+  a.status = c.status;
+  check_rc(fa4_fp8_cache_append(&c.f.c, &a, stream), "fa4_fp8_cache_append");
+}
+
+PyObject* append_fp8(PyObject* const* a) {
+  AppendCall c;
+  c.f = cache_of(a);
+  c.k = tensor_of(a[5], "k");
+  c.v = tensor_of(a[6], "v");
+  c.held = tensor_of(a[7], "cache_seqlens");
+  c.fresh = optional_tensor(a[8], "seqused_new");
+  c.cos = optional_tensor(a[9], "rotary_cos");
+  c.sin = optional_tensor(a[10], "rotary_sin");
+  c.interleaved = truth_of(a[11]);
+  c.q = optional_tensor(a[12], "q");
+  if (c.f.k.is_cuda()) c.status = status_word(c.f.k.device());
+  {
+    NoGil nogil;
+    run_append(c);
+  }
+  if (c.q_out.defined()) return THPVariable_Wrap(c.q_out);
+  Py_RETURN_NONE;
+}
+
+// k_cache v_cache k_scale v_scale page_table q seqused_k seqused_q softmax_scale causal window_left window_right
+// learnable_sink softcap num_splits return_lse out lse
+struct Fp8Call {
+  Fp8Cache f;
+  at::Tensor q, used, fresh, sink, out, lse;
+  bool default_softmax_scale = true, want_lse = false;
+  double softmax_scale = 0.0, softcap = 0.0;
+  long num_splits = 0;
+  Window win;
+  uint32_t* status = nullptr;
+};
+
+void run_fp8(Fp8Call& c) {
+  FA4_ASSERT(c.q.dim() == 4, "q must be (B, Sq, heads, head_dim), got %s", dims_of(c.q.sizes()).c_str());
+  const int64_t B = c.q.size(0), Sq = c.q.size(1), Hq = c.q.size(2);
+  describe_cache(c.f, B);
+  const at::Device device = c.f.k.device();
+  const int64_t Hkv = c.f.c.Hkv, D = c.f.c.D;
+  validate(c.q, "q", {B, Sq, Hq, D}, at::kBFloat16, device);
+  FA4_ASSERT(Hq > 0 && Hq % Hkv == 0, "num_head must be divisible by num_head_kv");
+  const at::Tensor used = counts_of(c.used, "seqused_k", B, device), fresh = counts_of(c.fresh, "seqused_q", B, device);
+  if (c.num_splits < 0 || c.num_splits > 128) fail(PyExc_ValueError, "num_splits must be in 0..128");
+  if (!(c.softcap >= 0.0) || !std::isfinite(c.softcap)) fail(PyExc_ValueError, "softcap must be a finite number >= 0");
+  const double softmax_scale = c.default_softmax_scale ? 1.0 / std::sqrt((double)D) : c.softmax_scale;
+  if (!(softmax_scale > 0.0) || !std::isfinite(softmax_scale)) fail(PyExc_ValueError, "softmax_scale must be a finite number > 0");
+  c10::cuda::OptionalCUDAGuard guard;
+  if (device.index() != c10::cuda::current_device()) guard.set_device(device);
+  void* stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
+  if (!c.out.defined()) {
+    c.out = new_tensor({B, Sq, Hq, D}, at::kBFloat16, device);
+    // (rows of padding are not written)
+    if (fresh.defined()) c.out.zero_();
+  } else {
+    validate(c.out, "out", {B, Sq, Hq, D}, at::kBFloat16, device);
+    FA4_ASSERT(c.out.stride(3) == 1 && (reinterpret_cast<uintptr_t>(c.out.data_ptr()) & 15u) == 0 && c.out.stride(0) % 8 == 0 &&
+                   c.out.stride(1) % 8 == 0 && c.out.stride(2) % 8 == 0,
+               "out must be 16-byte aligned, its last dimension contiguous, its strides multiples of 8");
+  }
+  if (c.lse.defined()) {
+    validate(c.lse, "lse", {B, Hq, Sq}, at::kFloat, device);
+    FA4_ASSERT(c.lse.is_contiguous(), "lse must be contiguous");
+  } else if (c.want_lse) {
+    c.lse = new_tensor({B, Hq, Sq}, at::kFloat, device);
+    if (fresh.defined()) c.lse.zero_();
+  }
+  if (B == 0 || Sq == 0) return;
+  const at::Tensor q = in_pieces(c.q), sink = sink_of(c.sink, Hq, device);
+  fa4_fp8_fwd p = {};
+  p.struct_size = sizeof p;
+  p.B = (int32_t)B; p.Sq = (int32_t)Sq; p.Hq = (int32_t)Hq;
+  p.q = q.data_ptr(); p.out = c.out.data_ptr();
+  p.lse = c.lse.defined() ? c.lse.data_ptr<float>() : nullptr;
+  p.q_stride_b = q.stride(0); p.q_stride_s = q.stride(1); p.q_stride_h = q.stride(2);
+  p.o_stride_b = c.out.stride(0); p.o_stride_s = c.out.stride(1); p.o_stride_h = c.out.stride(2);
+  p.seqused_k = used.data_ptr<int32_t>();
+  p.seqused_q = fresh.defined() ? fresh.data_ptr<int32_t>() : nullptr;
+  p.sink = sink.defined() ? sink.data_ptr<float>() : nullptr;
+  p.softmax_scale = (float)softmax_scale;
+  p.softcap = (float)c.softcap;
+  p.causal = c.win.causal;
+  p.window_left = c.win.left; p.window_right = c.win.right;
+  p.num_splits = (int32_t)c.num_splits;
+  p.status = c.status;
+  const int64_t bytes = fa4_fp8_cache_fwd_workspace_bytes(&c.f.c, &p);
+  if (bytes < 0) check_rc((int)bytes, "fa4_fp8_cache_fwd_workspace_bytes");
+  c10::DataPtr workspace;
+  if (bytes > 0) {
+    workspace = scratch_bytes(bytes);
+    p.workspace = workspace.get();
+    p.workspace_bytes = (uint64_t)bytes;
+  }
+  check_rc(fa4_fp8_cache_fwd(&c.f.c, &p, stream), "fa4_fp8_cache_fwd");
+}
+
+PyObject* fwd_fp8(PyObject* const* a) {
+  Fp8Call c;
+  c.f = cache_of(a);
+  c.q = tensor_of(a[5], "q");
+  c.used = tensor_of(a[6], "seqused_k");
+  c.fresh = optional_tensor(a[7], "seqused_q");
+  c.default_softmax_scale = is_none(a[8]);
+  if (!c.default_softmax_scale) c.softmax_scale = number_of(a[8]);
+  c.win = resolve_window(truth_of(a[9]), a[10], a[11]);
+  c.sink = optional_tensor(a[12], "learnable_sink");
+  if (!is_none(a[13])) c.softcap = number_of(a[13]);
+  c.num_splits = integer_of(a[14]);
+  c.want_lse = truth_of(a[15]);
+  c.out = optional_tensor(a[16], "out");
+  c.lse = optional_tensor(a[17], "lse");
+  if (c.f.k.is_cuda()) c.status = status_word(c.f.k.device());
+  {
+    NoGil nogil;
+    run_fp8(c);
+  }
+  return pair_of(a[16], c.out, a[17], c.lse);
+}
+
 // ---- the module -----------------------------------------------------------------------------------
 PyObject* choose_decode_splits(PyObject* const* a) {
   return PyLong_FromLongLong(decode_splits(integer_of(a[0]), integer_of(a[1]), integer_of(a[2]), integer_of(a[3])));
@@ -1036,6 +1296,8 @@ PyMethodDef methods[] = {method<fwd, 23>("fwd"),
                          method<quantize_qkv, 4>("quantize_qkv"),
                          method<host_pieces, 25>("host_pieces"),
                          method<window_of, 3>("resolve_window"),
+                         method<append_fp8, 13>("append_fp8"),
+                         method<fwd_fp8, 18>("fwd_fp8"),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_host", "Native host path of flash_attention_b200.", -1, methods,
                           nullptr, nullptr, nullptr, nullptr};

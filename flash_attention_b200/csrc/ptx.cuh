@@ -17,6 +17,7 @@ namespace fa4 {
 // host counts launches modulo 256) and runs normally beside a stale word.
 // ---------------------------------------------------------------------------------------------
 constexpr uint32_t kStatusWaitExpired = 1u;
+constexpr uint32_t kStatusBadIndex = 2u;   // stops no launch: what the index leads to is left out
 
 // (The attention kernels keep theirs in shared memory, written once by one thread: waits that block
 // pass its address to one out-of-line function, and no role holds these words in registers.)
@@ -31,7 +32,7 @@ struct WaitCtx {
 __device__ __forceinline__ bool status_poisoned(const uint32_t* g_status, uint32_t epoch) {
   if (g_status == nullptr) return false;
   const uint32_t v = *reinterpret_cast<const volatile uint32_t*>(g_status);
-  return v != 0u && ((v >> 8) & 0xffu) == epoch;
+  return (v >> 24) == kStatusWaitExpired && ((v >> 8) & 0xffu) == epoch;
 }
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
@@ -163,7 +164,7 @@ __device__ __forceinline__ bool mbar_poll(uint32_t bar, uint32_t parity, uint32_
 // thirty sites it was half of the code of the 64-key kernel, which on short tiles visits all of it
 // once per tile and then waits for instructions more than for anything else (a 127-key window:
 // 36 % of the instruction-cache requests missed, 5.5 of its 14 stalled warps per issue slot).
-__device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, const WaitCtx* w, uint32_t site,
+inline __device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, const WaitCtx* w, uint32_t site,
                                             uint32_t hint_ns) {
   const uint64_t t0 = globaltimer_ns();
   for (;;) {

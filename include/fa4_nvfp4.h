@@ -74,7 +74,10 @@ enum {
  * the word wherever results are consumed on the host. */
 enum {
   FA4_S_OK = 0,
-  FA4_S_WAIT_EXPIRED = 1 /* a bounded mbarrier wait ran out; `site` names the wait */
+  FA4_S_WAIT_EXPIRED = 1, /* a bounded mbarrier wait ran out; `site` names the wait */
+  FA4_S_BAD_INDEX = 2    /* 8-bit cache: an index on the device lies outside its range and what it leads to was left
+                            out; `site`: 120 a position behind the cache's end, 121 a page number, 122 a position without a row
+                            in the rotation's tables.  Stops nothing */
 };
 
 /* kernel variants */
@@ -471,6 +474,109 @@ int fa4_nvfp4_debug_wait_expiry(uint32_t* status, uint64_t budget_ns, void* cuda
  */
 #define FA4_NVFP4_STATIC_SCRATCH_BYTES (16u << 20)
 int fa4_nvfp4_fwd_linear_sf_noalloc(const fa4_nvfp4_params* p, void* cuda_stream);
+
+/*
+ * ---- KV cache in 8 bits ---------------------------------------------------------------------------------
+ *
+ * A second kind of KV cache beside the NVFP4 one: e4m3 keys and values, one fp32 scale for each block of `block`
+ * tokens and kv head, filled token by token (fa4_fp8_cache_append) and read by bf16 queries
+ * (fa4_fp8_cache_fwd).  The reference's calls of this kind are flash_attn_with_kvcache
+ * (hopper/flash_attn_interface.py: k, v, rotary_cos, rotary_sin, cache_seqlens, page_table), whose 8-bit scales
+ * are one per sequence and head; a scale per block of tokens lets a cache grow without a calibration.
+ *
+ *   k, v     (num_pages, page_size, Hkv, D) bytes, D = 64 or 128; the last dimension is contiguous, the strides of the others
+ *            are multiples of 16 bytes (so pools of (page, head, token) order are views), base 16-byte aligned
+ *   k_scale, v_scale  (num_pages, page_size / block, Hkv) fp32, contiguous: value = byte * scale
+ *   block    16, 32, 64 or 128; page_size a multiple of it
+ *   page_table (B, pages_per_seq) int32 on the device: token t of sequence b lies in page page_table[b][t / page_size].
+ *            NULL: contiguous caches, page b is sequence b's (num_pages = B at least, pages_per_seq = 1)
+ *
+ * Page numbers, lengths and positions live on the device, so the host cannot refuse bad ones: the kernels check
+ * them, leave the token (append) or the keys of the page (attention, as keys and values of zero) out and record FA4_S_BAD_INDEX in
+ * the status word.
+ */
+typedef struct fa4_fp8_cache {
+  uint32_t struct_size;      /* = sizeof(fa4_fp8_cache) */
+  int32_t num_pages, page_size, block;
+  int32_t Hkv, D;
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t k_stride_page, k_stride_token, k_stride_head;    /* bytes */
+  int64_t v_stride_page, v_stride_token, v_stride_head;
+  const int32_t* page_table;
+  int32_t pages_per_seq;
+  uint32_t reserved;         /* 0 */
+} fa4_fp8_cache;
+
+/*
+ * Keys and values of new tokens into the cache: token i (of S) of sequence b goes to position seqlens[b] + i, if
+ * i < seqused_new[b] (NULL: all).  seqlens is not changed.
+ *   Rotation (cos, sin non-NULL; (rotary_rows, rotary_dim / 2), fp32 or bf16, contiguous, row = position): of the first rotary_dim
+ *   elements of a key, pairs (x1, x2) -- elements i and i + rotary_dim / 2, or 2 i and 2 i + 1 if `interleaved` -- become
+ *   (x1 c - x2 s, x2 c + x1 s), in fp32.  q (B, S, Hq, D), if given, is rotated alike into q_out (bf16, contiguous),
+ *   all S rows of it.  rotary_dim % 16 == 0.
+ *   Scale of a block: the smallest power of two (2^-120 at least) by which the largest new value is at most 448; where
+ *   the block holds tokens already (its first position is in front of seqlens[b]) no less than the scale it
+ *   has.  If the scale grows the tokens it holds are rounded again: e4m3(byte * (old scale / new scale)).
+ *   A value that is not finite becomes the NaN code and does not count for the scale.  Bytes past the last new token are
+ *   not touched.
+ * bf16 k, v (B, S, Hkv, D), q: last dimension contiguous, strides in ELEMENTS and multiples of 8, 16-byte aligned.  A block must not
+ * belong to two sequences that append to it in one call.
+ */
+typedef struct fa4_fp8_append {
+  uint32_t struct_size;      /* = sizeof(fa4_fp8_append) */
+  int32_t B, S, Hq;
+  const void* k;
+  const void* v;
+  const void* q;             /* or NULL */
+  void* q_out;
+  int64_t k_stride_b, k_stride_s, k_stride_h;
+  int64_t v_stride_b, v_stride_s, v_stride_h;
+  int64_t q_stride_b, q_stride_s, q_stride_h;
+  const int32_t* seqlens;
+  const int32_t* seqused_new;
+  const void* cos;
+  const void* sin;
+  int32_t rotary_dim, rotary_rows;
+  int32_t rotary_bf16;       /* cos and sin are bf16, else fp32 */
+  int32_t interleaved;
+  uint32_t* status;          /* as in fa4_nvfp4_params */
+} fa4_fp8_append;
+int fa4_fp8_cache_append(const fa4_fp8_cache* cache, const fa4_fp8_append* a, void* cuda_stream);
+
+/*
+ * Attention of bf16 queries over the cache: sequence b attends to its first seqused_k[b] tokens (clamped to 0 ..
+ * pages_per_seq * page_size).  Query row i stands at position seqused_k[b] - seqused_q[b] + i (seqused_q NULL: Sq for all), which
+ * causal and window limits refer to; rows from seqused_q[b] on are neither computed nor written.
+ *   score = softmax_scale * k_scale * (q . k), soft cap, masks, sink as in fa4_nvfp4_ext
+ *   out = sum of softmax weight * v_scale * v: bf16 (B, Sq, Hq, D); lse fp32 (B, Hq, Sq) or NULL
+ * A row that sees no key gets zeros and an lse of -inf (of its sink).  What lies behind a sequence's last token may be anything,
+ * NaN included.  `workspace`: fa4_fp8_cache_fwd_workspace_bytes of device memory, 16-byte aligned, in use until the
+ * launches have run.  num_splits: 0 = chosen.
+ */
+typedef struct fa4_fp8_fwd {
+  uint32_t struct_size;      /* = sizeof(fa4_fp8_fwd) */
+  int32_t B, Sq, Hq;
+  const void* q;             /* strides in elements, multiples of 8; 16-byte aligned; last dimension contiguous */
+  void* out;
+  float* lse;
+  int64_t q_stride_b, q_stride_s, q_stride_h;
+  int64_t o_stride_b, o_stride_s, o_stride_h;
+  const int32_t* seqused_k;
+  const int32_t* seqused_q;  /* or NULL */
+  const float* sink;         /* Hq logits or NULL */
+  float softmax_scale, softcap;
+  int32_t causal, window_left, window_right;   /* -1: unlimited */
+  int32_t num_splits;
+  void* workspace;
+  uint64_t workspace_bytes;
+  uint32_t* status;
+  uint64_t wait_budget_ns;   /* 0 = default (2 s) */
+} fa4_fp8_fwd;
+int64_t fa4_fp8_cache_fwd_workspace_bytes(const fa4_fp8_cache* cache, const fa4_fp8_fwd* p);
+int fa4_fp8_cache_fwd(const fa4_fp8_cache* cache, const fa4_fp8_fwd* p, void* cuda_stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,462 @@
+"""The 8-bit KV cache on the GPU: appending against the oracle, attention over it against 64 bits.
+
+Tolerances.  Appended bytes and scales are the oracle's: rotation, scale and quotient are the same correctly rounded fp32 steps
+(the rounding to e4m3 is exact in 64 bits), so they are compared for equality; q is rounded to bf16 once from those.
+Attention: one output element is sum p v / sum p.  The weights are rounded to no fewer than 8 significant bits (2^-8 of
+each at most, half a step of bf16), scores are fp32 sums of exact products, so |error| <= 2^-8 sum p |v| / sum p, plus the output's
+own rounding of 2^-8 |out|, plus fp32 noise, for which 2^-13 sum p |v| is room.  lse: fp32 sums and hardware
+exponentials, 2^-18 of max(1, |lse|), with the scores' own fp32 rounding, 2^-20 of the largest |score| for D = 128 terms."""
+import math
+
+import pytest
+import torch
+
+import flash_attention_b200 as fa
+from oracle import fp8_cache_oracle as orc
+
+pytestmark = pytest.mark.gpu
+
+
+def make_cache(pages, size, H, D, block, seed, device, nan=True):
+    """A pool of random bytes (NaN where nothing is held yet: everything here, to begin with) and odd scales."""
+    g = torch.Generator().manual_seed(seed)
+    c = fa.FP8KVCache.empty(pages, size, H, D, block, device=device)
+    for t in (c.k, c.v):
+        t.view(torch.uint8).copy_(torch.full(t.shape, 0x7F, dtype=torch.uint8) if nan else
+                                  torch.randint(0, 0x78, t.shape, generator=g, dtype=torch.uint8))
+    for t in (c.k_scale, c.v_scale):
+        t.copy_(torch.full(t.shape, math.nan) if nan else torch.rand(t.shape, generator=g))
+    return c
+
+
+def fill(cache, tables, lens, seed, spread=1.0, outlier=False):
+    """Random keys and values for the first lens[b] tokens of every sequence: e4m3 values of a maximum / 448 scale."""
+    g = torch.Generator().manual_seed(seed)
+    pages, size, H, D = cache.k.shape
+    bt = cache.block
+    for t, sc, strong in ((cache.k, cache.k_scale, outlier), (cache.v, cache.v_scale, False)):
+        values, scales = t.cpu().view(torch.uint8).clone(), sc.cpu().clone()
+        for b, n in enumerate(lens):
+            for first in range(0, n, bt):
+                m = min(bt, n - first)
+                x = torch.randn(m, H, D, generator=g) * (spread ** torch.randn(1, H, 1, generator=g))
+                if strong:
+                    x[..., ::16] *= 8
+                s = x.abs().amax(dim=(0, 2)) / 448
+                page, off = tables[b][first // size], first % size
+                values[page, off:off + m] = (x / s[None, :, None]).clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8)
+                scales[page, off // bt] = s
+        t.view(torch.uint8).copy_(values)
+        sc.copy_(scales)
+
+
+def held_of(cache, table, n):
+    """float64 keys and values (n, H, D) of a sequence."""
+    got = []
+    for t, sc in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)):
+        x = t.cpu().view(torch.float8_e4m3fn).double() * sc.cpu().double().repeat_interleave(cache.block, dim=1)[..., None]
+        got.append(torch.cat([x[p] for p in table])[:n])
+    return got
+
+
+def tables_of(B, per, pages, seed):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randperm(pages, generator=g)[:B * per].view(B, per).tolist()
+
+
+def rope(rows, dim, dtype=torch.float32, seed=0):
+    ang = torch.arange(rows, dtype=torch.float64)[:, None] * 10000.0 ** (-torch.arange(dim // 2, dtype=torch.float64) / max(1, dim // 2))
+    return ang.cos().to(dtype), ang.sin().to(dtype)
+
+
+# ---- append ---------------------------------------------------------------------------------------------------
+
+APPENDS = [
+    # B, S, H, D, page, block, paged, held, fresh, rotary, interleaved, Hq, table dtype
+    (1, 1, 1, 128, 16, 16, True, [0], None, 128, False, 4, torch.float32),
+    (3, 1, 8, 128, 64, 64, True, [0, 63, 64], None, 128, False, 32, torch.bfloat16),
+    (3, 1, 2, 64, 48, 16, True, [47, 48, 15], [1, 0, 1], 32, True, 2, torch.float32),
+    (2, 4, 3, 128, 128, 128, True, [126, 0], None, 128, True, 6, torch.float32),
+    (2, 7, 2, 64, 96, 32, True, [30, 96], [7, 3], 64, False, 2, torch.float32),
+    (2, 16, 2, 128, 32, 32, False, [16, 3], None, 0, False, 0, torch.float32),
+    (1, 333, 2, 128, 192, 64, True, [1], None, 64, False, 3, torch.float32),
+    (2, 129, 1, 128, 256, 128, True, [127, 255], [129, 1], 128, False, 5, torch.float32),
+    (2, 50, 4, 64, 64, 64, True, [60, 0], [50, 9], 16, True, 4, torch.bfloat16),
+    (2, 300, 2, 128, 16, 16, True, [5, 31], [300, 17], 128, False, 2, torch.float32),
+    (1, 500, 2, 64, 512, 128, False, [12], None, 64, True, 9, torch.float32),
+]
+
+
+def append_both(cuda_device, case, seed, scale=1.0, poke=None):
+    B, S, H, D, size, block, paged, held, fresh, rotary, interleaved, Hq, dt = case
+    per = max(-(-(h + S) // size) for h in held)
+    if not paged:
+        size, per = per * size, 1
+    pages = B * per + 2
+    tables = tables_of(B, per, pages, seed) if paged else [[b] for b in range(B)]
+    cache = make_cache(pages, size, H, D, block, seed, cuda_device)
+    fill(cache, tables, held, seed)
+    g = torch.Generator().manual_seed(seed + 1)
+    # the three tensors of a projection lie side by side
+    qkv = (torch.randn(B, S, Hq + 2 * H, D, generator=g) * scale).bfloat16()
+    if poke:
+        poke(qkv[:, :, Hq:])
+    cos, sin = rope(max(held) + S, rotary, dt) if rotary else (None, None)
+    want = {n: getattr(cache, n).cpu().float().double() for n in ("k", "v", "k_scale", "v_scale")}
+    want_q = qkv[:, :, :Hq].clone()
+    for b in range(B):
+        n = S if fresh is None else fresh[b]
+        k, v = qkv[b, :n, Hq:Hq + H].float(), qkv[b, :n, Hq + H:].float()
+        if rotary:
+            k = orc.rotate(k, cos, sin, held[b], interleaved)
+            if Hq:
+                want_q[b] = orc.rotate(qkv[b, :, :Hq], cos, sin, held[b], interleaved).bfloat16()
+        orc.append(want["k"], want["k_scale"], k, held[b], tables[b], block)
+        orc.append(want["v"], want["v_scale"], v, held[b], tables[b], block)
+    dev = qkv.to(cuda_device)
+    q = fa.append_kv_fp8(cache, dev[:, :, Hq:Hq + H], dev[:, :, Hq + H:],
+                         torch.tensor(held, dtype=torch.int32, device=cuda_device),
+                         page_table=torch.tensor(tables, dtype=torch.int32, device=cuda_device) if paged else None,
+                         seqused_new=None if fresh is None else torch.tensor(fresh, dtype=torch.int32, device=cuda_device),
+                         rotary_cos=cos.to(cuda_device) if rotary else None, rotary_sin=sin.to(cuda_device) if rotary else None,
+                         rotary_interleaved=interleaved, q=dev[:, :, :Hq] if rotary and Hq else None)
+    torch.cuda.synchronize()
+    fa.check_status(cuda_device)
+    for name in ("k", "v", "k_scale", "v_scale"):
+        got = getattr(cache, name).cpu().float().double()
+        same = (got == want[name]) | (got.isnan() & want[name].isnan())
+        assert same.all(), f"{name}: {(~same).sum()} of {same.numel()} differ, first at {(~same).nonzero()[0].tolist()}"
+    if rotary and Hq:
+        assert torch.equal(q.cpu(), want_q)
+    else:
+        assert q is None
+
+
+@pytest.mark.parametrize("case", APPENDS)
+def test_append_gives_the_oracles_bytes(cuda_device, case):
+    append_both(cuda_device, case, seed=3)
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-3, 40.0, 1e30])
+def test_append_of_small_and_large_values(cuda_device, scale):
+    """The block's scale grows by far (or not at all) beside what it holds."""
+    append_both(cuda_device, APPENDS[1], seed=4, scale=scale)
+    append_both(cuda_device, APPENDS[6], seed=5, scale=scale)
+
+
+def test_append_of_values_that_are_not_finite(cuda_device):
+    def poke(kv):
+        kv[0, 0, 0, 5] = math.inf
+        kv[0, 0, -1, 7] = -math.inf
+        kv[-1, -1, -1, 9] = math.nan
+        kv[-1, 0, 0] = 0
+    append_both(cuda_device, APPENDS[5], seed=6, poke=poke)
+    append_both(cuda_device, APPENDS[0][:9] + (0, False, 0, torch.float32), seed=7, poke=poke)
+
+
+def test_tokens_one_by_one_leave_what_they_leave_at_once(cuda_device):
+    """(values of one scale: where a scale grows, small values are rounded twice)"""
+    g = torch.Generator().manual_seed(8)
+    k = torch.randn(2, 70, 2, 128, generator=g).clamp(-3.4, 3.4).bfloat16()
+    k[:, 0] = 3.4375                                 # every block's largest... of the first block: the rest follows
+    k[:, 32] = 3.4375
+    k[:, 64] = 3.4375
+    k = k.to(cuda_device)
+    caches = [make_cache(2, 96, 2, 128, 32, 1, cuda_device) for _ in range(2)]
+    at = lambda n: torch.full((2,), n, dtype=torch.int32, device=cuda_device)
+    fa.append_kv_fp8(caches[0], k, k, at(0))
+    for i in range(70):
+        fa.append_kv_fp8(caches[1], k[:, i:i + 1], k[:, i:i + 1], at(i))
+    fa.check_status(cuda_device)
+    for name in ("k", "v", "k_scale", "v_scale"):
+        a, b = (getattr(c, name).view(torch.uint8) for c in caches)
+        assert torch.equal(a, b)
+
+
+def test_append_leaves_out_what_has_no_place(cuda_device):
+    """Positions behind the cache's end, pages outside the pool, positions without a row in the tables: reported, the rest
+    written."""
+    cache = make_cache(4, 32, 1, 64, 32, 1, cuda_device)
+    k = torch.randn(3, 2, 1, 64, device=cuda_device, dtype=torch.bfloat16)
+    table = torch.tensor([[0, 1], [2, 7], [3, -1]], dtype=torch.int32, device=cuda_device)
+    before = [getattr(cache, n).view(torch.uint8).clone() for n in ("k", "v")]
+    for held, site in (([63, 0, 0], 120), ([0, 33, 0], 121), ([0, 0, 40], 121), ([-5, 0, 0], 120), ([2 ** 31 - 1, 0, 0], 120)):
+        fa.append_kv_fp8(cache, k, k, torch.tensor(held, dtype=torch.int32, device=cuda_device), page_table=table)
+        with pytest.raises(RuntimeError, match=f"code 2 .*site {site},"):
+            fa.check_status(cuda_device)
+    # sequence 1 held 33 in a page outside the pool and wrote nothing there; page 1 (of sequence 0) got its one token
+    assert torch.equal(cache.k.view(torch.uint8)[1, :31], before[0][1, :31])
+    assert not torch.equal(cache.k.view(torch.uint8)[1, 31], before[0][1, 31])
+    cos, sin = (t.to(cuda_device) for t in rope(3, 64))
+    fa.append_kv_fp8(cache, k[:1], k[:1], torch.tensor([2], dtype=torch.int32, device=cuda_device), page_table=table[:1],
+                     rotary_cos=cos, rotary_sin=sin)
+    with pytest.raises(RuntimeError, match="code 2 .*site 122,"):
+        fa.check_status(cuda_device)
+    fa.append_kv_fp8(cache, k, k, torch.tensor([1, 2, 3], dtype=torch.int32, device=cuda_device), page_table=table)
+    fa.check_status(cuda_device)
+
+
+def test_append_to_a_pool_of_another_order_and_from_unaligned_views(cuda_device):
+    """(page, head, token) pools are views; k and v that are no 16-byte pieces are copied."""
+    g = torch.Generator().manual_seed(9)
+    k = torch.randn(1, 40, 2, 64, generator=g).bfloat16().to(cuda_device)
+    plain = make_cache(3, 32, 2, 64, 16, 1, cuda_device)
+    other = make_cache(3, 32, 2, 64, 16, 1, cuda_device)
+    for n in ("k", "v"):
+        t = torch.full((3, 2, 32, 64), 0x7F, dtype=torch.uint8, device=cuda_device).view(torch.float8_e4m3fn)
+        setattr(other, n, t.transpose(1, 2))
+    odd = torch.empty(40 * 2 * 65 + 1, device=cuda_device, dtype=torch.bfloat16)[1:].view(1, 40, 2, 65)[..., 1:]
+    odd.copy_(k)
+    table = torch.tensor([[2, 0]], dtype=torch.int32, device=cuda_device)
+    at = torch.tensor([7], dtype=torch.int32, device=cuda_device)
+    for c in (plain, other):
+        c.k_scale.zero_()
+        c.v_scale.zero_()
+    fa.append_kv_fp8(plain, k, k, at, page_table=table)
+    fa.append_kv_fp8(other, odd, odd, at, page_table=table)
+    fa.check_status(cuda_device)
+    for n in ("k", "v", "k_scale", "v_scale"):
+        assert torch.equal(getattr(plain, n).contiguous().view(torch.uint8), getattr(other, n).contiguous().view(torch.uint8))
+
+
+# ---- attention ------------------------------------------------------------------------------------------------
+
+def attend_both(device, B, Sq, Hq, H, D, size, block, lens, fresh=None, paged=True, spread=1.0, seed=1, outlier=False, splits=0,
+                q_scale=1.0, **kw):
+    per = max(1, max(-(-n // size) for n in lens))
+    if not paged:
+        size, per = per * size, 1
+    pages = B * per + 2
+    tables = tables_of(B, per, pages, seed) if paged else [[b] for b in range(B)]
+    cache = make_cache(pages, size, H, D, block, seed, device)
+    fill(cache, tables, lens, seed, spread, outlier)
+    g = torch.Generator().manual_seed(seed + 2)
+    q = (torch.randn(B, Sq, Hq, D, generator=g) * q_scale).bfloat16()
+    sink = torch.randn(Hq, generator=g) * 2 if kw.pop("sink", False) else None
+    # entries of the table behind the last page are anybody's
+    wide = [t + [10 ** 9, -7] for t in tables]
+    for t, n in zip(wide, lens):
+        for i in range(-(-n // size), len(t)):
+            t[i] = 10 ** 9
+    out = torch.full((B, Sq, Hq, D), 7.0, dtype=torch.bfloat16, device=device)
+    lse = torch.full((B, Hq, Sq), 7.0, device=device)
+    got, got_lse = fa.flash_attn_fp8_cache_func(
+        q.to(device), cache, torch.tensor(lens, dtype=torch.int32, device=device),
+        page_table=torch.tensor(wide, dtype=torch.int32, device=device) if paged else None,
+        seqused_q=None if fresh is None else torch.tensor(fresh, dtype=torch.int32, device=device),
+        learnable_sink=None if sink is None else sink.to(device), num_splits=splits, return_lse=True, out=out, lse=lse, **kw)
+    torch.cuda.synchronize()
+    fa.check_status(device)
+    assert got is out and got_lse is lse
+    args = dict(softmax_scale=kw.get("softmax_scale"), causal=kw.get("causal", False), window=kw.get("window_size", (None, None)),
+                sink=sink, softcap=kw.get("softcap", 0.0))
+    for b in range(B):
+        n = Sq if fresh is None else fresh[b]
+        k, v = held_of(cache, tables[b], lens[b])
+        want, want_lse = orc.attend(q[b], k, v, n, **args)
+        mag, _ = orc.attend(q[b], k, v.abs(), n, **args)
+        o, l = out[b, :n].cpu().double(), lse[b, :, :n].cpu().double()
+        off = (o - want).abs()
+        room = 2.0 ** -8 * (mag + want.abs()) + 2.0 ** -13 * mag + 1e-30
+        assert (off <= room).all(), f"sequence {b}: {(off / room).max():.2f} of the room at {(off / room).argmax()}"
+        sees = want_lse > -math.inf
+        assert torch.equal(sees, l > -math.inf)
+        top = 1.0
+        if k.shape[0]:
+            top = float((q[b, :n].double().norm(dim=-1).max() if n else 0.0) * k.norm(dim=-1).max()) * (kw.get("softmax_scale") or D ** -0.5)
+        room = 2.0 ** -18 * want_lse[sees].abs().clamp(min=1.0) + 2.0 ** -20 * top
+        assert ((l[sees] - want_lse[sees]).abs() <= room).all(), f"lse off by {(l[sees] - want_lse[sees]).abs().max():.2e}, room {room.min():.2e}"
+        # rows behind the last one stay as they were
+        assert (out[b, n:] == 7.0).all() and (lse[b, :, n:] == 7.0).all()
+    return out, lse
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("group", [1, 4, 8, 16])
+@pytest.mark.parametrize("lens", [[1], [0, 5], [777, 128, 127], [16, 2049, 300, 129]])
+def test_one_token(cuda_device, D, group, lens):
+    attend_both(cuda_device, len(lens), 1, 2 * group, 2, D, 64, 64, lens, causal=True)
+
+
+@pytest.mark.parametrize("size,block,paged", [(16, 16, True), (48, 16, True), (32, 32, True), (96, 32, True), (128, 64, True),
+                                              (192, 64, True), (256, 128, True), (384, 128, True), (128, 16, True), (16, 16, False),
+                                              (64, 64, False), (128, 128, False)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_pages_and_blocks(cuda_device, size, block, paged, D):
+    attend_both(cuda_device, 3, 1, 8, 2, D, size, block, [500, 1030, 17], paged=paged, causal=True, spread=8.0)
+    attend_both(cuda_device, 2, 40, 8, 2, D, size, block, [500, 333], paged=paged, causal=True, spread=8.0)
+
+
+@pytest.mark.parametrize("Sq,group", [(2, 4), (3, 3), (4, 4), (5, 4), (8, 4), (7, 5), (33, 1), (9, 8), (64, 2), (130, 4), (257, 1)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_several_rows(cuda_device, Sq, group, causal):
+    attend_both(cuda_device, 2, Sq, 2 * group, 2, 128, 64, 64, [Sq + 300, Sq], causal=causal)
+    attend_both(cuda_device, 2, Sq, 2 * group, 2, 64, 64, 64, [Sq + 300, Sq], causal=causal)
+
+
+@pytest.mark.parametrize("window", [(0, 0), (15, None), (127, 0), (200, 3), (None, 5)])
+@pytest.mark.parametrize("Sq,group", [(1, 4), (4, 4), (70, 4)])
+def test_windows(cuda_device, window, Sq, group):
+    for D in (64, 128):
+        attend_both(cuda_device, 3, Sq, 2 * group, 2, D, 64, 32, [Sq + 700, Sq + 128, Sq], window_size=window,
+                    causal=window[1] is None, spread=4.0)
+
+
+@pytest.mark.parametrize("Sq,group", [(1, 4), (6, 2), (70, 4)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_sink_and_softcap(cuda_device, Sq, group, D):
+    lens = [Sq + 300, Sq + 5, 0]
+    attend_both(cuda_device, 3, Sq, 2 * group, 2, D, 64, 32, lens, causal=True, sink=True, fresh=[Sq, Sq, Sq])
+    attend_both(cuda_device, 3, Sq, 2 * group, 2, D, 64, 32, lens, causal=True, softcap=20.0, q_scale=4.0)
+    attend_both(cuda_device, 3, Sq, 2 * group, 2, D, 64, 32, lens, window_size=(40, 0), sink=True, softcap=5.0)
+
+
+@pytest.mark.parametrize("Sq,group", [(1, 4), (6, 2), (70, 4)])
+def test_padded_batches_and_rows_that_see_nothing(cuda_device, Sq, group):
+    """Rows behind seqused_q are left alone; with fewer keys than rows the first rows see nothing."""
+    for D in (64, 128):
+        attend_both(cuda_device, 4, Sq, 2 * group, 2, D, 64, 64, [300, 40, max(1, Sq // 2), 0], fresh=[Sq, max(1, Sq - 3), Sq, Sq], causal=True)
+        attend_both(cuda_device, 3, Sq, 2 * group, 2, D, 64, 64, [300, 40, 7], fresh=[0, Sq, 1], causal=True)
+
+
+@pytest.mark.parametrize("splits", [1, 2, 3, 7, 16, 128])
+@pytest.mark.parametrize("Sq,group,D", [(1, 8, 128), (5, 4, 128), (1, 4, 64), (60, 4, 128), (60, 4, 64)])
+def test_splits(cuda_device, splits, Sq, group, D):
+    attend_both(cuda_device, 2, Sq, group * 2, 2, D, 64, 64, [Sq + 1500, Sq + 100], causal=True, splits=splits, sink=True)
+    attend_both(cuda_device, 2, Sq, group * 2, 2, D, 64, 64, [Sq + 1500, Sq + 100], splits=splits, window_size=(300, 0))
+
+
+@pytest.mark.parametrize("Sq", [1, 70])
+@pytest.mark.parametrize("D", [64, 128])
+def test_strong_channels_and_unequal_blocks(cuda_device, Sq, D):
+    """Scores far apart, keys of a few strong channels, values whose blocks differ by orders of magnitude."""
+    attend_both(cuda_device, 2, Sq, 8, 2, D, 64, 16, [Sq + 900, Sq + 40], causal=True, spread=30.0, outlier=True, q_scale=6.0)
+    attend_both(cuda_device, 2, Sq, 8, 2, D, 64, 16, [Sq + 900, Sq + 40], causal=True, q_scale=1e-3)
+    attend_both(cuda_device, 1, Sq, 8, 2, D, 64, 16, [Sq + 900], causal=True, q_scale=30.0, softmax_scale=1.0)
+
+
+def test_many_sequences(cuda_device):
+    lens = [(37 * b) % 700 for b in range(150)]
+    attend_both(cuda_device, 150, 1, 4, 1, 128, 32, 32, lens, causal=True)
+    attend_both(cuda_device, 150, 2, 8, 2, 64, 32, 32, lens, causal=True)
+
+
+def test_a_prompt_appended_and_attended_step_by_step(cuda_device):
+    """The calls of a serving loop: a ragged batch of prompts in two pieces, then tokens one by one, one graph for the steps;
+    attention of all rows against the oracle over what the cache holds."""
+    B, H, G, D, size, block = 3, 2, 8, 128, 32, 32
+    lens, steps = [90, 41, 7], 6
+    per = -(-(max(lens) + steps) // size)
+    tables = tables_of(B, per, B * per + 1, 5)
+    table = torch.tensor(tables, dtype=torch.int32, device=cuda_device)
+    cache = make_cache(B * per + 1, size, H, D, block, 5, cuda_device)
+    g = torch.Generator().manual_seed(6)
+    T = max(lens) + steps
+    q, k, v = ((torch.randn(B, T, n, D, generator=g)).bfloat16().to(cuda_device) for n in (G, H, H))
+    cos, sin = (t.to(cuda_device) for t in rope(T, D))
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda_device)
+    outs = [[] for _ in range(B)]
+    held = [0] * B
+    turned = [[] for _ in range(B)]
+    for piece in (max(lens) // 2, max(lens) - max(lens) // 2):
+        n = [max(0, min(piece, lens[b] - held[b])) for b in range(B)]
+        part = [torch.stack([torch.cat([x[b, held[b]:held[b] + n[b]], x[b, :piece - n[b]]]) for b in range(B)]) for x in (q, k, v)]
+        qr = fa.append_kv_fp8(cache, part[1], part[2], i32(held), page_table=table, seqused_new=i32(n), rotary_cos=cos, rotary_sin=sin, q=part[0])
+        held = [h + m for h, m in zip(held, n)]
+        out, _ = fa.flash_attn_fp8_cache_func(qr, cache, i32(held), page_table=table, seqused_q=i32(n), causal=True)
+        for b in range(B):
+            outs[b].append(out[b, :n[b]].clone())
+            turned[b].append(qr[b, :n[b]].clone())
+    # one step, captured, the lengths counted on the device
+    at = i32(held)
+    one = [torch.zeros(B, 1, x.shape[2], D, dtype=torch.bfloat16, device=cuda_device) for x in (q, k, v)]
+
+    def step():
+        qr = fa.append_kv_fp8(cache, one[1], one[2], at, page_table=table, rotary_cos=cos, rotary_sin=sin, q=one[0])
+        at.add_(1)
+        return qr, fa.flash_attn_fp8_cache_func(qr, cache, at, page_table=table, causal=True, return_lse=True)
+    graph = torch.cuda.CUDAGraph()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for t, x in zip(one, (q, k, v)):
+            t.copy_(torch.stack([x[b, held[b]] for b in range(B)])[:, None])
+        step()
+        at.sub_(1)
+    torch.cuda.current_stream().wait_stream(side)
+    with torch.cuda.graph(graph):
+        qr, (out, _) = step()
+    for i in range(steps):
+        for t, x in zip(one, (q, k, v)):
+            t.copy_(torch.stack([x[b, lens[b] + i] for b in range(B)])[:, None])
+        graph.replay()
+        for b in range(B):
+            outs[b].append(out[b].clone())
+            turned[b].append(qr[b].clone())
+    torch.cuda.synchronize()
+    fa.check_status(cuda_device)
+    for b in range(B):
+        n = lens[b] + steps
+        kk, vv = held_of(cache, tables[b], n)
+        # (an early row met scales that grew later: blocks of one magnitude keep theirs within a factor of two, which a token
+        # of the same distribution raises without moving the bytes that stay above 2^-6)
+        want, _ = orc.attend(torch.cat(turned[b]).cpu(), kk, vv, n, causal=True)
+        mag, _ = orc.attend(torch.cat(turned[b]).cpu(), kk, vv.abs(), n, causal=True)
+        off = (torch.cat(outs[b]).cpu().double() - want).abs()
+        assert (off <= 2.0 ** -8 * (mag + want.abs()) + 2.0 ** -11 * mag).all()
+
+
+def test_another_stream_and_strided_operands(cuda_device):
+    """q and out as slices of larger tensors, on a side stream, the pool in (page, head, token) order."""
+    cache = make_cache(4, 64, 2, 128, 64, 1, cuda_device)
+    tables = [[2, 0], [3, 1]]
+    fill(cache, tables, [100, 65], 1)
+    moved = fa.FP8KVCache(*(getattr(cache, n).transpose(1, 2).contiguous().transpose(1, 2) for n in ("k", "v")), cache.k_scale, cache.v_scale)
+    table = torch.tensor(tables, dtype=torch.int32, device=cuda_device)
+    lens = torch.tensor([100, 65], dtype=torch.int32, device=cuda_device)
+    for Sq in (1, 33):
+        big = torch.randn(2, Sq, 24, 128, device=cuda_device).bfloat16()
+        want, _ = fa.flash_attn_fp8_cache_func(big[:, :, 8:16].contiguous(), cache, lens, page_table=table, causal=True)
+        torch.cuda.synchronize()
+        room = torch.zeros(2, Sq, 24, 128, device=cuda_device, dtype=torch.bfloat16)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            fa.flash_attn_fp8_cache_func(big[:, :, 8:16], moved, lens, page_table=table, causal=True, out=room[:, :, 8:16])
+        side.synchronize()
+        fa.check_status(cuda_device)
+        assert torch.equal(room[:, :, 8:16], want)
+        assert not room[:, :, :8].any() and not room[:, :, 16:].any()
+
+
+def test_same_call_gives_the_same_bits(cuda_device):
+    cache = make_cache(40, 64, 2, 128, 64, 1, cuda_device)
+    tables = [list(range(20)), list(range(20, 40))]
+    fill(cache, tables, [1280, 700], 1)
+    table = torch.tensor(tables, dtype=torch.int32, device=cuda_device)
+    lens = torch.tensor([1280, 700], dtype=torch.int32, device=cuda_device)
+    for Sq in (1, 4, 200):
+        q = torch.randn(2, Sq, 8, 128, device=cuda_device).bfloat16()
+        a = [fa.flash_attn_fp8_cache_func(q, cache, lens, page_table=table, causal=True, return_lse=True) for _ in range(8)]
+        torch.cuda.synchronize()
+        fa.check_status(cuda_device)
+        for out, lse in a[1:]:
+            assert torch.equal(out, a[0][0]) and torch.equal(lse, a[0][1])
+
+
+def test_bad_pages_are_reported(cuda_device):
+    """A page outside the pool stands for keys and values of zero."""
+    cache = make_cache(3, 64, 1, 128, 64, 1, cuda_device)
+    fill(cache, [[0, 1]], [128], 1)
+    lens = torch.tensor([128], dtype=torch.int32, device=cuda_device)
+    for Sq in (1, 40):
+        q = torch.randn(1, Sq, 4, 128, device=cuda_device).bfloat16()
+        for bad in (3, -1, 10 ** 9):
+            got, _ = fa.flash_attn_fp8_cache_func(q, cache, lens, page_table=torch.tensor([[0, bad]], dtype=torch.int32, device=cuda_device))
+            with pytest.raises(RuntimeError, match="code 2 .*site 121,"):
+                fa.check_status(cuda_device)
+            k, v = held_of(cache, [0], 64)
+            z = torch.zeros_like(k)
+            want, _ = orc.attend(q[0].cpu(), torch.cat([k, z]), torch.cat([v, z]), Sq)
+            mag, _ = orc.attend(q[0].cpu(), torch.cat([k, z]), torch.cat([v, z]).abs(), Sq)
+            assert ((got[0].cpu().double() - want).abs() <= 2.0 ** -8 * (mag + want.abs()) + 2.0 ** -13 * mag).all()
