@@ -1,4 +1,4 @@
-// Attention of bf16 queries over the 8-bit KV cache.
+// What the kernels of the attention over the 8-bit KV cache share: parameters, masks, the merge of splits.
 #pragma once
 #include "fp8_append.cuh"
 
@@ -14,9 +14,15 @@ struct Fp8Params {
   const float *k_scale, *v_scale;
   const int32_t *used, *fresh, *table;
   const float* sink;
+  int num_splits;
+  float* o_partial;                  // (splits, B, Sq, Hq, D) fp32, normalised
+  float* lse_partial;                // (splits, B, Hq, Sq), log2 units, sink left out
+  int box;                           // keys of a tensor-map box: 128, or what pages and tiles of 128 share
   int B, Sq, Hq, Hkv, group, D, log_block, num_pages, page_size, pages_per_seq, capacity;
-  FastDiv div_page, div_group;
-  float scale, softcap;              // softmax scale
+  int row_tiles;                     // of a kv head and sequence
+  FastDiv div_page, div_group, div_hq, div_sq, div_row_tiles;
+  // scores in log2 units: (q . k8) * ks * sl2, or cap_out * tanh((q . k8) * ks * cap_in) with a soft cap
+  float sl2, cap_in, cap_out;
   int win_left, win_right;           // -1: unlimited
   uint32_t* status;
   uint32_t epoch;
@@ -32,80 +38,95 @@ __device__ __forceinline__ int2 seen_by(const Fp8Params& p, int sk, int sq, int 
   return make_int2(lo, hi > lo ? hi : lo);
 }
 
-// One query row a CTA of 128 threads, keys in steps of 128: a thread has a key, then an output element.
-__global__ void __launch_bounds__(128) fp8_attn_rows_kernel(const __grid_constant__ Fp8Params p) {
-  __shared__ float s_q[128], s_p[128], s_red[4];
-  __shared__ int s_page[128];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int s = blockIdx.x / p.Hq, h = blockIdx.x - s * p.Hq, b = blockIdx.y, hk = h / p.group;
+// tanh in fp32 from the exponential: 1 - 2 / (1 + e^2x), off by a few 2^-24 (tanh.approx is off by 2^-11, 1 % of a weight at a
+// cap of 30).
+__device__ __forceinline__ float tanh_of(float x) {
+  const float e = ex2_approx(x * (2.f * 1.4426950408889634f));
+  return fmaf(-2.f, __frcp_rn(1.f + e), 1.f);
+}
+__device__ __forceinline__ float score_of(const Fp8Params& p, float dot, float row_factor) {
+  return p.cap_out != 0.f ? p.cap_out * tanh_of(dot * row_factor) : dot * row_factor;
+}
+
+// Valid keys and rows of a sequence.
+struct SeqLens {
+  int sk, sq;
+};
+__device__ __forceinline__ SeqLens lens_of(const Fp8Params& p, int b) {
+  SeqLens n;
+  n.sk = p.used[b];
+  n.sk = n.sk < 0 ? 0 : (n.sk < p.capacity ? n.sk : p.capacity);
+  n.sq = p.fresh != nullptr ? p.fresh[b] : p.Sq;
+  n.sq = n.sq < 0 ? 0 : (n.sq < p.Sq ? n.sq : p.Sq);
+  return n;
+}
+
+// A row's result from its sum `l` under the reference `m` (log2 units) and the sink of its head: the factor of the
+// accumulated values, and the LSE in natural units.
+struct RowEnd {
+  float factor, lse;
+};
+__device__ __forceinline__ RowEnd finish_row(float m, float l, const float* sink, int h) {
+  constexpr float kLn2 = 0.6931471805599453f;
+  RowEnd e;
+  float top = m, keep = 1.f;
+  if (sink != nullptr) {
+    const float x = sink[h] * 1.4426950408889634f;
+    top = fmaxf(m, x);
+    keep = m == -INFINITY ? 0.f : exp2f(m - top);
+    l = (m == -INFINITY ? 0.f : l * keep) + exp2f(x - top);
+  }
+  if (top == -INFINITY && l == 0.f) return {0.f, -INFINITY};    // (a row of NaN has l = NaN and goes on)
+  e.factor = keep / l;
+  e.lse = (top + log2f(l)) * kLn2;
+  return e;
+}
+
+// Merge of splits: a warp a row.
+constexpr int kFp8CombineWarps = 4;
+__global__ void __launch_bounds__(kFp8CombineWarps * 32) fp8_combine_kernel(const __grid_constant__ Fp8Params p) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t r = blockIdx.x * kFp8CombineWarps + (threadIdx.x >> 5), rows = (uint32_t)p.B * p.Sq * p.Hq;
   pdl_wait();
-  int sk = p.used[b], sq = p.fresh != nullptr ? p.fresh[b] : p.Sq;
-  sk = sk < 0 ? 0 : (sk < p.capacity ? sk : p.capacity);
-  if (s >= sq || s >= p.Sq) return;
-  sq = sq < p.Sq ? sq : p.Sq;
-  const int2 see = seen_by(p, sk, sq, s);
-  if (tid < p.D) s_q[tid] = __bfloat162float(p.q[b * p.q_b + s * p.q_s + h * p.q_h + tid]);
-  __syncthreads();
-  float m = -INFINITY, l = 0.f, o = 0.f;
-  if (p.sink != nullptr) {
-    m = p.sink[h];
-    l = 1.f;
-  }
-  for (int j0 = see.x; j0 < see.y; j0 += 128) {
-    const int j = j0 + tid;
-    float x = -INFINITY, vs = 0.f;
-    int page = -1;
-    if (j < see.y) {
-      const int pg = fast_div(j, p.div_page), off = j - pg * p.page_size;
-      page = p.table != nullptr ? p.table[(int64_t)b * p.pages_per_seq + pg] : b;
-      float dot = 0.f;
-      if (page >= 0 && page < p.num_pages) {
-        const int64_t at = ((int64_t)page * (p.page_size >> p.log_block) + (off >> p.log_block)) * p.Hkv + hk;
-        vs = p.v_scale[at];
-        const uint8_t* kr = p.kc + page * p.kc_page + off * p.kc_tok + hk * p.kc_head;
-        for (int d = 0; d < p.D; d += 4) {
-          float y[4];
-          unpack4_e4m3(*reinterpret_cast<const uint32_t*>(kr + d), y);
-          dot += s_q[d] * y[0] + s_q[d + 1] * y[1] + s_q[d + 2] * y[2] + s_q[d + 3] * y[3];
-        }
-        dot *= p.k_scale[at];
-      } else {
-        report_bad_index(p.status, p.epoch, kPageSite);
-        page = -1;
-      }
-      x = dot * p.scale;
-      if (p.softcap > 0.f) x = p.softcap * tanhf(x / p.softcap);
+  if (r >= rows) return;
+  const int bs = fast_div((int)r, p.div_hq), h = (int)r - bs * p.Hq, b = fast_div(bs, p.div_sq), s = bs - b * p.Sq;
+  if (p.fresh != nullptr && s >= p.fresh[b]) return;
+  const int64_t l_idx = ((int64_t)b * p.Hq + h) * p.Sq + s;
+  const int col = 4 * lane;
+  float m = -INFINITY, sum = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = 0; i0 < p.num_splits; i0 += 8) {
+    float l[8], top = m;
+    float4 v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      l[j] = i0 + j < p.num_splits ? p.lse_partial[(int64_t)(i0 + j) * rows + l_idx] : -INFINITY;
     }
-    float top = x;
-    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    if (lane == 0) s_red[warp] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(m, fmaxf(s_red[0], s_red[1])), fmaxf(s_red[2], s_red[3]));
-    const float ref = top == -INFINITY ? 0.f : top, keep = expf(m - ref);
-    const float w = j < see.y ? expf(x - ref) : 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      // (a split without a key wrote no values)
+      v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (l[j] != -INFINITY && col < p.D)
+        v[j] = *reinterpret_cast<const float4*>(p.o_partial + ((int64_t)(i0 + j) * rows + r) * p.D + col);
+      top = fmaxf(top, l[j]);
+    }
+    const float ref = top == -INFINITY ? 0.f : top, keep = exp2f(m - ref);
+    sum *= keep;
+    acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float w = exp2f(l[j] - ref);
+      sum += w;
+      acc.x = fmaf(w, v[j].x, acc.x); acc.y = fmaf(w, v[j].y, acc.y);
+      acc.z = fmaf(w, v[j].z, acc.z); acc.w = fmaf(w, v[j].w, acc.w);
+    }
     m = top;
-    s_p[tid] = w * vs;
-    s_page[tid] = page;
-    float sum = w;
-    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    __syncthreads();
-    if (lane == 0) s_red[warp] = sum;
-    __syncthreads();
-    l = l * keep + s_red[0] + s_red[1] + s_red[2] + s_red[3];
-    o *= keep;
-    if (tid < p.D) {
-      for (int i = 0; i < 128 && j0 + i < see.y; ++i) {
-        if (s_page[i] < 0) continue;
-        const int pg = fast_div(j0 + i, p.div_page), off = j0 + i - pg * p.page_size;
-        float y[4];
-        unpack4_e4m3(p.vc[s_page[i] * p.vc_page + off * p.vc_tok + hk * p.vc_head + tid], y);
-        o += s_p[i] * y[0];
-      }
-    }
-    __syncthreads();
   }
-  if (tid < p.D) p.out[b * p.o_b + s * p.o_s + h * p.o_h + tid] = __float2bfloat16(l > 0.f || !(l == l) ? o / l : 0.f);
-  if (tid == 0 && p.lse != nullptr) p.lse[((int64_t)b * p.Hq + h) * p.Sq + s] = m == -INFINITY ? -INFINITY : m + logf(l);
+  const RowEnd e = finish_row(m, sum, p.sink, h);
+  if (col < p.D)
+    *reinterpret_cast<uint2*>(p.out + b * p.o_b + s * p.o_s + h * p.o_h + col) =
+        make_uint2(pack_bf16x2(acc.x * e.factor, acc.y * e.factor), pack_bf16x2(acc.z * e.factor, acc.w * e.factor));
+  if (lane == 0 && p.lse != nullptr) p.lse[l_idx] = e.lse;
 }
 
 }  // namespace fa4

@@ -1,9 +1,10 @@
 // C ABI of the 8-bit KV cache (see include/fa4_nvfp4.h): argument validation and launches of the append and
 // of the attention over it.  Host code only; the kernels live in the .cuh files.
-#include "fp8_attn.cuh"
+#include "fp8_decode.cuh"
 #include "launch.cuh"
 
 #include <algorithm>
+#include <numeric>
 
 namespace {
 
@@ -121,7 +122,7 @@ int validate_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f) {
   if (f->B <= 0 || f->Sq <= 0 || f->Hq <= 0 || f->Hq % c->Hkv != 0) return -FA4_E_SHAPE;
   if (c->page_table == nullptr && f->B > c->num_pages) return -FA4_E_SHAPE;
   if (!(f->softmax_scale > 0.f) || !(f->softcap >= 0.f) || f->num_splits < 0 || f->num_splits > 128) return -FA4_E_SHAPE;
-  if ((int64_t)f->B * f->Sq * f->Hq > 0x0fffffffll || f->B > 65535) return -FA4_E_TOO_LARGE;
+  if ((int64_t)f->B * f->Sq * f->Hq > 0x0fffffffll || f->B > 65535 || (int64_t)f->Sq * f->Hq > (1 << 20)) return -FA4_E_TOO_LARGE;
   const int64_t strides[] = {f->q_stride_b, f->q_stride_s, f->q_stride_h, f->o_stride_b, f->o_stride_s, f->o_stride_h};
   for (int64_t s : strides)
     if ((s & 7) != 0) return -FA4_E_STRIDE;
@@ -131,42 +132,103 @@ int validate_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f) {
 
 }  // namespace
 
+namespace {
+
+// How a call is run: rows of a CTA and splits of the keys.
+struct Fp8Plan {
+  int rows, row_tiles, splits;
+};
+Fp8Plan plan_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f) {
+  Fp8Plan plan;
+  const int64_t rows = (int64_t)f->Sq * (f->Hq / c->Hkv);
+  plan.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
+  plan.row_tiles = (int)((rows + plan.rows - 1) / plan.rows);
+  const int64_t units = (int64_t)plan.row_tiles * c->Hkv * f->B, tiles = ((int64_t)c->pages_per_seq * c->page_size + 127) / 128;
+  const int64_t ctas = kSms * (plan.rows == 32 ? 1 : 2);
+  plan.splits = f->num_splits > 0 ? f->num_splits
+                                  : (int)std::max<int64_t>(1, std::min<int64_t>({128, ctas / units, tiles / 2}));
+  return plan;
+}
+int64_t workspace_of(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, const Fp8Plan& plan) {
+  return plan.splits > 1 ? (int64_t)plan.splits * f->B * f->Sq * f->Hq * (c->D + 1) * 4 : 0;
+}
+
+// The pool as (D, head, token of a page, page) bytes.
+bool encode_pool(CUtensorMap* m, const fa4_fp8_cache* c, const void* base, int64_t page, int64_t token, int64_t head, int box) {
+  const uint64_t dims[4] = {(uint64_t)c->D, (uint64_t)c->Hkv, (uint64_t)c->page_size, (uint64_t)c->num_pages};
+  const uint64_t strides[3] = {(uint64_t)head, (uint64_t)token, (uint64_t)page};
+  const uint32_t boxes[4] = {(uint32_t)c->D, 1, (uint32_t)box, 1};
+  return encode_u8_4d(m, base, dims, strides, boxes, c->D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
+}  // namespace
+
 extern "C" int64_t fa4_fp8_cache_fwd_workspace_bytes(const fa4_fp8_cache* c, const fa4_fp8_fwd* f) {
   if (int e = validate_fwd(c, f)) return e;
-  return 0;
+  return workspace_of(c, f, plan_fwd(c, f));
 }
 
 extern "C" int fa4_fp8_cache_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, void* cuda_stream) {
   if (int e = validate_fwd(c, f)) return e;
+  const Fp8Plan plan = plan_fwd(c, f);
+  const int64_t bytes = workspace_of(c, f, plan);
+  if (bytes > 0 && f->workspace == nullptr) return -FA4_E_NULL;
+  if (bytes > 0 && !aligned16(f->workspace)) return -FA4_E_ALIGN;
+  if (bytes > 0 && f->workspace_bytes < (uint64_t)bytes) return -FA4_E_TOO_LARGE;
   Fp8Params p = {};
   p.q = static_cast<const __nv_bfloat16*>(f->q);
   p.out = static_cast<__nv_bfloat16*>(f->out);
   p.lse = f->lse;
   p.q_b = f->q_stride_b; p.q_s = f->q_stride_s; p.q_h = f->q_stride_h;
   p.o_b = f->o_stride_b; p.o_s = f->o_stride_s; p.o_h = f->o_stride_h;
-  p.kc = static_cast<const uint8_t*>(c->k);
-  p.vc = static_cast<const uint8_t*>(c->v);
-  p.kc_page = c->k_stride_page; p.kc_tok = c->k_stride_token; p.kc_head = c->k_stride_head;
-  p.vc_page = c->v_stride_page; p.vc_tok = c->v_stride_token; p.vc_head = c->v_stride_head;
   p.k_scale = c->k_scale;
   p.v_scale = c->v_scale;
   p.used = f->seqused_k;
   p.fresh = f->seqused_q;
   p.table = c->page_table;
   p.sink = f->sink;
+  p.num_splits = plan.splits;
+  p.o_partial = static_cast<float*>(f->workspace);
+  p.lse_partial = bytes > 0 ? p.o_partial + (int64_t)plan.splits * f->B * f->Sq * f->Hq * c->D : nullptr;
+  p.row_tiles = plan.row_tiles;
+  // (a contiguous cache has no page borders: what lies behind its end is read as zeros)
+  p.box = c->page_table == nullptr ? 128 : std::gcd(c->page_size, 128);
   p.B = f->B; p.Sq = f->Sq; p.Hq = f->Hq; p.Hkv = c->Hkv; p.group = f->Hq / c->Hkv; p.D = c->D;
   p.log_block = log2_of(c->block);
   p.num_pages = c->num_pages; p.page_size = c->page_size; p.pages_per_seq = c->pages_per_seq;
   p.capacity = c->pages_per_seq * c->page_size;
   p.div_page = make_fastdiv((uint32_t)c->page_size);
   p.div_group = make_fastdiv((uint32_t)p.group);
-  p.scale = f->softmax_scale;
-  p.softcap = f->softcap;
+  p.div_hq = make_fastdiv((uint32_t)f->Hq);
+  p.div_sq = make_fastdiv((uint32_t)f->Sq);
+  p.div_row_tiles = make_fastdiv((uint32_t)plan.row_tiles);
+  constexpr float kLog2e = 1.4426950408889634f;
+  p.sl2 = f->softmax_scale * kLog2e;
+  p.cap_in = f->softcap > 0.f ? f->softmax_scale / f->softcap : 0.f;
+  p.cap_out = f->softcap * kLog2e;
   p.win_left = f->window_left;
   p.win_right = f->causal && f->window_right < 0 ? 0 : f->window_right;
   p.status = f->status;
   p.epoch = next_launch_epoch();
   p.budget_ns = f->wait_budget_ns ? f->wait_budget_ns : kDefaultBudgetNs;
-  return launch_pdl(fp8_attn_rows_kernel, dim3((unsigned)(f->Sq * f->Hq), (unsigned)f->B), 128, 0,
-                    static_cast<cudaStream_t>(cuda_stream), p);
+  CUtensorMap tm_k, tm_v;
+  if (!encode_pool(&tm_k, c, c->k, c->k_stride_page, c->k_stride_token, c->k_stride_head, p.box) ||
+      !encode_pool(&tm_v, c, c->v, c->v_stride_page, c->v_stride_token, c->v_stride_head, p.box))
+    return -FA4_E_TENSORMAP;
+  const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+  auto launch = [&](auto form) -> int {
+    using F = decltype(form);
+    return launch_pdl(fp8_decode_kernel<F>, dim3((unsigned)plan.splits, (unsigned)(c->Hkv * plan.row_tiles), (unsigned)f->B), F::kThreads, F::kRequest,
+                      stream, tm_k, tm_v, p);
+  };
+  using fp8d::Form;
+  const int rc = c->D == 128 ? (plan.rows == 8    ? launch(Form<128, 8, 1, 2, 3, 2>{})
+                                : plan.rows == 16 ? launch(Form<128, 16, 1, 2, 3, 2>{})
+                                                  : launch(Form<128, 16, 2, 2, 5, 1>{}))
+                             : (plan.rows == 8    ? launch(Form<64, 8, 1, 2, 6, 2>{})
+                                : plan.rows == 16 ? launch(Form<64, 16, 1, 2, 6, 2>{})
+                                                  : launch(Form<64, 16, 2, 2, 8, 1>{}));
+  if (rc != 0 || plan.splits == 1) return rc;
+  const int64_t rows = (int64_t)f->B * f->Sq * f->Hq;
+  return launch_pdl(fp8_combine_kernel, dim3((unsigned)((rows + kFp8CombineWarps - 1) / kFp8CombineWarps)), kFp8CombineWarps * 32, 0, stream, p);
 }

@@ -68,14 +68,15 @@ def attend(q, k, v, rows, softmax_scale=None, causal=False, window=(None, None),
     left, right = window
     if causal:
         right = 0
-    at = n - rows + torch.arange(rows)[:, None]
-    j = torch.arange(n)[None]
-    hidden = torch.zeros(rows, n, dtype=torch.bool)
+    at = n - rows + torch.arange(rows, device=k.device)[:, None]
+    j = torch.arange(n, device=k.device)[None]
+    hidden = torch.zeros(rows, n, dtype=torch.bool, device=k.device)
     if left is not None:
         hidden |= j < at - left
     if right is not None:
         hidden |= j > at + right
-    out, lse = torch.zeros(rows, G, D, dtype=torch.float64), torch.zeros(G, rows, dtype=torch.float64)
+    out = torch.zeros(rows, G, D, dtype=torch.float64, device=k.device)
+    lse = torch.zeros(G, rows, dtype=torch.float64, device=k.device)
     for g in range(G):
         s = q[:rows, g].double() @ k[:, g // (G // H)].double().T * scale
         if softcap:
@@ -83,7 +84,7 @@ def attend(q, k, v, rows, softmax_scale=None, causal=False, window=(None, None),
         s[hidden] = -math.inf
         if sink is not None:
             s = torch.cat([s, sink[g].double().expand(rows, 1)], dim=1)
-        total = torch.logsumexp(s, dim=1) if s.shape[1] else torch.full((rows,), -math.inf, dtype=torch.float64)
+        total = torch.logsumexp(s, dim=1) if s.shape[1] else torch.full((rows,), -math.inf, dtype=torch.float64, device=k.device)
         p = torch.exp(s - torch.where(total > -math.inf, total, 0.0)[:, None])[:, :n]
         # (a key that a row does not see adds nothing to it, whatever its value is)
         out[:, g] = p @ v[:, g // (G // H)].double()
