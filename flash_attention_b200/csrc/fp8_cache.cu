@@ -1,6 +1,6 @@
 // C ABI of the 8-bit KV cache (see include/fa4_nvfp4.h): argument validation and launches of the append and
 // of the attention over it.  Host code only; the kernels live in the .cuh files.
-#include "fp8_decode.cuh"
+#include "fp8_prefill.cuh"
 #include "launch.cuh"
 
 #include <algorithm>
@@ -141,10 +141,10 @@ struct Fp8Plan {
 Fp8Plan plan_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f) {
   Fp8Plan plan;
   const int64_t rows = (int64_t)f->Sq * (f->Hq / c->Hkv);
-  plan.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
+  plan.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 256;
   plan.row_tiles = (int)((rows + plan.rows - 1) / plan.rows);
   const int64_t units = (int64_t)plan.row_tiles * c->Hkv * f->B, tiles = ((int64_t)c->pages_per_seq * c->page_size + 127) / 128;
-  const int64_t ctas = kSms * (plan.rows == 32 ? 1 : 2);
+  const int64_t ctas = kSms * (plan.rows >= 32 ? 1 : 2);
   plan.splits = f->num_splits > 0 ? f->num_splits
                                   : (int)std::max<int64_t>(1, std::min<int64_t>({128, ctas / units, tiles / 2}));
   return plan;
@@ -221,8 +221,18 @@ extern "C" int fa4_fp8_cache_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, v
     return launch_pdl(fp8_decode_kernel<F>, dim3((unsigned)plan.splits, (unsigned)(c->Hkv * plan.row_tiles), (unsigned)f->B), F::kThreads, F::kRequest,
                       stream, tm_k, tm_v, p);
   };
+  // (a launch needs the registers that the kernel's budget counts on: see ensure_kernel)
+  auto launch_many = [&](auto kernel, uint32_t smem) -> int {
+    if (int e = ensure_kernel(kernel, smem, fp8p::kRegsLaunch)) return e;
+    return launch_pdl(kernel, dim3((unsigned)((int64_t)plan.row_tiles * c->Hkv * f->B * plan.splits)), fp8p::kThreads, smem, stream, tm_k, tm_v, p);
+  };
   using fp8d::Form;
-  const int rc = c->D == 128 ? (plan.rows == 8    ? launch(Form<128, 8, 1, 2, 3, 2>{})
+  const bool cap = f->softcap > 0.f;
+  const int rc = plan.rows == 256 ? (c->D == 128 ? (cap ? launch_many(fp8_prefill_kernel<128, true>, fp8p::Layout<128>::kRequest)
+                                                        : launch_many(fp8_prefill_kernel<128, false>, fp8p::Layout<128>::kRequest))
+                                                 : (cap ? launch_many(fp8_prefill_kernel<64, true>, fp8p::Layout<64>::kRequest)
+                                                        : launch_many(fp8_prefill_kernel<64, false>, fp8p::Layout<64>::kRequest)))
+               : c->D == 128 ? (plan.rows == 8    ? launch(Form<128, 8, 1, 2, 3, 2>{})
                                 : plan.rows == 16 ? launch(Form<128, 16, 1, 2, 3, 2>{})
                                                   : launch(Form<128, 16, 2, 2, 5, 1>{}))
                              : (plan.rows == 8    ? launch(Form<64, 8, 1, 2, 6, 2>{})
