@@ -14,13 +14,16 @@ struct Fp8Params {
   const float *k_scale, *v_scale;
   const int32_t *used, *fresh, *table;
   const float* sink;
-  int num_splits;
-  float* o_partial;                  // (splits, B, Sq, Hq, D) fp32, normalised
-  float* lse_partial;                // (splits, B, Hq, Sq), log2 units, sink left out
+  int num_splits;                    // 0: dealt by the lengths (decode kernel)
+  float* o_partial;                  // rows of D fp32, normalised; log2 of their sums, the sink left out
+  float* lse_partial;                //   many rows: (splits, B, Sq, Hq); decode: (slots, unit_rows)
+  int2* pieces;                      // decode, dealt: (B, Hkv) first CTA and number of pieces of a unit
+  int unit_rows;                     // Sq * group
+  int bundle, bundles;               // kv heads side by side (a divisor of Hkv), and how many such
   int box;                           // keys of a tensor-map box: 128, or what pages and tiles of 128 share
   int B, Sq, Hq, Hkv, group, D, log_block, num_pages, page_size, pages_per_seq, capacity;
   int row_tiles;                     // of a kv head and sequence
-  FastDiv div_page, div_group, div_hq, div_sq, div_row_tiles;
+  FastDiv div_page, div_group, div_hq, div_sq, div_groups;   // (groups of CTAs of the decode kernel)
   // scores in log2 units: (q . k8) * ks * sl2, or cap_out * tanh((q . k8) * ks * cap_in) with a soft cap
   float sl2, cap_in, cap_out;
   int win_left, win_right;           // -1: unlimited
@@ -32,9 +35,8 @@ struct Fp8Params {
 // The keys [lo, hi) that query row s of a sequence with `sk` keys and `sq` rows sees.
 __device__ __forceinline__ int2 seen_by(const Fp8Params& p, int sk, int sq, int s) {
   const int at = sk - sq + s;
-  int lo = 0, hi = sk;
-  if (p.win_left >= 0 && at - p.win_left > 0) lo = at - p.win_left;
-  if (p.win_right >= 0 && (int64_t)at + p.win_right + 1 < sk) hi = at + p.win_right + 1;
+  const int lo = p.win_left >= 0 && p.win_left < at ? at - p.win_left : 0;
+  const int hi = p.win_right >= 0 && p.win_right < sq - 1 - s ? at + p.win_right + 1 : sk;     // (no sum passes 2^31)
   return make_int2(lo, hi > lo ? hi : lo);
 }
 
@@ -73,49 +75,40 @@ __device__ __forceinline__ RowEnd finish_row(float m, float l, const float* sink
   if (sink != nullptr) {
     const float x = sink[h] * 1.4426950408889634f;
     top = fmaxf(m, x);
-    keep = m == -INFINITY ? 0.f : exp2f(m - top);
-    l = (m == -INFINITY ? 0.f : l * keep) + exp2f(x - top);
+    keep = m == -INFINITY ? 0.f : ex2_approx(m - top);
+    l = (m == -INFINITY ? 0.f : l * keep) + ex2_approx(x - top);
   }
   if (top == -INFINITY && l == 0.f) return {0.f, -INFINITY};    // (a row of NaN has l = NaN and goes on)
-  e.factor = keep / l;
-  e.lse = (top + log2f(l)) * kLn2;
+  e.factor = keep * __frcp_rn(l);
+  e.lse = (top + lg2_approx(l)) * kLn2;
   return e;
 }
 
-// Merge of splits: a warp a row.
+// Merge of a row's partial results by one warp; at(i): index of the i-th one's row.
 constexpr int kFp8CombineWarps = 4;
-__global__ void __launch_bounds__(kFp8CombineWarps * 32) fp8_combine_kernel(const __grid_constant__ Fp8Params p) {
-  const int lane = threadIdx.x & 31;
-  const uint32_t r = blockIdx.x * kFp8CombineWarps + (threadIdx.x >> 5), rows = (uint32_t)p.B * p.Sq * p.Hq;
-  pdl_wait();
-  if (r >= rows) return;
-  const int bs = fast_div((int)r, p.div_hq), h = (int)r - bs * p.Hq, b = fast_div(bs, p.div_sq), s = bs - b * p.Sq;
-  if (p.fresh != nullptr && s >= p.fresh[b]) return;
-  const int64_t l_idx = ((int64_t)b * p.Hq + h) * p.Sq + s;
+template <class At>
+__device__ __forceinline__ void merge_row(const Fp8Params& p, int b, int s, int h, int lane, int n, At at) {
   const int col = 4 * lane;
   float m = -INFINITY, sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = 0; i0 < p.num_splits; i0 += 8) {
+  for (int i0 = 0; i0 < n; i0 += 8) {
     float l[8], top = m;
     float4 v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      l[j] = i0 + j < p.num_splits ? p.lse_partial[(int64_t)(i0 + j) * rows + l_idx] : -INFINITY;
-    }
+    for (int j = 0; j < 8; ++j) l[j] = i0 + j < n ? p.lse_partial[at(i0 + j)] : -INFINITY;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      // (a split without a key wrote no values)
+      // (a part without a key wrote no values)
       v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (l[j] != -INFINITY && col < p.D)
-        v[j] = *reinterpret_cast<const float4*>(p.o_partial + ((int64_t)(i0 + j) * rows + r) * p.D + col);
+      if (l[j] != -INFINITY && col < p.D) v[j] = *reinterpret_cast<const float4*>(p.o_partial + at(i0 + j) * p.D + col);
       top = fmaxf(top, l[j]);
     }
-    const float ref = top == -INFINITY ? 0.f : top, keep = exp2f(m - ref);
+    const float ref = top == -INFINITY ? 0.f : top, keep = ex2_approx(m - ref);
     sum *= keep;
     acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float w = exp2f(l[j] - ref);
+      const float w = ex2_approx(l[j] - ref);
       sum += w;
       acc.x = fmaf(w, v[j].x, acc.x); acc.y = fmaf(w, v[j].y, acc.y);
       acc.z = fmaf(w, v[j].z, acc.z); acc.w = fmaf(w, v[j].w, acc.w);
@@ -126,7 +119,17 @@ __global__ void __launch_bounds__(kFp8CombineWarps * 32) fp8_combine_kernel(cons
   if (col < p.D)
     *reinterpret_cast<uint2*>(p.out + b * p.o_b + s * p.o_s + h * p.o_h + col) =
         make_uint2(pack_bf16x2(acc.x * e.factor, acc.y * e.factor), pack_bf16x2(acc.z * e.factor, acc.w * e.factor));
-  if (lane == 0 && p.lse != nullptr) p.lse[l_idx] = e.lse;
+  if (lane == 0 && p.lse != nullptr) p.lse[((int64_t)b * p.Hq + h) * p.Sq + s] = e.lse;
+}
+
+// The splits of the kernel for many rows: a warp a row.
+__global__ void __launch_bounds__(kFp8CombineWarps * 32) fp8_combine_kernel(const __grid_constant__ Fp8Params p) {
+  const uint32_t r = blockIdx.x * kFp8CombineWarps + (threadIdx.x >> 5), rows = (uint32_t)p.B * p.Sq * p.Hq;
+  pdl_wait();
+  if (r >= rows) return;
+  const int bs = fast_div((int)r, p.div_hq), h = (int)r - bs * p.Hq, b = fast_div(bs, p.div_sq), s = bs - b * p.Sq;
+  if (p.fresh != nullptr && s >= p.fresh[b]) return;
+  merge_row(p, b, s, h, threadIdx.x & 31, p.num_splits, [&](int i) { return (int64_t)i * rows + r; });
 }
 
 }  // namespace fa4

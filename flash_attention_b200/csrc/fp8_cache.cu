@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <numeric>
+#include <type_traits>
 
 namespace {
 
@@ -122,6 +123,8 @@ int validate_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f) {
   if (f->B <= 0 || f->Sq <= 0 || f->Hq <= 0 || f->Hq % c->Hkv != 0) return -FA4_E_SHAPE;
   if (c->page_table == nullptr && f->B > c->num_pages) return -FA4_E_SHAPE;
   if (!(f->softmax_scale > 0.f) || !(f->softcap >= 0.f) || f->num_splits < 0 || f->num_splits > 128) return -FA4_E_SHAPE;
+  // (tiles of all sequences and heads are counted in 32 bits)
+  if ((int64_t)f->B * c->Hkv * ((int64_t)c->pages_per_seq * c->page_size / 128 + 1) > 0x3fffffffll) return -FA4_E_TOO_LARGE;
   if ((int64_t)f->B * f->Sq * f->Hq > 0x0fffffffll || f->B > 65535 || (int64_t)f->Sq * f->Hq > (1 << 20)) return -FA4_E_TOO_LARGE;
   const int64_t strides[] = {f->q_stride_b, f->q_stride_s, f->q_stride_h, f->o_stride_b, f->o_stride_s, f->o_stride_h};
   for (int64_t s : strides)
@@ -134,30 +137,47 @@ int validate_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f) {
 
 namespace {
 
-// How a call is run: rows of a CTA and splits of the keys.
+// How a call is run.
 struct Fp8Plan {
-  int rows, row_tiles, splits;
+  bool decode;
+  int rows;          // decode: rows that the kernel is built for
+  int bundle;        // decode: kv heads side by side
+  int row_tiles;     // many rows: tiles of 256
+  int splits;        // 0: shares dealt on the device
+  int64_t slots;     // of partial results, and their rows
+  int64_t slot_rows;
 };
 Fp8Plan plan_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f) {
-  Fp8Plan plan;
-  const int64_t rows = (int64_t)f->Sq * (f->Hq / c->Hkv);
-  plan.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 256;
-  plan.row_tiles = (int)((rows + plan.rows - 1) / plan.rows);
-  const int64_t units = (int64_t)plan.row_tiles * c->Hkv * f->B, tiles = ((int64_t)c->pages_per_seq * c->page_size + 127) / 128;
-  const int64_t ctas = kSms * (plan.rows >= 32 ? 1 : 2);
-  plan.splits = f->num_splits > 0 ? f->num_splits
-                                  : (int)std::max<int64_t>(1, std::min<int64_t>({128, ctas / units, tiles / 2}));
+  Fp8Plan plan = {};
+  const int64_t rows = (int64_t)f->Sq * (f->Hq / c->Hkv), units = (int64_t)c->Hkv * f->B;
+  plan.decode = rows <= 32;
+  if (plan.decode) {
+    plan.rows = rows <= 16 ? 16 : 32;
+    plan.splits = f->num_splits;
+    for (plan.bundle = std::min(8, c->Hkv); c->Hkv % plan.bundle != 0;) --plan.bundle;
+    plan.slots = plan.splits == 0 ? 2 * kSms : plan.splits == 1 ? 0 : units * plan.splits;
+    plan.slot_rows = rows;
+  } else {
+    plan.row_tiles = (int)((rows + 255) / 256);
+    const int64_t tiles = ((int64_t)c->pages_per_seq * c->page_size + 127) / 128;
+    plan.splits = f->num_splits > 0 ? f->num_splits
+                                    : (int)std::max<int64_t>(1, std::min<int64_t>({128, kSms / (units * plan.row_tiles), tiles / 2}));
+    plan.slots = plan.splits == 1 ? 0 : plan.splits;
+    plan.slot_rows = (int64_t)f->B * f->Sq * f->Hq;
+  }
   return plan;
 }
+// Values, then sums, then (dealt) the pieces of the units.
 int64_t workspace_of(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, const Fp8Plan& plan) {
-  return plan.splits > 1 ? (int64_t)plan.splits * f->B * f->Sq * f->Hq * (c->D + 1) * 4 : 0;
+  const int64_t values = plan.slots * plan.slot_rows;
+  return values * (c->D + 1) * 4 + (plan.decode && plan.splits == 0 ? (values % 2) * 4 + (int64_t)f->B * c->Hkv * 8 : 0);
 }
 
-// The pool as (D, head, token of a page, page) bytes.
+// The pool as (D, token of a page, head, page) bytes.
 bool encode_pool(CUtensorMap* m, const fa4_fp8_cache* c, const void* base, int64_t page, int64_t token, int64_t head, int box) {
-  const uint64_t dims[4] = {(uint64_t)c->D, (uint64_t)c->Hkv, (uint64_t)c->page_size, (uint64_t)c->num_pages};
-  const uint64_t strides[3] = {(uint64_t)head, (uint64_t)token, (uint64_t)page};
-  const uint32_t boxes[4] = {(uint32_t)c->D, 1, (uint32_t)box, 1};
+  const uint64_t dims[4] = {(uint64_t)c->D, (uint64_t)c->page_size, (uint64_t)c->Hkv, (uint64_t)c->num_pages};
+  const uint64_t strides[3] = {(uint64_t)token, (uint64_t)head, (uint64_t)page};
+  const uint32_t boxes[4] = {(uint32_t)c->D, (uint32_t)box, 1, 1};
   return encode_u8_4d(m, base, dims, strides, boxes, c->D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
@@ -189,7 +209,11 @@ extern "C" int fa4_fp8_cache_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, v
   p.sink = f->sink;
   p.num_splits = plan.splits;
   p.o_partial = static_cast<float*>(f->workspace);
-  p.lse_partial = bytes > 0 ? p.o_partial + (int64_t)plan.splits * f->B * f->Sq * f->Hq * c->D : nullptr;
+  p.lse_partial = bytes > 0 ? p.o_partial + plan.slots * plan.slot_rows * c->D : nullptr;
+  p.pieces = bytes > 0 ? reinterpret_cast<int2*>(p.lse_partial + (plan.slots * plan.slot_rows + 1) / 2 * 2) : nullptr;
+  p.unit_rows = f->Sq * (f->Hq / c->Hkv);
+  p.bundle = plan.decode ? plan.bundle : 1;
+  p.bundles = c->Hkv / p.bundle;
   p.row_tiles = plan.row_tiles;
   // (a contiguous cache has no page borders: what lies behind its end is read as zeros)
   p.box = c->page_table == nullptr ? 128 : std::gcd(c->page_size, 128);
@@ -201,7 +225,6 @@ extern "C" int fa4_fp8_cache_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, v
   p.div_group = make_fastdiv((uint32_t)p.group);
   p.div_hq = make_fastdiv((uint32_t)f->Hq);
   p.div_sq = make_fastdiv((uint32_t)f->Sq);
-  p.div_row_tiles = make_fastdiv((uint32_t)plan.row_tiles);
   constexpr float kLog2e = 1.4426950408889634f;
   p.sl2 = f->softmax_scale * kLog2e;
   p.cap_in = f->softcap > 0.f ? f->softmax_scale / f->softcap : 0.f;
@@ -216,29 +239,35 @@ extern "C" int fa4_fp8_cache_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, v
       !encode_pool(&tm_v, c, c->v, c->v_stride_page, c->v_stride_token, c->v_stride_head, p.box))
     return -FA4_E_TENSORMAP;
   const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
-  auto launch = [&](auto form) -> int {
-    using F = decltype(form);
-    return launch_pdl(fp8_decode_kernel<F>, dim3((unsigned)plan.splits, (unsigned)(c->Hkv * plan.row_tiles), (unsigned)f->B), F::kThreads, F::kRequest,
-                      stream, tm_k, tm_v, p);
-  };
+  const bool cap = f->softcap > 0.f;
+  const int64_t rows = (int64_t)f->B * f->Sq * f->Hq;
+  const unsigned merge_grid = (unsigned)((rows + kFp8CombineWarps - 1) / kFp8CombineWarps);
+  if (plan.decode) {
+    const int64_t grid = plan.splits == 0 ? kSms / plan.bundle * plan.bundle : (int64_t)plan.splits * c->Hkv * f->B;
+    p.div_groups = make_fastdiv((uint32_t)(kSms / plan.bundle));
+    auto launch = [&](auto form) -> int {
+      using F = decltype(form);
+      return launch_pdl(fp8_decode_kernel<F>, dim3((unsigned)grid), F::kThreads, F::kRequest, stream, tm_k, tm_v, p);
+    };
+    using fp8d::Form;
+    auto launch_rows = [&](auto capped) -> int {
+      constexpr bool kCap = decltype(capped)::value;
+      if (c->D == 128) return plan.rows == 16 ? launch(Form<128, 16, kCap>{}) : launch(Form<128, 32, kCap>{});
+      return plan.rows == 16 ? launch(Form<64, 16, kCap>{}) : launch(Form<64, 32, kCap>{});
+    };
+    const int rc = cap ? launch_rows(std::true_type{}) : launch_rows(std::false_type{});
+    if (rc != 0 || plan.splits == 1) return rc;
+    return launch_pdl(fp8_merge_kernel, dim3(merge_grid), kFp8CombineWarps * 32, 0, stream, p);
+  }
   // (a launch needs the registers that the kernel's budget counts on: see ensure_kernel)
   auto launch_many = [&](auto kernel, uint32_t smem) -> int {
     if (int e = ensure_kernel(kernel, smem, fp8p::kRegsLaunch)) return e;
     return launch_pdl(kernel, dim3((unsigned)((int64_t)plan.row_tiles * c->Hkv * f->B * plan.splits)), fp8p::kThreads, smem, stream, tm_k, tm_v, p);
   };
-  using fp8d::Form;
-  const bool cap = f->softcap > 0.f;
-  const int rc = plan.rows == 256 ? (c->D == 128 ? (cap ? launch_many(fp8_prefill_kernel<128, true>, fp8p::Layout<128>::kRequest)
-                                                        : launch_many(fp8_prefill_kernel<128, false>, fp8p::Layout<128>::kRequest))
-                                                 : (cap ? launch_many(fp8_prefill_kernel<64, true>, fp8p::Layout<64>::kRequest)
-                                                        : launch_many(fp8_prefill_kernel<64, false>, fp8p::Layout<64>::kRequest)))
-               : c->D == 128 ? (plan.rows == 8    ? launch(Form<128, 8, 1, 2, 3, 2>{})
-                                : plan.rows == 16 ? launch(Form<128, 16, 1, 2, 3, 2>{})
-                                                  : launch(Form<128, 16, 2, 2, 5, 1>{}))
-                             : (plan.rows == 8    ? launch(Form<64, 8, 1, 2, 6, 2>{})
-                                : plan.rows == 16 ? launch(Form<64, 16, 1, 2, 6, 2>{})
-                                                  : launch(Form<64, 16, 2, 2, 8, 1>{}));
+  const int rc = c->D == 128 ? (cap ? launch_many(fp8_prefill_kernel<128, true>, fp8p::Layout<128>::kRequest)
+                                    : launch_many(fp8_prefill_kernel<128, false>, fp8p::Layout<128>::kRequest))
+                             : (cap ? launch_many(fp8_prefill_kernel<64, true>, fp8p::Layout<64>::kRequest)
+                                    : launch_many(fp8_prefill_kernel<64, false>, fp8p::Layout<64>::kRequest));
   if (rc != 0 || plan.splits == 1) return rc;
-  const int64_t rows = (int64_t)f->B * f->Sq * f->Hq;
-  return launch_pdl(fp8_combine_kernel, dim3((unsigned)((rows + kFp8CombineWarps - 1) / kFp8CombineWarps)), kFp8CombineWarps * 32, 0, stream, p);
+  return launch_pdl(fp8_combine_kernel, dim3(merge_grid), kFp8CombineWarps * 32, 0, stream, p);
 }

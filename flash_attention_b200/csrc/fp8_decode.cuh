@@ -1,28 +1,37 @@
 // Attention over the 8-bit KV cache for a handful of query rows (up to 32 rows of all query heads of a kv head).
 //
-// The bytes go from HBM to the tensor core as they are: keys and values are the A operands of kind::f8f6f4 products,
-// transposed (keys, then head dims on the 128 lanes, query rows on the N side), and nothing is converted.
+// The bytes go from HBM to the tensor core as they are: both products are kind::f8f6f4 and nothing of the cache is converted.
 //
-//   S^T (128 keys x N) = K (128 x D e4m3, K-major as loaded) . Q^T,     O^T (D x N) = V^T (MN-major as loaded) . P^T
+//   S (rows x 128 keys) = Q . K^T (K-major as loaded),     O^T (D x rows) = V^T (MN-major as loaded) . W^T
 //
-// A bf16 query has eight significant bits and an e4m3 value four, so a query row is TWO e4m3 rows: q = q1 + q2 / 16 with q1 =
-// e4m3(q 2^c) and q2 = 16 (q 2^c - q1), which is exact for elements down to 2^-13 of the row's largest (2^c brings that to 128..256;
-// smaller ones are off by 2^-20 of it).  Their scores are two columns of one product; S = S1 + S2 / 16.  The weights go the same
-// way: w = (w1 + w2 / 16) / 256, within 2^-9 of w down to 2^-14 and 2^-22 below that.  w is softmax weight times value scale, over
-// the largest of these that the row has in the TILE, not among all keys so far (a row whose first key outweighs the rest by 2^15 would
-// round the rest to nothing): the product of a tile is read out of tensor memory and added to the row's sums in fp32 registers,
-// 2 FMAs per row and thread.
+// A bf16 query has eight significant bits and an e4m3 value four, so a query row is two e4m3 rows, one behind the other along the
+// contraction: q 2^c = q1 + q2 with q1 = e4m3(q 2^c), which is exact for elements down to 2^-10 of the row's largest (2^c brings that to
+// 256 at most; smaller ones are off by 2^-18 of it).  The rows stand on the lanes of the A operand as often as they fit, so each of the four
+// warps of a tile finds all of them in its lanes, and a thread has one row and 16 neighbouring keys (32 with more than 16 rows):
+// nothing is transposed, and maxima take a shuffle and one exchange through shared memory.
 //
-// One CTA = (split, kv head, sequence): a contiguous share of the sequence's 128-key tiles.  Warps: softmax warpgroups first
-// (strand w takes every kStrands-th tile; with more than 16 rows two warpgroups share a tile's rows), then the loaders of K
-// and V, the issuers of the two products.  Every wait is bounded.  A warp whose wait ran out goes through the rest of its loop
+// Weights are two e4m3 rows as well, w = (w1 + w2 / 16) / 256, as neighbouring columns of one product: within 2^-9 of w down to 2^-14 and
+// 2^-22 below that.  w is softmax weight times value scale, over the largest of these that the row has in the TILE, not among all
+// keys so far (a row whose first key outweighs the rest by 2^15 would round the rest to nothing): the product of a tile is read out of
+// tensor memory and added to the row's sums in fp32 registers, two FMAs a row and thread.
+//
+// A CTA per SM works through its share of all tiles of the call: the lengths are on the device, and shares of equal size are what keeps HBM
+// busy to the end.  Up to eight kv heads go side by side through the same tokens, a CTA each: theirs lie next to each other in memory
+// (every head at its own place in the list: 4 x 65536 keys of 8 heads at 3.9 TB/s, HBM pages and translations missed).  A unit (sequence, kv head) that ends up in several CTAs is
+// merged by fp8_merge_kernel.  With a split count of the caller's a CTA has one split of one unit.
+//
+// Warps: kStrands softmax warpgroups, to which the tiles are dealt in turn, then the loaders of K and V and the issuers of the two products.  The
+// loaders run ahead through the pieces of a CTA.  Every wait is bounded.  A warp whose wait ran out goes through the rest of its loops
 // without waiting, so that the rendezvous of a warpgroup (bar.sync) always has all its threads.
 #pragma once
 #include "fp8_attn.cuh"
-#include "attn_decode.cuh"   // the transpose of lane groups, tensor-memory loads of few columns
+#include "attn_decode.cuh"   // tensor-memory loads of few columns
 
 namespace fa4 {
 namespace fp8d {
+
+// Smallest share of a CTA, in tiles.
+constexpr int kMinShare = 2;
 
 enum Site { kKFullS = 130, kKFreeS, kVFullS, kVFreeS, kSFullS, kSFreeS, kPFullS, kPvDoneS, kQReadyS };
 
@@ -41,6 +50,25 @@ template <int kD>
 __device__ __forceinline__ uint64_t tile_desc(uint32_t saddr) {
   return make_smem_desc(saddr, 0, 8 * kD, kD == 128 ? kSwizzle128 : kSwizzle64);
 }
+// The same descriptor `bytes` further on.
+__device__ __forceinline__ uint64_t desc_at(uint64_t desc, uint32_t bytes) {
+  uint32_t lo, hi;
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(desc));
+  lo += bytes >> 4;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(desc) : "r"(lo), "r"(hi));
+  return desc;
+}
+// A place in a ring of kN barriers and the parity of its present phase, without divisions.
+template <int kN>
+struct Ring {
+  uint32_t at = 0, parity = 0;
+  __device__ __forceinline__ void next() {
+    if (++at == kN) {
+      at = 0;
+      parity ^= 1u;
+    }
+  }
+};
 // Instruction descriptor of kind::f8f6f4, e4m3 x e4m3, fp32 accumulator: [4,6) D format 1, [7,10) A and [10,13) B format 0,
 // [15] A and [16] B MN-major, [17,23) N >> 3, [24,29) M >> 4.
 __host__ __device__ constexpr uint32_t make_idesc_e4m3(uint32_t m, uint32_t n, bool a_mn_major) {
@@ -58,47 +86,144 @@ __device__ __forceinline__ void mma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint6
 }
 __device__ __forceinline__ void group_sync(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
 
-// kRW: rows of a warpgroup; kHalves: warpgroups that share a tile's rows; kStages: K and V tiles in flight; kCtas: of an SM.
-template <int kD_, int kRW_, int kHalves_, int kStrands_, int kStages_, int kCtas_>
+// kR: rows (16 or 32).
+template <int kD_, int kR_, bool kCap_>
 struct Form {
-  static constexpr int kD = kD_, kRW = kRW_, kHalves = kHalves_, kStrands = kStrands_, kStages = kStages_, kCtas = kCtas_;
-  static constexpr int kR = kRW * kHalves, kN = 2 * kR, kGroups = kHalves * kStrands, kThreads = 128 * kGroups + 128;
+  static constexpr int kD = kD_, kR = kR_, kStrands = kR == 16 ? 3 : 2, kStages = kD == 128 ? 5 : 10, kThreads = 128 * kStrands + 128;
+  static constexpr bool kCap = kCap_;
+  static constexpr int kN = 2 * kR, kKeys = kR;       // keys of a thread: 128 lanes hold 128 / kR copies of the rows
   static constexpr uint32_t kTile = 128 * kD;
   // Scales of K and V come with K.  Its stage is free when the product is done, which is before the softmax has read them:
   // the tiles that a strand may still read (one each) keep theirs.
   static constexpr int kScales = kStages + kStrands;
-  static constexpr uint32_t kOffK = 0, kOffV = kOffK + kStages * kTile, kOffQ = kOffV + kStages * kTile,
-                            kOffP = kOffQ + (kN * kD + 1023) / 1024 * 1024,   // kStrands x (N rows x 128 keys)
+  static constexpr uint32_t kOffK = 0, kOffV = kOffK + kStages * kTile, kOffQ = kOffV + kStages * kTile,   // q1, q2: 128 x kD
+      kOffP = kOffQ + 2 * kTile,                                             // kStrands x (kN rows x 128 keys)
       kOffSc = kOffP + kStrands * kN * 128,                                  // scales of 16 keys: 8 of K, 8 of V a tile
-      kOffRed = kOffSc + kScales * 64,                                        // maxima: groups x 2 x 4 warps x rows
-      kOffFac = kOffRed + kGroups * 2 * 4 * kRW * 8,                         // (keep, add): groups x 2 x rows
-      kOffRow = kOffFac + kGroups * 2 * kRW * 8,                             // factor of a row's scores
-      kOffSum = kOffRow + kR * 4,                                            // groups x 4 warps x rows: sums
-      kOffRef = kOffSum + kGroups * 4 * kRW * 4,                             // groups x rows: last references
-      kOffBar = (kOffRef + kGroups * kRW * 4 + 7) / 8 * 8;
+      kOffRed = kOffSc + kScales * 64,                                       // maxima: strands x 2 x 4 warps x rows
+      kOffFac = kOffRed + kStrands * 2 * 4 * kR * 8,                         // (keep, add): strands x 2 x rows
+      kOffRow = kOffFac + kStrands * 2 * kR * 8,                             // factor of a row's scores
+      kOffSum = kOffRow + kR * 4,                                            // strands x 4 warps x rows: sums
+      kOffRef = kOffSum + kStrands * 4 * kR * 4,                             // strands x rows: last references
+      kOffBar = (kOffRef + kStrands * kR * 4 + 7) / 8 * 8;
   static constexpr uint32_t kKFull = 0, kKFree = kKFull + kStages, kVFull = kKFree + kStages, kVFree = kVFull + kStages,
                             kSFull = kVFree + kStages, kSFree = kSFull + kStrands, kPFull = kSFree + kStrands,
-                            kPvDone = kPFull + kStrands, kQReady = kPvDone + kStrands, kDrain = kQReady + 1, kBars = kDrain + 2;
+                            kPvDone = kPFull + kStrands, kQReady = kPvDone + kStrands, kVPart = kQReady + 1, kDrain = kVPart + 1, kBars = kDrain + 2;
   static constexpr uint32_t kOffMisc = (kOffBar + 8 * kBars + 15) / 16 * 16;
-  static constexpr uint32_t kRequest = kOffMisc + 16 + sizeof(WaitCtx) + 1024;
-  static_assert(kCtas * (kRequest + 1024) <= 228 * 1024, "shared memory of the decode kernel");
-  static constexpr uint32_t kS = 0, kO = kStrands * kN, kUsed = 2 * kStrands * kN;
-  static constexpr uint32_t kCols = kUsed <= 32 ? 32 : kUsed <= 64 ? 64 : kUsed <= 128 ? 128 : kUsed <= 256 ? 256 : 512;
-  static_assert(kCtas * kCols <= 512, "tensor memory of the decode kernel");
-  // the strands' sums meet in the memory of the K ring
-  static_assert(kR * kD * 4 * kStrands <= 2 * (int)kStages * (int)kTile, "merge of the strands");
+  static constexpr uint32_t kOffDeal = (kOffMisc + 16 + sizeof(WaitCtx) + 15) / 16 * 16;
+  static constexpr uint32_t kRequest = kOffDeal + 64 + 1024;
+  static_assert(kRequest <= 227 * 1024, "shared memory of the decode kernel");
+  static constexpr uint32_t kS = 0, kO = kStrands * 128;
+  static_assert(kO + kStrands * kN <= 512, "tensor memory of the decode kernel");
+  // the strands' sums meet in the memory of Q
+  static_assert(kR * kD * 4 * kStrands <= 2 * (int)kTile, "merge of the strands");
 };
+
+// A sequence as the kernel sees it: keys, query rows; the keys that some row sees, as tiles of 128.
+struct Seq {
+  int sk, sq, lo, hi, first, tiles;
+};
+__device__ __forceinline__ Seq seq_of(const Fp8Params& p, int sk, int sq) {
+  Seq q;
+  q.sk = sk;
+  q.sq = sq;
+  q.lo = seen_by(p, sk, sq, 0).x;
+  q.hi = sq > 0 ? seen_by(p, sk, sq, sq - 1).y : 0;
+  q.first = q.lo >> 7;
+  q.tiles = q.hi > q.lo ? ((q.hi + 127) >> 7) - q.first : 0;
+  return q;
+}
+// A unit's place in the list of all tiles: one that sees nothing takes a place too (its zeros are to be written), one without rows none.
+__device__ __forceinline__ int cost_of(const Seq& q) { return q.sq == 0 ? 0 : max(q.tiles, 1); }
+
+// The CTA's walk through its pieces: `bundle` heads of a sequence are worked on side by side by as many CTAs, so units of the walk are
+// (sequence, bundle).  One warp finds the start and leaves it in shared memory; every warp walks on by itself, with the lengths of the next
+// sequence on their way while a piece is worked on.
+struct alignas(16) Walk {
+  Seq cur;
+  int b, hb, at, left;       // unit, first place of the piece in it, places of this CTA from there on
+  int share;                 // places of a CTA
+  int next_sk, next_sq;
+
+  __device__ __forceinline__ bool more() const { return left > 0; }
+  __device__ __forceinline__ int places() const { return min(left, cost_of(cur) - at); }
+  __device__ __forceinline__ int tiles() const { return min(places(), cur.tiles - at); }
+  __device__ __forceinline__ void fetch(const Fp8Params& p) {
+    if (left <= cost_of(cur) - at) return;                     // (the last piece)
+    const SeqLens n = b + 1 < p.B ? lens_of(p, b + 1) : SeqLens{0, 0};
+    next_sk = n.sk;
+    next_sq = n.sq;
+  }
+  __device__ __forceinline__ void next(const Fp8Params& p) {
+    left -= places();
+    if (left <= 0) return;
+    at = 0;
+    if (++hb == p.bundles) {
+      hb = 0;
+      do {
+        if (++b >= p.B) {
+          left = 0;
+          return;
+        }
+        cur = seq_of(p, next_sk, next_sq);
+        fetch(p);
+      } while (cost_of(cur) == 0);
+    }
+  }
+};
+
+// Where group `group` of CTAs (of as many as p.div_groups divides by) starts, by one warp.
+__device__ __forceinline__ Walk deal_shares(const Fp8Params& p, int group, int lane) {
+  Walk w = {};
+  w.b = p.B;
+  auto read = [&](int b0) {
+    const SeqLens n = b0 + lane < p.B ? lens_of(p, b0 + lane) : SeqLens{0, 0};
+    return seq_of(p, n.sk, n.sq);
+  };
+  const Seq first = read(0);
+  int total = cost_of(first);
+#pragma unroll 1
+  for (int b0 = 32; b0 < p.B; b0 += 32) total += cost_of(read(b0));
+  total = __reduce_add_sync(0xffffffffu, total) * p.bundles;
+  const int groups = gridDim.x / p.bundle;
+  w.share = max(fast_div(total + groups - 1, p.div_groups), kMinShare);
+  const int from = group * w.share;
+  if (from >= total) return w;
+  int before = 0;
+#pragma unroll 1
+  for (int b0 = 0; b0 < p.B; b0 += 32) {
+    const Seq q = b0 == 0 ? first : read(b0);
+    int upto = cost_of(q) * p.bundles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    upto += before;
+    const uint32_t hit = __ballot_sync(0xffffffffu, from < upto);
+    if (hit != 0u) {
+      const int l = __ffs(hit) - 1;
+      w.b = b0 + l;
+      w.cur = seq_of(p, __shfl_sync(0xffffffffu, q.sk, l), __shfl_sync(0xffffffffu, q.sq, l));
+      const int c = cost_of(w.cur), into = from - (__shfl_sync(0xffffffffu, upto, l) - c * p.bundles);
+      w.hb = p.bundles > 1 ? into / c : 0;
+      w.at = into - w.hb * c;
+      w.left = w.share;
+      return w;
+    }
+    before = __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return w;
+}
 
 }  // namespace fp8d
 
 template <class F>
-__global__ void __launch_bounds__(F::kThreads, F::kCtas)
+__global__ void __launch_bounds__(F::kThreads, 1)
 fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                   const __grid_constant__ Fp8Params p) {
   using namespace fp8d;
   using dec::tmem_ld_cols;
-  constexpr int kD = F::kD, kRW = F::kRW, kR = F::kR, kN = F::kN, kStages = F::kStages, kStrands = F::kStrands, kHalves = F::kHalves,
-                kGroups = F::kGroups;
+  constexpr int kD = F::kD, kR = F::kR, kN = F::kN, kStages = F::kStages, kStrands = F::kStrands, kKeys = F::kKeys;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gbase = smem_raw + (base - smem_u32(smem_raw));
@@ -106,9 +231,9 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gbase + F::kOffMisc);
   volatile uint32_t* s_abort = reinterpret_cast<volatile uint32_t*>(gbase + F::kOffMisc + 4);
   WaitCtx& wc = *reinterpret_cast<WaitCtx*>(gbase + F::kOffMisc + 16);
+  Walk& s_walk = *reinterpret_cast<Walk*>(gbase + F::kOffDeal);
   const int tid = threadIdx.x, warp = warp_index(), lane = tid & 31;
-  const int split = blockIdx.x, hk = fast_div(blockIdx.y, p.div_row_tiles), b = blockIdx.z, r_first = (blockIdx.y - hk * p.row_tiles) * F::kR;
-  constexpr int kLoadK = 4 * kGroups, kLoadV = kLoadK + 1, kIssueS = kLoadK + 2, kIssueO = kLoadK + 3;
+  constexpr int kLoadK = 4 * kStrands, kLoadV = kLoadK + 1, kIssueS = kLoadK + 2, kIssueO = kLoadK + 3;
 
   if (tid == 0) {
     *s_abort = 0u;
@@ -121,11 +246,12 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     }
     for (int s = 0; s < kStrands; ++s) {
       mbar_init(bar(F::kSFull + s), 1);
-      mbar_init(bar(F::kSFree + s), 4 * kHalves);
-      mbar_init(bar(F::kPFull + s), 4 * kHalves);
+      mbar_init(bar(F::kSFree + s), 4);
+      mbar_init(bar(F::kPFull + s), 4);
       mbar_init(bar(F::kPvDone + s), 1);
     }
-    mbar_init(bar(F::kQReady), 4 * kGroups);
+    mbar_init(bar(F::kQReady), 4 * kStrands);
+    mbar_init(bar(F::kVPart), 1);
     mbar_init(bar(F::kDrain), 1);
     mbar_init(bar(F::kDrain + 1), 1);
     fence_barrier_init();
@@ -133,108 +259,176 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   if (warp == kLoadK && lane == 0) tma_prefetch_desc(&tm_k);
   if (warp == kLoadV && lane == 0) tma_prefetch_desc(&tm_v);
   if (warp == kIssueS) {
-    tmem_alloc(base + F::kOffMisc, F::kCols);
+    tmem_alloc(base + F::kOffMisc, 512);
     tmem_relinquish();
   }
   tc_fence_before_sync();
   pdl_wait();
-  const SeqLens len = lens_of(p, b);
-  // the keys that some row sees, as tiles; this CTA's share of them
-  const int R = max(0, min(F::kR, len.sq * p.group - r_first));      // live rows: row r = s * group + head in the group
-  const int lo_all = seen_by(p, len.sk, len.sq, fast_div(r_first, p.div_group)).x,
-            hi_all = R > 0 ? seen_by(p, len.sk, len.sq, fast_div(r_first + R - 1, p.div_group)).y : 0;
-  const int t_first = lo_all >> 7, t_total = hi_all > lo_all ? ((hi_all + 127) >> 7) - t_first : 0;
-  const int per = (t_total + p.num_splits - 1) / p.num_splits;
-  const int t0 = t_first + min(split * per, t_total), n = min(t_first + t_total - t0, per);
+  // CTA = group * bundle + head in the bundle; with a split count of the caller's, a group is one split of one unit
+  const int group = blockIdx.x / p.bundle, in_bundle = blockIdx.x - group * p.bundle;
+  if (warp == 0) {
+    Walk w = {};
+    if (p.num_splits > 0) {
+      const int unit = group / p.num_splits, split = group - unit * p.num_splits;
+      w.b = unit / p.bundles;
+      w.hb = unit - w.b * p.bundles;
+      const SeqLens len = lens_of(p, w.b);
+      w.cur = seq_of(p, len.sk, len.sq);
+      const int places = cost_of(w.cur);
+      w.share = p.num_splits == 1 ? places : (places + p.num_splits - 1) / p.num_splits;
+      w.at = split * w.share;
+      w.left = max(0, min(w.share, places - w.at));
+    } else {
+      w = deal_shares(p, group, lane);
+    }
+    if (lane == 0) s_walk = w;
+  }
   __syncthreads();
   tc_fence_after_sync();
   pdl_trigger();
   const uint32_t tmem = *tmem_slot;
   bool ok = true;
+  Walk walk = s_walk;
+  walk.fetch(p);
 
   if (warp == kLoadK || warp == kLoadV) {
     // ============================================ loaders ======================================
-    // Lane g (and g + 8) looks up keys 16 g .. 16 g + 15 of a tile: their page two tiles ahead and, in the loader of K, the scale of their
-    // keys (of their values) one tile ahead.  The lanes in front of a box issue its copy.  Boxes that no row sees are not
-    // loaded, their entries of the table not read.
+    // Four tiles at a time: lane 8 q + g looks up keys 16 g .. 16 g + 15 of the q-th, their page two batches ahead and, in the loader of
+    // K, the scales of their keys and values one batch ahead (a tile at a time, a CTA ran at a tile per memory latency, 1.1 us).  The
+    // lanes in front of a box issue its copy.  Boxes that no row sees are not loaded, their entries of the table not read.
     const bool is_k = warp == kLoadK;
     const CUtensorMap* tm = is_k ? &tm_k : &tm_v;
-    const float* scales = lane < 8 ? p.k_scale : p.v_scale;
     const uint32_t full0 = is_k ? F::kKFull : F::kVFull, free0 = is_k ? F::kKFree : F::kVFree;
     const uint32_t tile0 = base + (is_k ? F::kOffK : F::kOffV);
     float* s_scale = reinterpret_cast<float*>(gbase + F::kOffSc);
-    auto key_of = [&](int li) { return ((t0 + li) << 7) + 16 * (lane & 7); };
-    auto live = [&](int li) { return lane < 16 && li < n && key_of(li) < hi_all && key_of(li) + 16 > lo_all; };
-    // (page, first key of these 16 in it)
-    auto look_up = [&](int li) -> int2 {
-      int2 at = make_int2(-1, 0);
-      if (live(li)) {
-        const int key = key_of(li), pg = fast_div(key, p.div_page);
-        at = make_int2(p.table != nullptr ? p.table[(int64_t)b * p.pages_per_seq + pg] : b, key - pg * p.page_size);
+    const int per_box = p.box >> 4, gr = lane & 7;
+    int g = 0, slot = 0;
+    Ring<kStages> st;
+    bool first = true;                      // round of the ring
+    uint32_t parts = 0u;
+    for (; ok && walk.more(); walk.next(p)) {
+      const int n = walk.tiles(), t0 = walk.cur.first + walk.at, b = walk.b, hk = walk.hb * p.bundle + in_bundle, lo = walk.cur.lo, hi = walk.cur.hi;
+      // (page, first key of these 16 in it) for the batch from tile `li` on; page -1: no row sees them
+      auto look_up = [&](int li) -> int2 {
+        int2 at = make_int2(-1, 0);
+        const int mine = li + (lane >> 3), key = ((t0 + mine) << 7) + 16 * gr;
+        if (mine < n && key < hi && key + 16 > lo) {
+          const int pg = fast_div(key, p.div_page);
+          at = make_int2(p.table != nullptr ? p.table[(int64_t)b * p.pages_per_seq + pg] : b, key - pg * p.page_size);
+          if (at.x < 0 || at.x >= p.num_pages) {
+            report_bad_index(p.status, p.epoch, kPageSite);
+            at.x = p.num_pages;                     // (reads as zeros)
+          }
+        }
+        return at;
+      };
+      auto scales_at = [&](int2 at) -> float2 {
+        if (!is_k || at.x < 0 || at.x >= p.num_pages) return make_float2(0.f, 0.f);
+        const int64_t i = ((int64_t)at.x * (p.page_size >> p.log_block) + (at.y >> p.log_block)) * p.Hkv + hk;
+        return make_float2(p.k_scale[i], p.v_scale[i]);
+      };
+      int2 at = look_up(0), at1 = look_up(4);
+      float2 sc = scales_at(at);
+      for (int l0 = 0; ok && l0 < n; l0 += 4) {
+        const int2 at2 = look_up(l0 + 8);
+        const float2 sc1 = scales_at(at1);
+        // a box is loaded if any of its keys is seen; the keys in front of those have no page here: that of the box is the first one looked up
+        const uint32_t seen = __ballot_sync(0xffffffffu, at.x >= 0);
+        const uint32_t in_box = (seen >> lane) & ((1u << per_box) - 1u);
+        const bool heads = (gr & (per_box - 1)) == 0 && in_box != 0u;
+        const uint32_t boxes = __ballot_sync(0xffffffffu, heads);
+        const int src = heads ? lane + __ffs(in_box) - 1 : lane;
+        const int page = __shfl_sync(0xffffffffu, at.x, src & 31), off = __shfl_sync(0xffffffffu, at.y, src & 31) - 16 * (src - lane);
+        const int end = min(4, n - l0);
+#pragma unroll 1
+        for (int q = 0; q < end; ++q) {
+          const uint32_t full = bar(full0 + st.at);
+          if (ok && !first) ok = mbar_wait_relaxed<256>(bar(free0 + st.at), st.parity ^ 1u, wc, is_k ? kKFreeS : kVFreeS);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          // A tile of values that are not all seen goes through a barrier of its own: the others may be anything, and 0 * NaN is NaN, so they are
+          // made zeros before the tile is given on.
+          const int key0 = (t0 + l0 + q) << 7;
+          const bool part = !is_k && (key0 < lo || key0 + 128 > hi);
+          const uint32_t lands = part ? bar(F::kVPart) : full;
+          if (lane == 0) mbar_arrive_expect_tx(lands, __popc((boxes >> (8 * q)) & 0xffu) * (uint32_t)p.box * kD);
+          __syncwarp();
+          if ((lane >> 3) == q) {
+            if (heads) tma_load_4d(tile0 + st.at * F::kTile + 16 * gr * kD, tm, lands, 0, off, hk, page);
+            if (is_k) {
+              float* to = s_scale + slot * 16 + gr;
+              to[0] = sc.x;
+              to[8] = sc.y;
+            }
+          }
+          if (is_k) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full);
+          }
+          if (part) {
+            ok = __all_sync(0xffffffffu, mbar_wait(lands, parts, wc, kVFullS));
+            if (!ok) break;
+            parts ^= 1u;
+            for (int r = lane; r < 128; r += 32)
+              if (key0 + r < lo || key0 + r >= hi) {
+                uint4* v = reinterpret_cast<uint4*>(gbase + F::kOffV + st.at * F::kTile + r * kD);
+#pragma unroll
+                for (int i = 0; i < kD / 16; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
+              }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full);
+          }
+          st.next();
+          if (st.at == 0) first = false;
+          if (++slot == F::kScales) slot = 0;
+          ++g;
+        }
+        at = at1; at1 = at2; sc = sc1;
       }
-      return at;
-    };
-    auto scale_at = [&](int2 at) -> float {
-      return is_k && at.x >= 0 && at.x < p.num_pages
-                 ? scales[((int64_t)at.x * (p.page_size >> p.log_block) + (at.y >> p.log_block)) * p.Hkv + hk] : 0.f;
-    };
-    int2 at = look_up(0), at1 = look_up(1);
-    float sc = scale_at(at);
-    int li = 0;
-    for (; li < n; ++li) {
-      const uint32_t st = li % kStages;
-      const int2 at2 = look_up(li + 2);
-      const float sc1 = scale_at(at1);
-      if (li >= kStages && ok) ok = mbar_wait(bar(free0 + st), (li / kStages - 1) & 1, wc, is_k ? kKFreeS : kVFreeS);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      // a box is loaded if any of its keys is seen
-      const uint32_t seen = __ballot_sync(0xffffffffu, live(li)) & 0xffu;
-      const int per_box = p.box >> 4;
-      const bool mine = lane < 8 && (lane & (per_box - 1)) == 0 && ((seen >> lane) & ((1u << per_box) - 1u)) != 0u;
-      const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, mine));
-      if (lane == 0) mbar_arrive_expect_tx(bar(full0 + st), boxes * (uint32_t)p.box * kD);
-      __syncwarp();
-      // (the keys in front of those that are seen have no page here: that of the box is the first one looked up)
-      const uint32_t in_box = (seen >> lane) & ((1u << per_box) - 1u);
-      const int src = mine ? lane + __ffs(in_box) - 1 : lane;
-      const int page = __shfl_sync(0xffffffffu, at.x, src & 31), off = __shfl_sync(0xffffffffu, at.y, src & 31) - 16 * (src - lane);
-      if (mine) {
-        const bool fine = page >= 0 && page < p.num_pages;
-        if (!fine) report_bad_index(p.status, p.epoch, kPageSite);
-        tma_load_4d(tile0 + st * F::kTile + 16 * lane * kD, tm, bar(full0 + st), 0, hk, off, fine ? page : p.num_pages);
-      }
-      if (is_k) {
-        // (those of V as logarithms: -inf where nothing is seen or the scale is 0)
-        if (lane < 16) s_scale[li % F::kScales * 16 + lane] = lane < 8 ? sc : lg2_approx(sc);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(full0 + st));
-      }
-      at = at1; at1 = at2; sc = sc1;
     }
     if (!ok && lane == 0) {
       // bounded drain: let the copies on their way land before the CTA's memory is released
       const uint64_t begun = globaltimer_ns();
-      for (int i = li > kStages ? li - kStages : 0; i < li; ++i)
+      for (int i = g > kStages ? g - kStages : 0; i < g; ++i)
         while (!mbar_try_wait(bar(full0 + i % kStages), (i / kStages) & 1) && globaltimer_ns() - begun < 50ull * 1000 * 1000) {}
     }
   } else if (warp == kIssueS) {
-    // ============================================ K . Q^T ======================================
-    if (elect_one() && n > 0) {
-      constexpr uint32_t idesc = make_idesc_e4m3(128, kN, false);
-      ok = mbar_wait(bar(F::kQReady), 0, wc, kQReadyS);
-      for (int li = 0; ok && li < n; ++li) {
-        const uint32_t st = li % kStages, sd = li % kStrands;
-        ok = mbar_wait(bar(F::kKFull + st), (li / kStages) & 1, wc, kKFullS);
-        if (ok && li >= kStrands) ok = mbar_wait(bar(F::kSFree + sd), (li / kStrands - 1) & 1, wc, kSFreeS);
-        if (!ok) break;
-        tc_fence_after_sync();
+    // ============================================ Q . K^T ======================================
+    // (An issuing thread gets an instruction every eight clocks or so, its code never stays in the scheduler's cache beside the softmax
+    // warps'.  With divisions for the ring places, descriptors made anew and votes in the loop the issuer of V^T W^T took 2000
+    // clocks a tile and paced the kernel: 4 x 65536 keys 139 us.)
+    if (elect_one()) {
+      constexpr uint32_t idesc = make_idesc_e4m3(128, 128, false);
+      const uint64_t dq = tile_desc<kD>(base + F::kOffQ), dk = tile_desc<kD>(base + F::kOffK);
+      Ring<kStages> st;
+      Ring<kStrands> sd;
+      bool first = true;                    // round of the strands
+      // (pieces without a tile have no Q: a phase of the barrier for each that has some)
+      uint32_t piece = 0;
+      for (; ok && walk.more(); walk.next(p)) {
+        const int n = walk.tiles();
+        if (n > 0) {
+          ok = mbar_wait(bar(F::kQReady), piece, wc, kQReadyS);
+          piece ^= 1u;
+        }
+#pragma unroll 1
+        for (int li = 0; ok && li < n; ++li) {
+          ok = mbar_wait(bar(F::kKFull + st.at), st.parity, wc, kKFullS);
+          if (ok && !first) ok = mbar_wait(bar(F::kSFree + sd.at), sd.parity ^ 1u, wc, kSFreeS);
+          if (!ok) break;
+          tc_fence_after_sync();
+          const uint64_t kt = desc_at(dk, st.at * F::kTile);
+          const uint32_t to = tmem + F::kS + 128 * sd.at;
 #pragma unroll
-        for (int ks = 0; ks < kD / 32; ++ks)
-          mma_e4m3(tmem + F::kS + sd * kN, tile_desc<kD>(base + F::kOffK + st * F::kTile + 32 * ks),
-                   tile_desc<kD>(base + F::kOffQ + 32 * ks), idesc, ks > 0);
-        tc_commit(bar(F::kKFree + st));
-        tc_commit(bar(F::kSFull + sd));
+          for (int ks = 0; ks < kD / 16; ++ks)
+            mma_e4m3(to, desc_at(dq, ks / (kD / 32) * F::kTile + 32 * (ks % (kD / 32))), desc_at(kt, 32 * (ks % (kD / 32))), idesc, ks > 0);
+          tc_commit(bar(F::kKFree + st.at));
+          tc_commit(bar(F::kSFull + sd.at));
+          st.next();
+          sd.next();
+          if (sd.at == 0) first = false;
+        }
       }
       if (!ok) {
         const uint64_t begun = globaltimer_ns();
@@ -243,270 +437,305 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       }
     }
   } else if (warp == kIssueO) {
-    // ============================================ V^T . P^T ====================================
-    constexpr uint32_t idesc = make_idesc_e4m3(128, kN, true);
-    for (int li = 0; li < n; ++li) {
-      const uint32_t st = li % kStages, sd = li % kStrands;
-      const int key0 = (t0 + li) << 7;
-      const bool lead = elect_one();
-      if (lead) ok = mbar_wait(bar(F::kVFull + st), (li / kStages) & 1, wc, kVFullS);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      if (key0 < lo_all || key0 + 128 > hi_all) {
-        // values that no row sees may be anything, and 0 * NaN is NaN
-        __syncwarp();
-        for (int r = lane; r < 128; r += 32)
-          if (key0 + r < lo_all || key0 + r >= hi_all) {
-            uint4* v = reinterpret_cast<uint4*>(gbase + F::kOffV + st * F::kTile + r * kD);
-#pragma unroll
-            for (int i = 0; i < kD / 16; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
-          }
-        fence_proxy_async_smem();
-        __syncwarp();
-      }
-      if (lead) {
-        ok = mbar_wait(bar(F::kPFull + sd), (li / kStrands) & 1, wc, kPFullS);
-        if (ok) {
+    // ============================================ V^T . W^T ====================================
+    if (elect_one()) {
+      constexpr uint32_t idesc = make_idesc_e4m3(128, kN, true);
+      const uint64_t dv = tile_desc<kD>(base + F::kOffV), dw = tile_desc<128>(base + F::kOffP);
+      Ring<kStages> st;
+      Ring<kStrands> sd;
+      for (; ok && walk.more(); walk.next(p)) {
+        const int n = walk.tiles();
+#pragma unroll 1
+        for (int li = 0; li < n; ++li) {
+          ok = mbar_wait(bar(F::kVFull + st.at), st.parity, wc, kVFullS) && mbar_wait(bar(F::kPFull + sd.at), sd.parity, wc, kPFullS);
+          if (!ok) break;
           tc_fence_after_sync();
+          const uint64_t vt = desc_at(dv, st.at * F::kTile), wt = desc_at(dw, sd.at * kN * 128);
+          const uint32_t to = tmem + F::kO + sd.at * kN;
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks)
-            mma_e4m3(tmem + F::kO + sd * kN, tile_desc<kD>(base + F::kOffV + st * F::kTile + 32 * ks * kD),
-                     tile_desc<128>(base + F::kOffP + sd * kN * 128 + 32 * ks), idesc, ks > 0);
-          tc_commit(bar(F::kVFree + st));
-          tc_commit(bar(F::kPvDone + sd));
+          for (int ks = 0; ks < 4; ++ks) mma_e4m3(to, desc_at(vt, 32 * ks * kD), desc_at(wt, 32 * ks), idesc, ks > 0);
+          tc_commit(bar(F::kVFree + st.at));
+          tc_commit(bar(F::kPvDone + sd.at));
+          st.next();
+          sd.next();
         }
       }
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-    }
-    if (!ok && elect_one()) {
-      const uint64_t begun = globaltimer_ns();
-      tc_commit(bar(F::kDrain + 1));
-      while (!mbar_try_wait(bar(F::kDrain + 1), 0) && globaltimer_ns() - begun < 50ull * 1000 * 1000) {}
+      if (!ok) {
+        const uint64_t begun = globaltimer_ns();
+        tc_commit(bar(F::kDrain + 1));
+        while (!mbar_try_wait(bar(F::kDrain + 1), 0) && globaltimer_ns() - begun < 50ull * 1000 * 1000) {}
+      }
     }
   } else {
     // ============================================ softmax ======================================
-    const int wg = warp >> 2, wq = warp & 3, sd = wg / kHalves, half = wg % kHalves, t = tid & 127;
+    const int sd = warp >> 2, wq = warp & 3, t = tid & 127;
     const uint32_t lanes = static_cast<uint32_t>(wq * 32) << 16;
-    float2* s_red = reinterpret_cast<float2*>(gbase + F::kOffRed) + wg * 2 * 4 * kRW;
-    float2* s_fac = reinterpret_cast<float2*>(gbase + F::kOffFac) + wg * 2 * kRW;
+    float2* s_red = reinterpret_cast<float2*>(gbase + F::kOffRed) + sd * 2 * 4 * kR;
+    float2* s_fac = reinterpret_cast<float2*>(gbase + F::kOffFac) + sd * 2 * kR;
     float* s_row = reinterpret_cast<float*>(gbase + F::kOffRow);
-
-    // ---- Q^T: a row's pieces of eight elements by neighbouring lanes
-    {
-      constexpr int kPieces = kD / 8;
-      for (int i = tid; i < kR * kPieces; i += 128 * kGroups) {
-        const int r = i / kPieces, ch = i % kPieces;
-        uint4 u = make_uint4(0u, 0u, 0u, 0u);
-        if (r < R) {
-          const int s = fast_div(r_first + r, p.div_group), h = hk * p.group + r_first + r - s * p.group;
-          u = *reinterpret_cast<const uint4*>(p.q + b * p.q_b + s * p.q_s + h * p.q_h + 8 * ch);
-        }
-        float x[8];
-        unpack8(u, x);
-        uint32_t top = 0u;                      // (bit patterns: NaN is the largest)
-#pragma unroll
-        for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(x[k]) & 0x7fffffffu);
-#pragma unroll
-        for (int o = 1; o < kPieces; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        // 2^c with largest * 2^c in [128, 256); a row that is not finite becomes NaN whole
-        const int e = max((int)(top >> 23), 17);
-        const float up = __uint_as_float((uint32_t)(254 + 7 - e) << 23), down = __uint_as_float((uint32_t)(e - 7) << 23);
-        uint32_t w[4];
-        if (top >= 0x7f800000u) {
-          w[0] = w[1] = w[2] = w[3] = 0x7f7f7f7fu;
-        } else {
-          float y[8], rest[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) x[k] *= up;
-          w[0] = pack4_e4m3(x[0], x[1], x[2], x[3]);
-          w[1] = pack4_e4m3(x[4], x[5], x[6], x[7]);
-          unpack4_e4m3(w[0], y);
-          unpack4_e4m3(w[1], y + 4);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) rest[k] = (x[k] - y[k]) * 16.f;
-          w[2] = pack4_e4m3(rest[0], rest[1], rest[2], rest[3]);
-          w[3] = pack4_e4m3(rest[4], rest[5], rest[6], rest[7]);
-        }
-        *reinterpret_cast<uint2*>(gbase + F::kOffQ + row_piece<kD>(r, ch >> 1) + (ch & 1) * 8) = make_uint2(w[0], w[1]);
-        *reinterpret_cast<uint2*>(gbase + F::kOffQ + row_piece<kD>(kR + r, ch >> 1) + (ch & 1) * 8) = make_uint2(w[2], w[3]);
-        if (ch == 0) s_row[r] = (p.cap_out != 0.f ? p.cap_in : p.sl2) * down;
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(F::kQReady));
-      // (the factors of the rows are read by all warps: they have met where all have arrived)
-      ok = __all_sync(0xffffffffu, mbar_wait(bar(F::kQReady), 0, wc, kQReadyS));
-    }
-    // After the transpose below a thread has one row, and the kRW keys of its lane group.
-    const int my = lane & (kRW - 1), row = half * kRW + my, grp = lane / kRW, key_in = wq * 32 + grp * kRW;
-    int lo = 0, hi = 0;
-    if (row < R) {
-      const int2 see = seen_by(p, len.sk, len.sq, fast_div(r_first + row, p.div_group));
-      lo = see.x;
-      hi = see.y;
-    }
-    const float factor = s_row[row];
-    float m_run = -INFINITY, l = 0.f, acc[kRW];
-#pragma unroll
-    for (int r = 0; r < kRW; ++r) acc[r] = 0.f;
-    // O^T of the strand's last tile, into the sums
-    auto take = [&](int u) {
-      if (ok) ok = mbar_wait(bar(F::kPvDone + sd), u & 1, wc, kPvDoneS);
-      ok = __all_sync(0xffffffffu, ok);
-      tc_fence_after_sync();
-      float o1[kRW], o2[kRW];
-      tmem_ld_cols<kRW>(tmem + lanes + F::kO + sd * kN + half * kRW, reinterpret_cast<uint32_t*>(o1));
-      tmem_ld_cols<kRW>(tmem + lanes + F::kO + sd * kN + kR + half * kRW, reinterpret_cast<uint32_t*>(o2));
-      tc_wait_ld();
-      tc_fence_before_sync();
-      const float2* fac = s_fac + (u & 1) * kRW;
-#pragma unroll
-      for (int r = 0; r < kRW; ++r) acc[r] = fmaf(acc[r], fac[r].x, fmaf(o2[r], 0.0625f, o1[r]) * fac[r].y);
-    };
-    int u = 0;
-    for (int li = sd; li < n; li += kStrands, ++u) {
-      // (only barriers of this strand are waited for: a stage's barrier may be two phases behind, and a wait on parities
-      // does not tell that from done)
-      const int key0 = (t0 + li) << 7;
-      if (ok) ok = mbar_wait(bar(F::kSFull + sd), u & 1, wc, kSFullS);
-      ok = __all_sync(0xffffffffu, ok);
-      tc_fence_after_sync();
-      float x[kRW], lv;
-      {
-        float x2[kRW];
-        tmem_ld_cols<kRW>(tmem + lanes + F::kS + sd * kN + half * kRW, reinterpret_cast<uint32_t*>(x));
-        tmem_ld_cols<kRW>(tmem + lanes + F::kS + sd * kN + kR + half * kRW, reinterpret_cast<uint32_t*>(x2));
-        tc_wait_ld();
-        tc_fence_before_sync();
-        // (the scales were there before the product: one barrier for both)
-        const float* sc = reinterpret_cast<const float*>(gbase + F::kOffSc) + li % F::kScales * 16;
-        const float ks = sc[t >> 4];
-        lv = sc[8 + (key_in >> 4)];
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(F::kSFree + sd));
-#pragma unroll
-        for (int r = 0; r < kRW; ++r) x[r] = fmaf(x2[r], 0.0625f, x[r]) * ks;
-      }
-      dec::lane_group_transpose<kRW>(x, lane);
-      float top = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < kRW; ++j) {
-        const int key = key0 + key_in + j;
-        x[j] = key >= lo && key < hi ? score_of(p, x[j], factor) : -INFINITY;
-        top = fmaxf(top, x[j]);
-      }
-      float top_v = top + lv;              // of the weights with the values' scales
-#pragma unroll
-      for (int o = kRW; o < 32; o <<= 1) {
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        top_v = fmaxf(top_v, __shfl_xor_sync(0xffffffffu, top_v, o));
-      }
-      float2* red = s_red + (u & 1) * 4 * kRW;
-      if (lane < kRW) red[wq * kRW + lane] = make_float2(top, top_v);
-      group_sync(1 + wg);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float2 of = red[k * kRW + my];
-        top = fmaxf(top, of.x);
-        top_v = fmaxf(top_v, of.y);
-      }
-      const float ref = top == -INFINITY ? 0.f : top, up = lv - (top_v == -INFINITY ? 0.f : top_v) + 8.f;
-      const float m_new = fmaxf(m_run, top), keep = m_new == -INFINITY ? 0.f : ex2_approx(m_run - m_new),
-                  add = m_new == -INFINITY ? 0.f : ex2_approx(top - m_new),
-                  add_v = m_new == -INFINITY ? 0.f : ex2_approx(top_v - m_new);
-      float w[kRW], sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < kRW; ++j) {
-        sum += ex2_approx(x[j] - ref);
-        w[j] = ex2_approx(x[j] + up);
-      }
-      l = fmaf(l, keep, sum * add);
-      m_run = m_new;
-      // the sums of the tile before, and with them its P^T, are done with
-      if (u > 0) take(u - 1);
-      if (wq == 0 && lane < kRW) s_fac[(u & 1) * kRW + lane] = make_float2(keep, add_v * (1.f / 256.f));
-      {
-        uint8_t* pt = gbase + F::kOffP + sd * kN * 128;
-        uint32_t w1[kRW / 4], w2[kRW / 4];
-#pragma unroll
-        for (int j = 0; j < kRW / 4; ++j) {
-          float y[4];
-          w1[j] = pack4_e4m3(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
-          unpack4_e4m3(w1[j], y);
-          w2[j] = pack4_e4m3((w[4 * j] - y[0]) * 16.f, (w[4 * j + 1] - y[1]) * 16.f, (w[4 * j + 2] - y[2]) * 16.f,
-                             (w[4 * j + 3] - y[3]) * 16.f);
-        }
-        uint8_t *a1 = pt + sw128_offset(row, key_in >> 4) + (key_in & 15), *a2 = pt + sw128_offset(kR + row, key_in >> 4) + (key_in & 15);
-        if constexpr (kRW == 8) {
-          *reinterpret_cast<uint2*>(a1) = make_uint2(w1[0], w1[1]);
-          *reinterpret_cast<uint2*>(a2) = make_uint2(w2[0], w2[1]);
-        } else {
-          *reinterpret_cast<uint4*>(a1) = make_uint4(w1[0], w1[1], w1[2], w1[3]);
-          *reinterpret_cast<uint4*>(a2) = make_uint4(w2[0], w2[1], w2[2], w2[3]);
-        }
-      }
-      fence_proxy_async_smem();
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(F::kPFull + sd));
-    }
-    if (u > 0) {
-      // (the factors of the last tile, written before its rendezvous... by one warp: meet once more)
-      group_sync(1 + wg);
-      take(u - 1);
-    }
-    // ---- the row's sum over its lanes and warps, then the strands
-#pragma unroll
-    for (int o = kRW; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
     float* s_sum = reinterpret_cast<float*>(gbase + F::kOffSum);
     float* s_ref = reinterpret_cast<float*>(gbase + F::kOffRef);
-    if (lane < kRW) s_sum[(wg * 4 + wq) * kRW + lane] = l;
-    if (wq == 0 && lane < kRW) s_ref[wg * kRW + lane] = m_run;
-    auto all_groups = [] { asm volatile("bar.sync 15, %0;" ::"n"(128 * kGroups) : "memory"); };
-    all_groups();                                                    // (every tile is done with: the rings are free)
-    float* s_acc = reinterpret_cast<float*>(gbase + F::kOffK);       // strands x rows x kD
-    if (t < kD) {
+    float* s_acc = reinterpret_cast<float*>(gbase + F::kOffQ);       // strands x rows x kD
+    auto all_strands = [] { asm volatile("bar.sync 15, %0;" ::"n"(128 * kStrands) : "memory"); };
+    const int my = lane & (kR - 1), grp = lane / kR, key_in = wq * 32 + grp * kKeys;
+    int g = 0;
+    bool again = false;
+    for (int piece = 0; walk.more(); walk.next(p)) {
+      if (again) all_strands();                                        // (the sums of the last piece are read: Q may be written)
+      again = true;
+      const Seq seq = walk.cur;
+      const int n = walk.tiles(), t0 = seq.first + walk.at, b = walk.b, hk = walk.hb * p.bundle + in_bundle, R = seq.sq * p.group;
+      // ---- Q: a row's pieces of eight elements by neighbouring lanes, to all copies of the row
+      if (n > 0) {
+        constexpr int kPieces = kD / 8;
+        for (int i = tid; i < kR * kPieces; i += 128 * kStrands) {
+          const int r = i / kPieces, ch = i % kPieces;
+          uint4 u = make_uint4(0u, 0u, 0u, 0u);
+          if (r < R) {
+            const int s = fast_div(r, p.div_group), h = hk * p.group + r - s * p.group;
+            u = *reinterpret_cast<const uint4*>(p.q + b * p.q_b + s * p.q_s + h * p.q_h + 8 * ch);
+          }
+          float x[8];
+          unpack8(u, x);
+          uint32_t top = 0u;                      // (bit patterns: NaN is the largest)
 #pragma unroll
-      for (int r = 0; r < kRW; ++r) s_acc[(sd * kR + half * kRW + r) * kD + t] = acc[r];
-    }
-    all_groups();
-    // a warp a row, four elements a lane
-    const bool whole = *s_abort == 0u;
+          for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(x[k]) & 0x7fffffffu);
+#pragma unroll
+          for (int o = 1; o < kPieces; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+          // 2^c with largest * 2^c in [128, 256); a row that is not finite becomes NaN whole
+          const int e = max((int)(top >> 23), 17);
+          const float up = __uint_as_float((uint32_t)(254 + 7 - e) << 23), down = __uint_as_float((uint32_t)(e - 7) << 23);
+          uint32_t w[4];
+          if (top >= 0x7f800000u) {
+            w[0] = w[1] = w[2] = w[3] = 0x7f7f7f7fu;
+          } else {
+            float y[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] *= up;
+            w[0] = pack4_e4m3(x[0], x[1], x[2], x[3]);
+            w[1] = pack4_e4m3(x[4], x[5], x[6], x[7]);
+            unpack4_e4m3(w[0], y);
+            unpack4_e4m3(w[1], y + 4);
+            w[2] = pack4_e4m3(x[0] - y[0], x[1] - y[1], x[2] - y[2], x[3] - y[3]);
+            w[3] = pack4_e4m3(x[4] - y[4], x[5] - y[5], x[6] - y[6], x[7] - y[7]);
+          }
+#pragma unroll
+          for (int k = 0; k < 128 / kR; ++k) {
+            uint8_t* to = gbase + F::kOffQ + row_piece<kD>(k * kR + r, ch >> 1) + (ch & 1) * 8;
+            *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+            *reinterpret_cast<uint2*>(to + F::kTile) = make_uint2(w[2], w[3]);
+          }
+          if (ch == 0) s_row[r] = (F::kCap ? p.cap_in : p.sl2) * down;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(F::kQReady));
+        // (the factors of the rows are read by all warps: they have met where all have arrived)
+        if (ok) ok = mbar_wait(bar(F::kQReady), piece++ & 1, wc, kQReadyS);
+        ok = __all_sync(0xffffffffu, ok);
+      }
+      int lo = 0, hi = 0;
+      if (my < R) {
+        const int2 see = seen_by(p, seq.sk, seq.sq, fast_div(my, p.div_group));
+        lo = see.x;
+        hi = see.y;
+      }
+      // the keys that all rows see
+      const int lo_in = seq.sq > 0 ? seen_by(p, seq.sk, seq.sq, seq.sq - 1).x : 0, hi_in = seen_by(p, seq.sk, seq.sq, 0).y;
+      const float factor = s_row[my];
+      float m_run = -INFINITY, l = 0.f, acc[kR];
+#pragma unroll
+      for (int r = 0; r < kR; ++r) acc[r] = 0.f;
+      // O^T of the strand's tile before, into the sums
+      auto take = [&](int u) {
+        if (ok) ok = mbar_wait(bar(F::kPvDone + sd), u & 1, wc, kPvDoneS);
+        ok = __all_sync(0xffffffffu, ok);
+        tc_fence_after_sync();
+        float o1[kR], o2[kR];
+        tmem_ld_cols<kR>(tmem + lanes + F::kO + sd * kN, reinterpret_cast<uint32_t*>(o1));
+        tmem_ld_cols<kR>(tmem + lanes + F::kO + sd * kN + kR, reinterpret_cast<uint32_t*>(o2));
+        tc_wait_ld();
+        tc_fence_before_sync();
+        const float4* fac = reinterpret_cast<const float4*>(s_fac + (u & 1) * kR);
+#pragma unroll
+        for (int r = 0; r < kR; r += 2) {
+          const float4 f = fac[r / 2];
+          acc[r] = fmaf(acc[r], f.x, fmaf(o2[r], 0.0625f, o1[r]) * f.y);
+          acc[r + 1] = fmaf(acc[r + 1], f.z, fmaf(o2[r + 1], 0.0625f, o1[r + 1]) * f.w);
+        }
+      };
+      // this strand's tiles: those with running number sd, sd + kStrands, ... of the CTA
+      // (and one round more, for the last tile's product)
+      const int g0 = g, li0 = (sd + kStrands - g0 % kStrands) % kStrands, u0 = (g0 + li0) / kStrands;
 #pragma unroll 1
-    for (int r = warp; r < R && whole; r += 4 * kGroups) {
-      const int hf = r / kRW, rw = r % kRW, col = 4 * lane;
-      float m = -INFINITY, sum = 0.f;
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int li = li0, u = u0; li < n + kStrands; li += kStrands, ++u) {
+        const bool live = li < n;
+        const int key0 = (t0 + li) << 7;
+        float x[kKeys], up[kKeys / 16], keep = 0.f, add_v = 0.f;
+        if (live) {
+        // (only barriers of this strand are waited for: a stage's barrier may be two phases behind, and a wait on parities
+        // does not tell that from done)
+        if (ok) ok = mbar_wait(bar(F::kSFull + sd), u & 1, wc, kSFullS);
+        ok = __all_sync(0xffffffffu, ok);
+        tc_fence_after_sync();
+        float ks[kKeys / 16], lv[kKeys / 16];
+        {
+          float y[32];
+          tmem_ld32(tmem + lanes + F::kS + 128 * sd + 32 * wq, reinterpret_cast<uint32_t*>(y));
+          tc_wait_ld();
+          tc_fence_before_sync();
+          // (the scales were there before the product: one barrier for both)
+          const float* sc = reinterpret_cast<const float*>(gbase + F::kOffSc) + (g0 + li) % F::kScales * 16;
 #pragma unroll
-      for (int k = 0; k < kStrands; ++k) m = fmaxf(m, s_ref[(k * kHalves + hf) * kRW + rw]);
+          for (int i = 0; i < kKeys / 16; ++i) {
+            ks[i] = sc[(key_in >> 4) + i] * factor;
+            lv[i] = lg2_approx(sc[8 + (key_in >> 4) + i]);       // (-inf where nothing is seen or the scale is 0)
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(F::kSFree + sd));
 #pragma unroll
-      for (int k = 0; k < kStrands; ++k) {
-        const int g = k * kHalves + hf;
-        const float f = m == -INFINITY ? 1.f : ex2_approx(s_ref[g * kRW + rw] - m);
-        const float* s4 = s_sum + g * 4 * kRW + rw;
-        sum = fmaf(f, ((s4[0] + s4[kRW]) + s4[2 * kRW]) + s4[3 * kRW], sum);
-        if (col < kD) {
-          const float4 a = *reinterpret_cast<const float4*>(s_acc + (k * kR + r) * kD + col);
-          o.x = fmaf(f, a.x, o.x); o.y = fmaf(f, a.y, o.y); o.z = fmaf(f, a.z, o.z); o.w = fmaf(f, a.w, o.w);
+          for (int j = 0; j < kKeys; ++j) {
+            x[j] = (kR == 16 && grp != 0 ? y[(16 + j) & 31] : y[j]) * ks[j / 16];
+            if constexpr (F::kCap) x[j] = p.cap_out * tanh_of(x[j]);
+          }
+        }
+        if (key0 < lo_in || key0 + 128 > hi_in) {
+#pragma unroll
+          for (int j = 0; j < kKeys; ++j) {
+            const int key = key0 + key_in + j;
+            x[j] = key >= lo && key < hi ? x[j] : -INFINITY;
+          }
+        }
+        float top = -INFINITY, top_v = -INFINITY;     // of the scores; of the weights with the values' scales
+#pragma unroll
+        for (int i = 0; i < kKeys / 16; ++i) {
+          float m = fmaxf(x[16 * i], x[16 * i + 1]);
+#pragma unroll
+          for (int j = 2; j < 16; j += 2) m = fmax3(m, x[16 * i + j], x[16 * i + j + 1]);
+          top = fmaxf(top, m);
+          top_v = fmaxf(top_v, m + lv[i]);
+        }
+#pragma unroll
+        for (int o = kR; o < 32; o <<= 1) {
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          top_v = fmaxf(top_v, __shfl_xor_sync(0xffffffffu, top_v, o));
+        }
+        float2* red = s_red + (u & 1) * 4 * kR;
+        if (lane < kR) red[wq * kR + lane] = make_float2(top, top_v);
+        group_sync(1 + sd);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 of = red[k * kR + my];
+          top = fmaxf(top, of.x);
+          top_v = fmaxf(top_v, of.y);
+        }
+        const float ref = top == -INFINITY ? 0.f : top, ref_v = top_v == -INFINITY ? 0.f : top_v;
+        const float m_new = fmaxf(m_run, top), base_m = m_new == -INFINITY ? 0.f : m_new, add = ex2_approx(top - base_m);
+        keep = ex2_approx(m_run - base_m);
+        add_v = ex2_approx(top_v - base_m);
+        // a weight times this is 256 at most (bounded for scales further apart than fp32 reaches)
+#pragma unroll
+        for (int i = 0; i < kKeys / 16; ++i) {
+          const float e = lv[i] + (ref - ref_v) + 8.f;
+          up[i] = ex2_approx(e > 100.f ? 100.f : e);
+        }
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < kKeys; ++j) {
+          x[j] = ex2_approx(x[j] - ref);
+          sum += x[j];
+          x[j] *= up[j / 16];
+        }
+        l = fmaf(l, keep, sum * add);
+        m_run = m_new;
+        } else {
+          if (u == u0) break;
+          group_sync(1 + sd);         // (the factors of the last tile are written by one warp)
+        }
+        // the sums of the tile before, and with them its W^T, are done with
+        if (u > u0) take(u - 1);
+        if (!live) break;
+        if (wq == 0 && lane < kR) s_fac[(u & 1) * kR + lane] = make_float2(keep, add_v * (1.f / 256.f));
+#pragma unroll
+        for (int i = 0; i < kKeys / 16; ++i) {
+          uint32_t w1[4], w2[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float* w = x + 16 * i + 4 * j;
+            float y[4];
+            w1[j] = pack4_e4m3(w[0], w[1], w[2], w[3]);
+            unpack4_e4m3(w1[j], y);
+            w2[j] = pack4_e4m3((w[0] - y[0]) * 16.f, (w[1] - y[1]) * 16.f, (w[2] - y[2]) * 16.f, (w[3] - y[3]) * 16.f);
+          }
+          uint8_t* pt = gbase + F::kOffP + sd * kN * 128;
+          *reinterpret_cast<uint4*>(pt + sw128_offset(my, (key_in >> 4) + i)) = make_uint4(w1[0], w1[1], w1[2], w1[3]);
+          *reinterpret_cast<uint4*>(pt + sw128_offset(kR + my, (key_in >> 4) + i)) = make_uint4(w2[0], w2[1], w2[2], w2[3]);
+        }
+        fence_proxy_async_smem();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(F::kPFull + sd));
+      }
+      g += n;
+      // ---- the row's sum over its lanes and warps, then the strands
+#pragma unroll
+      for (int o = kR; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+      if (lane < kR) s_sum[(sd * 4 + wq) * kR + lane] = l;
+      if (wq == 0 && lane < kR) s_ref[sd * kR + lane] = m_run;
+      all_strands();                                                   // (every product of the piece is done: Q is free)
+      if (t < kD) {
+#pragma unroll
+        for (int r = 0; r < kR; ++r) s_acc[(sd * kR + r) * kD + t] = acc[r];
+      }
+      all_strands();
+      // where the result goes: the output if the whole unit was this piece, else a slot of partial results
+      const int places = cost_of(seq), unit = b * p.Hkv + hk;
+      bool direct;
+      int64_t slot;
+      if (p.num_splits > 0) {
+        direct = p.num_splits == 1;
+        slot = (int64_t)unit * p.num_splits + group % p.num_splits;
+      } else {
+        direct = walk.places() == places;
+        slot = 2 * (int64_t)blockIdx.x + (walk.at == 0 ? 1 : 0);
+        if (tid == 0 && walk.at == 0) {
+          const int share = s_walk.share, rest = places - walk.places();
+          p.pieces[unit] = make_int2(blockIdx.x, 1 + (rest + share - 1) / share);
         }
       }
-      const int s = fast_div(r_first + r, p.div_group), h = hk * p.group + r_first + r - s * p.group;
-      const int64_t l_idx = ((int64_t)b * p.Hq + h) * p.Sq + s;
-      if (p.num_splits == 1) {
-        const RowEnd e = finish_row(m, sum, p.sink, h);
-        if (col < kD)
-          *reinterpret_cast<uint2*>(p.out + b * p.o_b + s * p.o_s + h * p.o_h + col) =
-              make_uint2(pack_bf16x2(o.x * e.factor, o.y * e.factor), pack_bf16x2(o.z * e.factor, o.w * e.factor));
-        if (lane == 0 && p.lse != nullptr) p.lse[l_idx] = e.lse;
-      } else {
-        const int64_t rows = (int64_t)p.B * p.Sq * p.Hq, part = (int64_t)split * rows;
-        const bool none = m == -INFINITY && sum == 0.f;
-        const float f = 1.f / sum;
-        if (col < kD && !none)
-          *reinterpret_cast<float4*>(p.o_partial + (part + ((int64_t)b * p.Sq + s) * p.Hq + h) * kD + col) =
-              make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
-        if (lane == 0) p.lse_partial[part + l_idx] = none ? -INFINITY : m + log2f(sum);
+      // a warp a row, four elements a lane
+      const bool whole = *s_abort == 0u;
+#pragma unroll 1
+      for (int r = warp; r < R && whole; r += 4 * kStrands) {
+        const int col = 4 * lane;
+        float m = -INFINITY, sum = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < kStrands; ++k) m = fmaxf(m, s_ref[k * kR + r]);
+#pragma unroll
+        for (int k = 0; k < kStrands; ++k) {
+          const float f = m == -INFINITY ? 1.f : ex2_approx(s_ref[k * kR + r] - m);
+          const float* s4 = s_sum + k * 4 * kR + r;
+          sum = fmaf(f, ((s4[0] + s4[kR]) + s4[2 * kR]) + s4[3 * kR], sum);
+          if (col < kD) {
+            const float4 a = *reinterpret_cast<const float4*>(s_acc + (k * kR + r) * kD + col);
+            o.x = fmaf(f, a.x, o.x); o.y = fmaf(f, a.y, o.y); o.z = fmaf(f, a.z, o.z); o.w = fmaf(f, a.w, o.w);
+          }
+        }
+        if (direct) {
+          const int s = fast_div(r, p.div_group), h = hk * p.group + r - s * p.group;
+          const RowEnd e = finish_row(m, sum, p.sink, h);
+          if (col < kD)
+            *reinterpret_cast<uint2*>(p.out + b * p.o_b + s * p.o_s + h * p.o_h + col) =
+                make_uint2(pack_bf16x2(o.x * e.factor, o.y * e.factor), pack_bf16x2(o.z * e.factor, o.w * e.factor));
+          if (lane == 0 && p.lse != nullptr) p.lse[((int64_t)b * p.Hq + h) * p.Sq + s] = e.lse;
+        } else {
+          const bool none = m == -INFINITY && sum == 0.f;
+          const float f = __frcp_rn(sum);
+          if (col < kD && !none)
+            *reinterpret_cast<float4*>(p.o_partial + (slot * p.unit_rows + r) * kD + col) = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+          if (lane == 0) p.lse_partial[slot * p.unit_rows + r] = none ? -INFINITY : m + lg2_approx(sum);
+        }
       }
     }
   }
@@ -514,8 +743,36 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   __syncthreads();
   if (warp == kIssueS) {
     tc_fence_after_sync();
-    tmem_dealloc(tmem, F::kCols);
+    tmem_dealloc(tmem, 512);
   }
+}
+
+// The units that several CTAs had a piece of: a warp a row.
+__global__ void __launch_bounds__(kFp8CombineWarps * 32) fp8_merge_kernel(const __grid_constant__ Fp8Params p) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t r = blockIdx.x * kFp8CombineWarps + (threadIdx.x >> 5), rows = (uint32_t)p.B * p.Sq * p.Hq;
+  pdl_wait();
+  if (r >= rows) return;
+  const int bs = fast_div((int)r, p.div_hq), h = (int)r - bs * p.Hq, b = fast_div(bs, p.div_sq), s = bs - b * p.Sq;
+  if (p.fresh != nullptr && s >= p.fresh[b]) return;
+  const int hk = fast_div(h, p.div_group), row = s * p.group + h - hk * p.group, unit = b * p.Hkv + hk;
+  int64_t first, step;
+  int pieces = p.num_splits;
+  if (pieces > 0) {
+    // (the splits that have a part of the unit)
+    first = (int64_t)unit * pieces;
+    step = 1;
+    const SeqLens len = lens_of(p, b);
+    const int places = fp8d::cost_of(fp8d::seq_of(p, len.sk, len.sq)), per = (places + pieces - 1) / pieces;
+    pieces = (places + per - 1) / per;
+  } else {
+    const int2 at = p.pieces[unit];
+    pieces = at.y;
+    first = 2 * (int64_t)at.x;          // (a CTA has two slots: of the unit it begins in the middle of, of the one it leaves there)
+    step = 2 * p.bundle;
+  }
+  if (p.num_splits == 0 && pieces <= 1) return;
+  merge_row(p, b, s, h, lane, pieces, [&](int i) { return (first + i * step + (i == 0 && p.num_splits == 0 ? 1 : 0)) * p.unit_rows + row; });
 }
 
 }  // namespace fa4

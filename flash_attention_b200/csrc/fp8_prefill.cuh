@@ -243,7 +243,7 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         if (mine) {
           const bool fine = page >= 0 && page < p.num_pages;
           if (!fine) report_bad_index(p.status, p.epoch, kPageSite);
-          tma_load_4d(tile + 16 * lane * kD, tm, full, 0, hk, off, fine ? page : p.num_pages);
+          tma_load_4d(tile + 16 * lane * kD, tm, full, 0, off, hk, fine ? page : p.num_pages);
         }
         if (is_k) {
           // (Q K^T of step i - 2 is done before this step is converted, and so the softmax of step i - 3: four slots are enough)
@@ -262,11 +262,17 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       if (elect_one() && n > 0) {
         constexpr uint32_t idesc_s = make_idesc_f16(128, 128, false), idesc_o = make_idesc_f16(128, kD, true);
         // (products run in the order they are issued: Q K^T of a tile's next step may overwrite the weights that W V in front of it reads)
-        auto score = [&](int t, int i) {
+        // (descriptors are moved, not made anew: see the issuers of the decode kernel)
+        using fp8d::desc_at;
+        const uint64_t dq = half_desc(base + L::kOffQ), dk = half_desc(base + L::kOffK), dv = half_desc(base + L::kOffV);
+        auto score = [&](uint32_t t, uint32_t buf) {
+          const uint64_t qt = desc_at(dq, t * L::kTile16), kt = desc_at(dk, buf * L::kTile16);
+          const uint32_t to = tmem + kColS + 128 * t;
 #pragma unroll
-          for (int ks = 0; ks < kD / 16; ++ks)
-            mma_f16_ss(tmem + kColS + 128 * t, half_desc(base + L::kOffQ + t * L::kTile16 + (ks >> 2) * L::kHalf + (ks & 3) * 32),
-                       half_desc(base + L::kOffK + (i & 1) * L::kTile16 + (ks >> 2) * L::kHalf + (ks & 3) * 32), idesc_s, ks > 0);
+          for (int ks = 0; ks < kD / 16; ++ks) {
+            const uint32_t at = (ks >> 2) * L::kHalf + (ks & 3) * 32;
+            mma_f16_ss(to, desc_at(qt, at), desc_at(kt, at), idesc_s, ks > 0);
+          }
           tc_commit(bar(L::kSFull + t));
         };
         ok = mbar_wait(bar(L::kQReady), 0, wc, kQReadyS) && mbar_wait(bar(L::kKFull), 0, wc, kHalfFullS);
@@ -275,23 +281,29 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
           for (int t = 0; t < tiles; ++t) score(t, 0);
           tc_commit(bar(L::kKFree));
         }
+        uint32_t buf = 0, parity = 0;          // of step i
+#pragma unroll 1
         for (int i = 0; ok && i < n; ++i) {
-          ok = mbar_wait(bar(L::kVFull + (i & 1)), (i >> 1) & 1, wc, kHalfFullS);
-          if (ok && i + 1 < n) ok = mbar_wait(bar(L::kKFull + ((i + 1) & 1)), ((i + 1) >> 1) & 1, wc, kHalfFullS);
+          const bool more = i + 1 < n;
+          ok = mbar_wait(bar(L::kVFull + buf), parity, wc, kHalfFullS);
+          if (ok && more) ok = mbar_wait(bar(L::kKFull + (buf ^ 1u)), parity ^ buf, wc, kHalfFullS);
+          const uint64_t vt = desc_at(dv, buf * L::kTile16);
+#pragma unroll 1
           for (int t = 0; ok && t < tiles; ++t) {
             ok = mbar_wait(bar(L::kPFull + t), i & 1, wc, kPFullS);
             if (!ok) break;
             tc_fence_after_sync();
+            const uint32_t to = tmem + kColO + kD * t, w = tmem + kColS + 128 * t;
 #pragma unroll
-            for (int ks = 0; ks < 8; ++ks)
-              mma_f16_ts(tmem + kColO + kD * t, tmem + kColS + 128 * t + 8 * ks, half_desc(base + L::kOffV + (i & 1) * L::kTile16 + 2048 * ks), idesc_o,
-                         i > 0 || ks > 0);
-            if (i + 1 < n) score(t, i + 1);
+            for (int ks = 0; ks < 8; ++ks) mma_f16_ts(to, w + 8 * ks, desc_at(vt, 2048 * ks), idesc_o, i > 0 || ks > 0);
+            if (more) score(t, buf ^ 1u);
           }
           if (ok) {
-            tc_commit(bar(L::kVFree + (i & 1)));
-            if (i + 1 < n) tc_commit(bar(L::kKFree + ((i + 1) & 1)));
+            tc_commit(bar(L::kVFree + buf));
+            if (more) tc_commit(bar(L::kKFree + (buf ^ 1u)));
           }
+          parity ^= buf;
+          buf ^= 1u;
         }
         if (ok) {
           tc_commit(bar(L::kODone));
@@ -461,7 +473,7 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       const float scale = (direct ? end.factor : 1.f / l) * vs_down;
       if (ok && row < R) {
         if (direct && p.lse != nullptr) p.lse[l_idx] = end.lse;
-        if (!direct) p.lse_partial[part + l_idx] = none ? -INFINITY : m_ref + log2f(l);
+        if (!direct) p.lse_partial[part + ((int64_t)b * p.Sq + s) * p.Hq + h] = none ? -INFINITY : m_ref + log2f(l);
       }
 #pragma unroll 1
       for (int c = 0; c < kD / 32; ++c) {
