@@ -137,6 +137,14 @@ int validate_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f) {
 
 namespace {
 
+// The most tiles of 128 keys that rows of one sequence may see.
+int64_t longest_unit(const fa4_fp8_cache* c, const fa4_fp8_fwd* f) {
+  const int64_t all = ((int64_t)c->pages_per_seq * c->page_size + 127) / 128;
+  if (f->window_left < 0) return all;
+  const bool open = f->window_right < 0 && !f->causal;         // (to the right)
+  return open ? all : std::min(all, ((int64_t)f->window_left + std::max(0, f->window_right) + f->Sq + 126) / 128 + 1);
+}
+
 // How a call is run.
 struct Fp8Plan {
   bool decode;
@@ -154,6 +162,9 @@ Fp8Plan plan_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f) {
   if (plan.decode) {
     plan.rows = rows <= 16 ? 16 : 32;
     plan.splits = f->num_splits;
+    // Dealing the shares and merging the pieces costs about as much as ten tiles.  us, dealt / a CTA a unit: 128 units of a window of nine
+    // tiles, head dim 64 19.0 / 12.6, 8 units of seven tiles 10.5 / 9.2; but 256 units of up to 64 tiles 57.6 / 71.1.
+    if (plan.splits == 0 && units <= kSms && longest_unit(c, f) <= 10) plan.splits = 1;
     for (plan.bundle = std::min(8, c->Hkv); c->Hkv % plan.bundle != 0;) --plan.bundle;
     plan.slots = plan.splits == 0 ? 2 * kSms : plan.splits == 1 ? 0 : units * plan.splits;
     plan.slot_rows = rows;

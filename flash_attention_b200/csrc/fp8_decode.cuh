@@ -94,12 +94,13 @@ struct Form {
   static constexpr int kN = 2 * kR, kKeys = kR;       // keys of a thread: 128 lanes hold 128 / kR copies of the rows
   static constexpr uint32_t kTile = 128 * kD;
   // Scales of K and V come with K.  Its stage is free when the product is done, which is before the softmax has read them:
-  // the tiles that a strand may still read (one each) keep theirs.
-  static constexpr int kScales = kStages + kStrands;
+  // the tiles that a strand may still read (one each) keep theirs, beside a batch that is written at once.
+  static constexpr int kScales = kStages + kStrands + 4;
   static constexpr uint32_t kOffK = 0, kOffV = kOffK + kStages * kTile, kOffQ = kOffV + kStages * kTile,   // q1, q2: 128 x kD
       kOffP = kOffQ + 2 * kTile,                                             // kStrands x (kN rows x 128 keys)
       kOffSc = kOffP + kStrands * kN * 128,                                  // scales of 16 keys: 8 of K, 8 of V a tile
-      kOffRed = kOffSc + kScales * 64,                                       // maxima: strands x 2 x 4 warps x rows
+      kOffBox = (kOffSc + kScales * 64 + 15) / 16 * 16,                                        // what the copies of a batch need: 2 x 32 (page, key in it)
+      kOffRed = kOffBox + 512,                                       // maxima: strands x 2 x 4 warps x rows
       kOffFac = kOffRed + kStrands * 2 * 4 * kR * 8,                         // (keep, add): strands x 2 x rows
       kOffRow = kOffFac + kStrands * 2 * kR * 8,                             // factor of a row's scores
       kOffSum = kOffRow + kR * 4,                                            // strands x 4 warps x rows: sums
@@ -239,7 +240,7 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     *s_abort = 0u;
     wc = WaitCtx{s_abort, p.status, p.budget_ns, p.epoch};
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(bar(F::kKFull + s), 2);    // the copies' bytes, and the scales
+      mbar_init(bar(F::kKFull + s), 1);    // (the scales are written in front of the copies)
       mbar_init(bar(F::kVFull + s), 1);
       mbar_init(bar(F::kKFree + s), 1);
       mbar_init(bar(F::kVFree + s), 1);
@@ -294,96 +295,116 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   if (warp == kLoadK || warp == kLoadV) {
     // ============================================ loaders ======================================
     // Four tiles at a time: lane 8 q + g looks up keys 16 g .. 16 g + 15 of the q-th, their page two batches ahead and, in the loader of
-    // K, the scales of their keys and values one batch ahead (a tile at a time, a CTA ran at a tile per memory latency, 1.1 us).  The
-    // lanes in front of a box issue its copy.  Boxes that no row sees are not loaded, their entries of the table not read.
+    // K, the scales of their keys and values one batch ahead (a tile at a time, a CTA ran at a tile per memory latency).  What the copies need goes
+    // through shared memory to one thread, which issues them (with all lanes in that loop a tile took 900 clocks).  Boxes that no row
+    // sees are not loaded, their entries of the table not read.
     const bool is_k = warp == kLoadK;
     const CUtensorMap* tm = is_k ? &tm_k : &tm_v;
-    const uint32_t full0 = is_k ? F::kKFull : F::kVFull, free0 = is_k ? F::kKFree : F::kVFree;
+    const uint32_t full0 = bar(is_k ? F::kKFull : F::kVFull), free0 = bar(is_k ? F::kKFree : F::kVFree);
     const uint32_t tile0 = base + (is_k ? F::kOffK : F::kOffV);
     float* s_scale = reinterpret_cast<float*>(gbase + F::kOffSc);
+    int2* s_box = reinterpret_cast<int2*>(gbase + F::kOffBox) + (is_k ? 0 : 32);
     const int per_box = p.box >> 4, gr = lane & 7;
-    int g = 0, slot = 0;
-    Ring<kStages> st;
+    int g = 0, slot = 0;                    // tiles before the batch; its place among the scales
+    Ring<kStages> st;                       // (of the issuing thread)
     bool first = true;                      // round of the ring
     uint32_t parts = 0u;
     for (; ok && walk.more(); walk.next(p)) {
       const int n = walk.tiles(), t0 = walk.cur.first + walk.at, b = walk.b, hk = walk.hb * p.bundle + in_bundle, lo = walk.cur.lo, hi = walk.cur.hi;
-      // (page, first key of these 16 in it) for the batch from tile `li` on; page -1: no row sees them
+      // (page, first key of these 16 in it) for the batch from tile `li` on; key -1: no row sees them
       auto look_up = [&](int li) -> int2 {
-        int2 at = make_int2(-1, 0);
+        int2 at = make_int2(0, -1);
         const int mine = li + (lane >> 3), key = ((t0 + mine) << 7) + 16 * gr;
         if (mine < n && key < hi && key + 16 > lo) {
           const int pg = fast_div(key, p.div_page);
           at = make_int2(p.table != nullptr ? p.table[(int64_t)b * p.pages_per_seq + pg] : b, key - pg * p.page_size);
-          if (at.x < 0 || at.x >= p.num_pages) {
-            report_bad_index(p.status, p.epoch, kPageSite);
-            at.x = p.num_pages;                     // (reads as zeros)
-          }
         }
         return at;
       };
       auto scales_at = [&](int2 at) -> float2 {
-        if (!is_k || at.x < 0 || at.x >= p.num_pages) return make_float2(0.f, 0.f);
+        if (!is_k || at.y < 0 || at.x < 0 || at.x >= p.num_pages) return make_float2(0.f, 0.f);
         const int64_t i = ((int64_t)at.x * (p.page_size >> p.log_block) + (at.y >> p.log_block)) * p.Hkv + hk;
         return make_float2(p.k_scale[i], p.v_scale[i]);
       };
       int2 at = look_up(0), at1 = look_up(4);
       float2 sc = scales_at(at);
-      for (int l0 = 0; ok && l0 < n; l0 += 4) {
-        const int2 at2 = look_up(l0 + 8);
-        const float2 sc1 = scales_at(at1);
+#pragma unroll 1
+      for (int l0 = 0; l0 < n; l0 += 4) {
         // a box is loaded if any of its keys is seen; the keys in front of those have no page here: that of the box is the first one looked up
-        const uint32_t seen = __ballot_sync(0xffffffffu, at.x >= 0);
+        const uint32_t seen = __ballot_sync(0xffffffffu, at.y >= 0);
         const uint32_t in_box = (seen >> lane) & ((1u << per_box) - 1u);
         const bool heads = (gr & (per_box - 1)) == 0 && in_box != 0u;
         const uint32_t boxes = __ballot_sync(0xffffffffu, heads);
         const int src = heads ? lane + __ffs(in_box) - 1 : lane;
-        const int page = __shfl_sync(0xffffffffu, at.x, src & 31), off = __shfl_sync(0xffffffffu, at.y, src & 31) - 16 * (src - lane);
+        int page = __shfl_sync(0xffffffffu, at.x, src & 31);
+        const int off = __shfl_sync(0xffffffffu, at.y, src & 31) - 16 * (src - lane);
+        if (heads) {
+          if (page < 0 || page >= p.num_pages) {
+            report_bad_index(p.status, p.epoch, kPageSite);
+            page = p.num_pages;                       // (reads as zeros)
+          }
+          s_box[lane] = make_int2(page, off);
+        }
         const int end = min(4, n - l0);
+        if (is_k && (lane >> 3) < end) {
+          // (the scales of the batch, as far ahead of the softmax as the ring of them allows)
+          int to = slot + (lane >> 3);
+          to = (to >= F::kScales ? to - F::kScales : to) * 16 + gr;
+          s_scale[to] = sc.x;
+          s_scale[to + 8] = sc.y;
+        }
+        const int2 at2 = look_up(l0 + 8);
+        const float2 sc1 = scales_at(at1);
+        __syncwarp();
+        // A tile of values that are not all seen (the first and the last of a unit may be) goes through a barrier of its own: the others may be
+        // anything, and 0 * NaN is NaN, so they are made zeros before the tile is given on.
+        auto in_part = [&](int q) { const int key0 = (t0 + l0 + q) << 7; return !is_k && (key0 < lo || key0 + 128 > hi); };
+        for (int q0 = 0; q0 < end && ok;) {
+          int q1 = q0;
+          while (q1 < end && !in_part(q1)) ++q1;
+          const bool part = q1 < end;
+          uint32_t last = 0u;                       // the last one's stage
+          const bool lead = elect_one();            // (the same lane each time)
+          if (lead) {
 #pragma unroll 1
-        for (int q = 0; q < end; ++q) {
-          const uint32_t full = bar(full0 + st.at);
-          if (ok && !first) ok = mbar_wait_relaxed<256>(bar(free0 + st.at), st.parity ^ 1u, wc, is_k ? kKFreeS : kVFreeS);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          // A tile of values that are not all seen goes through a barrier of its own: the others may be anything, and 0 * NaN is NaN, so they are
-          // made zeros before the tile is given on.
-          const int key0 = (t0 + l0 + q) << 7;
-          const bool part = !is_k && (key0 < lo || key0 + 128 > hi);
-          const uint32_t lands = part ? bar(F::kVPart) : full;
-          if (lane == 0) mbar_arrive_expect_tx(lands, __popc((boxes >> (8 * q)) & 0xffu) * (uint32_t)p.box * kD);
-          __syncwarp();
-          if ((lane >> 3) == q) {
-            if (heads) tma_load_4d(tile0 + st.at * F::kTile + 16 * gr * kD, tm, lands, 0, off, hk, page);
-            if (is_k) {
-              float* to = s_scale + slot * 16 + gr;
-              to[0] = sc.x;
-              to[8] = sc.y;
+            for (int q = q0; q < q1 + part; ++q) {
+              const uint32_t lands = q < q1 ? full0 + 8 * st.at : bar(F::kVPart);
+              if (!first) ok = mbar_wait_relaxed<256>(free0 + 8 * st.at, st.parity ^ 1u, wc, is_k ? kKFreeS : kVFreeS);
+              if (!ok) break;
+              last = st.at;
+              const uint32_t mine = (boxes >> (8 * q)) & 0xffu;
+              mbar_arrive_expect_tx(lands, __popc(mine) * (uint32_t)p.box * kD);
+              for (uint32_t m = mine; m != 0u; m &= m - 1u) {
+                const int i = __ffs(m) - 1;
+                const int2 from = s_box[8 * q + i];
+                tma_load_4d(tile0 + last * F::kTile + 16 * i * kD, tm, lands, 0, from.y, hk, from.x);
+              }
+              st.next();
+              if (st.at == 0) first = false;
             }
           }
-          if (is_k) {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(full);
-          }
-          if (part) {
-            ok = __all_sync(0xffffffffu, mbar_wait(lands, parts, wc, kVFullS));
-            if (!ok) break;
+          ok = __all_sync(0xffffffffu, ok);
+          if (part && ok) {
+            ok = __all_sync(0xffffffffu, mbar_wait(bar(F::kVPart), parts, wc, kVFullS));
             parts ^= 1u;
+            last = __shfl_sync(0xffffffffu, last, __ffs(__ballot_sync(0xffffffffu, lead)) - 1);
+            const int key0 = (t0 + l0 + q1) << 7;
             for (int r = lane; r < 128; r += 32)
               if (key0 + r < lo || key0 + r >= hi) {
-                uint4* v = reinterpret_cast<uint4*>(gbase + F::kOffV + st.at * F::kTile + r * kD);
+                uint4* v = reinterpret_cast<uint4*>(gbase + F::kOffV + last * F::kTile + r * kD);
 #pragma unroll
                 for (int i = 0; i < kD / 16; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
               }
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(full);
+            if (lane == 0) mbar_arrive(full0 + 8 * last);
           }
-          st.next();
-          if (st.at == 0) first = false;
-          if (++slot == F::kScales) slot = 0;
-          ++g;
+          q0 = q1 + part;
         }
+        if (!ok) break;
+        g += end;
+        slot += end;
+        if (slot >= F::kScales) slot -= F::kScales;
         at = at1; at1 = at2; sc = sc1;
       }
     }
@@ -391,7 +412,7 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       // bounded drain: let the copies on their way land before the CTA's memory is released
       const uint64_t begun = globaltimer_ns();
       for (int i = g > kStages ? g - kStages : 0; i < g; ++i)
-        while (!mbar_try_wait(bar(full0 + i % kStages), (i / kStages) & 1) && globaltimer_ns() - begun < 50ull * 1000 * 1000) {}
+        while (!mbar_try_wait(full0 + 8 * (i % kStages), (i / kStages) & 1) && globaltimer_ns() - begun < 50ull * 1000 * 1000) {}
     }
   } else if (warp == kIssueS) {
     // ============================================ Q . K^T ======================================
