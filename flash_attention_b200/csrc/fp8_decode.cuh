@@ -86,6 +86,143 @@ __device__ __forceinline__ void mma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint6
 }
 __device__ __forceinline__ void group_sync(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
 
+// A warp that loads the tiles of keys or of values, as far ahead as its ring of kStages places allows.
+//
+// Four tiles at a time: lane 8 q + g looks up keys 16 g .. 16 g + 15 of the q-th, their page two batches ahead and, in the loader of
+// K, the scales of their keys and values one batch ahead (a tile at a time, a CTA ran at a tile per memory latency).  What the copies need goes
+// through shared memory to one thread, which issues them (with all lanes in that loop a tile took 900 clocks).  Boxes that no row
+// sees are not loaded, their entries of the table not read.  The scales are written in front of the copies: the barrier of K's tile is
+// theirs too.
+struct FeederSites {
+  uint32_t free, lands;      // where a wait may run out
+};
+template <int kD, int kStages, int kScales>
+struct Feeder {
+  static constexpr uint32_t kTile = 128 * kD;
+  const CUtensorMap* tm;
+  uint32_t full0, free0, part;      // barriers: of the ring's places; of a tile of values that are not all seen (0: such tiles are no matter)
+  uint32_t tiles;                   // shared memory of the ring
+  uint8_t* ring;                    //   the same, for plain stores
+  float* scales;                    // kScales x (8 of K, 8 of V), or null
+  int2* box;                        // 32 places
+  float v_factor;                   // on the scales of values
+  FeederSites site;
+  Ring<kStages> st;                 // (of the issuing thread)
+  bool first = true;                // round of the ring
+  int g = 0, slot = 0;              // tiles so far; place of the next among the scales
+  uint32_t parts = 0u;
+
+  // Tiles t0 .. t0 + n - 1 of kv head hk of sequence b, in which keys [lo, hi) are seen.  False: a wait ran out.
+  __device__ __forceinline__ bool piece(const Fp8Params& p, const WaitCtx& wc, int n, int t0, int b, int hk, int lo, int hi) {
+    const int lane = threadIdx.x & 31, per_box = p.box >> 4, gr = lane & 7;
+    bool ok = true;
+    // (page, first key of these 16 in it) for the batch from tile `li` on; key -1: no row sees them
+    auto look_up = [&](int li) -> int2 {
+      int2 at = make_int2(0, -1);
+      const int mine = li + (lane >> 3), key = ((t0 + mine) << 7) + 16 * gr;
+      if (mine < n && key < hi && key + 16 > lo) {
+        const int pg = fast_div(key, p.div_page);
+        at = make_int2(p.table != nullptr ? p.table[(int64_t)b * p.pages_per_seq + pg] : b, key - pg * p.page_size);
+      }
+      return at;
+    };
+    auto scales_at = [&](int2 at) -> float2 {
+      if (scales == nullptr || at.y < 0 || at.x < 0 || at.x >= p.num_pages) return make_float2(0.f, 0.f);
+      const int64_t i = ((int64_t)at.x * (p.page_size >> p.log_block) + (at.y >> p.log_block)) * p.Hkv + hk;
+      return make_float2(p.k_scale[i], p.v_scale[i]);
+    };
+    int2 at = look_up(0), at1 = look_up(4);
+    float2 sc = scales_at(at);
+#pragma unroll 1
+    for (int l0 = 0; l0 < n; l0 += 4) {
+      // a box is loaded if any of its keys is seen; the keys in front of those have no page here: that of the box is the first one looked up
+      const uint32_t seen = __ballot_sync(0xffffffffu, at.y >= 0);
+      const uint32_t in_box = (seen >> lane) & ((1u << per_box) - 1u);
+      const bool heads = (gr & (per_box - 1)) == 0 && in_box != 0u;
+      const uint32_t boxes = __ballot_sync(0xffffffffu, heads);
+      const int src = heads ? lane + __ffs(in_box) - 1 : lane;
+      int page = __shfl_sync(0xffffffffu, at.x, src & 31);
+      const int off = __shfl_sync(0xffffffffu, at.y, src & 31) - 16 * (src - lane);
+      if (heads) {
+        if (page < 0 || page >= p.num_pages) {
+          report_bad_index(p.status, p.epoch, kPageSite);
+          page = p.num_pages;                       // (reads as zeros)
+        }
+        box[lane] = make_int2(page, off);
+      }
+      const int end = min(4, n - l0);
+      if (scales != nullptr && (lane >> 3) < end) {
+        // (the scales of the batch, as far ahead of the softmax as the ring of them allows)
+        int to = slot + (lane >> 3);
+        to = (to >= kScales ? to - kScales : to) * 16 + gr;
+        scales[to] = sc.x;
+        scales[to + 8] = sc.y * v_factor;
+      }
+      const int2 at2 = look_up(l0 + 8);
+      const float2 sc1 = scales_at(at1);
+      __syncwarp();
+      // A tile of values that are not all seen (the first and the last of a unit may be) goes through a barrier of its own: the others may be
+      // anything, and 0 * NaN is NaN, so they are made zeros before the tile is given on.
+      auto in_part = [&](int q) { const int key0 = (t0 + l0 + q) << 7; return part != 0u && (key0 < lo || key0 + 128 > hi); };
+      for (int q0 = 0; q0 < end && ok;) {
+        int q1 = q0;
+        while (q1 < end && !in_part(q1)) ++q1;
+        const bool is_part = q1 < end;
+        uint32_t last = 0u;                       // the last one's place
+        const bool lead = elect_one();            // (the same lane each time)
+        if (lead) {
+#pragma unroll 1
+          for (int q = q0; q < q1 + is_part; ++q) {
+            const uint32_t lands = q < q1 ? full0 + 8 * st.at : part;
+            if (!first) ok = mbar_wait_relaxed<256>(free0 + 8 * st.at, st.parity ^ 1u, wc, site.free);
+            if (!ok) break;
+            last = st.at;
+            const uint32_t mine = (boxes >> (8 * q)) & 0xffu;
+            mbar_arrive_expect_tx(lands, __popc(mine) * (uint32_t)p.box * kD);
+            for (uint32_t m = mine; m != 0u; m &= m - 1u) {
+              const int i = __ffs(m) - 1;
+              const int2 from = box[8 * q + i];
+              tma_load_4d(tiles + last * kTile + 16 * i * kD, tm, lands, 0, from.y, hk, from.x);
+            }
+            st.next();
+            if (st.at == 0) first = false;
+          }
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        if (is_part && ok) {
+          ok = __all_sync(0xffffffffu, mbar_wait(part, parts, wc, site.lands));
+          parts ^= 1u;
+          last = __shfl_sync(0xffffffffu, last, __ffs(__ballot_sync(0xffffffffu, lead)) - 1);
+          const int key0 = (t0 + l0 + q1) << 7;
+          for (int r = lane; r < 128; r += 32)
+            if (key0 + r < lo || key0 + r >= hi) {
+              uint4* v = reinterpret_cast<uint4*>(ring + last * kTile + r * kD);
+#pragma unroll
+              for (int i = 0; i < kD / 16; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
+            }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(full0 + 8 * last);
+        }
+        q0 = q1 + is_part;
+      }
+      if (!ok) return false;
+      g += end;
+      slot += end;
+      if (slot >= kScales) slot -= kScales;
+      at = at1; at1 = at2; sc = sc1;
+    }
+    return true;
+  }
+  // After a wait that ran out: let the copies on their way land, within limits, before the CTA's memory is released.
+  __device__ __forceinline__ void drain() const {
+    if ((threadIdx.x & 31) != 0) return;
+    const uint64_t begun = globaltimer_ns();
+    for (int i = g > kStages ? g - kStages : 0; i < g + 4; ++i)
+      while (!mbar_try_wait(full0 + 8 * (i % kStages), (i / kStages) & 1) && globaltimer_ns() - begun < 50ull * 1000 * 1000) {}
+  }
+};
+
 // kR: rows (16 or 32).
 template <int kD_, int kR_, bool kCap_>
 struct Form {
@@ -294,126 +431,21 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 
   if (warp == kLoadK || warp == kLoadV) {
     // ============================================ loaders ======================================
-    // Four tiles at a time: lane 8 q + g looks up keys 16 g .. 16 g + 15 of the q-th, their page two batches ahead and, in the loader of
-    // K, the scales of their keys and values one batch ahead (a tile at a time, a CTA ran at a tile per memory latency).  What the copies need goes
-    // through shared memory to one thread, which issues them (with all lanes in that loop a tile took 900 clocks).  Boxes that no row
-    // sees are not loaded, their entries of the table not read.
     const bool is_k = warp == kLoadK;
-    const CUtensorMap* tm = is_k ? &tm_k : &tm_v;
-    const uint32_t full0 = bar(is_k ? F::kKFull : F::kVFull), free0 = bar(is_k ? F::kKFree : F::kVFree);
-    const uint32_t tile0 = base + (is_k ? F::kOffK : F::kOffV);
-    float* s_scale = reinterpret_cast<float*>(gbase + F::kOffSc);
-    int2* s_box = reinterpret_cast<int2*>(gbase + F::kOffBox) + (is_k ? 0 : 32);
-    const int per_box = p.box >> 4, gr = lane & 7;
-    int g = 0, slot = 0;                    // tiles before the batch; its place among the scales
-    Ring<kStages> st;                       // (of the issuing thread)
-    bool first = true;                      // round of the ring
-    uint32_t parts = 0u;
-    for (; ok && walk.more(); walk.next(p)) {
-      const int n = walk.tiles(), t0 = walk.cur.first + walk.at, b = walk.b, hk = walk.hb * p.bundle + in_bundle, lo = walk.cur.lo, hi = walk.cur.hi;
-      // (page, first key of these 16 in it) for the batch from tile `li` on; key -1: no row sees them
-      auto look_up = [&](int li) -> int2 {
-        int2 at = make_int2(0, -1);
-        const int mine = li + (lane >> 3), key = ((t0 + mine) << 7) + 16 * gr;
-        if (mine < n && key < hi && key + 16 > lo) {
-          const int pg = fast_div(key, p.div_page);
-          at = make_int2(p.table != nullptr ? p.table[(int64_t)b * p.pages_per_seq + pg] : b, key - pg * p.page_size);
-        }
-        return at;
-      };
-      auto scales_at = [&](int2 at) -> float2 {
-        if (!is_k || at.y < 0 || at.x < 0 || at.x >= p.num_pages) return make_float2(0.f, 0.f);
-        const int64_t i = ((int64_t)at.x * (p.page_size >> p.log_block) + (at.y >> p.log_block)) * p.Hkv + hk;
-        return make_float2(p.k_scale[i], p.v_scale[i]);
-      };
-      int2 at = look_up(0), at1 = look_up(4);
-      float2 sc = scales_at(at);
-#pragma unroll 1
-      for (int l0 = 0; l0 < n; l0 += 4) {
-        // a box is loaded if any of its keys is seen; the keys in front of those have no page here: that of the box is the first one looked up
-        const uint32_t seen = __ballot_sync(0xffffffffu, at.y >= 0);
-        const uint32_t in_box = (seen >> lane) & ((1u << per_box) - 1u);
-        const bool heads = (gr & (per_box - 1)) == 0 && in_box != 0u;
-        const uint32_t boxes = __ballot_sync(0xffffffffu, heads);
-        const int src = heads ? lane + __ffs(in_box) - 1 : lane;
-        int page = __shfl_sync(0xffffffffu, at.x, src & 31);
-        const int off = __shfl_sync(0xffffffffu, at.y, src & 31) - 16 * (src - lane);
-        if (heads) {
-          if (page < 0 || page >= p.num_pages) {
-            report_bad_index(p.status, p.epoch, kPageSite);
-            page = p.num_pages;                       // (reads as zeros)
-          }
-          s_box[lane] = make_int2(page, off);
-        }
-        const int end = min(4, n - l0);
-        if (is_k && (lane >> 3) < end) {
-          // (the scales of the batch, as far ahead of the softmax as the ring of them allows)
-          int to = slot + (lane >> 3);
-          to = (to >= F::kScales ? to - F::kScales : to) * 16 + gr;
-          s_scale[to] = sc.x;
-          s_scale[to + 8] = sc.y;
-        }
-        const int2 at2 = look_up(l0 + 8);
-        const float2 sc1 = scales_at(at1);
-        __syncwarp();
-        // A tile of values that are not all seen (the first and the last of a unit may be) goes through a barrier of its own: the others may be
-        // anything, and 0 * NaN is NaN, so they are made zeros before the tile is given on.
-        auto in_part = [&](int q) { const int key0 = (t0 + l0 + q) << 7; return !is_k && (key0 < lo || key0 + 128 > hi); };
-        for (int q0 = 0; q0 < end && ok;) {
-          int q1 = q0;
-          while (q1 < end && !in_part(q1)) ++q1;
-          const bool part = q1 < end;
-          uint32_t last = 0u;                       // the last one's stage
-          const bool lead = elect_one();            // (the same lane each time)
-          if (lead) {
-#pragma unroll 1
-            for (int q = q0; q < q1 + part; ++q) {
-              const uint32_t lands = q < q1 ? full0 + 8 * st.at : bar(F::kVPart);
-              if (!first) ok = mbar_wait_relaxed<256>(free0 + 8 * st.at, st.parity ^ 1u, wc, is_k ? kKFreeS : kVFreeS);
-              if (!ok) break;
-              last = st.at;
-              const uint32_t mine = (boxes >> (8 * q)) & 0xffu;
-              mbar_arrive_expect_tx(lands, __popc(mine) * (uint32_t)p.box * kD);
-              for (uint32_t m = mine; m != 0u; m &= m - 1u) {
-                const int i = __ffs(m) - 1;
-                const int2 from = s_box[8 * q + i];
-                tma_load_4d(tile0 + last * F::kTile + 16 * i * kD, tm, lands, 0, from.y, hk, from.x);
-              }
-              st.next();
-              if (st.at == 0) first = false;
-            }
-          }
-          ok = __all_sync(0xffffffffu, ok);
-          if (part && ok) {
-            ok = __all_sync(0xffffffffu, mbar_wait(bar(F::kVPart), parts, wc, kVFullS));
-            parts ^= 1u;
-            last = __shfl_sync(0xffffffffu, last, __ffs(__ballot_sync(0xffffffffu, lead)) - 1);
-            const int key0 = (t0 + l0 + q1) << 7;
-            for (int r = lane; r < 128; r += 32)
-              if (key0 + r < lo || key0 + r >= hi) {
-                uint4* v = reinterpret_cast<uint4*>(gbase + F::kOffV + last * F::kTile + r * kD);
-#pragma unroll
-                for (int i = 0; i < kD / 16; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
-              }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(full0 + 8 * last);
-          }
-          q0 = q1 + part;
-        }
-        if (!ok) break;
-        g += end;
-        slot += end;
-        if (slot >= F::kScales) slot -= F::kScales;
-        at = at1; at1 = at2; sc = sc1;
-      }
-    }
-    if (!ok && lane == 0) {
-      // bounded drain: let the copies on their way land before the CTA's memory is released
-      const uint64_t begun = globaltimer_ns();
-      for (int i = g > kStages ? g - kStages : 0; i < g; ++i)
-        while (!mbar_try_wait(full0 + 8 * (i % kStages), (i / kStages) & 1) && globaltimer_ns() - begun < 50ull * 1000 * 1000) {}
-    }
+    Feeder<kD, kStages, F::kScales> feed;
+    feed.tm = is_k ? &tm_k : &tm_v;
+    feed.full0 = bar(is_k ? F::kKFull : F::kVFull);
+    feed.free0 = bar(is_k ? F::kKFree : F::kVFree);
+    feed.part = is_k ? 0u : bar(F::kVPart);
+    feed.tiles = base + (is_k ? F::kOffK : F::kOffV);
+    feed.ring = gbase + (is_k ? F::kOffK : F::kOffV);
+    feed.scales = is_k ? reinterpret_cast<float*>(gbase + F::kOffSc) : nullptr;
+    feed.box = reinterpret_cast<int2*>(gbase + F::kOffBox) + (is_k ? 0 : 32);
+    feed.v_factor = 1.f;
+    feed.site = is_k ? FeederSites{kKFreeS, kKFullS} : FeederSites{kVFreeS, kVFullS};
+    for (; ok && walk.more(); walk.next(p))
+      ok = feed.piece(p, wc, walk.tiles(), walk.cur.first + walk.at, walk.b, walk.hb * p.bundle + in_bundle, walk.cur.lo, walk.cur.hi);
+    if (!ok) feed.drain();
   } else if (warp == kIssueS) {
     // ============================================ Q . K^T ======================================
     // (An issuing thread gets an instruction every eight clocks or so, its code never stays in the scheduler's cache beside the softmax
