@@ -1,63 +1,61 @@
 // Attention over the 8-bit KV cache for many query rows (pieces of prompts).
 //
-// With a tile of query rows the products are bound by the tensor cores, so keys and values are turned into fp16 once for 256 rows
-// (two tiles of 128 rows, of all query heads of a kv head: row r = token r / group, head r % group) and everything runs as
-// kind::f16 products, in which an e4m3 value, a bf16 query (times a power of two) and their products are exact.
+//   S (128 rows x 128 keys) = Q . K^T  in e4m3: the keys as they are loaded, a bf16 query as two e4m3 rows (see the decode kernel)
+//   O (128 rows x D) += W . V          in fp16: values widened to fp16 (exact), weights from tensor memory
 //
-//   S (128 rows x 128 keys) = Q . K^T,    O (128 rows x D) += W . V,    W = 2^(t - m) vs / vs_max * 2^6 as fp16, from tensor memory
+// W = 2^(t - m) vs / vs_max * 2^6 with t the score in log2 units, m a row's reference, which follows the maximum when it falls behind by
+// more than 8 (then O is multiplied), and vs / vs_max the scale of a block of values over the largest that this CTA meets: a weight is below
+// 2^16 and has its eleven bits down to 2^-20 of that.  Two e4m3 rows would not do here: O stays in tensor memory, so the reference is one of all
+// keys so far, and what lies 2^13 below it would lose its bits.  The row sum takes the weight without vs, in fp32.
 //
-// t is the score in log2 units, m a row's reference, which follows the maximum when it falls behind by more than 8 (then O
-// is multiplied); vs / vs_max the scale of a block of values over the largest that this CTA meets, so a weight is below 2^16
-// and has its eleven bits down to 2^-20 of that; the row sum takes the weight without vs, in fp32.
+// A CTA has two tiles of 128 rows (row r = token r / group, head r % group of a kv head), a softmax warpgroup each (thread = row).  S of a
+// tile is two halves of 64 columns.  A softmax warpgroup takes the upper half (keys 64-127) to registers first, and Q K^T of the next step's upper half
+// may overwrite it at once; W goes where the lower half was, then W V and Q K^T of the next lower half follow it.  So the softmax, which
+// is what bounds the kernel (the exponentials of 256 rows x 128 keys take 2048 clocks, the products 2048 beside them), finds its next
+// scores waiting.  With one product of 128 columns the softmax waited 1500 of 4000 clocks for W V and Q K^T: B = 1, 1024 rows of 32 heads
+// on 16384 keys 294 us.
 //
-// Warps: 0-3 and 4-7 the softmax of a tile each (thread = row), 8-11 turn K and V tiles into fp16 (cvt.f16x2.e4m3x2 runs at 64 a clock and
-// beside the exponentials: a step of 128 keys takes 256 clocks of it, the exponentials of 256 rows 2048), 12 and 14 load,
-// 13 issues the products: W V of a step and Q K^T of the next one for one tile while the other tile's softmax runs.  Tensor memory: S 2 x 128
-// columns, in whose place W is written, O 2 x D.  Every wait is bounded (those of the softmax warps, which
-// leave no registers for a call, by the issuer's: see mbar_wait_flag); a warp whose wait ran out goes on without waiting.
+// Warps: 0-3 and 4-7 softmax, 8-11 widen the tiles of V (cvt.f16x2.e4m3x2 runs at 64 a clock beside the exponentials), 12 and 14 load, 13 issues
+// the products.  Every wait is bounded (those of the softmax warps, which leave no registers for a call, by the issuer's: see mbar_wait_flag); a warp
+// whose wait ran out goes on without waiting.
 #pragma once
 #include "fp8_decode.cuh"
 
 namespace fa4 {
 namespace fp8p {
 
-enum Site { kRawFullS = 140, kRawFreeS, kHalfFullS, kHalfFreeS, kSFullS, kPFullS, kODoneS, kQReadyS };
+enum Site { kKFullS = 140, kKFreeS, kRawFullS, kRawFreeS, kHalfFullS, kHalfFreeS, kUFreeS, kPFullS, kODoneS, kQReadyS };
 
 // Registers: 512 threads launch with 128; the softmax takes what the others give back.
 constexpr int kThreads = 512, kRegsLaunch = 128, kRegsSoftmax = 192, kRegsConvert = 64, kRegsService = 64;
 static_assert(2 * kRegsSoftmax + kRegsConvert + kRegsService <= 4 * kRegsLaunch, "register budget of the 8-bit prefill kernel");
+constexpr uint32_t kHalf = 128 * 128;                                // 128 rows x 64 fp16
 
 template <int kD>
 struct Layout {
-  static constexpr uint32_t kHalf = 128 * 128;                       // 128 rows x 64 fp16
+  static constexpr int kStagesK = 3, kStagesV = 2;                   // tiles of bytes
+  // (Q K^T of step i is done before its place is loaded anew; the softmax is at step i - 1 then, and a batch of scales four ahead)
+  static constexpr int kScales = kStagesK + 6;
   static constexpr uint32_t kTile16 = kHalf * (kD / 64), kTile8 = 128 * kD;
-  static constexpr uint32_t kOffQ = 0, kOffK = 2 * kTile16, kOffV = kOffK + 2 * kTile16, kOffRawK = kOffV + 2 * kTile16,
-                            kOffRawV = kOffRawK + kTile8, kOffSc = kOffRawV + kTile8,   // scales of 16 keys: 4 steps x (8 of K, 8 of V)
-      kOffBar = kOffSc + 4 * 64;
-  static constexpr uint32_t kRawKFull = 0, kRawKFree = 1, kRawVFull = 2, kRawVFree = 3, kKFull = 4 /* 2 */, kKFree = 6, kVFull = 8,
-                            kVFree = 10, kSFull = 12, kPFull = 14, kODone = 16, kQReady = 17, kDrain = 18, kBars = 19;
+  static constexpr uint32_t kOffQ = 0 /* 2 tiles x (q1, q2) */, kOffK = 4 * kTile8, kOffRawV = kOffK + kStagesK * kTile8,
+                            kOffV = kOffRawV + kStagesV * kTile8, kOffSc = kOffV + 2 * kTile16, kOffBox = kOffSc + kScales * 64,
+                            kOffBar = kOffBox + 512;
+  static constexpr uint32_t kKFull = 0, kKFree = kKFull + kStagesK, kRawFull = kKFree + kStagesK, kRawFree = kRawFull + kStagesV,
+                            kVFull = kRawFree + kStagesV, kVFree = kVFull + 2, kUFull = kVFree + 2, kLFull = kUFull + 2, kUFree = kLFull + 2,
+                            kPFull = kUFree + 2, kPvDone = kPFull + 2, kODone = kPvDone + 2, kQReady = kODone + 1, kDrain = kQReady + 1,
+                            kBars = kDrain + 1;
   static constexpr uint32_t kOffMisc = (kOffBar + 8 * kBars + 15) / 16 * 16;
   static constexpr uint32_t kRequest = kOffMisc + 32 + sizeof(WaitCtx) + 1024;
   static_assert(kRequest <= 227 * 1024, "shared memory of the 8-bit prefill kernel");
 };
 constexpr uint32_t kColS = 0, kColO = 256;
 
-// K-major rows of 64 fp16 (128 bytes, 128-byte swizzle, groups of eight rows 1024 bytes apart).  Read MN-major the same groups
-// are eight steps of the contraction, and the next 64 of the other side lie 16 KB on.
-__device__ __forceinline__ uint64_t half_desc(uint32_t saddr) { return make_smem_desc(saddr, 128 * 128, 1024, kSwizzle128); }
+// A widened tile: halves of 64 columns, rows of 128 bytes (128-byte swizzle, groups of eight rows 1024 bytes apart).  Read MN-major the groups
+// are eight steps of the contraction, and the next 64 columns lie a half on.
+__device__ __forceinline__ uint64_t half_desc(uint32_t saddr) { return make_smem_desc(saddr, kHalf, 1024, kSwizzle128); }
 // Instruction descriptor of kind::f16, fp16 x fp16, fp32 accumulator.
 __host__ __device__ constexpr uint32_t make_idesc_f16(uint32_t m, uint32_t n, bool b_mn_major) {
   return (1u << 4) | (b_mn_major ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((m >> 4) << 24);
-}
-__device__ __forceinline__ void mma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n"
-      ".reg .pred p;\n"
-      "setp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
-      "}\n"
-      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-      : "memory");
 }
 __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -118,6 +116,8 @@ __global__ void __launch_bounds__(fp8p::kThreads, 1)
 fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                    const __grid_constant__ Fp8Params p) {
   using namespace fp8p;
+  using fp8d::desc_at;
+  using fp8d::Ring;
   using L = Layout<kD>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -149,17 +149,22 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     *s_abort = 0u;
     *s_top = 0u;
     wc = WaitCtx{s_abort, p.status, p.budget_ns, p.epoch};
-    mbar_init(bar(L::kRawKFull), 2);         // the copies' bytes, and the scales
-    mbar_init(bar(L::kRawVFull), 1);
-    mbar_init(bar(L::kRawKFree), 4);
-    mbar_init(bar(L::kRawVFree), 4);
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(bar(L::kKFull + s), 4);
-      mbar_init(bar(L::kVFull + s), 4);
+    for (int s = 0; s < L::kStagesK; ++s) {
+      mbar_init(bar(L::kKFull + s), 1);
       mbar_init(bar(L::kKFree + s), 1);
+    }
+    for (int s = 0; s < L::kStagesV; ++s) {
+      mbar_init(bar(L::kRawFull + s), 1);
+      mbar_init(bar(L::kRawFree + s), 4);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(bar(L::kVFull + s), 4);
       mbar_init(bar(L::kVFree + s), 1);
-      mbar_init(bar(L::kSFull + s), 1);
+      mbar_init(bar(L::kUFull + s), 1);
+      mbar_init(bar(L::kLFull + s), 1);
+      mbar_init(bar(L::kUFree + s), 4);
       mbar_init(bar(L::kPFull + s), 4);
+      mbar_init(bar(L::kPvDone + s), 1);
     }
     mbar_init(bar(L::kODone), 1);
     mbar_init(bar(L::kQReady), 8);
@@ -199,108 +204,91 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
 
   if (warp >= 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsService));
-    if (warp == 12 || warp == 14) {
-      // ============================================ loaders ======================================
-      // (as in the decode kernel: lane g and g + 8 have keys 16 g .. 16 g + 15 of a step)
-      const bool is_k = warp == 12;
-      const CUtensorMap* tm = is_k ? &tm_k : &tm_v;
-      const float* scales = lane < 8 ? p.k_scale : p.v_scale;
-      const uint32_t full = bar(is_k ? L::kRawKFull : L::kRawVFull), free = bar(is_k ? L::kRawKFree : L::kRawVFree);
-      const uint32_t tile = base + (is_k ? L::kOffRawK : L::kOffRawV);
-      float* s_scale = reinterpret_cast<float*>(gbase + L::kOffSc);
-      auto key_of = [&](int i) { return ((t0 + i) << 7) + 16 * (lane & 7); };
-      auto live = [&](int i) { return lane < 16 && i < n && key_of(i) < hi_all && key_of(i) + 16 > lo_all; };
-      auto look_up = [&](int i) -> int2 {
-        int2 at = make_int2(-1, 0);
-        if (live(i)) {
-          const int key = key_of(i), pg = fast_div(key, p.div_page);
-          at = make_int2(p.table != nullptr ? p.table[(int64_t)b * p.pages_per_seq + pg] : b, key - pg * p.page_size);
-        }
-        return at;
-      };
-      auto scale_at = [&](int2 at) -> float {
-        return is_k && at.x >= 0 && at.x < p.num_pages
-                   ? scales[((int64_t)at.x * (p.page_size >> p.log_block) + (at.y >> p.log_block)) * p.Hkv + hk] * (lane < 8 ? 1.f : vs_up) : 0.f;
-      };
-      int2 at = look_up(0), at1 = look_up(1);
-      float sc = scale_at(at);
-      int i = 0;
-      for (; i < n; ++i) {
-        const int2 at2 = look_up(i + 2);
-        const float sc1 = scale_at(at1);
-        if (i > 0 && ok) ok = mbar_wait_relaxed<512>(free, (i - 1) & 1, wc, kRawFreeS);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        const uint32_t seen = __ballot_sync(0xffffffffu, live(i)) & 0xffu;
-        const int per_box = p.box >> 4;
-        const uint32_t in_box = (seen >> lane) & ((1u << per_box) - 1u);
-        const bool mine = lane < 8 && (lane & (per_box - 1)) == 0 && in_box != 0u;
-        const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, mine));
-        if (lane == 0) mbar_arrive_expect_tx(full, boxes * (uint32_t)p.box * kD);
-        __syncwarp();
-        const int src = mine ? lane + __ffs(in_box) - 1 : lane;
-        const int page = __shfl_sync(0xffffffffu, at.x, src & 31), off = __shfl_sync(0xffffffffu, at.y, src & 31) - 16 * (src - lane);
-        if (mine) {
-          const bool fine = page >= 0 && page < p.num_pages;
-          if (!fine) report_bad_index(p.status, p.epoch, kPageSite);
-          tma_load_4d(tile + 16 * lane * kD, tm, full, 0, off, hk, fine ? page : p.num_pages);
-        }
-        if (is_k) {
-          // (Q K^T of step i - 2 is done before this step is converted, and so the softmax of step i - 3: four slots are enough)
-          if (lane < 16) s_scale[(i & 3) * 16 + lane] = sc;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(full);
-        }
-        at = at1; at1 = at2; sc = sc1;
-      }
-      if (!ok && i > 0 && lane == 0) {
-        const uint64_t begun = globaltimer_ns();
-        while (!mbar_try_wait(full, (i - 1) & 1) && globaltimer_ns() - begun < 50ull * 1000 * 1000) {}
-      }
+    if (warp == 12) {
+      fp8d::Feeder<kD, L::kStagesK, L::kScales> feed;
+      feed.tm = &tm_k;
+      feed.full0 = bar(L::kKFull);
+      feed.free0 = bar(L::kKFree);
+      feed.part = 0u;
+      feed.tiles = base + L::kOffK;
+      feed.ring = gbase + L::kOffK;
+      feed.scales = reinterpret_cast<float*>(gbase + L::kOffSc);
+      feed.box = reinterpret_cast<int2*>(gbase + L::kOffBox);
+      feed.v_factor = vs_up;
+      feed.site = {kKFreeS, kKFullS};
+      if (!feed.piece(p, wc, n, t0, b, hk, lo_all, hi_all)) feed.drain();
+    } else if (warp == 14) {
+      fp8d::Feeder<kD, L::kStagesV, L::kScales> feed;
+      feed.tm = &tm_v;
+      feed.full0 = bar(L::kRawFull);
+      feed.free0 = bar(L::kRawFree);
+      feed.part = 0u;
+      feed.tiles = base + L::kOffRawV;
+      feed.ring = gbase + L::kOffRawV;
+      feed.scales = nullptr;
+      feed.box = reinterpret_cast<int2*>(gbase + L::kOffBox) + 32;
+      feed.v_factor = 1.f;
+      feed.site = {kRawFreeS, kRawFullS};
+      if (!feed.piece(p, wc, n, t0, b, hk, lo_all, hi_all)) feed.drain();
     } else if (warp == 13) {
       // ============================================ products =====================================
+      // (Products run in the order they are issued: Q K^T of a tile's next lower half overwrites the weights that W V in front of it reads.
+      // Descriptors are moved, not made anew: see the issuers of the decode kernel.)
       if (elect_one() && n > 0) {
-        constexpr uint32_t idesc_s = make_idesc_f16(128, 128, false), idesc_o = make_idesc_f16(128, kD, true);
-        // (products run in the order they are issued: Q K^T of a tile's next step may overwrite the weights that W V in front of it reads)
-        // (descriptors are moved, not made anew: see the issuers of the decode kernel)
-        using fp8d::desc_at;
-        const uint64_t dq = half_desc(base + L::kOffQ), dk = half_desc(base + L::kOffK), dv = half_desc(base + L::kOffV);
-        auto score = [&](uint32_t t, uint32_t buf) {
-          const uint64_t qt = desc_at(dq, t * L::kTile16), kt = desc_at(dk, buf * L::kTile16);
-          const uint32_t to = tmem + kColS + 128 * t;
+        constexpr uint32_t idesc_s = fp8d::make_idesc_e4m3(128, 64, false), idesc_o = make_idesc_f16(128, kD, true);
+        const uint64_t dq = fp8d::tile_desc<kD>(base + L::kOffQ), dk = fp8d::tile_desc<kD>(base + L::kOffK), dv = half_desc(base + L::kOffV);
+        // scores of tile t, upper or lower keys of the K tile at place `at`
+        auto score = [&](uint32_t t, uint32_t at, bool upper) {
+          const uint64_t qt = desc_at(dq, 2 * t * L::kTile8), kt = desc_at(dk, at * L::kTile8 + (upper ? 64 * kD : 0));
+          const uint32_t to = tmem + kColS + 128 * t + (upper ? 64 : 0);
 #pragma unroll
-          for (int ks = 0; ks < kD / 16; ++ks) {
-            const uint32_t at = (ks >> 2) * L::kHalf + (ks & 3) * 32;
-            mma_f16_ss(to, desc_at(qt, at), desc_at(kt, at), idesc_s, ks > 0);
-          }
-          tc_commit(bar(L::kSFull + t));
+          for (int ks = 0; ks < kD / 16; ++ks)
+            fp8d::mma_e4m3(to, desc_at(qt, ks / (kD / 32) * L::kTile8 + 32 * (ks % (kD / 32))), desc_at(kt, 32 * (ks % (kD / 32))), idesc_s, ks > 0);
+          tc_commit(bar((upper ? L::kUFull : L::kLFull) + t));
         };
-        ok = mbar_wait(bar(L::kQReady), 0, wc, kQReadyS) && mbar_wait(bar(L::kKFull), 0, wc, kHalfFullS);
+        Ring<L::kStagesK> kk;
+        ok = mbar_wait(bar(L::kQReady), 0, wc, kQReadyS) && mbar_wait(bar(L::kKFull), 0, wc, kKFullS);
         if (ok) {
           tc_fence_after_sync();
-          for (int t = 0; t < tiles; ++t) score(t, 0);
+          for (int t = 0; t < tiles; ++t) score(t, 0, true);
+          for (int t = 0; t < tiles; ++t) score(t, 0, false);
           tc_commit(bar(L::kKFree));
+          kk.next();
         }
-        uint32_t buf = 0, parity = 0;          // of step i
+        uint32_t buf = 0, parity = 0;          // of V of step i
 #pragma unroll 1
         for (int i = 0; ok && i < n; ++i) {
           const bool more = i + 1 < n;
-          ok = mbar_wait(bar(L::kVFull + buf), parity, wc, kHalfFullS);
-          if (ok && more) ok = mbar_wait(bar(L::kKFull + (buf ^ 1u)), parity ^ buf, wc, kHalfFullS);
+          if (more) {
+            ok = mbar_wait(bar(L::kKFull + kk.at), kk.parity, wc, kKFullS);
+#pragma unroll 1
+            for (int t = 0; ok && t < tiles; ++t) {
+              ok = mbar_wait(bar(L::kUFree + t), i & 1, wc, kUFreeS);
+              if (!ok) break;
+              tc_fence_after_sync();
+              score(t, kk.at, true);
+            }
+          }
+          if (ok) ok = mbar_wait(bar(L::kVFull + buf), parity, wc, kHalfFullS);
           const uint64_t vt = desc_at(dv, buf * L::kTile16);
 #pragma unroll 1
           for (int t = 0; ok && t < tiles; ++t) {
             ok = mbar_wait(bar(L::kPFull + t), i & 1, wc, kPFullS);
             if (!ok) break;
             tc_fence_after_sync();
-            const uint32_t to = tmem + kColO + kD * t, w = tmem + kColS + 128 * t;
+            const uint32_t to = tmem + kColO + kD * t, from = tmem + kColS + 128 * t;
+            // (the weights of the upper keys come first)
 #pragma unroll
-            for (int ks = 0; ks < 8; ++ks) mma_f16_ts(to, w + 8 * ks, desc_at(vt, 2048 * ks), idesc_o, i > 0 || ks > 0);
-            if (more) score(t, buf ^ 1u);
+            for (int ks = 0; ks < 8; ++ks) mma_f16_ts(to, from + 8 * ks, desc_at(vt, 2048 * (ks ^ 4)), idesc_o, i > 0 || ks > 0);
+            tc_commit(bar(L::kPvDone + t));
+            if (more) score(t, kk.at, false);
           }
           if (ok) {
             tc_commit(bar(L::kVFree + buf));
-            if (more) tc_commit(bar(L::kKFree + (buf ^ 1u)));
+            if (more) {
+              tc_commit(bar(L::kKFree + kk.at));
+              kk.next();
+            }
           }
           parity ^= buf;
           buf ^= 1u;
@@ -317,26 +305,26 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       }
     }
   } else if (warp >= 8) {
-    // ============================================ e4m3 -> fp16 ===================================
+    // ============================================ V: e4m3 -> fp16 ================================
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsConvert));
+    Ring<L::kStagesV> raw;
+    Ring<2> to;
+#pragma unroll 1
     for (int i = 0; i < n; ++i) {
       const int key0 = (t0 + i) << 7;
-#pragma unroll
-      for (int v = 0; v < 2; ++v) {
-        const uint32_t full = bar(v ? L::kVFull : L::kKFull) + 8 * (i & 1);
-        if (ok) ok = mbar_wait(bar(v ? L::kRawVFull : L::kRawKFull), i & 1, wc, kRawFullS);
-        if (ok && i >= 2) ok = mbar_wait(bar(v ? L::kVFree : L::kKFree) + 8 * (i & 1), ((i >> 1) - 1) & 1, wc, kHalfFreeS);
-        ok = __all_sync(0xffffffffu, ok);
-        // (values that no row sees may be anything, and 0 * NaN is NaN)
-        widen_tile<kD>(gbase + (v ? L::kOffRawV : L::kOffRawK), gbase + (v ? L::kOffV : L::kOffK) + (i & 1) * L::kTile16, warp - 8, lane,
-                       v ? lo_all - key0 : 0, v ? hi_all - key0 : 128);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(bar(v ? L::kRawVFree : L::kRawKFree));
-          mbar_arrive(full);
-        }
+      if (ok) ok = mbar_wait(bar(L::kRawFull + raw.at), raw.parity, wc, kRawFullS);
+      if (ok && i >= 2) ok = mbar_wait(bar(L::kVFree + to.at), to.parity ^ 1u, wc, kHalfFreeS);
+      ok = __all_sync(0xffffffffu, ok);
+      // (values that no row sees may be anything, and 0 * NaN is NaN)
+      widen_tile<kD>(gbase + L::kOffRawV + raw.at * L::kTile8, gbase + L::kOffV + to.at * L::kTile16, warp - 8, lane, lo_all - key0, hi_all - key0);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(bar(L::kRawFree + raw.at));
+        mbar_arrive(bar(L::kVFull + to.at));
       }
+      raw.next();
+      to.next();
     }
   } else {
     // ============================================ softmax ======================================
@@ -345,13 +333,13 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tm_s = tmem + lanes + kColS + 128 * tile, tm_o = tmem + lanes + kColO + kD * tile;
     const int s = fast_div(r_first + row, p.div_group), h = hk * p.group + r_first + row - s * p.group;
-    // ---- Q: the thread's row, times the power of two that brings its largest element to 128 .. 256
+    // ---- Q: the thread's row as two e4m3 rows, times the power of two that brings its largest element to 128 .. 256
     float factor = 0.f;
     {
-      uint8_t* qt = gbase + L::kOffQ + tile * L::kTile16;
+      uint8_t* qt = gbase + L::kOffQ + 2 * tile * L::kTile8;
+      const __nv_bfloat16* src = p.q + b * p.q_b + (int64_t)s * p.q_s + h * p.q_h;
       uint4 u[kD / 8];
       uint32_t top = 0u;
-      const __nv_bfloat16* src = p.q + b * p.q_b + (int64_t)s * p.q_s + h * p.q_h;
 #pragma unroll
       for (int c = 0; c < kD / 8; ++c) u[c] = row < R ? *reinterpret_cast<const uint4*>(src + 8 * c) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
@@ -362,15 +350,27 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       }
       const int e = max((int)(top >> 23), 17);
       const float up = __uint_as_float((uint32_t)(254 + 7 - e) << 23), down = __uint_as_float((uint32_t)(e - 7) << 23);
+      const bool fine = top < 0x7f800000u;                   // (a row that is not finite becomes NaN whole)
       factor = (kCap ? p.cap_in : p.sl2) * down;
 #pragma unroll
-      for (int c = 0; c < kD / 8; ++c) {
-        float x[8];
-        unpack8(u[c], x);
-        uint4 o = make_uint4(pack_f16x2(x[0] * up, x[1] * up), pack_f16x2(x[2] * up, x[3] * up), pack_f16x2(x[4] * up, x[5] * up),
-                             pack_f16x2(x[6] * up, x[7] * up));
-        if (top >= 0x7f800000u) o = make_uint4(0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u);   // (not finite: NaN whole)
-        *reinterpret_cast<uint4*>(qt + (c >> 3) * L::kHalf + fp8d::sw128_offset(t, c & 7)) = o;
+      for (int c = 0; c < kD / 16; ++c) {
+        uint32_t q1[4], q2[4];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float x[8], y[8];
+          unpack8(u[2 * c + k], x);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] *= up;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            q1[2 * k + i] = fine ? pack4_e4m3(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]) : 0x7f7f7f7fu;
+            unpack4_e4m3(q1[2 * k + i], y + 4 * i);
+            q2[2 * k + i] = pack4_e4m3(x[4 * i] - y[4 * i], x[4 * i + 1] - y[4 * i + 1], x[4 * i + 2] - y[4 * i + 2], x[4 * i + 3] - y[4 * i + 3]);
+          }
+        }
+        uint8_t* to = qt + fp8d::row_piece<kD>(t, c);
+        *reinterpret_cast<uint4*>(to) = make_uint4(q1[0], q1[1], q1[2], q1[3]);
+        *reinterpret_cast<uint4*>(to + L::kTile8) = make_uint4(q2[0], q2[1], q2[2], q2[3]);
       }
       fence_proxy_async_smem();
       __syncwarp();
@@ -385,78 +385,107 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     float m_ref = -INFINITY;
     float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
     if (tile < tiles) {
-      for (int i = 0; i < n; ++i) {
-        if (ok) ok = mbar_wait_flag(bar(L::kSFull + tile), i & 1, s_abort);
-        ok = __all_sync(0xffffffffu, ok);
-        tc_fence_after_sync();
-        float x[128];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(tm_s + 32 * c, reinterpret_cast<uint32_t*>(x + 32 * c));
-        tc_wait_ld();
-        const float4* sc4 = reinterpret_cast<const float4*>(gbase + L::kOffSc + (i & 3) * 64);
-        const float4 ka = sc4[0], kb = sc4[1];
-        const float ks[8] = {ka.x, ka.y, ka.z, ka.w, kb.x, kb.y, kb.z, kb.w};
-#pragma unroll
-        for (int g = 0; g < 8; ++g) {
-          const float2 f = make_float2(ks[g] * factor, ks[g] * factor);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            float2 y = __fmul2_rn(make_float2(x[16 * g + 2 * j], x[16 * g + 2 * j + 1]), f);
-            if constexpr (kCap) y = make_float2(p.cap_out * tanh_of(y.x), p.cap_out * tanh_of(y.y));
-            x[16 * g + 2 * j] = y.x;
-            x[16 * g + 2 * j + 1] = y.y;
-          }
-        }
-        const int lo_in = lo - ((t0 + i) << 7), hi_in = hi - ((t0 + i) << 7);
-        if (__any_sync(0xffffffffu, lo_in > 0 || hi_in < 128)) {
-#pragma unroll
-          for (int j = 0; j < 128; ++j) x[j] = j >= lo_in && j < hi_in ? x[j] : -INFINITY;
-        }
-        float top = fmaxf(x[0], x[1]);
-#pragma unroll
-        for (int j = 2; j < 128; j += 2) top = fmax3(top, x[j], x[j + 1]);
-        // the reference follows when the row's weights would pass 2^8
-        float fac = 1.f;
-        const bool moved = top > m_ref + 8.f;
-        if (moved) {
-          fac = ex2_approx(m_ref - top);
-          m_ref = top;
-          l2[0].x *= fac; l2[0].y *= fac; l2[1].x *= fac; l2[1].y *= fac;
-        }
-        if (i > 0 && __any_sync(0xffffffffu, moved)) {
-          // (the scores of this step are behind W V of the last one)
+      int slot = 0;
 #pragma unroll 1
-          for (int c = 0; c < kD / 16; ++c) {
-            float o[16];
-            dec::tmem_ld16(tm_o + 16 * c, reinterpret_cast<uint32_t*>(o));
-            tc_wait_ld();
+      for (int i = 0; i < n; ++i) {
+        const float* sc = reinterpret_cast<const float*>(gbase + L::kOffSc) + slot * 16;
+        if (++slot == L::kScales) slot = 0;
+        uint32_t wu[32];
+        // 64 scores to weights (two to a word); `upper`: keys 64-127 of the step
+        auto weights = [&](float (&x)[64], const bool upper, uint32_t (&pw)[32]) {
+          const float4 ks = *reinterpret_cast<const float4*>(sc + (upper ? 4 : 0));
+          const float kf[4] = {ks.x * factor, ks.y * factor, ks.z * factor, ks.w * factor};
 #pragma unroll
-            for (int j = 0; j < 16; ++j) o[j] *= fac;
-            dec::tmem_st16(tm_o + 16 * c, reinterpret_cast<const uint32_t*>(o));
+          for (int j = 0; j < 32; ++j) {
+            float2 y = __fmul2_rn(make_float2(x[2 * j], x[2 * j + 1]), make_float2(kf[j >> 3], kf[j >> 3]));
+            if constexpr (kCap) y = make_float2(p.cap_out * tanh_of(y.x), p.cap_out * tanh_of(y.y));
+            x[2 * j] = y.x;
+            x[2 * j + 1] = y.y;
           }
-        }
-        const float ref = m_ref == -INFINITY ? 0.f : -m_ref;
-        const float2 ref2 = make_float2(ref, ref);
-        const float4 va = sc4[2], vb = sc4[3];
-        const float vs[8] = {va.x, va.y, va.z, va.w, vb.x, vb.y, vb.z, vb.w};
+          const int key0 = ((t0 + i) << 7) + (upper ? 64 : 0), lo_in = lo - key0, hi_in = hi - key0;
+          if (__any_sync(0xffffffffu, lo_in > 0 || hi_in < 64)) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t pw[16];
+            for (int j = 0; j < 64; ++j) x[j] = j >= lo_in && j < hi_in ? x[j] : -INFINITY;
+          }
+          float top = fmaxf(x[0], x[1]);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const int k = 32 * c + 2 * j;
-            const float2 y = __fadd2_rn(make_float2(x[k], x[k + 1]), ref2);
+          for (int j = 2; j < 64; j += 2) top = fmax3(top, x[j], x[j + 1]);
+          // the reference follows when the row's weights would pass 2^8
+          const bool moved = top > m_ref + 8.f;
+          if (__any_sync(0xffffffffu, moved)) {
+            const float fac = moved ? ex2_approx(m_ref - top) : 1.f;
+            if (moved) m_ref = top;
+            l2[0].x *= fac; l2[0].y *= fac; l2[1].x *= fac; l2[1].y *= fac;
+            if (i > 0) {
+              // O, and in the upper half: behind W V of the step before (whose lower scores were behind that of the one before)
+              if (upper) {
+                if (ok) ok = mbar_wait_flag(bar(L::kPvDone + tile), (i - 1) & 1, s_abort);
+                ok = __all_sync(0xffffffffu, ok);
+                tc_fence_after_sync();
+              }
+#pragma unroll 1
+              for (int c = 0; c < kD / 16; ++c) {
+                float o[16];
+                dec::tmem_ld16(tm_o + 16 * c, reinterpret_cast<uint32_t*>(o));
+                tc_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) o[j] *= fac;
+                dec::tmem_st16(tm_o + 16 * c, reinterpret_cast<const uint32_t*>(o));
+              }
+            }
+            if (!upper && fac != 1.f) {
+              // the weights of the upper half were made under the old reference
+              const __half2 f2 = __float2half2_rn(fac);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&wu[j]), f2);
+                wu[j] = *reinterpret_cast<const uint32_t*>(&y);
+              }
+            }
+          }
+          const float ref = m_ref == -INFINITY ? 0.f : -m_ref;
+          const float2 ref2 = make_float2(ref, ref);
+          const float4 vs4 = *reinterpret_cast<const float4*>(sc + 8 + (upper ? 4 : 0));
+          const float vs[4] = {vs4.x, vs4.y, vs4.z, vs4.w};
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const float2 y = __fadd2_rn(make_float2(x[2 * j], x[2 * j + 1]), ref2);
             const float2 e = make_float2(ex2_approx(y.x), ex2_approx(y.y));
             l2[j & 1] = __fadd2_rn(l2[j & 1], e);
-            const float2 wv = __fmul2_rn(e, make_float2(vs[k >> 4], vs[k >> 4]));
+            const float2 wv = __fmul2_rn(e, make_float2(vs[j >> 3], vs[j >> 3]));
             pw[j] = pack_f16x2(wv.x, wv.y);
           }
-          dec::tmem_st16(tm_s + 16 * c, pw);
+        };
+        {
+          if (ok) ok = mbar_wait_flag(bar(L::kUFull + tile), i & 1, s_abort);
+          ok = __all_sync(0xffffffffu, ok);
+          tc_fence_after_sync();
+          float x[64];
+          tmem_ld32(tm_s + 64, reinterpret_cast<uint32_t*>(x));
+          tmem_ld32(tm_s + 96, reinterpret_cast<uint32_t*>(x + 32));
+          tc_wait_ld();
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(L::kUFree + tile));
+          weights(x, true, wu);
         }
-        tc_wait_st();
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(L::kPFull + tile));
+        {
+          if (ok) ok = mbar_wait_flag(bar(L::kLFull + tile), i & 1, s_abort);
+          ok = __all_sync(0xffffffffu, ok);
+          tc_fence_after_sync();
+          float x[64];
+          uint32_t wl[32];
+          tmem_ld32(tm_s, reinterpret_cast<uint32_t*>(x));
+          tmem_ld32(tm_s + 32, reinterpret_cast<uint32_t*>(x + 32));
+          tc_wait_ld();
+          weights(x, false, wl);
+          tmem_st32(tm_s, wu);
+          tmem_st32(tm_s + 32, wl);
+          tc_wait_st();
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(L::kPFull + tile));
+        }
       }
       // ---- the row's result
       if (n > 0) {
@@ -470,10 +499,10 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       const RowEnd end = finish_row(m_ref, l, p.sink, h);
       const bool direct = p.num_splits == 1;
       const int64_t rows = (int64_t)p.B * p.Sq * p.Hq, part = (int64_t)split * rows;
-      const float scale = (direct ? end.factor : 1.f / l) * vs_down;
+      const float scale = (direct ? end.factor : __frcp_rn(l)) * vs_down;
       if (ok && row < R) {
         if (direct && p.lse != nullptr) p.lse[l_idx] = end.lse;
-        if (!direct) p.lse_partial[part + ((int64_t)b * p.Sq + s) * p.Hq + h] = none ? -INFINITY : m_ref + log2f(l);
+        if (!direct) p.lse_partial[part + ((int64_t)b * p.Sq + s) * p.Hq + h] = none ? -INFINITY : m_ref + lg2_approx(l);
       }
 #pragma unroll 1
       for (int c = 0; c < kD / 32; ++c) {
