@@ -40,14 +40,16 @@ __device__ __forceinline__ int2 seen_by(const Fp8Params& p, int sk, int sq, int 
   return make_int2(lo, hi > lo ? hi : lo);
 }
 
-// tanh in fp32 from the exponential: 1 - 2 / (1 + e^2x), off by a few 2^-24 (tanh.approx is off by 2^-11, 1 % of a weight at a
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// tanh in fp32 from the exponential: 1 - 2 / (1 + e^2x), off by a few 2^-23 (tanh.approx is off by 2^-11, 1 % of a weight at a
 // cap of 30).
 __device__ __forceinline__ float tanh_of(float x) {
   const float e = ex2_approx(x * (2.f * 1.4426950408889634f));
-  return fmaf(-2.f, __frcp_rn(1.f + e), 1.f);
-}
-__device__ __forceinline__ float score_of(const Fp8Params& p, float dot, float row_factor) {
-  return p.cap_out != 0.f ? p.cap_out * tanh_of(dot * row_factor) : dot * row_factor;
+  return fmaf(-2.f, rcp_approx(1.f + e), 1.f);
 }
 
 // Valid keys and rows of a sequence.
@@ -79,7 +81,7 @@ __device__ __forceinline__ RowEnd finish_row(float m, float l, const float* sink
     l = (m == -INFINITY ? 0.f : l * keep) + ex2_approx(x - top);
   }
   if (top == -INFINITY && l == 0.f) return {0.f, -INFINITY};    // (a row of NaN has l = NaN and goes on)
-  e.factor = keep * __frcp_rn(l);
+  e.factor = keep * rcp_approx(l);
   e.lse = (top + lg2_approx(l)) * kLn2;
   return e;
 }

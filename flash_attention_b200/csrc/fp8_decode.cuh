@@ -784,7 +784,7 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           if (lane == 0 && p.lse != nullptr) p.lse[((int64_t)b * p.Hq + h) * p.Sq + s] = e.lse;
         } else {
           const bool none = m == -INFINITY && sum == 0.f;
-          const float f = __frcp_rn(sum);
+          const float f = rcp_approx(sum);
           if (col < kD && !none)
             *reinterpret_cast<float4*>(p.o_partial + (slot * p.unit_rows + r) * kD + col) = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
           if (lane == 0) p.lse_partial[slot * p.unit_rows + r] = none ? -INFINITY : m + lg2_approx(sum);

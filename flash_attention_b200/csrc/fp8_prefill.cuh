@@ -259,17 +259,21 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
 #pragma unroll 1
         for (int i = 0; ok && i < n; ++i) {
           const bool more = i + 1 < n;
+          // (what is most often there already is asked for at once: a wait of its own costs 110 clocks even then)
           if (more) {
-            ok = mbar_wait(bar(L::kKFull + kk.at), kk.parity, wc, kKFullS);
+            const uint32_t two = tiles - 1;
+            const bool kf = mbar_poll(bar(L::kKFull + kk.at), kk.parity), vf = mbar_poll(bar(L::kVFull + buf), parity),
+                       u0 = mbar_poll(bar(L::kUFree), i & 1), u1 = mbar_poll(bar(L::kUFree + two), i & 1);
+            if (!(kf && vf && u0 && u1))
+              ok = mbar_wait(bar(L::kKFull + kk.at), kk.parity, wc, kKFullS) && mbar_wait(bar(L::kVFull + buf), parity, wc, kHalfFullS) &&
+                   mbar_wait(bar(L::kUFree), i & 1, wc, kUFreeS) && mbar_wait(bar(L::kUFree + two), i & 1, wc, kUFreeS);
+            if (!ok) break;
+            tc_fence_after_sync();
 #pragma unroll 1
-            for (int t = 0; ok && t < tiles; ++t) {
-              ok = mbar_wait(bar(L::kUFree + t), i & 1, wc, kUFreeS);
-              if (!ok) break;
-              tc_fence_after_sync();
-              score(t, kk.at, true);
-            }
+            for (int t = 0; t < tiles; ++t) score(t, kk.at, true);
+          } else {
+            ok = mbar_wait(bar(L::kVFull + buf), parity, wc, kHalfFullS);
           }
-          if (ok) ok = mbar_wait(bar(L::kVFull + buf), parity, wc, kHalfFullS);
           const uint64_t vt = desc_at(dv, buf * L::kTile16);
 #pragma unroll 1
           for (int t = 0; ok && t < tiles; ++t) {
@@ -499,7 +503,7 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       const RowEnd end = finish_row(m_ref, l, p.sink, h);
       const bool direct = p.num_splits == 1;
       const int64_t rows = (int64_t)p.B * p.Sq * p.Hq, part = (int64_t)split * rows;
-      const float scale = (direct ? end.factor : __frcp_rn(l)) * vs_down;
+      const float scale = (direct ? end.factor : rcp_approx(l)) * vs_down;
       if (ok && row < R) {
         if (direct && p.lse != nullptr) p.lse[l_idx] = end.lse;
         if (!direct) p.lse_partial[part + ((int64_t)b * p.Sq + s) * p.Hq + h] = none ? -INFINITY : m_ref + lg2_approx(l);
