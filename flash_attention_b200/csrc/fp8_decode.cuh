@@ -105,7 +105,6 @@ struct Feeder {
   uint8_t* ring;                    //   the same, for plain stores
   float* scales;                    // kScales x (8 of K, 8 of V), or null
   int2* box;                        // 32 places
-  float v_factor;                   // on the scales of values
   FeederSites site;
   Ring<kStages> st;                 // (of the issuing thread)
   bool first = true;                // round of the ring
@@ -156,7 +155,7 @@ struct Feeder {
         int to = slot + (lane >> 3);
         to = (to >= kScales ? to - kScales : to) * 16 + gr;
         scales[to] = sc.x;
-        scales[to + 8] = sc.y * v_factor;
+        scales[to + 8] = sc.y;
       }
       const int2 at2 = look_up(l0 + 8);
       const float2 sc1 = scales_at(at1);
@@ -441,7 +440,6 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     feed.ring = gbase + (is_k ? F::kOffK : F::kOffV);
     feed.scales = is_k ? reinterpret_cast<float*>(gbase + F::kOffSc) : nullptr;
     feed.box = reinterpret_cast<int2*>(gbase + F::kOffBox) + (is_k ? 0 : 32);
-    feed.v_factor = 1.f;
     feed.site = is_k ? FeederSites{kKFreeS, kKFullS} : FeederSites{kVFreeS, kVFullS};
     for (; ok && walk.more(); walk.next(p))
       ok = feed.piece(p, wc, walk.tiles(), walk.cur.first + walk.at, walk.b, walk.hb * p.bundle + in_bundle, walk.cur.lo, walk.cur.hi);

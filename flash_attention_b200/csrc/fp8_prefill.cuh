@@ -38,8 +38,8 @@ struct Layout {
   static constexpr int kScales = kStagesK + 6;
   static constexpr uint32_t kTile16 = kHalf * (kD / 64), kTile8 = 128 * kD;
   static constexpr uint32_t kOffQ = 0 /* 2 tiles x (q1, q2) */, kOffK = 4 * kTile8, kOffRawV = kOffK + kStagesK * kTile8,
-                            kOffV = kOffRawV + kStagesV * kTile8, kOffSc = kOffV + 2 * kTile16, kOffBox = kOffSc + kScales * 64,
-                            kOffBar = kOffBox + 512;
+                            kOffV = kOffRawV + kStagesV * kTile8, kOffSc = kOffV + 2 * kTile16, kOffBox = kOffSc + kScales * 64, kOffRow = kOffBox + 512 /* factor of a row's scores */,
+                            kOffBar = kOffRow + 256 * 4;
   static constexpr uint32_t kKFull = 0, kKFree = kKFull + kStagesK, kRawFull = kKFree + kStagesK, kRawFree = kRawFull + kStagesV,
                             kVFull = kRawFree + kStagesV, kVFree = kVFull + 2, kUFull = kVFree + 2, kLFull = kUFull + 2, kUFree = kLFull + 2,
                             kPFull = kUFree + 2, kPvDone = kPFull + 2, kODone = kPvDone + 2, kQReady = kODone + 1, kDrain = kQReady + 1,
@@ -167,7 +167,7 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       mbar_init(bar(L::kPvDone + s), 1);
     }
     mbar_init(bar(L::kODone), 1);
-    mbar_init(bar(L::kQReady), 8);
+    mbar_init(bar(L::kQReady), 12);
     mbar_init(bar(L::kDrain), 1);
     fence_barrier_init();
   }
@@ -182,11 +182,55 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   tc_fence_after_sync();
   pdl_trigger();
   const uint32_t tmem = *tmem_slot;
-  // the largest scale of values among this CTA's keys
-  const int first_key = max(lo_all, t0 << 7), end_key = min(hi_all, (t0 + n) << 7);
-  {
+  bool ok = true;
+  float vs_up = 1.f, vs_down = 1.f;
+  if (warp < 12) {
+    // ---- Q by all but the service warps, a row's pieces of eight elements by neighbouring lanes: a row as two e4m3 rows, times the
+    //      power of two that brings its largest element to 128 .. 256.  All on their way at once, to where V's widened tiles
+    //      will be (one after another from registers took 14000 clocks).
+    constexpr int kPieces = kD / 8;
+    float* s_row = reinterpret_cast<float*>(gbase + L::kOffRow);
+#pragma unroll 4
+    for (int i = tid; i < 256 * kPieces; i += 384) {
+      const int r = i / kPieces, ch = i % kPieces, s = fast_div(r_first + r, p.div_group), h = hk * p.group + r_first + r - s * p.group;
+      const __nv_bfloat16* src = r < R ? p.q + b * p.q_b + (int64_t)s * p.q_s + h * p.q_h + 8 * ch : p.q;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(base + L::kOffV + 16 * i), "l"(src), "r"(r < R ? 16 : 0) : "memory");
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll 1
+    for (int i = tid; i < 256 * kPieces; i += 384) {
+      const int r = i / kPieces, ch = i % kPieces;
+      const uint4 u = *reinterpret_cast<const uint4*>(gbase + L::kOffV + 16 * i);
+      float x[8], y[8];
+      unpack8(u, x);
+      uint32_t top = 0u;                      // (bit patterns: NaN is the largest)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(x[k]) & 0x7fffffffu);
+#pragma unroll
+      for (int o = 1; o < kPieces; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const int e = max((int)(top >> 23), 17);
+      const float up = __uint_as_float((uint32_t)(254 + 7 - e) << 23), down = __uint_as_float((uint32_t)(e - 7) << 23);
+      const bool fine = top < 0x7f800000u;                   // (a row that is not finite becomes NaN whole)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] *= up;
+      uint2 q1 = make_uint2(pack4_e4m3(x[0], x[1], x[2], x[3]), pack4_e4m3(x[4], x[5], x[6], x[7]));
+      unpack4_e4m3(q1.x, y);
+      unpack4_e4m3(q1.y, y + 4);
+      const uint2 q2 = make_uint2(pack4_e4m3(x[0] - y[0], x[1] - y[1], x[2] - y[2], x[3] - y[3]),
+                                  pack4_e4m3(x[4] - y[4], x[5] - y[5], x[6] - y[6], x[7] - y[7]));
+      if (!fine) q1 = make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
+      uint8_t* to = gbase + L::kOffQ + 2 * (r >> 7) * L::kTile8 + fp8d::row_piece<kD>(r & 127, ch >> 1) + (ch & 1) * 8;
+      *reinterpret_cast<uint2*>(to) = q1;
+      *reinterpret_cast<uint2*>(to + L::kTile8) = q2;
+      if (ch == 0) s_row[r] = (kCap ? p.cap_in : p.sl2) * down;
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(L::kQReady));
+    // the largest scale of values among this CTA's keys
+    const int first_key = max(lo_all, t0 << 7), end_key = min(hi_all, (t0 + n) << 7);
     uint32_t top = 0u;
-    for (int64_t blk = (first_key >> p.log_block) + tid; (blk << p.log_block) < end_key && n > 0; blk += kThreads) {
+    for (int64_t blk = (first_key >> p.log_block) + tid; (blk << p.log_block) < end_key && n > 0; blk += 384) {
       const int key = (int)(blk << p.log_block), pg = fast_div(key, p.div_page), off = key - pg * p.page_size;
       const int page = p.table != nullptr ? p.table[(int64_t)b * p.pages_per_seq + pg] : b;
       if (page >= 0 && page < p.num_pages)
@@ -194,13 +238,14 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     }
     top = __reduce_max_sync(0xffffffffu, top);
     if (lane == 0 && top > 0u) atomicMax(s_top, top);
+    asm volatile("bar.sync 1, 384;" ::: "memory");
+    // 2^6 / its power of two, and back (1 and 1 where it is no ordinary number)
+    const uint32_t top_e = *s_top >> 23;
+    if (top_e >= 20 && top_e <= 240) {
+      vs_up = __uint_as_float((254u + 6u - top_e) << 23);
+      vs_down = __uint_as_float((top_e - 6u) << 23);
+    }
   }
-  __syncthreads();
-  // 2^6 / its power of two, and back (1 and 1 where it is no ordinary number)
-  const uint32_t top_e = *s_top >> 23;
-  const bool ordinary = top_e >= 20 && top_e <= 240;
-  const float vs_up = ordinary ? __uint_as_float((254u + 6u - top_e) << 23) : 1.f, vs_down = ordinary ? __uint_as_float((top_e - 6u) << 23) : 1.f;
-  bool ok = true;
 
   if (warp >= 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsService));
@@ -214,7 +259,6 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       feed.ring = gbase + L::kOffK;
       feed.scales = reinterpret_cast<float*>(gbase + L::kOffSc);
       feed.box = reinterpret_cast<int2*>(gbase + L::kOffBox);
-      feed.v_factor = vs_up;
       feed.site = {kKFreeS, kKFullS};
       if (!feed.piece(p, wc, n, t0, b, hk, lo_all, hi_all)) feed.drain();
     } else if (warp == 14) {
@@ -227,7 +271,6 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       feed.ring = gbase + L::kOffRawV;
       feed.scales = nullptr;
       feed.box = reinterpret_cast<int2*>(gbase + L::kOffBox) + 32;
-      feed.v_factor = 1.f;
       feed.site = {kRawFreeS, kRawFullS};
       if (!feed.piece(p, wc, n, t0, b, hk, lo_all, hi_all)) feed.drain();
     } else if (warp == 13) {
@@ -337,49 +380,7 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tm_s = tmem + lanes + kColS + 128 * tile, tm_o = tmem + lanes + kColO + kD * tile;
     const int s = fast_div(r_first + row, p.div_group), h = hk * p.group + r_first + row - s * p.group;
-    // ---- Q: the thread's row as two e4m3 rows, times the power of two that brings its largest element to 128 .. 256
-    float factor = 0.f;
-    {
-      uint8_t* qt = gbase + L::kOffQ + 2 * tile * L::kTile8;
-      const __nv_bfloat16* src = p.q + b * p.q_b + (int64_t)s * p.q_s + h * p.q_h;
-      uint4 u[kD / 8];
-      uint32_t top = 0u;
-#pragma unroll
-      for (int c = 0; c < kD / 8; ++c) u[c] = row < R ? *reinterpret_cast<const uint4*>(src + 8 * c) : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-      for (int c = 0; c < kD / 8; ++c) {
-        const uint32_t w4[4] = {u[c].x, u[c].y, u[c].z, u[c].w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) top = max(top, max((w4[k] << 16) & 0x7fffffffu, w4[k] & 0x7fff0000u));
-      }
-      const int e = max((int)(top >> 23), 17);
-      const float up = __uint_as_float((uint32_t)(254 + 7 - e) << 23), down = __uint_as_float((uint32_t)(e - 7) << 23);
-      const bool fine = top < 0x7f800000u;                   // (a row that is not finite becomes NaN whole)
-      factor = (kCap ? p.cap_in : p.sl2) * down;
-#pragma unroll
-      for (int c = 0; c < kD / 16; ++c) {
-        uint32_t q1[4], q2[4];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          float x[8], y[8];
-          unpack8(u[2 * c + k], x);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] *= up;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            q1[2 * k + i] = fine ? pack4_e4m3(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]) : 0x7f7f7f7fu;
-            unpack4_e4m3(q1[2 * k + i], y + 4 * i);
-            q2[2 * k + i] = pack4_e4m3(x[4 * i] - y[4 * i], x[4 * i + 1] - y[4 * i + 1], x[4 * i + 2] - y[4 * i + 2], x[4 * i + 3] - y[4 * i + 3]);
-          }
-        }
-        uint8_t* to = qt + fp8d::row_piece<kD>(t, c);
-        *reinterpret_cast<uint4*>(to) = make_uint4(q1[0], q1[1], q1[2], q1[3]);
-        *reinterpret_cast<uint4*>(to + L::kTile8) = make_uint4(q2[0], q2[1], q2[2], q2[3]);
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(L::kQReady));
-    }
+    const float factor = reinterpret_cast<const float*>(gbase + L::kOffRow)[row];
     int lo = 0, hi = 0;
     if (row < R) {
       const int2 see = seen_by(p, len.sk, len.sq, s);
@@ -450,7 +451,7 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
           const float ref = m_ref == -INFINITY ? 0.f : -m_ref;
           const float2 ref2 = make_float2(ref, ref);
           const float4 vs4 = *reinterpret_cast<const float4*>(sc + 8 + (upper ? 4 : 0));
-          const float vs[4] = {vs4.x, vs4.y, vs4.z, vs4.w};
+          const float vs[4] = {vs4.x * vs_up, vs4.y * vs_up, vs4.z * vs_up, vs4.w * vs_up};
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
             const float2 y = __fadd2_rn(make_float2(x[2 * j], x[2 * j + 1]), ref2);
@@ -508,6 +509,9 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         if (direct && p.lse != nullptr) p.lse[l_idx] = end.lse;
         if (!direct) p.lse_partial[part + ((int64_t)b * p.Sq + s) * p.Hq + h] = none ? -INFINITY : m_ref + lg2_approx(l);
       }
+      // Output rows go through the memory of the tile's Q (a warp's own 32 rows; every product is done), to be written by lanes side by side.
+      uint8_t* stage = gbase + L::kOffQ + 2 * tile * L::kTile8 + (t & ~31) * (2 * kD);
+      constexpr int kChunks = kD / 8;
 #pragma unroll 1
       for (int c = 0; c < kD / 32; ++c) {
         float o[32];
@@ -518,17 +522,27 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
 #pragma unroll
           for (int j = 0; j < 32; ++j) o[j] = 0.f;
         }
-        if (!ok || row >= R) {
-        } else if (direct) {
-          uint4* dst = reinterpret_cast<uint4*>(p.out + b * p.o_b + (int64_t)s * p.o_s + h * p.o_h + 32 * c);
+        if (direct) {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            dst[j] = make_uint4(pack_bf16x2(o[8 * j] * scale, o[8 * j + 1] * scale), pack_bf16x2(o[8 * j + 2] * scale, o[8 * j + 3] * scale),
-                                pack_bf16x2(o[8 * j + 4] * scale, o[8 * j + 5] * scale), pack_bf16x2(o[8 * j + 6] * scale, o[8 * j + 7] * scale));
-        } else if (!none) {
+            *reinterpret_cast<uint4*>(stage + lane * (2 * kD) + (((4 * c + j) ^ (lane & 7)) << 4)) =
+                make_uint4(pack_bf16x2(o[8 * j] * scale, o[8 * j + 1] * scale), pack_bf16x2(o[8 * j + 2] * scale, o[8 * j + 3] * scale),
+                           pack_bf16x2(o[8 * j + 4] * scale, o[8 * j + 5] * scale), pack_bf16x2(o[8 * j + 6] * scale, o[8 * j + 7] * scale));
+        } else if (ok && row < R && !none) {
           float4* dst = reinterpret_cast<float4*>(p.o_partial + (part + ((int64_t)b * p.Sq + s) * p.Hq + h) * kD + 32 * c);
 #pragma unroll
           for (int j = 0; j < 8; ++j) dst[j] = make_float4(o[4 * j] * scale, o[4 * j + 1] * scale, o[4 * j + 2] * scale, o[4 * j + 3] * scale);
+        }
+      }
+      if (direct && ok) {
+        __syncwarp();
+#pragma unroll 4
+        for (int i = 0; i < kChunks; ++i) {
+          const int rr = i * (32 / kChunks) + lane / kChunks, c = lane % kChunks, at = r_first + (row & ~31) + rr;
+          const int ss = fast_div(at, p.div_group), hh = hk * p.group + at - ss * p.group;
+          if ((row & ~31) + rr < R)
+            *reinterpret_cast<uint4*>(p.out + b * p.o_b + (int64_t)ss * p.o_s + hh * p.o_h + 8 * c) =
+                *reinterpret_cast<const uint4*>(stage + rr * (2 * kD) + ((c ^ (rr & 7)) << 4));
         }
       }
     }
