@@ -9,9 +9,13 @@
 // exact but for values that fall below 2^-6 of the new scale.  So tokens that come one by one leave (but for those) the bytes
 // of the block quantised at once.
 //
-// A unit is one block of one sequence, kv head and K or V, which one CTA owns: maxima need no atomics, old bytes are read and
-// written by the same CTA.  A thread has 16 elements of a row, as two 16-byte pieces that hold eight whole pairs,
-// in fp32 from the load to the store: memory is read once.
+// A unit is one block of one sequence, kv head and K or V, which one CTA (for a few tokens: one warp) owns: maxima need no atomics, old
+// bytes are read and written by the same threads.  A thread has 16 elements of a row, as two 16-byte pieces that hold eight whole
+// pairs.  With several rows it turns each twice, for the maximum and for the bytes, the second time from L1.
+//
+// What bounds it: a prompt moves 2 B in and 1 B out an element, but an element takes 8 (V) to 15 (K) instructions, and issue and ALU pipe come
+// close to the HBM.  So what is not finite is looked for by one multiply-add an element and treated on a path of its own (27
+// instructions an element without it).
 #pragma once
 #include "ptx.cuh"
 #include <cuda_bf16.h>
@@ -39,6 +43,7 @@ struct AppendParams {
   int rotary_dim, rotary_rows, rotary_bf16, interleaved;
   int B, S, Hq, Hkv, D, log_block, num_pages, page_size, pages_per_seq;
   int blocks;                        // units of a sequence and head: blocks that S tokens may touch
+  int units;
   int kv_ctas;                       // CTAs of keys and values, in front of those of q
   int q_heads, q_head_groups;        // heads of a thread; groups of them
   FastDiv div_blocks, div_hkv2, div_page, div_groups, div_s;
@@ -137,79 +142,110 @@ __device__ __forceinline__ float scale_for(float top) {
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
-// x / scale, where `inv` is not 0 by the exact reciprocal of a power of two.
-__device__ __forceinline__ float over(float x, float scale, float inv) {
-  return inv != 0.f ? __fmul_rn(x, inv) : __fdiv_rn(x, scale);
+// x / scale with r = RN(1 / scale): the product and one residual step, the correctly rounded quotient (Markstein 1990) wherever
+// it is an ordinary number; NaN where x is not finite (an infinity less itself).
+__device__ __forceinline__ float quotient(float x, float scale, float r) {
+  const float q = __fmul_rn(x, r);
+  return __fmaf_rn(__fmaf_rn(-q, scale, x), r, q);
 }
 
-// One unit.  kThreads: of the CTA, or 32 (a warp a unit, for a few new tokens: maxima stay in registers).  kRows: rows of a
-// thread.
-template <int kThreads, int kRows>
-__device__ __forceinline__ void append_unit(const AppendParams& p, int unit, int tid, float* s_max) {
+// Where a unit lies.
+struct AppendUnit {
+  const __nv_bfloat16* src;          // of the token at position `held`
+  uint8_t* dst;                      // of position `start`
+  float* scale;
+  float before;                      // its scale, if it holds tokens already (`kept`)
+  int held, start, t0, t1;           // tokens in front of the call; first position of the block; new ones in it
+  bool is_v, kept, any;
+};
+__device__ __forceinline__ AppendUnit find_unit(const AppendParams& p, int unit, bool report) {
+  AppendUnit u = {};
   // unit = ((b * Hkv + head) * 2 + is_v) * blocks + blk
   const int rest = fast_div(unit, p.div_blocks), blk = unit - rest * p.blocks;
   const int b = fast_div(rest, p.div_hkv2), hv = rest - b * 2 * p.Hkv, head = hv >> 1;
-  const bool is_v = (hv & 1) != 0;
-  const int held = p.seqlens[b];
+  u.is_v = (hv & 1) != 0;
+  u.held = p.seqlens[b];
   int n = p.fresh != nullptr ? p.fresh[b] : p.S;
   n = n < 0 ? 0 : (n < p.S ? n : p.S);
-  if (n == 0) return;
-  if (held < 0) {
-    if (tid == 0) report_bad_index(p.status, p.epoch, kPositionSite);
-    return;
+  if (n == 0) return u;
+  if (u.held < 0) {
+    if (report) report_bad_index(p.status, p.epoch, kPositionSite);
+    return u;
   }
   const int bt = 1 << p.log_block;
   // (positions stay below 2^31: those of the cache do, and the first one behind it ends the unit)
-  const int64_t start64 = (int64_t)((held >> p.log_block) + blk) << p.log_block;
-  if (start64 >= (int64_t)held + n) return;
-  if (start64 >= (int64_t)p.pages_per_seq * p.page_size) {
-    if (tid == 0) report_bad_index(p.status, p.epoch, kPositionSite);
-    return;
+  const int64_t start = (int64_t)((u.held >> p.log_block) + blk) << p.log_block, end = (int64_t)u.held + n;
+  if (start >= end) return u;
+  if (start >= (int64_t)p.pages_per_seq * p.page_size) {
+    if (report) report_bad_index(p.status, p.epoch, kPositionSite);
+    return u;
   }
-  const int start = (int)start64;
-  const int t0 = held > start ? held : start;
-  const int t1 = (int64_t)held + n < (int64_t)start + bt ? held + n : start + bt;
-  const int pg = fast_div(start, p.div_page), off = start - pg * p.page_size;
+  u.start = (int)start;
+  u.t0 = u.held > u.start ? u.held : u.start;
+  u.t1 = end < start + bt ? (int)end : u.start + bt;
+  const int pg = fast_div(u.start, p.div_page), off = u.start - pg * p.page_size;
   const int page = p.table != nullptr ? p.table[(int64_t)b * p.pages_per_seq + pg] : b;
   if (page < 0 || page >= p.num_pages) {
-    if (tid == 0) report_bad_index(p.status, p.epoch, kPageSite);
-    return;
+    if (report) report_bad_index(p.status, p.epoch, kPageSite);
+    return u;
   }
-  float* scale_at = (is_v ? p.v_scale : p.k_scale) +
-                    ((int64_t)page * (p.page_size >> p.log_block) + (off >> p.log_block)) * p.Hkv + head;
-  uint8_t* dst = is_v ? p.vc + page * p.vc_page + off * p.vc_tok + head * p.vc_head
-                      : p.kc + page * p.kc_page + off * p.kc_tok + head * p.kc_head;
-  const int64_t dst_tok = is_v ? p.vc_tok : p.kc_tok;
-  const bool kept = held > start;
-  const float before = kept ? *scale_at : 0.f;
+  u.any = true;
+  u.scale = (u.is_v ? p.v_scale : p.k_scale) + ((int64_t)page * (p.page_size >> p.log_block) + (off >> p.log_block)) * p.Hkv + head;
+  u.dst = u.is_v ? p.vc + page * p.vc_page + off * p.vc_tok + head * p.vc_head : p.kc + page * p.kc_page + off * p.kc_tok + head * p.kc_head;
+  u.src = u.is_v ? p.v + b * p.v_b + head * p.v_h : p.k + b * p.k_b + head * p.k_h;
+  u.kept = u.held > u.start;
+  u.before = u.kept ? *u.scale : 0.f;
+  return u;
+}
 
-  const int log_chunks = p.D == 128 ? 3 : 2;                   // chunks of 16 in a row
+// kThreads threads of a unit (32: a warp, whose maxima stay in registers), a row each or (kMany) several.
+template <int kThreads, bool kMany>
+__device__ __forceinline__ void append_unit(const AppendParams& p, int unit, int tid, float* s_max) {
+  const AppendUnit u = find_unit(p, unit, tid == 0);
+  if (!u.any) return;
+  const int log_chunks = p.D == 128 ? 3 : 2;                 // chunks of 16 in a row
   const int c = tid & ((1 << log_chunks) - 1), row0 = tid >> log_chunks, step = kThreads >> log_chunks;
-  const bool rotate = !is_v && p.cos != nullptr;
-  Chunk ch = {16 * c, 16 * c + 8, false};
-  if (rotate) ch = chunk_of(p, c);
-  const __nv_bfloat16* src = is_v ? p.v + b * p.v_b + head * p.v_h : p.k + b * p.k_b + head * p.k_h;
-  const int64_t src_tok = is_v ? p.v_s : p.k_s;
-  float x[kRows][16];
-  float top = 0.f;
+  const Chunk ch = !u.is_v && p.cos != nullptr ? chunk_of(p, c) : Chunk{16 * c, 16 * c + 8, false};
+  const int64_t src_tok = u.is_v ? p.v_s : p.k_s, dst_tok = u.is_v ? p.vc_tok : p.kc_tok;
+  auto row_of = [&](int t, float (&x)[16]) {                 // the thread's piece of the row at position t, turned
+    const __nv_bfloat16* row = u.src + (t - u.held) * src_tok;
+    unpack8(*reinterpret_cast<const uint4*>(row + ch.a), x);
+    unpack8(*reinterpret_cast<const uint4*>(row + ch.b), x + 8);
+    if (ch.turned) turn16(x, load_angles(p, t < p.rotary_rows ? t : p.rotary_rows - 1, c), p.interleaved != 0);
+  };
+  // zero is NaN if an element is not finite
+  float x[16], top = 0.f, zero = 0.f;
+  auto take = [&](const float (&v)[16]) {
 #pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    const int t = t0 + row0 + r * step;
-    if (t < t1) {
-      const __nv_bfloat16* row = src + (t - held) * src_tok;
-      unpack8(*reinterpret_cast<const uint4*>(row + ch.a), x[r]);
-      unpack8(*reinterpret_cast<const uint4*>(row + ch.b), x[r] + 8);
-      if (ch.turned) {
-        const bool there = t < p.rotary_rows;
-        if (!there) report_bad_index(p.status, p.epoch, kRotationSite);
-        turn16(x[r], load_angles(p, there ? t : p.rotary_rows - 1, c), p.interleaved != 0);
-      }
+    for (int i = 0; i < 16; ++i) {
+      top = fmaxf(top, fabsf(v[i]));
+      zero = fmaf(v[i], 0.f, zero);
+    }
+  };
+  if constexpr (kMany) {
+#pragma unroll 2
+    for (int t = u.t0 + row0; t < u.t1; t += step) {
+      float y[16];
+      row_of(t, y);
+      take(y);
+    }
+  } else if (u.t0 + row0 < u.t1) {
+    row_of(u.t0 + row0, x);
+    take(x);
+  }
+  if (ch.turned && row0 == 0 && u.t1 > p.rotary_rows) report_bad_index(p.status, p.epoch, kRotationSite);
+  const bool fine = zero == 0.f;
+  if (!fine) {
+    top = 0.f;
+#pragma unroll 1
+    for (int t = u.t0 + row0; t < u.t1; t += step) {
+      if constexpr (kMany) row_of(t, x);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float m = fabsf(x[r][i]);
-        if (m < INFINITY) top = fmaxf(top, m);
-        else x[r][i] = __uint_as_float(0x7fffffffu);           // (and NaN: what is not finite)
+        const float m = fabsf(x[i]);
+        top = fmaxf(top, m < INFINITY ? m : 0.f);
       }
+      if constexpr (!kMany) break;
     }
   }
 #pragma unroll
@@ -221,49 +257,60 @@ __device__ __forceinline__ void append_unit(const AppendParams& p, int unit, int
     for (int w = 0; w < kThreads / 32; ++w) top = fmaxf(top, s_max[w]);
   }
   const float need = scale_for(top);
-  const float scale = kept ? fmaxf(before, need) : need;
-  // (old scales need not be powers of two)
-  const bool pow2 = (__float_as_uint(scale) & 0x7fffffu) == 0u && scale >= 0x1p-126f && scale <= 0x1p126f;
-  const float inv = pow2 ? __uint_as_float((254u << 23) - __float_as_uint(scale)) : 0.f;
-  if (kept && scale != before) {
-    const float again = __fdiv_rn(before, scale);
-    for (int t = row0; t < t0 - start; t += step) {
-      uint4* at = reinterpret_cast<uint4*>(dst + t * dst_tok + 16 * c);
-      uint4 u = *at;
-      uint32_t* w = &u.x;
+  const float scale = u.kept ? fmaxf(u.before, need) : need;
+  if (u.kept && scale != u.before) {
+    const float again = __fdiv_rn(u.before, scale);
+#pragma unroll 1
+    for (int t = row0; t < u.t0 - u.start; t += step) {
+      uint4* held = reinterpret_cast<uint4*>(u.dst + t * dst_tok + 16 * c);
+      uint4 v = *held;
+      uint32_t* w = &v.x;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float y[4];
         unpack4_e4m3(w[i], y);
         w[i] = pack4_e4m3(__fmul_rn(y[0], again), __fmul_rn(y[1], again), __fmul_rn(y[2], again), __fmul_rn(y[3], again));
       }
-      *at = u;
+      *held = v;
     }
   }
+  // (old scales need not be powers of two)
+  const bool product = fine && (__float_as_uint(scale) & 0x7fffffu) == 0u;
+  const float inv = __frcp_rn(scale);
+  auto bytes_of = [&](int t, float (&v)[16]) {
+    if (product) {
 #pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    const int t = t0 + row0 + r * step;
-    if (t < t1) {
-      uint32_t w[4];
+      for (int i = 0; i < 16; ++i) v[i] = __fmul_rn(v[i], inv);
+    } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        w[i] = pack4_e4m3(over(x[r][4 * i], scale, inv), over(x[r][4 * i + 1], scale, inv),
-                          over(x[r][4 * i + 2], scale, inv), over(x[r][4 * i + 3], scale, inv));
-      uint8_t* at = dst + (t - start) * dst_tok;
-      if (ch.b == ch.a + 8) {
-        *reinterpret_cast<uint4*>(at + ch.a) = make_uint4(w[0], w[1], w[2], w[3]);
-      } else {
-        *reinterpret_cast<uint2*>(at + ch.a) = make_uint2(w[0], w[1]);
-        *reinterpret_cast<uint2*>(at + ch.b) = make_uint2(w[2], w[3]);
-      }
+      for (int i = 0; i < 16; ++i) v[i] = quotient(v[i], scale, inv);
     }
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = pack4_e4m3(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    uint8_t* to = u.dst + (t - u.start) * dst_tok;
+    if (ch.b == ch.a + 8) {
+      *reinterpret_cast<uint4*>(to + ch.a) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+      *reinterpret_cast<uint2*>(to + ch.a) = make_uint2(w[0], w[1]);
+      *reinterpret_cast<uint2*>(to + ch.b) = make_uint2(w[2], w[3]);
+    }
+  };
+  if constexpr (kMany) {
+#pragma unroll 2
+    for (int t = u.t0 + row0; t < u.t1; t += step) {
+      float y[16];
+      row_of(t, y);
+      bytes_of(t, y);
+    }
+  } else if (u.t0 + row0 < u.t1) {
+    bytes_of(u.t0 + row0, x);
   }
   if constexpr (kThreads == 32) __syncwarp();                  // (every lane has read it)
-  if (tid == 0) *scale_at = scale;
+  if (tid == 0) *u.scale = scale;
 }
 
 // Rows of q: a thread turns one chunk of `q_heads` heads of a row, whose angles it loads once.
-template <int kThreads>
 __device__ __forceinline__ void rotate_queries(const AppendParams& p, int64_t item) {
   const int log_chunks = p.D == 128 ? 3 : 2;
   const int c = (int)item & ((1 << log_chunks) - 1);
@@ -300,21 +347,19 @@ __device__ __forceinline__ void rotate_queries(const AppendParams& p, int64_t it
 }
 
 // kThreads = 32: a warp a unit, four units a CTA; else a CTA a unit.  The CTAs from kv_ctas on turn q.
-template <int kThreads, int kRows>
+template <int kThreads, bool kMany>
 __global__ void __launch_bounds__(kThreads == 32 ? 128 : kThreads)
 fp8_append_kernel(const __grid_constant__ AppendParams p) {
   constexpr int kCta = kThreads == 32 ? 128 : kThreads;
   __shared__ float s_max[kCta / 32];
   pdl_wait();
   if ((int)blockIdx.x >= p.kv_ctas) {
-    rotate_queries<kCta>(p, (int64_t)(blockIdx.x - p.kv_ctas) * kCta + threadIdx.x);
-    return;
-  }
-  if constexpr (kThreads == 32) {
+    rotate_queries(p, (int64_t)(blockIdx.x - p.kv_ctas) * kCta + threadIdx.x);
+  } else if constexpr (kThreads == 32) {
     const int unit = blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (unit < p.B * p.Hkv * 2 * p.blocks) append_unit<32, kRows>(p, unit, threadIdx.x & 31, s_max);
+    if (unit < p.units) append_unit<32, kMany>(p, unit, threadIdx.x & 31, s_max);
   } else {
-    append_unit<kThreads, kRows>(p, blockIdx.x, threadIdx.x, s_max);
+    append_unit<kThreads, kMany>(p, blockIdx.x, threadIdx.x, s_max);
   }
 }
 

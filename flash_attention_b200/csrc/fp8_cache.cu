@@ -98,19 +98,21 @@ extern "C" int fa4_fp8_cache_append(const fa4_fp8_cache* c, const fa4_fp8_append
   p.q_head_groups = with_q ? (a->Hq + p.q_heads - 1) / p.q_heads : 1;
   p.div_groups = make_fastdiv((uint32_t)p.q_head_groups);
   const int64_t q_threads = with_q ? (int64_t)a->B * a->S * p.q_head_groups * chunks : 0;
-  auto launch = [&](auto kernel, int threads, int64_t ctas) -> int {
-    p.kv_ctas = (int)ctas;
-    const int64_t grid = ctas + (q_threads + threads - 1) / threads;
-    return launch_pdl(kernel, dim3((unsigned)grid), (unsigned)threads, 0, static_cast<cudaStream_t>(cuda_stream), p);
-  };
+  p.units = (int)units;
+  const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
   // pieces of 16 elements that a unit may have
   const int64_t pieces = std::min<int64_t>(a->S, c->block) * chunks;
-  if (pieces <= 32) return launch(fp8_append_kernel<32, 1>, 128, (units + 3) / 4);
-  if (pieces <= 64) return launch(fp8_append_kernel<64, 1>, 64, units);
-  if (pieces <= 128) return launch(fp8_append_kernel<128, 1>, 128, units);
-  if (pieces <= 256) return launch(fp8_append_kernel<256, 1>, 256, units);
-  if (pieces <= 512) return launch(fp8_append_kernel<256, 2>, 256, units);
-  return launch(fp8_append_kernel<256, 4>, 256, units);
+  auto launch = [&](auto kernel, int threads, int64_t ctas) -> int {
+    p.kv_ctas = (int)ctas;
+    return launch_pdl(kernel, dim3((unsigned)(ctas + (q_threads + threads - 1) / threads)), (unsigned)threads, 0, stream, p);
+  };
+  // About four rows a thread: what a unit costs a thread once (its place, the scale) is as much as a row's 16 elements.  us, 2 x 8192 tokens of 8
+  // heads without q, blocks of 16 / 32 / 64 tokens: a row a thread (two for 64) 56 / 54 / 43, four 40 / 38 / 38.
+  if (pieces <= 32) return launch(fp8_append_kernel<32, false>, 128, (units + 3) / 4);
+  if (pieces <= 128) return launch(fp8_append_kernel<32, true>, 128, (units + 3) / 4);
+  if (pieces <= 256) return launch(fp8_append_kernel<64, true>, 64, units);
+  if (pieces <= 512) return launch(fp8_append_kernel<128, true>, 128, units);
+  return launch(fp8_append_kernel<256, true>, 256, units);
 }
 
 namespace {
