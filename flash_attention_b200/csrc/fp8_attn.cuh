@@ -9,8 +9,6 @@ struct Fp8Params {
   __nv_bfloat16* out;
   float* lse;
   int64_t q_b, q_s, q_h, o_b, o_s, o_h;   // elements
-  const uint8_t *kc, *vc;
-  int64_t kc_page, kc_tok, kc_head, vc_page, vc_tok, vc_head;   // bytes
   const float *k_scale, *v_scale;
   const int32_t *used, *fresh, *table;
   const float* sink;
@@ -22,7 +20,7 @@ struct Fp8Params {
   int bundle, bundles;               // kv heads side by side (a divisor of Hkv), and how many such
   int box;                           // keys of a tensor-map box: 128, or what pages and tiles of 128 share
   int B, Sq, Hq, Hkv, group, D, log_block, num_pages, page_size, pages_per_seq, capacity;
-  int row_tiles;                     // of a kv head and sequence
+  int row_tiles, cta_rows;           // many rows: tiles of 128 or 256 rows of a kv head and sequence
   FastDiv div_page, div_group, div_hq, div_sq, div_groups;   // (groups of CTAs of the decode kernel)
   // scores in log2 units: (q . k8) * ks * sl2, or cap_out * tanh((q . k8) * ks * cap_in) with a soft cap
   float sl2, cap_in, cap_out;

@@ -152,11 +152,34 @@ struct Fp8Plan {
   bool decode;
   int rows;          // decode: rows that the kernel is built for
   int bundle;        // decode: kv heads side by side
-  int row_tiles;     // many rows: tiles of 256
+  int row_tiles, cta_rows;   // many rows: tiles of 128 or 256
   int splits;        // 0: shares dealt on the device
   int64_t slots;     // of partial results, and their rows
   int64_t slot_rows;
 };
+// Rows of a CTA and splits of the kernel for many rows.  Chosen splits: 256 rows, whatever the batch.  CTAs that are more than the SMs: 256 rows, one
+// split.  Else what takes the least time by these figures (us): a CTA 10 with 128 rows and 13 with 256, a step of 128 keys 2.0 and 1.85 (the softmax of one tile
+// wait for the products more often), a merge 5 and the partial results, written and read once at 4 TB/s.  Measured, 128 rows / 256 rows / 256 in two
+// splits, D = 128: 333 rows of 16 heads on as many keys 13.7 / 17.0 / 21.9, 512 of 32 heads on 1024 keys 21.9 / 26.9 / 32.6, on 4096 keys
+// 57.5 / 70.9 / 55.5, three sequences of up to 333 rows of 16 heads on up to 2048 keys 41.0 / 47.4 / 40.4.
+void plan_many(int64_t rows, int64_t units, int64_t tiles, int64_t values, int chosen, Fp8Plan* plan) {
+  double least = 0;
+  for (const int cta_rows : {256, 128}) {
+    const int64_t row_tiles = (rows + cta_rows - 1) / cta_rows, room = kSms / (units * row_tiles);
+    if (cta_rows == 128 && (room == 0 || chosen > 0)) break;
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>({128, room, tiles / 2}));
+    for (int64_t splits = chosen > 0 ? chosen : 1; splits <= (chosen > 0 ? chosen : most); ++splits) {
+      const double merge = splits == 1 ? 0. : 5. + (double)(splits * values) * 8 / 4e6;
+      const double us = (cta_rows == 256 ? 13. : 10.) + (cta_rows == 256 ? 1.85 : 2.) * (double)((tiles + splits - 1) / splits) + merge;
+      if (plan->cta_rows == 0 || us < least) {
+        least = us;
+        plan->cta_rows = cta_rows;
+        plan->row_tiles = (int)row_tiles;
+        plan->splits = (int)splits;
+      }
+    }
+  }
+}
 Fp8Plan plan_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f) {
   Fp8Plan plan = {};
   const int64_t rows = (int64_t)f->Sq * (f->Hq / c->Hkv), units = (int64_t)c->Hkv * f->B;
@@ -171,10 +194,8 @@ Fp8Plan plan_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f) {
     plan.slots = plan.splits == 0 ? 2 * kSms : plan.splits == 1 ? 0 : units * plan.splits;
     plan.slot_rows = rows;
   } else {
-    plan.row_tiles = (int)((rows + 255) / 256);
     const int64_t tiles = ((int64_t)c->pages_per_seq * c->page_size + 127) / 128;
-    plan.splits = f->num_splits > 0 ? f->num_splits
-                                    : (int)std::max<int64_t>(1, std::min<int64_t>({128, kSms / (units * plan.row_tiles), tiles / 2}));
+    plan_many(rows, units, tiles, (int64_t)f->B * f->Sq * f->Hq * c->D, f->num_splits, &plan);
     plan.slots = plan.splits == 1 ? 0 : plan.splits;
     plan.slot_rows = (int64_t)f->B * f->Sq * f->Hq;
   }
@@ -228,6 +249,7 @@ extern "C" int fa4_fp8_cache_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, v
   p.bundle = plan.decode ? plan.bundle : 1;
   p.bundles = c->Hkv / p.bundle;
   p.row_tiles = plan.row_tiles;
+  p.cta_rows = plan.cta_rows;
   // (a contiguous cache has no page borders: what lies behind its end is read as zeros)
   p.box = c->page_table == nullptr ? 128 : std::gcd(c->page_size, 128);
   p.B = f->B; p.Sq = f->Sq; p.Hq = f->Hq; p.Hkv = c->Hkv; p.group = f->Hq / c->Hkv; p.D = c->D;

@@ -109,6 +109,35 @@ __device__ __forceinline__ void widen_tile(const uint8_t* raw, uint8_t* to, int 
   }
 }
 
+// x to cap * tanh(x).  While no score of the warp's 64 keys is beyond 0.75 (a cap lies well above what scores mostly are), tanh x / x is a polynomial in
+// x^2 through its values at the six Chebyshev nodes of [0, 0.75^2]: off by 1.6e-7 of the value with the rounding in fp32, and without the two
+// special functions of tanh_of, which with the weight's own would bound the kernel.
+__device__ __forceinline__ void cap_scores(float (&x)[64], float cap) {
+  float far = fabsf(x[0]);
+#pragma unroll
+  for (int j = 1; j < 63; j += 2) far = fmax3(far, fabsf(x[j]), fabsf(x[j + 1]));
+  far = fmaxf(far, fabsf(x[63]));
+  if (__any_sync(0xffffffffu, far > 0.75f)) {
+#pragma unroll
+    for (int j = 0; j < 64; ++j) x[j] = cap * tanh_of(x[j]);
+  } else {
+    constexpr float kC[6] = {0.99999997f, -0.33332954f, 0.13325339f, -0.053341115f, 0.019576216f, -0.0047115222f};
+    float2 c[6];
+#pragma unroll
+    for (int k = 0; k < 6; ++k) c[k] = make_float2(cap * kC[k], cap * kC[k]);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      const float2 v = make_float2(x[2 * j], x[2 * j + 1]), z = __fmul2_rn(v, v);
+      float2 y = c[5];
+#pragma unroll
+      for (int k = 4; k >= 0; --k) y = __ffma2_rn(y, z, c[k]);
+      y = __fmul2_rn(y, v);
+      x[2 * j] = y.x;
+      x[2 * j + 1] = y.y;
+    }
+  }
+}
+
 }  // namespace fp8p
 
 template <int kD, bool kCap>
@@ -134,10 +163,10 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   w /= p.num_splits;
   const int hk = w % p.Hkv;
   w /= p.Hkv;
-  const int b = w % p.B, r_first = (p.row_tiles - 1 - w / p.B) * 256;
+  const int b = w % p.B, r_first = (p.row_tiles - 1 - w / p.B) * p.cta_rows;
   pdl_wait();
   const SeqLens len = lens_of(p, b);
-  const int R = min(256, len.sq * p.group - r_first);
+  const int R = min(p.cta_rows, len.sq * p.group - r_first);
   if (R <= 0) return;
   const int lo_all = seen_by(p, len.sk, len.sq, fast_div(r_first, p.div_group)).x,
             hi_all = seen_by(p, len.sk, len.sq, fast_div(r_first + R - 1, p.div_group)).y;
@@ -191,14 +220,23 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     constexpr int kPieces = kD / 8;
     float* s_row = reinterpret_cast<float*>(gbase + L::kOffRow);
 #pragma unroll 4
-    for (int i = tid; i < 256 * kPieces; i += 384) {
+    for (int i = tid; i < p.cta_rows * kPieces; i += 384) {
       const int r = i / kPieces, ch = i % kPieces, s = fast_div(r_first + r, p.div_group), h = hk * p.group + r_first + r - s * p.group;
       const __nv_bfloat16* src = r < R ? p.q + b * p.q_b + (int64_t)s * p.q_s + h * p.q_h + 8 * ch : p.q;
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(base + L::kOffV + 16 * i), "l"(src), "r"(r < R ? 16 : 0) : "memory");
     }
+    // the largest scale of values among this CTA's keys, while Q is on its way
+    const int first_key = max(lo_all, t0 << 7), end_key = min(hi_all, (t0 + n) << 7);
+    uint32_t vs_top = 0u;
+    for (int64_t blk = (first_key >> p.log_block) + tid; (blk << p.log_block) < end_key && n > 0; blk += 384) {
+      const int key = (int)(blk << p.log_block), pg = fast_div(key, p.div_page), off = key - pg * p.page_size;
+      const int page = p.table != nullptr ? p.table[(int64_t)b * p.pages_per_seq + pg] : b;
+      if (page >= 0 && page < p.num_pages)
+        vs_top = max(vs_top, __float_as_uint(p.v_scale[((int64_t)page * (p.page_size >> p.log_block) + (off >> p.log_block)) * p.Hkv + hk]) & 0x7fffffffu);
+    }
     asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll 1
-    for (int i = tid; i < 256 * kPieces; i += 384) {
+    for (int i = tid; i < p.cta_rows * kPieces; i += 384) {
       const int r = i / kPieces, ch = i % kPieces;
       const uint4 u = *reinterpret_cast<const uint4*>(gbase + L::kOffV + 16 * i);
       float x[8], y[8];
@@ -227,17 +265,8 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) mbar_arrive(bar(L::kQReady));
-    // the largest scale of values among this CTA's keys
-    const int first_key = max(lo_all, t0 << 7), end_key = min(hi_all, (t0 + n) << 7);
-    uint32_t top = 0u;
-    for (int64_t blk = (first_key >> p.log_block) + tid; (blk << p.log_block) < end_key && n > 0; blk += 384) {
-      const int key = (int)(blk << p.log_block), pg = fast_div(key, p.div_page), off = key - pg * p.page_size;
-      const int page = p.table != nullptr ? p.table[(int64_t)b * p.pages_per_seq + pg] : b;
-      if (page >= 0 && page < p.num_pages)
-        top = max(top, __float_as_uint(p.v_scale[((int64_t)page * (p.page_size >> p.log_block) + (off >> p.log_block)) * p.Hkv + hk]) & 0x7fffffffu);
-    }
-    top = __reduce_max_sync(0xffffffffu, top);
-    if (lane == 0 && top > 0u) atomicMax(s_top, top);
+    vs_top = __reduce_max_sync(0xffffffffu, vs_top);
+    if (lane == 0 && vs_top > 0u) atomicMax(s_top, vs_top);
     asm volatile("bar.sync 1, 384;" ::: "memory");
     // 2^6 / its power of two, and back (1 and 1 where it is no ordinary number)
     const uint32_t top_e = *s_top >> 23;
@@ -403,10 +432,10 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
             float2 y = __fmul2_rn(make_float2(x[2 * j], x[2 * j + 1]), make_float2(kf[j >> 3], kf[j >> 3]));
-            if constexpr (kCap) y = make_float2(p.cap_out * tanh_of(y.x), p.cap_out * tanh_of(y.y));
             x[2 * j] = y.x;
             x[2 * j + 1] = y.y;
           }
+          if constexpr (kCap) cap_scores(x, p.cap_out);
           const int key0 = ((t0 + i) << 7) + (upper ? 64 : 0), lo_in = lo - key0, hi_in = hi - key0;
           if (__any_sync(0xffffffffu, lo_in > 0 || hi_in < 64)) {
 #pragma unroll
