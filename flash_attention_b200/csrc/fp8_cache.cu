@@ -128,6 +128,7 @@ int validate_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f) {
   // (tiles of all sequences and heads are counted in 32 bits)
   if ((int64_t)f->B * c->Hkv * ((int64_t)c->pages_per_seq * c->page_size / 128 + 1) > 0x3fffffffll) return -FA4_E_TOO_LARGE;
   if ((int64_t)f->B * f->Sq * f->Hq > 0x0fffffffll || f->B > 65535 || (int64_t)f->Sq * f->Hq > (1 << 20)) return -FA4_E_TOO_LARGE;
+  if ((int64_t)f->B * c->Hkv * std::max(1, f->num_splits) > 0x7fffffffll) return -FA4_E_TOO_LARGE;       // (CTAs)
   const int64_t strides[] = {f->q_stride_b, f->q_stride_s, f->q_stride_h, f->o_stride_b, f->o_stride_s, f->o_stride_h};
   for (int64_t s : strides)
     if ((s & 7) != 0) return -FA4_E_STRIDE;
@@ -139,12 +140,12 @@ int validate_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f) {
 
 namespace {
 
-// The most tiles of 128 keys that rows of one sequence may see.
-int64_t longest_unit(const fa4_fp8_cache* c, const fa4_fp8_fwd* f) {
+// The most tiles of 128 keys that `tokens` rows of a sequence one behind the other may see.
+int64_t most_tiles(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, int64_t tokens) {
   const int64_t all = ((int64_t)c->pages_per_seq * c->page_size + 127) / 128;
   if (f->window_left < 0) return all;
   const bool open = f->window_right < 0 && !f->causal;         // (to the right)
-  return open ? all : std::min(all, ((int64_t)f->window_left + std::max(0, f->window_right) + f->Sq + 126) / 128 + 1);
+  return open ? all : std::min(all, ((int64_t)f->window_left + std::max(0, f->window_right) + tokens + 126) / 128 + 1);
 }
 
 // How a call is run.
@@ -162,10 +163,13 @@ struct Fp8Plan {
 // wait for the products more often), a merge 5 and the partial results, written and read once at 4 TB/s.  Measured, 128 rows / 256 rows / 256 in two
 // splits, D = 128: 333 rows of 16 heads on as many keys 13.7 / 17.0 / 21.9, 512 of 32 heads on 1024 keys 21.9 / 26.9 / 32.6, on 4096 keys
 // 57.5 / 70.9 / 55.5, three sequences of up to 333 rows of 16 heads on up to 2048 keys 41.0 / 47.4 / 40.4.
-void plan_many(int64_t rows, int64_t units, int64_t tiles, int64_t values, int chosen, Fp8Plan* plan) {
+void plan_many(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, Fp8Plan* plan) {
+  const int group = f->Hq / c->Hkv, chosen = f->num_splits;
+  const int64_t rows = (int64_t)f->Sq * group, units = (int64_t)c->Hkv * f->B, values = (int64_t)f->B * f->Sq * f->Hq * c->D;
   double least = 0;
   for (const int cta_rows : {256, 128}) {
-    const int64_t row_tiles = (rows + cta_rows - 1) / cta_rows, room = kSms / (units * row_tiles);
+    const int64_t row_tiles = (rows + cta_rows - 1) / cta_rows, room = kSms / (units * row_tiles),
+                  tiles = most_tiles(c, f, std::min<int64_t>(f->Sq, (cta_rows - 1) / group + 2));
     if (cta_rows == 128 && (room == 0 || chosen > 0)) break;
     const int64_t most = std::max<int64_t>(1, std::min<int64_t>({128, room, tiles / 2}));
     for (int64_t splits = chosen > 0 ? chosen : 1; splits <= (chosen > 0 ? chosen : most); ++splits) {
@@ -189,13 +193,12 @@ Fp8Plan plan_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f) {
     plan.splits = f->num_splits;
     // Dealing the shares and merging the pieces costs about as much as ten tiles.  us, dealt / a CTA a unit: 128 units of a window of nine
     // tiles, head dim 64 19.0 / 12.6, 8 units of seven tiles 10.5 / 9.2; but 256 units of up to 64 tiles 57.6 / 71.1.
-    if (plan.splits == 0 && units <= kSms && longest_unit(c, f) <= 10) plan.splits = 1;
+    if (plan.splits == 0 && units <= kSms && most_tiles(c, f, f->Sq) <= 10) plan.splits = 1;
     for (plan.bundle = std::min(8, c->Hkv); c->Hkv % plan.bundle != 0;) --plan.bundle;
     plan.slots = plan.splits == 0 ? 2 * kSms : plan.splits == 1 ? 0 : units * plan.splits;
     plan.slot_rows = rows;
   } else {
-    const int64_t tiles = ((int64_t)c->pages_per_seq * c->page_size + 127) / 128;
-    plan_many(rows, units, tiles, (int64_t)f->B * f->Sq * f->Hq * c->D, f->num_splits, &plan);
+    plan_many(c, f, &plan);
     plan.slots = plan.splits == 1 ? 0 : plan.splits;
     plan.slot_rows = (int64_t)f->B * f->Sq * f->Hq;
   }

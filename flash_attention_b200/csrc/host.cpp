@@ -985,7 +985,7 @@ struct Fp8Cache {
 at::Tensor in_pieces(const at::Tensor& t) {
   bool ok = t.stride(-1) == 1 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0;
   for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && t.stride(i) % 8 == 0;
-  return ok ? t : t.contiguous();
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);     // (contiguous() gives one back that merely starts in between)
 }
 
 at::Tensor counts_of(const at::Tensor& t, const char* name, int64_t B, const at::Device& device) {
@@ -1006,6 +1006,8 @@ void describe_cache(Fp8Cache& f, int64_t B) {
   if (D != 64 && D != 128)
     fail(PyExc_NotImplementedError, "head dim %lld is not built for the 8-bit cache; supported: 64 and 128", (long long)D);
   FA4_ASSERT(pages > 0 && size > 0 && H > 0, "the cache is empty");
+  FA4_ASSERT(pages <= 0x7fffffff && size <= 0x7fffffff && H <= 0x7fffffff && (!f.table.defined() || f.table.dim() != 2 || f.table.size(1) <= 0x7fffffff),
+             "the cache or its page table is too large");
   const int64_t blocks = f.k_scale.dim() == 3 ? f.k_scale.size(1) : 0;
   FA4_ASSERT(blocks > 0 && size % blocks == 0 && (size / blocks == 16 || size / blocks == 32 || size / blocks == 64 || size / blocks == 128),
              "k_scale must be (num_pages, page_size / block, heads) for blocks of 16, 32, 64 or 128 tokens, got %s", dims_of(f.k_scale.sizes()).c_str());
@@ -1065,6 +1067,7 @@ void run_append(AppendCall& c) {
   FA4_ASSERT(c.k.dim() == 4 && c.v.dim() == 4 && c.k.sizes() == c.v.sizes(), "k and v must be (B, S, heads, head_dim) both, got %s and %s",
              dims_of(c.k.sizes()).c_str(), dims_of(c.v.sizes()).c_str());
   const int64_t B = c.k.size(0), S = c.k.size(1), H = c.k.size(2), D = c.k.size(3);
+  FA4_ASSERT(B <= 0x7fffffff && S <= 0x7fffffff && (!c.q.defined() || c.q.dim() != 4 || c.q.size(2) <= 0xffff), "k, v or q too large");
   describe_cache(c.f, B);
   const at::Device device = c.f.k.device();
   validate(c.k, "k", {B, S, c.f.c.Hkv, c.f.c.D}, at::kBFloat16, device);
@@ -1152,6 +1155,7 @@ struct Fp8Call {
 void run_fp8(Fp8Call& c) {
   FA4_ASSERT(c.q.dim() == 4, "q must be (B, Sq, heads, head_dim), got %s", dims_of(c.q.sizes()).c_str());
   const int64_t B = c.q.size(0), Sq = c.q.size(1), Hq = c.q.size(2);
+  FA4_ASSERT(B <= 0x7fffffff && Sq <= 0x7fffffff && Hq <= 0x7fffffff, "q too large");
   describe_cache(c.f, B);
   const at::Device device = c.f.k.device();
   const int64_t Hkv = c.f.c.Hkv, D = c.f.c.D;

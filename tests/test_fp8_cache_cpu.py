@@ -101,6 +101,27 @@ def test_bad_attention_calls_are_refused(kw, rc):
     assert L.fa4_fp8_cache_fwd_workspace_bytes(ctypes.byref(cache()), ctypes.byref(fwd(**kw))) == rc
 
 
+@pytest.mark.parametrize("Sq,splits", [(1, 2), (100, 2), (1, 128), (100, 128)])
+def test_a_workspace_that_is_none_is_refused(Sq, splits):
+    """(8 pages x 4 a sequence: nothing is launched)"""
+    L = fa.lib()
+    L.fa4_fp8_cache_fwd_workspace_bytes.restype = ctypes.c_int64
+    c, f = cache(), fwd(Sq=Sq, num_splits=splits)
+    need = L.fa4_fp8_cache_fwd_workspace_bytes(ctypes.byref(c), ctypes.byref(f))
+    # partial results of every split: D values and a sum for each of B x Sq x Hq rows
+    assert need == splits * 2 * Sq * 8 * 129 * 4
+    for kw, rc in ((dict(), NULL), (dict(workspace=4104, workspace_bytes=need), ALIGN), (dict(workspace=4096, workspace_bytes=need - 1), LARGE)):
+        assert L.fa4_fp8_cache_fwd(ctypes.byref(c), ctypes.byref(fwd(Sq=Sq, num_splits=splits, **kw)), None) == rc
+
+
+def test_sizes_beyond_a_launch_are_refused():
+    L = fa.lib()
+    L.fa4_fp8_cache_fwd_workspace_bytes.restype = ctypes.c_int64
+    assert L.fa4_fp8_cache_fwd_workspace_bytes(ctypes.byref(cache(Hkv=1 << 10)), ctypes.byref(fwd(B=1 << 15, Hq=1 << 10, num_splits=128))) == LARGE
+    # tiles of all sequences and heads
+    assert L.fa4_fp8_cache_fwd_workspace_bytes(ctypes.byref(cache(Hkv=1 << 10, pages_per_seq=1 << 12)), ctypes.byref(fwd(B=1 << 10, Hq=1 << 10))) == LARGE
+
+
 def test_exports():
     for name in _lib.EXPORTS_FP8:
         assert hasattr(fa.lib(), name)

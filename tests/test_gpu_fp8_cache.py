@@ -493,8 +493,205 @@ def test_long_contexts_on_a_full_gpu(cuda_device, B, Sq, Hq, H, D, size, block, 
         want, want_lse = orc.attend(q[b], kb, vb, Sq, causal=True)
         mag, _ = orc.attend(q[b], kb, vb.abs(), Sq, causal=True)
         off = (got[0][0][b].double() - want).abs()
-        # 2^-8 of each weight in the worst case; of thousands that are independent, far less: what a wrong scale of one tile would
-        # show against is the root of the sum of squares, sqrt(sum p^2 v^2) <= sqrt(max p) sqrt(sum p v^2); here five of these
+        # 2^-8 of each weight in the worst case.  Thousands of independent roundings do not add up like that: the output's own have a root
+        # mean square below 2^-8 / sqrt(3) of it, those of the weights (2^-9 of each at most) one below 2^-9 sqrt(sum p^2 v^2), and with values of
+        # random signs that root is the size of an output.  So the norm is off by less than 2^-8 of it, which a wrong scale of one tile is not.
         assert (off <= 2.0 ** -8 * (mag + want.abs())).all()
         assert off.norm() <= 2.0 ** -8 * want.norm()
         assert (got[0][1][b].double() - want_lse).abs().max() <= 2.0 ** -18 * want_lse.abs().max()
+
+
+@pytest.mark.parametrize("B,Sq,Hq,H,D,n", [(1, 64, 8, 2, 128, 64), (1, 200, 8, 2, 64, 1000), (1, 130, 16, 1, 128, 5000), (3, 150, 8, 4, 128, 1500), (9, 100, 16, 4, 64, 700),
+                                           (2, 600, 16, 8, 128, 600), (1, 33, 8, 8, 128, 9000), (2, 40, 40, 1, 128, 300)])
+def test_rows_of_a_cta_and_splits(cuda_device, B, Sq, Hq, H, D, n):
+    """Many rows, few or many CTAs, short or long: tiles of 128 and of 256 rows, with and without splits."""
+    attend_both(cuda_device, B, Sq, Hq, H, D, 64, 64, [n - 17 * b for b in range(B)], fresh=[Sq - 11 * b for b in range(B)], causal=True)
+    attend_both(cuda_device, B, Sq, Hq, H, D, 64, 64, [n - 17 * b for b in range(B)], window_size=(300, 20))
+
+
+@pytest.mark.parametrize("softcap", [0.5, 2.0, 8.0, 50.0])
+@pytest.mark.parametrize("Sq", [1, 70])
+def test_soft_caps_below_and_above_the_scores(cuda_device, Sq, softcap):
+    """Scores of a few units: warps whose scores are all below 0.75 of the cap, all above, and both."""
+    for D, q_scale in ((64, 1.0), (128, 3.0)):
+        attend_both(cuda_device, 2, Sq, 8, 2, D, 64, 64, [Sq + 700, Sq + 5], causal=True, softcap=softcap, q_scale=q_scale)
+
+
+@pytest.mark.parametrize("B,Sq,Hq,H", [(9, 3, 24, 12), (9, 1, 14, 7), (9, 2, 11, 11), (70, 4, 8, 8), (9, 40, 24, 12)])
+@pytest.mark.parametrize("splits", [0, 2])
+def test_sequences_without_rows_or_keys_between_others(cuda_device, B, Sq, Hq, H, splits):
+    lens = [(b * 211) % 900 if b % 4 else 0 for b in range(B)]
+    fresh = [0 if b % 3 == 1 else max(1, Sq - b % 3) for b in range(B)]
+    attend_both(cuda_device, B, Sq, Hq, H, 64, 32, 32, lens, fresh=fresh, causal=True, splits=splits)
+    attend_both(cuda_device, B, Sq, Hq, H, 128, 32, 32, lens, fresh=[0] * (B - 1) + [1], causal=True, splits=splits)
+
+
+def batch_of(device, B, n, H=2, D=128, size=64, seed=1):
+    """A cache of B sequences of n tokens, its table."""
+    per = -(-n // size)
+    cache = make_cache(B * per + 1, size, H, D, 64, seed, "cpu")
+    cache = fa.FP8KVCache(*(getattr(cache, f).to(device) for f in ("k", "v", "k_scale", "v_scale")))
+    tables = tables_of(B, per, B * per + 1, seed)
+    fill(cache, tables, [n] * B, seed)
+    return cache, torch.tensor(tables, dtype=torch.int32, device=device)
+
+
+@pytest.mark.parametrize("Sq", [1, 6, 100])
+@pytest.mark.parametrize("splits", [1, 3])
+def test_a_chosen_split_count_gives_the_bits_of_the_entry_alone(cuda_device, Sq, splits):
+    cache, table = batch_of(cuda_device, 5, 1000)
+    lens = torch.tensor([1000, 3, 640, 641, 129], dtype=torch.int32, device=cuda_device)
+    q = torch.randn(5, Sq, 8, 128, device=cuda_device).bfloat16()
+    out, lse = fa.flash_attn_fp8_cache_func(q, cache, lens, page_table=table, causal=True, num_splits=splits, return_lse=True)
+    for b in range(5):
+        o, l = fa.flash_attn_fp8_cache_func(q[b:b + 1], cache, lens[b:b + 1], page_table=table[b:b + 1], causal=True, num_splits=splits, return_lse=True)
+        assert torch.equal(o[0], out[b]) and torch.equal(l[0], lse[b])
+    fa.check_status(cuda_device)
+
+
+def test_keys_that_no_row_sees_may_be_anything(cuda_device):
+    """NaN bytes and NaN scales in front of a window and behind the last token; pages of the table there that do not exist."""
+    cache, table = batch_of(cuda_device, 2, 1000)
+    lens = torch.tensor([950, 700], dtype=torch.int32, device=cuda_device)
+    for Sq, Hq in ((1, 8), (6, 8), (50, 8), (200, 8)):
+        for cap in (0.0, 10.0):
+            q = torch.randn(2, Sq, Hq, 128, device=cuda_device).bfloat16()
+            args = dict(page_table=table, window_size=(100, 0), softcap=cap, return_lse=True)
+            want = fa.flash_attn_fp8_cache_func(q, cache, lens, **args)
+            bad = fa.FP8KVCache(cache.k.clone(), cache.v.clone(), cache.k_scale.clone(), cache.v_scale.clone())
+            gone = table.clone()
+            for b, n in enumerate([950, 700]):
+                first = max(0, n - Sq - 100)       # row 0 stands at n - Sq and sees 100 keys in front of it
+                for i, page in enumerate(table[b].tolist()):
+                    seen_lo, seen_hi = max(0, first - 64 * i), min(64, n - 64 * i)
+                    if seen_hi <= 0 or seen_lo >= 64:
+                        gone[b, i] = -5
+                        bad.k_scale[page] = bad.v_scale[page] = math.nan
+                        seen_lo, seen_hi = 64, 64
+                    for t in (bad.k, bad.v):
+                        t[page, :seen_lo].view(torch.uint8).fill_(0x7F)
+                        t[page, max(0, seen_hi):].view(torch.uint8).fill_(0x7F)
+            args["page_table"] = gone
+            got = fa.flash_attn_fp8_cache_func(q, bad, lens, **args)
+            fa.check_status(cuda_device)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_calls_on_two_streams_at_once(cuda_device):
+    """Workspaces and results of calls that run side by side are their own."""
+    cache, table = batch_of(cuda_device, 4, 2000)
+    lens = torch.tensor([2000, 1500, 77, 1999], dtype=torch.int32, device=cuda_device)
+    sizes = [(1, 4, 0), (5, 4, 0), (120, 8, 0), (1, 4, 4), (120, 8, 3)]
+    qs = [[torch.randn(4, Sq, Hq, 128, device=cuda_device).bfloat16() for _ in range(2)] for Sq, Hq, _ in sizes]
+    run = lambda q, sp: fa.flash_attn_fp8_cache_func(q, cache, lens, page_table=table, causal=True, num_splits=sp)[0]
+    want = [[run(q, size[2]) for q in pair] for pair, size in zip(qs, sizes)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        for i, (pair, size) in enumerate(zip(qs, sizes)):
+            for j in (0, 1):
+                with torch.cuda.stream(streams[j]):
+                    got[j].append((i, run(pair[j], size[2])))
+    torch.cuda.synchronize()
+    fa.check_status(cuda_device)
+    for j in (0, 1):
+        for i, out in got[j]:
+            assert torch.equal(out, want[i][j])
+
+
+@pytest.mark.parametrize("Sq,splits", [(1, 0), (6, 0), (1, 3), (90, 0), (90, 2)])
+def test_a_replayed_graph_reads_the_lengths_anew(cuda_device, Sq, splits):
+    cache, table = batch_of(cuda_device, 4, 1500)
+    q = torch.randn(4, Sq, 8, 128, device=cuda_device).bfloat16()
+    lens = torch.tensor([1, 1, 1, 1], dtype=torch.int32, device=cuda_device)
+    rows = torch.tensor([Sq] * 4, dtype=torch.int32, device=cuda_device)
+    out, lse = torch.zeros_like(q), torch.zeros(4, 8, Sq, device=cuda_device)
+    run = lambda **kw: fa.flash_attn_fp8_cache_func(q, cache, lens, page_table=table, seqused_q=rows, causal=True, num_splits=splits, return_lse=True, **kw)
+    run()
+    torch.cuda.synchronize()
+    graph, twin = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run(out=out, lse=lse)
+    with torch.cuda.graph(twin):
+        again = run()
+    for new, n in (([1500, 3, 0, 900], [Sq, 1, Sq, 0]), ([64, 1499, 1024, 1], [Sq] * 4), ([0, 0, 0, 0], [Sq] * 4), ([1500] * 4, [Sq, 0, 0, Sq])):
+        lens.copy_(torch.tensor(new, dtype=torch.int32))
+        rows.copy_(torch.tensor(n, dtype=torch.int32))
+        want = run()
+        out.zero_()
+        lse.zero_()
+        graph.replay()
+        twin.replay()
+        fa.check_status(cuda_device)
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+        for a, w in zip(again, want):
+            assert torch.equal(a, w)
+
+
+def test_offsets_that_pass_32_bits(cuda_device):
+    """Pages 2^31 + 2^20 bytes apart: the bytes and the results of a compact pool."""
+    far = (1 << 31) + (1 << 20)
+    compact = make_cache(3, 256, 2, 128, 64, 1, cuda_device)
+    room = [torch.empty(2 * far + 256 * 2 * 128, dtype=torch.uint8, device=cuda_device) for _ in range(2)]
+    wide = fa.FP8KVCache(*(t.as_strided((3, 256, 2, 128), (far, 256, 128, 1)) for t in room), torch.empty_like(compact.k_scale), torch.empty_like(compact.v_scale))
+    k, v = (torch.randn(1, 600, 2, 128, device=cuda_device).bfloat16() for _ in range(2))
+    table = torch.tensor([[2, 1, 0]], dtype=torch.int32, device=cuda_device)
+    for c in (compact, wide):
+        c.k_scale.zero_()
+        c.v_scale.zero_()
+        for x in (c.k, c.v):
+            for page in range(3):
+                x[page].view(torch.uint8).fill_(0x7F)
+        fa.append_kv_fp8(c, k, v, torch.zeros(1, dtype=torch.int32, device=cuda_device), page_table=table)
+        fa.append_kv_fp8(c, k[:, :1], v[:, :1], torch.full((1,), 600, dtype=torch.int32, device=cuda_device), page_table=table)
+    for a, b in ((compact.k, wide.k), (compact.v, wide.v)):
+        assert all(torch.equal(a[p].view(torch.uint8), b[p]) for p in range(3))
+    lens = torch.tensor([601], dtype=torch.int32, device=cuda_device)
+    for Sq in (1, 100):
+        q = torch.randn(1, Sq, 4, 128, device=cuda_device).bfloat16()
+        got = [fa.flash_attn_fp8_cache_func(q, c, lens, page_table=table, causal=True)[0] for c in (compact, wide)]
+        assert torch.equal(*got)
+    fa.check_status(cuda_device)
+
+
+def test_operands_that_start_between_pieces_are_copied(cuda_device):
+    """Contiguous, but two bytes behind a 16-byte boundary."""
+    cache, table = batch_of(cuda_device, 1, 200)
+    lens = torch.tensor([150], dtype=torch.int32, device=cuda_device)
+    for Sq in (1, 40):
+        q = torch.randn(1, Sq, 8, 128, device=cuda_device).bfloat16()
+        odd = torch.empty(q.numel() + 1, dtype=q.dtype, device=cuda_device)[1:].view(q.shape)
+        odd.copy_(q)
+        got = [fa.flash_attn_fp8_cache_func(x, cache, lens, page_table=table, causal=True)[0] for x in (q, odd)]
+        assert torch.equal(*got)
+        twin = fa.FP8KVCache(*(getattr(cache, n).clone() for n in ("k", "v", "k_scale", "v_scale")))
+        for c, x in ((cache, q), (twin, odd)):
+            fa.append_kv_fp8(c, x[:, :, :2], x[:, :, 2:4].contiguous(), lens, page_table=table)
+        assert torch.equal(cache.k.view(torch.uint8), twin.k.view(torch.uint8)) and torch.equal(cache.v.view(torch.uint8), twin.v.view(torch.uint8))
+
+
+def test_refusals_on_the_gpu(cuda_device):
+    cache, table = batch_of(cuda_device, 2, 100)
+    lens = torch.tensor([90, 80], dtype=torch.int32, device=cuda_device)
+    q = torch.zeros(2, 1, 8, 128, dtype=torch.bfloat16, device=cuda_device)
+    ok = dict(page_table=table)
+    call = lambda q=q, cache=cache, lens=lens, **kw: fa.flash_attn_fp8_cache_func(q, cache, lens, **dict(ok, **kw))
+    for bad in (dict(q=q.half()), dict(q=q[:, :, :3]), dict(q=q[:1]), dict(lens=lens.long()), dict(lens=lens[:1]), dict(page_table=table.long()),
+                dict(page_table=table[:1]), dict(seqused_q=lens.cpu()), dict(out=q[..., :64]), dict(out=torch.zeros(2, 1, 8, 132, dtype=q.dtype, device=cuda_device)[..., 4:]),
+                dict(lse=torch.zeros(2, 1, 8, device=cuda_device)), dict(learnable_sink=torch.zeros(3, device=cuda_device)), dict(softcap=-1.0),
+                dict(softcap=math.inf), dict(softmax_scale=0.0), dict(num_splits=129), dict(num_splits=-1)):
+        with pytest.raises((AssertionError, ValueError, TypeError, RuntimeError, NotImplementedError)):
+            call(**bad)
+    k = torch.zeros(2, 3, 2, 128, dtype=torch.bfloat16, device=cuda_device)
+    cos = torch.zeros(200, 64, device=cuda_device)
+    put = lambda k=k, v=k, lens=lens, **kw: fa.append_kv_fp8(cache, k, v, lens, **dict(ok, **kw))
+    for bad in (dict(k=k.float()), dict(v=k[:, :2]), dict(k=k[:, :, :1], v=k[:, :, :1]), dict(lens=lens.float()), dict(seqused_new=lens[:1]), dict(q=k),
+                dict(rotary_cos=cos), dict(rotary_cos=cos, rotary_sin=cos.bfloat16()), dict(rotary_cos=cos[:, :4], rotary_sin=cos[:, :4]),
+                dict(rotary_cos=cos.cpu(), rotary_sin=cos.cpu()), dict(rotary_cos=cos, rotary_sin=cos, q=k[:, :1]), dict(page_table=None, k=k.repeat(9, 1, 1, 1), v=k.repeat(9, 1, 1, 1), lens=lens.repeat(9))):
+        with pytest.raises((AssertionError, ValueError, TypeError, RuntimeError, NotImplementedError)):
+            put(**bad)
+    torch.cuda.synchronize()
+    fa.check_status(cuda_device)
