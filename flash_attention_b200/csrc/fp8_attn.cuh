@@ -95,12 +95,18 @@ __device__ __forceinline__ void merge_row(const Fp8Params& p, int b, int s, int 
     float l[8], top = m;
     float4 v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) l[j] = i0 + j < n ? p.lse_partial[at(i0 + j)] : -INFINITY;
+    for (int j = 0; j < 8; ++j) {
+      l[j] = -INFINITY;
+      v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i0 + j < n) {
+        l[j] = p.lse_partial[at(i0 + j)];
+        if (col < p.D) v[j] = *reinterpret_cast<const float4*>(p.o_partial + at(i0 + j) * p.D + col);
+      }
+    }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      // (a part without a key wrote no values)
-      v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (l[j] != -INFINITY && col < p.D) v[j] = *reinterpret_cast<const float4*>(p.o_partial + at(i0 + j) * p.D + col);
+      // (a part without a key wrote no values; they are asked for with the sums all the same)
+      if (l[j] == -INFINITY) v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
       top = fmaxf(top, l[j]);
     }
     const float ref = top == -INFINITY ? 0.f : top, keep = ex2_approx(m - ref);

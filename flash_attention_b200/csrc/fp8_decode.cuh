@@ -805,8 +805,11 @@ __global__ void __launch_bounds__(kFp8CombineWarps * 32) fp8_merge_kernel(const 
   pdl_wait();
   if (r >= rows) return;
   const int bs = fast_div((int)r, p.div_hq), h = (int)r - bs * p.Hq, b = fast_div(bs, p.div_sq), s = bs - b * p.Sq;
-  if (p.fresh != nullptr && s >= p.fresh[b]) return;
   const int hk = fast_div(h, p.div_group), row = s * p.group + h - hk * p.group, unit = b * p.Hkv + hk;
+  // (asked for together; a sequence without rows has no pieces noted)
+  const int rows_here = p.fresh != nullptr ? p.fresh[b] : p.Sq;
+  const int2 at = p.num_splits == 0 ? p.pieces[unit] : make_int2(0, 0);
+  if (s >= rows_here) return;
   int64_t first, step;
   int pieces = p.num_splits;
   if (pieces > 0) {
@@ -817,7 +820,6 @@ __global__ void __launch_bounds__(kFp8CombineWarps * 32) fp8_merge_kernel(const 
     const int places = fp8d::cost_of(fp8d::seq_of(p, len.sk, len.sq)), per = (places + pieces - 1) / pieces;
     pieces = (places + per - 1) / per;
   } else {
-    const int2 at = p.pieces[unit];
     pieces = at.y;
     first = 2 * (int64_t)at.x;          // (a CTA has two slots: of the unit it begins in the middle of, of the one it leaves there)
     step = 2 * p.bundle;
