@@ -428,22 +428,33 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         // 64 scores to weights (two to a word); `upper`: keys 64-127 of the step
         auto weights = [&](float (&x)[64], const bool upper, uint32_t (&pw)[32]) {
           const float4 ks = *reinterpret_cast<const float4*>(sc + (upper ? 4 : 0));
-          const float kf[4] = {ks.x * factor, ks.y * factor, ks.z * factor, ks.w * factor};
+          float kf[4] = {ks.x * factor, ks.y * factor, ks.z * factor, ks.w * factor};
+          if constexpr (kCap) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            float2 y = __fmul2_rn(make_float2(x[2 * j], x[2 * j + 1]), make_float2(kf[j >> 3], kf[j >> 3]));
-            x[2 * j] = y.x;
-            x[2 * j + 1] = y.y;
+            for (int j = 0; j < 32; ++j) {
+              const float2 y = __fmul2_rn(make_float2(x[2 * j], x[2 * j + 1]), make_float2(kf[j >> 3], kf[j >> 3]));
+              x[2 * j] = y.x;
+              x[2 * j + 1] = y.y;
+            }
+            cap_scores(x, p.cap_out);
+          } else {
+            // (the factors go into the exponents' multiply-add and the groups' maxima; 0 would make NaN of a masked score)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) kf[k] = kf[k] == 0.f ? 1.17549435e-38f : kf[k];
           }
-          if constexpr (kCap) cap_scores(x, p.cap_out);
           const int key0 = ((t0 + i) << 7) + (upper ? 64 : 0), lo_in = lo - key0, hi_in = hi - key0;
           if (__any_sync(0xffffffffu, lo_in > 0 || hi_in < 64)) {
 #pragma unroll
             for (int j = 0; j < 64; ++j) x[j] = j >= lo_in && j < hi_in ? x[j] : -INFINITY;
           }
-          float top = fmaxf(x[0], x[1]);
+          float top = -INFINITY;
 #pragma unroll
-          for (int j = 2; j < 64; j += 2) top = fmax3(top, x[j], x[j + 1]);
+          for (int k = 0; k < 4; ++k) {
+            float m = fmaxf(x[16 * k], x[16 * k + 1]);
+#pragma unroll
+            for (int j = 2; j < 16; j += 2) m = fmax3(m, x[16 * k + j], x[16 * k + j + 1]);
+            top = fmaxf(top, kCap ? m : m * kf[k]);
+          }
           // the reference follows when the row's weights would pass 2^8
           const bool moved = top > m_ref + 8.f;
           if (__any_sync(0xffffffffu, moved)) {
@@ -483,7 +494,8 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
           const float vs[4] = {vs4.x * vs_up, vs4.y * vs_up, vs4.z * vs_up, vs4.w * vs_up};
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
-            const float2 y = __fadd2_rn(make_float2(x[2 * j], x[2 * j + 1]), ref2);
+            const float2 xx = make_float2(x[2 * j], x[2 * j + 1]);
+            const float2 y = kCap ? __fadd2_rn(xx, ref2) : __ffma2_rn(xx, make_float2(kf[j >> 3], kf[j >> 3]), ref2);
             const float2 e = make_float2(ex2_approx(y.x), ex2_approx(y.y));
             l2[j & 1] = __fadd2_rn(l2[j & 1], e);
             const float2 wv = __fmul2_rn(e, make_float2(vs[j >> 3], vs[j >> 3]));
