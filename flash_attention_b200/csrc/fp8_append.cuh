@@ -13,9 +13,12 @@
 // bytes are read and written by the same threads.  A thread has 16 elements of a row, as two 16-byte pieces that hold eight whole
 // pairs.  With several rows it turns each twice, for the maximum and for the bytes, the second time from L1.
 //
-// What bounds it: a prompt moves 2 B in and 1 B out an element, but an element takes 8 (V) to 15 (K) instructions, and issue and ALU pipe come
-// close to the HBM.  So what is not finite is looked for by one multiply-add an element and treated on a path of its own (27
-// instructions an element without it).
+// What bounds it: 2 x 8192 tokens of 8 kv heads with 32 query heads, D = 128, blocks of 128: 87 us, 41 of them keys and values (101 MB, 2.5 TB/s), the rest q
+// (268 MB, 5.8 TB/s).  Keys and values wait for loads (11 warps of an average instruction's latency, issue slots 42 % busy, 32 warps of an SM
+// with 63 registers): a row is read twice, the angles of a key come from L1.  Not finite values are looked for by one multiply-add an element and
+// treated on a path of their own; with that and the rows a thread has, keys and values went from 57 to 41.  More rows in flight (loops unrolled by four
+// rather than two) 45, the loads of four query heads in front of their stores 45 with q's part unchanged: fewer warps.  A few tokens are a
+// launch: 64 sequences of one token 2.9 us in a graph.
 #pragma once
 #include "ptx.cuh"
 #include <cuda_bf16.h>

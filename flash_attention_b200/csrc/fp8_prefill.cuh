@@ -10,10 +10,15 @@
 //
 // A CTA has two tiles of 128 rows (row r = token r / group, head r % group of a kv head), a softmax warpgroup each (thread = row).  S of a
 // tile is two halves of 64 columns.  A softmax warpgroup takes the upper half (keys 64-127) to registers first, and Q K^T of the next step's upper half
-// may overwrite it at once; W goes where the lower half was, then W V and Q K^T of the next lower half follow it.  So the softmax, which
-// is what bounds the kernel (the exponentials of 256 rows x 128 keys take 2048 clocks, the products 2048 beside them), finds its next
-// scores waiting.  With one product of 128 columns the softmax waited 1500 of 4000 clocks for W V and Q K^T: B = 1, 1024 rows of 32 heads
-// on 16384 keys 294 us.
+// may overwrite it at once; W goes where the lower half was, then W V and Q K^T of the next lower half follow it.  So the softmax finds its next
+// scores waiting (with one product of 128 columns it waited 1500 of 4000 clocks for W V and Q K^T: 294 us for the first call below).
+//
+// What bounds it: no unit alone.  A step of 256 rows x 128 keys takes about 3300 clocks: the exponentials 2048, the products 2560 (Q K^T in halves of 64
+// columns 48 clocks an instruction, bound by shared memory), 1700 issue slots a scheduler, in chains between two warps of a scheduler.  D = 128, B = 1:
+// 1024 rows of 32 heads on 16384 keys 238 us (162 at the measured rate of bf16 products), tensor pipe 62 %, exponential unit 62 %, issue slots 53 %
+// busy; 8192 rows of 64 heads on as many keys 1000-1080 us (669), causal.  A CTA's start and end take 12000 clocks, 8000 of them Q.
+// Exponentials by polynomials: one in eight 253, one in four 261 (more instructions between the others); the logarithm of a value scale in the
+// exponents where a half has one: 248; the lower scores loaded in front of the upper exponentials or between them: 282, 247.
 //
 // Warps: 0-3 and 4-7 softmax, 8-11 widen the tiles of V (cvt.f16x2.e4m3x2 runs at 64 a clock beside the exponentials), 12 and 14 load, 13 issues
 // the products.  Every wait is bounded (those of the softmax warps, which leave no registers for a call, by the issuer's: see mbar_wait_flag); a warp
