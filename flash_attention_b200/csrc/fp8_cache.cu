@@ -127,7 +127,7 @@ int validate_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f) {
   if (!(f->softmax_scale > 0.f) || !(f->softcap >= 0.f) || f->num_splits < 0 || f->num_splits > 128) return -FA4_E_SHAPE;
   // (tiles of all sequences and heads are counted in 32 bits)
   if ((int64_t)f->B * c->Hkv * ((int64_t)c->pages_per_seq * c->page_size / 128 + 1) > 0x3fffffffll) return -FA4_E_TOO_LARGE;
-  if ((int64_t)f->B * f->Sq * f->Hq > 0x0fffffffll || f->B > 65535 || (int64_t)f->Sq * f->Hq > (1 << 20)) return -FA4_E_TOO_LARGE;
+  if ((int64_t)f->B * f->Sq * f->Hq > 0x0fffffffll || f->B > 65535) return -FA4_E_TOO_LARGE;
   if ((int64_t)f->B * c->Hkv * std::max(1, f->num_splits) > 0x7fffffffll) return -FA4_E_TOO_LARGE;       // (CTAs)
   const int64_t strides[] = {f->q_stride_b, f->q_stride_s, f->q_stride_h, f->o_stride_b, f->o_stride_s, f->o_stride_h};
   for (int64_t s : strides)

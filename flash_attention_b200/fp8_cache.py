@@ -22,8 +22,8 @@ class FP8KVCache:
 
     k, v              (num_pages, page_size, heads, head_dim) float8_e4m3fn (or its bytes as uint8); head_dim 64 or 128, contiguous;
                       the other strides are multiples of 16 bytes, so a pool stored as (page, head, token) is passed transposed
-    k_scale, v_scale  (num_pages, page_size / block, heads) fp32, contiguous: value = byte * scale.  ``block`` tokens (16, 32,
-                      64 or 128) share a scale
+    k_scale, v_scale  (num_pages, page_size / block, heads) fp32, contiguous: value = byte * scale, no scale below 0.  ``block`` tokens
+                      (16, 32, 64 or 128) share a scale
     """
     k: torch.Tensor
     v: torch.Tensor
@@ -80,7 +80,7 @@ def append_kv_fp8(
 
     The scale of a block is the smallest power of two that leaves its values at most 448; it grows with the tokens, and those
     in the block are then rounded to the new one (exact but for values 2^15 below the largest).  A value that is not finite is
-    stored as NaN.  One launch, no synchronisation; can be captured in a graph.  Positions behind the cache's or the
+    stored as NaN.  Nothing here is differentiable.  One launch, no synchronisation; can be captured in a graph.  Positions behind the cache's or the
     tables' end and page numbers outside the pool cannot be refused here (they are on the device): such
     tokens are left out, or turned by the tables' last row, and :func:`check_status` raises.  No block may belong to two sequences that append to it in one call.
     """
@@ -111,7 +111,8 @@ def flash_attn_fp8_cache_func(
     ``window_size`` refer to.  ``learnable_sink``, ``softcap``, ``num_splits`` (0: chosen), ``out`` and ``lse`` as in
     :func:`flash_attn_fp4_func`; a row that sees nothing gets zeros and an lse of -inf.
 
-    The cache behind a sequence's last token may hold anything, NaN included.  A NaN in a value that some row of a sequence sees may
+    Not differentiable.  A length beyond the cache's or the table's end counts as that end, a negative one as 0 (they are on the device and cannot be
+    refused).  The cache behind a sequence's last token may hold anything, NaN included.  A NaN in a value that some row of a sequence sees may
     reach the other rows of that sequence too.  Page numbers outside the pool stand for keys and values of zero, and
     :func:`check_status` raises.
     """

@@ -695,3 +695,45 @@ def test_refusals_on_the_gpu(cuda_device):
             put(**bad)
     torch.cuda.synchronize()
     fa.check_status(cuda_device)
+
+
+def test_blocks_whose_scale_is_zero(cuda_device):
+    """Keys and values of zero, among others, next to masked keys."""
+    cache, table = batch_of(cuda_device, 1, 600)
+    g = torch.Generator().manual_seed(3)
+    for t in (cache.k_scale, cache.v_scale):
+        t.mul_((torch.rand(t.shape, generator=g) < 0.6).to(t))
+    lens = torch.tensor([590], dtype=torch.int32, device=cuda_device)
+    k, v = held_of(cache, table[0].tolist(), 590)
+    assert (k.abs().amax(dim=-1) == 0).any() and (v.abs().amax(dim=-1) == 0).any()
+    for Sq in (1, 6, 90):
+        for kw in (dict(causal=True), dict(window_size=(70, 0)), dict(causal=True, softcap=10.0)):
+            q = torch.randn(1, Sq, 8, 128, generator=g).bfloat16()
+            out, lse = fa.flash_attn_fp8_cache_func(q.to(cuda_device), cache, lens, page_table=table, return_lse=True, **kw)
+            fa.check_status(cuda_device)
+            args = dict(causal=kw.get("causal", False), window=kw.get("window_size", (None, None)), softcap=kw.get("softcap", 0.0))
+            want, want_lse = orc.attend(q[0], k, v, Sq, **args)
+            mag, _ = orc.attend(q[0], k, v.abs(), Sq, **args)
+            assert ((out[0].cpu().double() - want).abs() <= 2.0 ** -8 * (mag + want.abs()) + 2.0 ** -13 * mag).all()
+            assert ((lse[0].cpu().double() - want_lse).abs() <= 2.0 ** -17 * want_lse.abs().clamp(min=1.0)).all()
+
+
+def test_lengths_beyond_the_end_count_as_the_end(cuda_device):
+    cache, table = batch_of(cuda_device, 2, 256)
+    for Sq in (1, 50):
+        q = torch.randn(2, Sq, 8, 128, device=cuda_device).bfloat16()
+        call = lambda n: fa.flash_attn_fp8_cache_func(q, cache, torch.tensor(n, dtype=torch.int32, device=cuda_device), page_table=table, causal=True, return_lse=True)
+        for a, b in zip(call([2 ** 31 - 1, -5]), call([256, 0])):
+            assert torch.equal(a, b)
+        fa.check_status(cuda_device)
+
+
+def test_more_than_a_million_rows(cuda_device):
+    cache, table = batch_of(cuda_device, 1, 200)
+    lens = torch.tensor([200], dtype=torch.int32, device=cuda_device)
+    q = torch.randn(1, 40000, 32, 128, device=cuda_device, dtype=torch.bfloat16)
+    out, lse = fa.flash_attn_fp8_cache_func(q, cache, lens, page_table=table, num_splits=1, return_lse=True)
+    for a, b in ((0, 4096), (20000, 20001 + 64), (39936, 40000)):
+        o, l = fa.flash_attn_fp8_cache_func(q[:, a:b], cache, lens, page_table=table, num_splits=1, return_lse=True)
+        assert torch.equal(o, out[:, a:b]) and torch.equal(l, lse[:, :, a:b])
+    fa.check_status(cuda_device)
