@@ -88,6 +88,9 @@ APPENDS = [
     (2, 50, 4, 64, 64, 64, True, [60, 0], [50, 9], 16, True, 4, torch.bfloat16),
     (2, 300, 2, 128, 16, 16, True, [5, 31], [300, 17], 128, False, 2, torch.float32),
     (1, 500, 2, 64, 512, 128, False, [12], None, 64, True, 9, torch.float32),
+    # queries enough for four heads a thread, the last group of a row with fewer
+    (2, 3300, 1, 128, 256, 128, True, [3, 0], [3300, 1000], 128, False, 6, torch.float32),
+    (1, 9000, 1, 64, 128, 64, False, [0], None, 32, True, 9, torch.bfloat16),
 ]
 
 
