@@ -16,7 +16,8 @@
 // What bounds it: no unit alone.  A step of 256 rows x 128 keys takes about 3300 clocks: the exponentials 2048, the products 2560 (Q K^T in halves of 64
 // columns 48 clocks an instruction, bound by shared memory), 1700 issue slots a scheduler, in chains between two warps of a scheduler.  D = 128, B = 1:
 // 1024 rows of 32 heads on 16384 keys 238 us (162 at the measured rate of bf16 products), tensor pipe 62 %, exponential unit 62 %, issue slots 53 %
-// busy; 8192 rows of 64 heads on as many keys 1000-1080 us (669), causal.  A CTA's start and end take 12000 clocks, 8000 of them Q.
+// busy; 8192 rows of 64 heads on as many keys, causal, 940 us at first and 1080 under the power cap
+// (669, or 793 at the sustained rate).  A CTA's start and end take 12000 clocks, 8000 of them Q.
 // Exponentials by polynomials: one in eight 253, one in four 261 (more instructions between the others); the logarithm of a value scale in the
 // exponents where a half has one: 248; the lower scores loaded in front of the upper exponentials or between them: 282, 247.
 //
