@@ -515,7 +515,7 @@ def test_rows_of_a_cta_and_splits(cuda_device, B, Sq, Hq, H, D, n):
 @pytest.mark.parametrize("softcap", [0.5, 2.0, 8.0, 50.0])
 @pytest.mark.parametrize("Sq", [1, 70])
 def test_soft_caps_below_and_above_the_scores(cuda_device, Sq, softcap):
-    """Scores of a few units: warps whose scores are all below 0.75 of the cap, all above, and both."""
+    """Scores of a few units: warps whose scores are all well below the cap, all above, and both."""
     for D, q_scale in ((64, 1.0), (128, 3.0)):
         attend_both(cuda_device, 2, Sq, 8, 2, D, 64, 64, [Sq + 700, Sq + 5], causal=True, softcap=softcap, q_scale=q_scale)
 
