@@ -196,6 +196,7 @@ Fp8Plan plan_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f) {
     // Dealing the shares and merging the pieces costs about as much as ten tiles.  us, dealt / a CTA a unit: 128 units of a window of nine
     // tiles, head dim 64 19.0 / 12.6, 8 units of seven tiles 10.5 / 9.2; but 256 units of up to 64 tiles 57.6 / 71.1.
     if (plan.splits == 0 && units <= kSms && most_tiles(c, f, f->Sq) <= 10) plan.splits = 1;
+    // (us, up to 8 / 4 heads side by side, which are 144 / 148 CTAs: 32 sequences of up to 8192 keys 55 / 60, drafted tokens on pages of 16 29 / 32.5)
     for (plan.bundle = std::min(8, c->Hkv); c->Hkv % plan.bundle != 0;) --plan.bundle;
     plan.slots = plan.splits == 0 ? 2 * kSms : plan.splits == 1 ? 0 : units * plan.splits;
     plan.slot_rows = rows;
