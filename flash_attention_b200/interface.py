@@ -58,8 +58,11 @@ def check_status(device=None) -> None:
     if v != 0:
         w.zero_()
         code, site, epoch, blk = v >> 24, (v >> 16) & 0xFF, (v >> 8) & 0xFF, v & 0xFF
-        raise RuntimeError(f"fa4_nvfp4 kernel failure: code {code} (1 = bounded wait expired, "
-                           f"2 = index outside its range), site {site}, launch epoch {epoch}, block {blk} (mod 256)")
+        if code == 2:
+            raise RuntimeError(f"fa4_nvfp4: code 2 (an index on the device is outside its range, and what it leads to was left out), "
+                               f"site {site}, launch epoch {epoch}, block {blk} (mod 256)")
+        raise RuntimeError(f"fa4_nvfp4 kernel failure: code {code} (1 = bounded wait expired), "
+                           f"wait site {site}, launch epoch {epoch}, block {blk} (mod 256)")
 
 
 def flash_attn_fp4_func(
