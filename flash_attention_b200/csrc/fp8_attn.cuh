@@ -43,11 +43,12 @@ __device__ __forceinline__ float rcp_approx(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// tanh in fp32 from the exponential: 1 - 2 / (1 + e^2x), off by a few 2^-23 (tanh.approx is off by 2^-11, 1 % of a weight at a
-// cap of 30).
+// tanh in fp32 (tanh.approx is off by 2^-11, 1 % of a weight at a cap of 30): from 0.5 on 1 - 2 / (1 + e^2x), off by a few 2^-23; below, where that
+// loses the bits that cancel, x times a polynomial in x^2 through the values of tanh x / x at the five Chebyshev nodes of [0, 0.25].
 __device__ __forceinline__ float tanh_of(float x) {
-  const float e = ex2_approx(x * (2.f * 1.4426950408889634f));
-  return fmaf(-2.f, rcp_approx(1.f + e), 1.f);
+  const float e = ex2_approx(x * (2.f * 1.4426950408889634f)), far = fmaf(-2.f, rcp_approx(1.f + e), 1.f), z = x * x;
+  const float near = x * fmaf(fmaf(fmaf(fmaf(0.017131344f, z, -0.052984239f), z, 0.13324751f), z, -0.33333068f), z, 1.f);
+  return fabsf(x) < 0.5f ? near : far;
 }
 
 // Valid keys and rows of a sequence.

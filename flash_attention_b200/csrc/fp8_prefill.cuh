@@ -116,8 +116,8 @@ __device__ __forceinline__ void widen_tile(const uint8_t* raw, uint8_t* to, int 
 }
 
 // x to cap * tanh(x).  While no score of the warp's 64 keys is beyond 0.5 (a cap lies well above what scores mostly are), tanh x / x is a polynomial in
-// x^2 through its values at the four Chebyshev nodes of [0, 0.5^2]: off by 6e-7 of the value, 3e-7 of the cap at most, which is what tanh_of is off by, and
-// without its two special functions, which with the weight's own would bound the kernel.  Three sequences of up to 333 rows on up to 2048 keys:
+// x^2 through its values at the four Chebyshev nodes of [0, 0.5^2]: off by 6e-7 of the value, and
+// without the two special functions of tanh_of, which with the weight's own would bound the kernel.  Three sequences of up to 333 rows on up to 2048 keys:
 // tanh_of alone 56 us, six nodes of [0, 0.75^2] 49.1, four 46.7.
 __device__ __forceinline__ void cap_scores(float (&x)[64], float cap) {
   float far = fabsf(x[0]);

@@ -39,6 +39,8 @@ def append(values, scales, new, held, table, block):
     """Tokens `new` (n, heads, D) behind the `held` ones of a sequence whose pages are `table`; values (pages, size, heads, D)
     and scales (pages, size / block, heads), both float64 of what the cache stands for in units of the scale, are changed."""
     n, H, _ = new.shape
+    if n == 0:
+        return
     size = values.shape[1]
     new = new.double()
     for first in range(held // block * block, held + n, block):

@@ -9,7 +9,8 @@ products of at most |q| |k| scale = T together: 2^-24 of T for each addition, sq
 is off by delta = 2^-20 T, a weight by the factor e^delta, and the quotient of two sums of weights by e^2delta: another
 (e^2delta - 1) sum p |v| / sum p.  (T is 10 in an ordinary case and this is nothing; with T in the thousands it is as much as the
 rest, with T in the millions, as in the test of far scores, fp32 scores tell only the largest ones apart.)  lse: fp32 sums and hardware
-exponentials, 2^-18 of max(1, |lse|), and the same delta."""
+exponentials, 2^-18 of max(1, |lse|), and the same delta.  Weights keep their bits down to 2^-14 (many rows: 2^-20) of
+the largest: no case here has an element that is made by smaller ones alone."""
 import math
 
 import pytest
@@ -740,3 +741,11 @@ def test_more_than_a_million_rows(cuda_device):
         o, l = fa.flash_attn_fp8_cache_func(q[:, a:b], cache, lens, page_table=table, num_splits=1, return_lse=True)
         assert torch.equal(o, out[:, a:b]) and torch.equal(l, lse[:, :, a:b])
     fa.check_status(cuda_device)
+
+
+@pytest.mark.parametrize("Sq", [1, 70])
+def test_soft_cap_of_small_scores(cuda_device, Sq):
+    """Scores far below the cap are the scores: lse of one key is its score, to the room of a score itself."""
+    for n in (1, 3):
+        attend_both(cuda_device, 6, Sq, 8, 2, 128, 64, 64, [n] * 6, softcap=50.0, spread=8.0, seed=5)
+        attend_both(cuda_device, 6, Sq, 8, 2, 64, 64, 64, [n] * 6, softcap=50.0, spread=8.0, seed=6)
