@@ -76,8 +76,9 @@ __device__ __forceinline__ RowEnd finish_row(float m, float l, const float* sink
   if (sink != nullptr) {
     const float x = sink[h] * 1.4426950408889634f;
     top = fmaxf(m, x);
-    keep = m == -INFINITY ? 0.f : ex2_approx(m - top);
-    l = (m == -INFINITY ? 0.f : l * keep) + ex2_approx(x - top);
+    const float ref = top == -INFINITY ? 0.f : top;               // (a sink of -inf in a row that sees nothing: it adds 0)
+    keep = ex2_approx(m - ref);
+    l = (m == -INFINITY ? 0.f : l * keep) + ex2_approx(x - ref);
   }
   if (top == -INFINITY && l == 0.f) return {0.f, -INFINITY};    // (a row of NaN has l = NaN and goes on)
   e.factor = keep * rcp_approx(l);

@@ -749,3 +749,29 @@ def test_soft_cap_of_small_scores(cuda_device, Sq):
     for n in (1, 3):
         attend_both(cuda_device, 6, Sq, 8, 2, 128, 64, 64, [n] * 6, softcap=50.0, spread=8.0, seed=5)
         attend_both(cuda_device, 6, Sq, 8, 2, 64, 64, 64, [n] * 6, softcap=50.0, spread=8.0, seed=6)
+
+
+@pytest.mark.parametrize("splits", [0, 1, 3])
+@pytest.mark.parametrize("Sq,group", [(1, 4), (6, 2), (70, 4)])
+def test_sinks_that_are_switched_off(cuda_device, Sq, group, splits):
+    """A sink of -inf adds nothing: a row that sees no key either gets zeros and -inf, the others what they get without sinks."""
+    Hq = 2 * group
+    off = torch.arange(Hq) % 3 == 0
+    sink = torch.where(off, -math.inf, torch.linspace(-2.0, 2.0, Hq))
+    cache, table = batch_of(cuda_device, 4, 1000)
+    lens = torch.tensor([1000, 0, max(1, Sq // 2), Sq], dtype=torch.int32, device=cuda_device)
+    q = torch.randn(4, Sq, Hq, 128, generator=torch.Generator().manual_seed(1)).bfloat16().to(cuda_device)
+    call = lambda **kw: fa.flash_attn_fp8_cache_func(q, cache, lens, page_table=table, causal=True, num_splits=splits, return_lse=True, **kw)
+    out, lse = (x.cpu() for x in call(learnable_sink=sink.to(cuda_device)))
+    plain, plain_lse = (x.cpu() for x in call())
+    fa.check_status(cuda_device)
+    assert torch.equal(out[:, :, off], plain[:, :, off]) and torch.equal(lse[:, off], plain_lse[:, off])
+    blind = plain_lse[:, 0] == -math.inf                    # (B, Sq): alike for all heads
+    assert blind[1].all() and blind[2, :Sq - max(1, Sq // 2)].all() and not blind[0].any()
+    assert not out[blind].any()
+    # the sink alone, times log2 e and times ln 2: two products and two constants off by 2^-24 each
+    alone = sink[None, :, None].expand_as(lse).transpose(1, 2)[blind]
+    got = lse.transpose(1, 2)[blind]
+    assert torch.equal(got == -math.inf, alone == -math.inf)
+    live = alone > -math.inf
+    assert ((got - alone)[live].abs() <= 2.0 ** -22 * alone[live].abs()).all()
