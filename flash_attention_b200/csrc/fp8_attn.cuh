@@ -78,7 +78,7 @@ __device__ __forceinline__ RowEnd finish_row(float m, float l, const float* sink
     top = fmaxf(m, x);
     const float ref = top == -INFINITY ? 0.f : top;               // (a sink of -inf in a row that sees nothing: it adds 0)
     keep = ex2_approx(m - ref);
-    l = (m == -INFINITY ? 0.f : l * keep) + ex2_approx(x - ref);
+    l = fmaf(l, keep, ex2_approx(x - ref));                        // (of a row of NaN alone m is -inf and l NaN)
   }
   if (top == -INFINITY && l == 0.f) return {0.f, -INFINITY};    // (a row of NaN has l = NaN and goes on)
   e.factor = keep * rcp_approx(l);

@@ -775,3 +775,19 @@ def test_sinks_that_are_switched_off(cuda_device, Sq, group, splits):
     assert torch.equal(got == -math.inf, alone == -math.inf)
     live = alone > -math.inf
     assert ((got - alone)[live].abs() <= 2.0 ** -22 * alone[live].abs()).all()
+
+
+@pytest.mark.parametrize("Sq", [1, 6, 70])
+@pytest.mark.parametrize("splits", [0, 1, 3])
+def test_rows_of_nan_beside_a_sink(cuda_device, Sq, splits):
+    """A sequence whose keys are all NaN: out and lse are NaN, with a sink too; its neighbour is what it was."""
+    cache, table = batch_of(cuda_device, 2, 300)
+    for page in table[0].tolist():
+        cache.k[page].view(torch.uint8).fill_(0x7F)
+    lens = torch.tensor([300, 290], dtype=torch.int32, device=cuda_device)
+    q = torch.randn(2, Sq, 8, 128, device=cuda_device).bfloat16()
+    for sink in (None, torch.linspace(-1.0, 1.0, 8, device=cuda_device)):
+        out, lse = fa.flash_attn_fp8_cache_func(q, cache, lens, page_table=table, learnable_sink=sink, num_splits=splits, return_lse=True)
+        fa.check_status(cuda_device)
+        assert out[0].isnan().all() and lse[0].isnan().all()
+        assert out[1].isfinite().all() and lse[1].isfinite().all()
