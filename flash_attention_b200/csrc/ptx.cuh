@@ -12,9 +12,10 @@ namespace fa4 {
 // status word (global) + abort flag (shared): the no-hang contract
 //
 // Status word: (code << 24) | (site << 16) | (launch epoch << 8) | (blockIdx.x & 0xff).  The first
-// failure stays in the word until the host reads and clears it (compare-and-swap from 0), but it
+// failure stays in the word until the host reads and clears it, but it
 // stops only the CTAs of the launch that recorded it: a later launch carries another epoch (the
-// host counts launches modulo 256) and runs normally beside a stale word.
+// host counts launches modulo 256) and runs normally beside a stale word.  A bad index stopped
+// nothing, so an expired wait takes its place.
 // ---------------------------------------------------------------------------------------------
 constexpr uint32_t kStatusWaitExpired = 1u;
 constexpr uint32_t kStatusBadIndex = 2u;   // stops no launch: what the index leads to is left out
@@ -48,8 +49,10 @@ __device__ __forceinline__ uint64_t globaltimer_ns() {
 __device__ __forceinline__ void report_status(const WaitCtx& w, uint32_t code, uint32_t site) {
   *w.s_abort = 1u;
   if (w.g_status != nullptr) {
-    atomicCAS(w.g_status, 0u,
-              (code << 24) | ((site & 0xffu) << 16) | ((w.epoch & 0xffu) << 8) | (blockIdx.x & 0xffu));
+    // (a plain look and an exchange: of two waits that run out at once either may stay.  A compare-and-swap that tries again
+    // behind a bad index costs the 64-key kernel registers, 12 -> 20 bytes spilled)
+    if ((*reinterpret_cast<volatile uint32_t*>(w.g_status) >> 24) != kStatusWaitExpired)
+      atomicExch(w.g_status, (code << 24) | ((site & 0xffu) << 16) | ((w.epoch & 0xffu) << 8) | (blockIdx.x & 0xffu));
   }
 }
 

@@ -35,7 +35,8 @@ class DeviceStatus:
     synchronises) and raises if a kernel gave up; the attention call itself never synchronises.
     A launch whose wait ran out leaves its outputs unwritten and returns normally, like any
     asynchronous CUDA failure: call :func:`check_status` wherever results are consumed on the host.
-    The word keeps the first failure until it is read, but only the launch that recorded it stops
+    The word keeps the first failure until it is read (an expired wait takes the place of a bad index,
+    which stopped nothing), but only the launch that recorded it stops
     early (the kernels compare a per-launch epoch), so later calls are not affected by a stale word.
     """
     _words = {}

@@ -77,7 +77,7 @@ enum {
   FA4_S_WAIT_EXPIRED = 1, /* a bounded mbarrier wait ran out; `site` names the wait */
   FA4_S_BAD_INDEX = 2    /* 8-bit cache: an index on the device lies outside its range and what it leads to was left
                             out; `site`: 120 a position behind the cache's end, 121 a page number, 122 a position without a row
-                            in the rotation's tables.  Stops nothing */
+                            in the rotation's tables.  Stops nothing, and gives way to FA4_S_WAIT_EXPIRED */
 };
 
 /* kernel variants */

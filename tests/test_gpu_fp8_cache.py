@@ -791,3 +791,15 @@ def test_rows_of_nan_beside_a_sink(cuda_device, Sq, splits):
         fa.check_status(cuda_device)
         assert out[0].isnan().all() and lse[0].isnan().all()
         assert out[1].isfinite().all() and lse[1].isfinite().all()
+
+
+def test_an_expired_wait_takes_the_place_of_a_bad_index(cuda_device):
+    """A bad index stopped nothing; behind it a wait that runs out is what the caller has to know.  The first expired wait stays."""
+    word = fa.interface.DeviceStatus.word(cuda_device)
+    expire = lambda: fa.lib().fa4_nvfp4_debug_wait_expiry(word.data_ptr(), 5_000_000, None)
+    for before, after in ((0x02780503, "site 99,"), (0, "site 99,"), (0x01640700, "site 100, launch epoch 7,")):
+        word.fill_(before)
+        assert expire() == 0
+        with pytest.raises(RuntimeError, match=f"code 1 .*bounded wait expired.*{after}"):
+            fa.check_status(cuda_device)
+        fa.check_status(cuda_device)
