@@ -436,6 +436,12 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         auto weights = [&](float (&x)[64], const bool upper, uint32_t (&pw)[32]) {
           const float4 ks = *reinterpret_cast<const float4*>(sc + (upper ? 4 : 0));
           float kf[4] = {ks.x * factor, ks.y * factor, ks.z * factor, ks.w * factor};
+          const int key0 = ((t0 + i) << 7) + (upper ? 64 : 0), lo_in = lo - key0, hi_in = hi - key0;
+          const bool part = __any_sync(0xffffffffu, lo_in > 0 || hi_in < 64);
+          auto hide = [&](float as) {
+#pragma unroll
+            for (int j = 0; j < 64; ++j) x[j] = j >= lo_in && j < hi_in ? x[j] : as;
+          };
           if constexpr (kCap) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
@@ -443,17 +449,15 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
               x[2 * j] = y.x;
               x[2 * j + 1] = y.y;
             }
+            // (what a row does not see may be anything and has no say in how the others are capped)
+            if (part) hide(0.f);
             cap_scores(x, p.cap_out);
           } else {
             // (the factors go into the exponents' multiply-add and the groups' maxima; 0 would make NaN of a masked score)
 #pragma unroll
             for (int k = 0; k < 4; ++k) kf[k] = kf[k] == 0.f ? 1.17549435e-38f : kf[k];
           }
-          const int key0 = ((t0 + i) << 7) + (upper ? 64 : 0), lo_in = lo - key0, hi_in = hi - key0;
-          if (__any_sync(0xffffffffu, lo_in > 0 || hi_in < 64)) {
-#pragma unroll
-            for (int j = 0; j < 64; ++j) x[j] = j >= lo_in && j < hi_in ? x[j] : -INFINITY;
-          }
+          if (part) hide(-INFINITY);
           float top = -INFINITY;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {

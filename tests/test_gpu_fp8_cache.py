@@ -803,3 +803,26 @@ def test_an_expired_wait_takes_the_place_of_a_bad_index(cuda_device):
         with pytest.raises(RuntimeError, match=f"code 1 .*bounded wait expired.*{after}"):
             fa.check_status(cuda_device)
         fa.check_status(cuda_device)
+
+
+@pytest.mark.parametrize("byte", [0x7E, 0xFE, 0x7F])
+@pytest.mark.parametrize("softcap", [0.0, 3.0, 10.0, 50.0])
+def test_bytes_that_no_row_sees_leave_the_bits(cuda_device, byte, softcap):
+    """The largest values, of either sign, and NaN in front of the window and behind the last token, in blocks that are seen too."""
+    cache, table = batch_of(cuda_device, 2, 1000)
+    lens = [950, 700]
+    n = torch.tensor(lens, dtype=torch.int32, device=cuda_device)
+    for Sq in (1, 6, 50, 200):
+        q = torch.randn(2, Sq, 8, 128, generator=torch.Generator().manual_seed(Sq)).bfloat16().to(cuda_device)
+        call = lambda c: fa.flash_attn_fp8_cache_func(q, c, n, page_table=table, window_size=(100, 0), softcap=softcap, return_lse=True)
+        want = call(cache)
+        bad = fa.FP8KVCache(cache.k.clone(), cache.v.clone(), cache.k_scale, cache.v_scale)
+        for b, m in enumerate(lens):
+            first = max(0, m - Sq - 100)
+            for i, page in enumerate(table[b].tolist()):
+                for t in (bad.k, bad.v):
+                    t[page, :min(64, max(0, first - 64 * i))].view(torch.uint8).fill_(byte)
+                    t[page, min(64, max(0, m - 64 * i)):].view(torch.uint8).fill_(byte)
+        got = call(bad)
+        fa.check_status(cuda_device)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
