@@ -488,6 +488,7 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
                 for (int j = 0; j < 16; ++j) o[j] *= fac;
                 dec::tmem_st16(tm_o + 16 * c, reinterpret_cast<const uint32_t*>(o));
               }
+              tc_wait_st();                // (the lower half may read them again)
             }
             if (!upper && fac != 1.f) {
               // the weights of the upper half were made under the old reference

@@ -46,3 +46,15 @@ def test_a_decode_warp_writes_only_its_own_hand_over_slot():
                     env = {"wg": wg, "wq": wq, "lane": lane, "my_row": lane, "kR": k_r, "kMaxRows": k_max_rows}
                     if eval(cond.replace("&&", "and"), env):
                         assert eval(index, env) == (wg * 4 + wq) * k_max_rows + lane, (cond, index, wg, wq)
+
+
+def test_accumulators_that_were_stored_are_awaited_before_they_are_read_again():
+    """Many rows over the 8-bit cache: a row's reference may move in both halves of a step, and tensor-memory stores and
+    loads of one thread are ordered by tcgen05.wait alone.  Behind each loop that stores O stands a wait for its stores."""
+    text = re.sub(r"//.*", "", open(os.path.join(CSRC, "fp8_prefill.cuh")).read())
+    stores = [m.end() for m in re.finditer(r"tmem_st\d+\(tm_o\b[^;]*;", text)]
+    assert stores
+    for at in stores:
+        rest = text[at:]
+        wait = rest.index("tc_wait_st()")
+        assert "tmem_ld" not in rest[:wait] and re.fullmatch(r"\s*}\s*", rest[:wait])
