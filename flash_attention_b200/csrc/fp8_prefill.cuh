@@ -8,10 +8,11 @@
 // 2^16 and has its eleven bits down to 2^-20 of that.  Two e4m3 rows would not do here: O stays in tensor memory, so the reference is one of all
 // keys so far, and what lies 2^13 below it would lose its bits.  The row sum takes the weight without vs, in fp32.
 //
-// A CTA has two tiles of 128 rows (row r = token r / group, head r % group of a kv head), a softmax warpgroup each (thread = row).  S of a
-// tile is two halves of 64 columns.  A softmax warpgroup takes the upper half (keys 64-127) to registers first, and Q K^T of the next step's upper half
-// may overwrite it at once; W goes where the lower half was, then W V and Q K^T of the next lower half follow it.  So the softmax finds its next
-// scores waiting (with one product of 128 columns it waited 1500 of 4000 clocks for W V and Q K^T: 294 us for the first call below).
+// A CTA has two tiles of 128 rows (row r = token r / group, head r % group of a kv head), a softmax warpgroup each (thread = row).  The scores of a
+// tile have two halves of 64 columns, which the steps take in turn: the upper scores (keys 64-127) come first, the lower ones to the same columns when
+// those are in registers, the weights of both where the lower scores were.  Meanwhile the next step's upper scores go to the other half.  So the softmax finds
+// its next scores waiting (with one product of 128 columns it waited 1500 of 4000 clocks for W V and Q K^T: 294 us for the first call below), and no product
+// overwrites weights that another one may still read (Q K^T behind W V by issue alone 236 us, upper scores always in the same half and W V waited for 254-267).
 //
 // What bounds it: no unit alone.  A step of 256 rows x 128 keys takes about 3300 clocks: the exponentials 2048, the products 2560 (Q K^T in halves of 64
 // columns 48 clocks an instruction, bound by shared memory), 1700 issue slots a scheduler, in chains between two warps of a scheduler.  D = 128, B = 1:
@@ -30,7 +31,7 @@
 namespace fa4 {
 namespace fp8p {
 
-enum Site { kKFullS = 140, kKFreeS, kRawFullS, kRawFreeS, kHalfFullS, kHalfFreeS, kUFreeS, kPFullS, kODoneS, kQReadyS };
+enum Site { kKFullS = 140, kKFreeS, kRawFullS, kRawFreeS, kHalfFullS, kHalfFreeS, kUFreeS, kPFullS, kODoneS, kQReadyS, kPvDoneS };
 
 // Registers: 512 threads launch with 128; the softmax takes what the others give back.
 constexpr int kThreads = 512, kRegsLaunch = 128, kRegsSoftmax = 192, kRegsConvert = 64, kRegsService = 64;
@@ -311,15 +312,15 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       if (!feed.piece(p, wc, n, t0, b, hk, lo_all, hi_all)) feed.drain();
     } else if (warp == 13) {
       // ============================================ products =====================================
-      // (Products run in the order they are issued: Q K^T of a tile's next lower half overwrites the weights that W V in front of it reads.
+      // (Products are ordered by issue only where they share an accumulator and a shape: what is overwritten is waited for.
       // Descriptors are moved, not made anew: see the issuers of the decode kernel.)
       if (elect_one() && n > 0) {
         constexpr uint32_t idesc_s = fp8d::make_idesc_e4m3(128, 64, false), idesc_o = make_idesc_f16(128, kD, true);
         const uint64_t dq = fp8d::tile_desc<kD>(base + L::kOffQ), dk = fp8d::tile_desc<kD>(base + L::kOffK), dv = half_desc(base + L::kOffV);
-        // scores of tile t, upper or lower keys of the K tile at place `at`
-        auto score = [&](uint32_t t, uint32_t at, bool upper) {
+        // scores of tile t, upper or lower keys of the K tile at place `at`, to a half of its columns
+        auto score = [&](uint32_t t, uint32_t at, bool upper, uint32_t half) {
           const uint64_t qt = desc_at(dq, 2 * t * L::kTile8), kt = desc_at(dk, at * L::kTile8 + (upper ? 64 * kD : 0));
-          const uint32_t to = tmem + kColS + 128 * t + (upper ? 64 : 0);
+          const uint32_t to = tmem + kColS + 128 * t + 64 * half;
 #pragma unroll
           for (int ks = 0; ks < kD / 16; ++ks)
             fp8d::mma_e4m3(to, desc_at(qt, ks / (kD / 32) * L::kTile8 + 32 * (ks % (kD / 32))), desc_at(kt, 32 * (ks % (kD / 32))), idesc_s, ks > 0);
@@ -329,8 +330,8 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         ok = mbar_wait(bar(L::kQReady), 0, wc, kQReadyS) && mbar_wait(bar(L::kKFull), 0, wc, kKFullS);
         if (ok) {
           tc_fence_after_sync();
-          for (int t = 0; t < tiles; ++t) score(t, 0, true);
-          for (int t = 0; t < tiles; ++t) score(t, 0, false);
+          for (int t = 0; t < tiles; ++t) score(t, 0, true, 1);
+          for (int t = 0; t < tiles; ++t) score(t, 0, false, 0);
           tc_commit(bar(L::kKFree));
           kk.next();
         }
@@ -338,18 +339,20 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
 #pragma unroll 1
         for (int i = 0; ok && i < n; ++i) {
           const bool more = i + 1 < n;
+          const uint32_t half = (i + 1) & 1;   // of step i + 1
           // (what is most often there already is asked for at once: a wait of its own costs 110 clocks even then)
           if (more) {
-            const uint32_t two = tiles - 1;
+            // what was in that half: the upper scores of step 0, the weights of step i - 1
+            const uint32_t two = tiles - 1, gone = bar(i == 0 ? L::kUFree : L::kPvDone), site = i == 0 ? kUFreeS : kPvDoneS, phase = i == 0 ? 0 : half;
             const bool kf = mbar_poll(bar(L::kKFull + kk.at), kk.parity), vf = mbar_poll(bar(L::kVFull + buf), parity),
-                       u0 = mbar_poll(bar(L::kUFree), i & 1), u1 = mbar_poll(bar(L::kUFree + two), i & 1);
-            if (!(kf && vf && u0 && u1))
+                       g0 = mbar_poll(gone, phase), g1 = mbar_poll(gone + 8 * two, phase);
+            if (!(kf && vf && g0 && g1))
               ok = mbar_wait(bar(L::kKFull + kk.at), kk.parity, wc, kKFullS) && mbar_wait(bar(L::kVFull + buf), parity, wc, kHalfFullS) &&
-                   mbar_wait(bar(L::kUFree), i & 1, wc, kUFreeS) && mbar_wait(bar(L::kUFree + two), i & 1, wc, kUFreeS);
+                   mbar_wait(gone, phase, wc, site) && mbar_wait(gone + 8 * two, phase, wc, site);
             if (!ok) break;
             tc_fence_after_sync();
 #pragma unroll 1
-            for (int t = 0; t < tiles; ++t) score(t, kk.at, true);
+            for (int t = 0; t < tiles; ++t) score(t, kk.at, true, half);
           } else {
             ok = mbar_wait(bar(L::kVFull + buf), parity, wc, kHalfFullS);
           }
@@ -359,12 +362,18 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
             ok = mbar_wait(bar(L::kPFull + t), i & 1, wc, kPFullS);
             if (!ok) break;
             tc_fence_after_sync();
-            const uint32_t to = tmem + kColO + kD * t, from = tmem + kColS + 128 * t;
+            const uint32_t to = tmem + kColO + kD * t, from = tmem + kColS + 128 * t + 64 * (i & 1);
             // (the weights of the upper keys come first)
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks) mma_f16_ts(to, from + 8 * ks, desc_at(vt, 2048 * (ks ^ 4)), idesc_o, i > 0 || ks > 0);
             tc_commit(bar(L::kPvDone + t));
-            if (more) score(t, kk.at, false);
+            if (more) {
+              // (the softmax takes the upper scores as soon as it has handed its weights on)
+              ok = mbar_wait(bar(L::kUFree + t), half, wc, kUFreeS);
+              if (!ok) break;
+              tc_fence_after_sync();
+              score(t, kk.at, false, half);
+            }
           }
           if (ok) {
             tc_commit(bar(L::kVFree + buf));
@@ -432,6 +441,7 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         const float* sc = reinterpret_cast<const float*>(gbase + L::kOffSc) + slot * 16;
         if (++slot == L::kScales) slot = 0;
         uint32_t wu[32];
+        const uint32_t tm_half = tm_s + 64 * (i & 1);
         // 64 scores to weights (two to a word); `upper`: keys 64-127 of the step
         auto weights = [&](float (&x)[64], const bool upper, uint32_t (&pw)[32]) {
           const float4 ks = *reinterpret_cast<const float4*>(sc + (upper ? 4 : 0));
@@ -473,7 +483,7 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
             if (moved) m_ref = top;
             l2[0].x *= fac; l2[0].y *= fac; l2[1].x *= fac; l2[1].y *= fac;
             if (i > 0) {
-              // O, and in the upper half: behind W V of the step before (whose lower scores were behind that of the one before)
+              // O, behind W V of the step before (whose end the barrier of the lower scores implies)
               if (upper) {
                 if (ok) ok = mbar_wait_flag(bar(L::kPvDone + tile), (i - 1) & 1, s_abort);
                 ok = __all_sync(0xffffffffu, ok);
@@ -519,8 +529,9 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
           ok = __all_sync(0xffffffffu, ok);
           tc_fence_after_sync();
           float x[64];
-          tmem_ld32(tm_s + 64, reinterpret_cast<uint32_t*>(x));
-          tmem_ld32(tm_s + 96, reinterpret_cast<uint32_t*>(x + 32));
+          const uint32_t from = i == 0 ? tm_s + 64 : tm_half;
+          tmem_ld32(from, reinterpret_cast<uint32_t*>(x));
+          tmem_ld32(from + 32, reinterpret_cast<uint32_t*>(x + 32));
           tc_wait_ld();
           tc_fence_before_sync();
           __syncwarp();
@@ -533,12 +544,12 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
           tc_fence_after_sync();
           float x[64];
           uint32_t wl[32];
-          tmem_ld32(tm_s, reinterpret_cast<uint32_t*>(x));
-          tmem_ld32(tm_s + 32, reinterpret_cast<uint32_t*>(x + 32));
+          tmem_ld32(tm_half, reinterpret_cast<uint32_t*>(x));
+          tmem_ld32(tm_half + 32, reinterpret_cast<uint32_t*>(x + 32));
           tc_wait_ld();
           weights(x, false, wl);
-          tmem_st32(tm_s, wu);
-          tmem_st32(tm_s + 32, wl);
+          tmem_st32(tm_half, wu);
+          tmem_st32(tm_half + 32, wl);
           tc_wait_st();
           tc_fence_before_sync();
           __syncwarp();

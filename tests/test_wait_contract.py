@@ -58,3 +58,18 @@ def test_accumulators_that_were_stored_are_awaited_before_they_are_read_again():
         rest = text[at:]
         wait = rest.index("tc_wait_st()")
         assert "tmem_ld" not in rest[:wait] and re.fullmatch(r"\s*}\s*", rest[:wait])
+
+
+def test_products_wait_for_what_they_overwrite():
+    """Many rows over the 8-bit cache: tensor memory that one product reads and another overwrites.  Products of different accumulators may run in
+    any order, so the scores of step i + 1 go to the half of the columns that W V of step i does not read, and each product that writes there waits for
+    what was there: the weights of step i - 1 (W V done), the upper scores (taken by the softmax) for the lower ones."""
+    loop = _role("fp8_prefill.cuh", "products")
+    loop = loop[loop.index("uint32_t buf = 0"):]
+    assert "half = (i + 1) & 1;" in loop and re.search(r"from = [^;]*\+ 64 \* \(i & 1\);", loop)
+    assert re.search(r"gone = bar\(i == 0 \? L::kUFree : L::kPvDone\)", loop)
+    waits = r"mbar_wait\(%s, %s, wc, \w+\)"
+    first, second = [m.start() for m in re.finditer(r"score\(", loop)]
+    assert "true, half" in loop[first:first + 40] and "false, half" in loop[second:second + 40]
+    assert re.search(waits % ("gone", "phase"), loop[:first]) and re.search(waits % (r"gone \+ 8 \* two", "phase"), loop[:first])
+    assert re.search(waits % (r"bar\(L::kUFree \+ t\)", "half") + r";\s*if \(!ok\) break;\s*tc_fence_after_sync\(\);\s*$", loop[:second])
