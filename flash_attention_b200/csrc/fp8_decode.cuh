@@ -101,14 +101,16 @@ __device__ __forceinline__ void group_sync(int id) { asm volatile("bar.sync %0, 
 struct FeederSites {
   uint32_t free, lands;      // where a wait may run out
 };
-template <int kD, int kStages, int kScales>
+// kLogs: behind the scales the logarithms of the values', to base 2.
+template <int kD, int kStages, int kScales, bool kLogs = false>
 struct Feeder {
   static constexpr uint32_t kTile = 128 * kD;
+  static constexpr int kWords = kLogs ? 24 : 16;
   const CUtensorMap* tm;
   uint32_t full0, free0, part;      // barriers: of the ring's places; of a tile of values that are not all seen (0: such tiles are no matter)
   uint32_t tiles;                   // shared memory of the ring
   uint8_t* ring;                    //   the same, for plain stores
-  float* scales;                    // kScales x (8 of K, 8 of V), or null
+  float* scales;                    // kScales x (8 of K, 8 of V, logarithms of those), or null
   int2* box;                        // 32 places
   FeederSites site;
   Ring<kStages> st;                 // (of the issuing thread)
@@ -158,9 +160,10 @@ struct Feeder {
       if (scales != nullptr && (lane >> 3) < end) {
         // (the scales of the batch, as far ahead of the softmax as the ring of them allows)
         int to = slot + (lane >> 3);
-        to = (to >= kScales ? to - kScales : to) * 16 + gr;
+        to = (to >= kScales ? to - kScales : to) * kWords + gr;
         scales[to] = sc.x;
         scales[to + 8] = sc.y;
+        if constexpr (kLogs) scales[to + 16] = lg2_approx(sc.y);
       }
       const int2 at2 = look_up(l0 + 8);
       const float2 sc1 = scales_at(at1);

@@ -3,10 +3,10 @@
 //   S (128 rows x 128 keys) = Q . K^T  in e4m3: the keys as they are loaded, a bf16 query as two e4m3 rows (see the decode kernel)
 //   O (128 rows x D) += W . V          in fp16: values widened to fp16 (exact), weights from tensor memory
 //
-// W = 2^(t - m) vs / vs_max * 2^6 with t the score in log2 units, m a row's reference, which follows the maximum when it falls behind by
-// more than 8 (then O is multiplied), and vs / vs_max the scale of a block of values over the largest that this CTA meets: a weight is below
-// 2^16 and has its eleven bits down to 2^-20 of that.  Two e4m3 rows would not do here: O stays in tensor memory, so the reference is one of all
-// keys so far, and what lies 2^13 below it would lose its bits.  The row sum takes the weight without vs, in fp32.
+// W = 2^(t - v) vs 2^6 with t the score in log2 units, vs the scale of the key's block of values and v a row's reference, which follows the row's largest
+// t + log2 vs when it falls behind by more than 8 (then O is multiplied): a weight is 2^14 at most and has its eleven bits down to 2^-20 of that
+// reference, whatever values the rows beside it see.  Two e4m3 rows would not do here: O stays in tensor memory, so the reference is one of all
+// keys so far, and what lies 2^13 below it would lose its bits.  The row sum takes 2^(t - m) in fp32, m a reference of the scores alone.
 //
 // A CTA has two tiles of 128 rows (row r = token r / group, head r % group of a kv head), a softmax warpgroup each (thread = row).  The scores of a
 // tile have two halves of 64 columns, which the steps take in turn: the upper scores (keys 64-127) come first, the lower ones to the same columns when
@@ -45,7 +45,7 @@ struct Layout {
   static constexpr int kScales = kStagesK + 6;
   static constexpr uint32_t kTile16 = kHalf * (kD / 64), kTile8 = 128 * kD;
   static constexpr uint32_t kOffQ = 0 /* 2 tiles x (q1, q2) */, kOffK = 4 * kTile8, kOffRawV = kOffK + kStagesK * kTile8,
-                            kOffV = kOffRawV + kStagesV * kTile8, kOffSc = kOffV + 2 * kTile16, kOffBox = kOffSc + kScales * 64, kOffRow = kOffBox + 512 /* factor of a row's scores */,
+                            kOffV = kOffRawV + kStagesV * kTile8, kOffSc = kOffV + 2 * kTile16, kOffBox = kOffSc + kScales * 96, kOffRow = kOffBox + 512 /* factor of a row's scores */,
                             kOffBar = kOffRow + 256 * 4;
   static constexpr uint32_t kKFull = 0, kKFree = kKFull + kStagesK, kRawFull = kKFree + kStagesK, kRawFree = kRawFull + kStagesV,
                             kVFull = kRawFree + kStagesV, kVFree = kVFull + 2, kUFull = kVFree + 2, kLFull = kUFull + 2, kUFree = kLFull + 2,
@@ -78,6 +78,12 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+// The smaller of two, NaN if one is.
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
 }
 // Four e4m3 bytes as two pairs of fp16.
 __device__ __forceinline__ uint2 widen4(uint32_t w) {
@@ -162,7 +168,6 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   auto bar = [&](uint32_t idx) -> uint32_t { return base + L::kOffBar + 8u * idx; };
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gbase + L::kOffMisc);
   volatile uint32_t* s_abort = reinterpret_cast<volatile uint32_t*>(gbase + L::kOffMisc + 4);
-  uint32_t* s_top = reinterpret_cast<uint32_t*>(gbase + L::kOffMisc + 8);
   WaitCtx& wc = *reinterpret_cast<WaitCtx*>(gbase + L::kOffMisc + 32);
   const int tid = threadIdx.x, warp = warp_index(), lane = tid & 31;
   // row tiles from the last one on (with a causal mask the longest comes first), the kv heads and sequences of one next to each other
@@ -184,7 +189,6 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   const int tiles = R > 128 ? 2 : 1;
   if (tid == 0) {
     *s_abort = 0u;
-    *s_top = 0u;
     wc = WaitCtx{s_abort, p.status, p.budget_ns, p.epoch};
     for (int s = 0; s < L::kStagesK; ++s) {
       mbar_init(bar(L::kKFull + s), 1);
@@ -220,7 +224,6 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   pdl_trigger();
   const uint32_t tmem = *tmem_slot;
   bool ok = true;
-  float vs_up = 1.f, vs_down = 1.f;
   if (warp < 12) {
     // ---- Q by all but the service warps, a row's pieces of eight elements by neighbouring lanes: a row as two e4m3 rows, times the
     //      power of two that brings its largest element to 128 .. 256.  All on their way at once, to where V's widened tiles
@@ -232,15 +235,6 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       const int r = i / kPieces, ch = i % kPieces, s = fast_div(r_first + r, p.div_group), h = hk * p.group + r_first + r - s * p.group;
       const __nv_bfloat16* src = r < R ? p.q + b * p.q_b + (int64_t)s * p.q_s + h * p.q_h + 8 * ch : p.q;
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(base + L::kOffV + 16 * i), "l"(src), "r"(r < R ? 16 : 0) : "memory");
-    }
-    // the largest scale of values among this CTA's keys, while Q is on its way
-    const int first_key = max(lo_all, t0 << 7), end_key = min(hi_all, (t0 + n) << 7);
-    uint32_t vs_top = 0u;
-    for (int64_t blk = (first_key >> p.log_block) + tid; (blk << p.log_block) < end_key && n > 0; blk += 384) {
-      const int key = (int)(blk << p.log_block), pg = fast_div(key, p.div_page), off = key - pg * p.page_size;
-      const int page = p.table != nullptr ? p.table[(int64_t)b * p.pages_per_seq + pg] : b;
-      if (page >= 0 && page < p.num_pages)
-        vs_top = max(vs_top, __float_as_uint(p.v_scale[((int64_t)page * (p.page_size >> p.log_block) + (off >> p.log_block)) * p.Hkv + hk]) & 0x7fffffffu);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll 1
@@ -273,21 +267,13 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) mbar_arrive(bar(L::kQReady));
-    vs_top = __reduce_max_sync(0xffffffffu, vs_top);
-    if (lane == 0 && vs_top > 0u) atomicMax(s_top, vs_top);
-    asm volatile("bar.sync 1, 384;" ::: "memory");
-    // 2^6 / its power of two, and back (1 and 1 where it is no ordinary number)
-    const uint32_t top_e = *s_top >> 23;
-    if (top_e >= 20 && top_e <= 240) {
-      vs_up = __uint_as_float((254u + 6u - top_e) << 23);
-      vs_down = __uint_as_float((top_e - 6u) << 23);
-    }
+    asm volatile("bar.sync 1, 384;" ::: "memory");             // (the factors of the rows)
   }
 
   if (warp >= 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsService));
     if (warp == 12) {
-      fp8d::Feeder<kD, L::kStagesK, L::kScales> feed;
+      fp8d::Feeder<kD, L::kStagesK, L::kScales, true> feed;
       feed.tm = &tm_k;
       feed.full0 = bar(L::kKFull);
       feed.free0 = bar(L::kKFree);
@@ -432,13 +418,13 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       lo = see.x;
       hi = see.y;
     }
-    float m_ref = -INFINITY;
+    float m_ref = -INFINITY, v_ref = -INFINITY, v_up = 0.f;     // references of the sum and of O; 2^(m_ref - v_ref + 6)
     float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
     if (tile < tiles) {
       int slot = 0;
 #pragma unroll 1
       for (int i = 0; i < n; ++i) {
-        const float* sc = reinterpret_cast<const float*>(gbase + L::kOffSc) + slot * 16;
+        const float* sc = reinterpret_cast<const float*>(gbase + L::kOffSc) + slot * 24;
         if (++slot == L::kScales) slot = 0;
         uint32_t wu[32];
         const uint32_t tm_half = tm_s + 64 * (i & 1);
@@ -468,20 +454,30 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
             for (int k = 0; k < 4; ++k) kf[k] = kf[k] == 0.f ? 1.17549435e-38f : kf[k];
           }
           if (part) hide(-INFINITY);
-          float top = -INFINITY;
+          const float4 lv4 = *reinterpret_cast<const float4*>(sc + 16 + (upper ? 4 : 0));
+          const float lv[4] = {lv4.x, lv4.y, lv4.z, lv4.w};
+          float top = -INFINITY, top_v = -INFINITY;             // of the scores; of the weights with the values' scales
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             float m = fmaxf(x[16 * k], x[16 * k + 1]);
 #pragma unroll
             for (int j = 2; j < 16; j += 2) m = fmax3(m, x[16 * k + j], x[16 * k + j + 1]);
             top = fmaxf(top, kCap ? m : m * kf[k]);
+            top_v = fmaxf(top_v, kCap ? m + lv[k] : fmaf(m, kf[k], lv[k]));
           }
-          // the reference follows when the row's weights would pass 2^8
-          const bool moved = top > m_ref + 8.f;
+          // the references follow when the row's weights would pass 2^8, without or with the values' scales
+          const bool moved = top > m_ref + 8.f || top_v > v_ref + 8.f;
           if (__any_sync(0xffffffffu, moved)) {
-            const float fac = moved ? ex2_approx(m_ref - top) : 1.f;
-            if (moved) m_ref = top;
-            l2[0].x *= fac; l2[0].y *= fac; l2[1].x *= fac; l2[1].y *= fac;
+            float fac = 1.f;
+            if (moved) {
+              // (2^-120: the smallest scale of an append; below it, or at 0, the weights lose range, not v_up)
+              const float m_new = fmaxf(m_ref, top), v_new = fmaxf(fmaxf(v_ref, top_v), m_new - 120.f), keep = ex2_approx(m_ref - m_new);
+              fac = ex2_approx(v_ref - v_new);
+              l2[0].x *= keep; l2[0].y *= keep; l2[1].x *= keep; l2[1].y *= keep;
+              m_ref = m_new;
+              v_ref = v_new;
+              v_up = ex2_approx(m_new - v_new + 6.f);
+            }
             if (i > 0) {
               // O, behind W V of the step before (whose end the barrier of the lower scores implies)
               if (upper) {
@@ -513,7 +509,8 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
           const float ref = m_ref == -INFINITY ? 0.f : -m_ref;
           const float2 ref2 = make_float2(ref, ref);
           const float4 vs4 = *reinterpret_cast<const float4*>(sc + 8 + (upper ? 4 : 0));
-          const float vs[4] = {vs4.x * vs_up, vs4.y * vs_up, vs4.z * vs_up, vs4.w * vs_up};
+          // (finite: a key whose score lies 2^100 lower has a weight of 0, whatever its scale)
+          const float vs[4] = {min_nan(vs4.x * v_up, 3e38f), min_nan(vs4.y * v_up, 3e38f), min_nan(vs4.z * v_up, 3e38f), min_nan(vs4.w * v_up, 3e38f)};
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
             const float2 xx = make_float2(x[2 * j], x[2 * j + 1]);
@@ -568,7 +565,8 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       const RowEnd end = finish_row(m_ref, l, p.sink, h);
       const bool direct = p.num_splits == 1;
       const int64_t rows = (int64_t)p.B * p.Sq * p.Hq, part = (int64_t)split * rows;
-      const float scale = (direct ? end.factor : rcp_approx(l)) * vs_down;
+      // (2^(v_ref - m_ref - 6) in two steps: it may be as small as 2^-126 beside a large O)
+      const float down = m_ref == -INFINITY ? 0.f : ex2_approx(0.5f * (v_ref - m_ref - 6.f)), scale = (direct ? end.factor : rcp_approx(l)) * down;
       if (ok && row < R) {
         if (direct && p.lse != nullptr) p.lse[l_idx] = end.lse;
         if (!direct) p.lse_partial[part + ((int64_t)b * p.Sq + s) * p.Hq + h] = none ? -INFINITY : m_ref + lg2_approx(l);
@@ -586,16 +584,18 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
 #pragma unroll
           for (int j = 0; j < 32; ++j) o[j] = 0.f;
         }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) o[j] = o[j] * scale * down;
         if (direct) {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             *reinterpret_cast<uint4*>(stage + lane * (2 * kD) + (((4 * c + j) ^ (lane & 7)) << 4)) =
-                make_uint4(pack_bf16x2(o[8 * j] * scale, o[8 * j + 1] * scale), pack_bf16x2(o[8 * j + 2] * scale, o[8 * j + 3] * scale),
-                           pack_bf16x2(o[8 * j + 4] * scale, o[8 * j + 5] * scale), pack_bf16x2(o[8 * j + 6] * scale, o[8 * j + 7] * scale));
+                make_uint4(pack_bf16x2(o[8 * j], o[8 * j + 1]), pack_bf16x2(o[8 * j + 2], o[8 * j + 3]), pack_bf16x2(o[8 * j + 4], o[8 * j + 5]),
+                           pack_bf16x2(o[8 * j + 6], o[8 * j + 7]));
         } else if (ok && row < R && !none) {
           float4* dst = reinterpret_cast<float4*>(p.o_partial + (part + ((int64_t)b * p.Sq + s) * p.Hq + h) * kD + 32 * c);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) dst[j] = make_float4(o[4 * j] * scale, o[4 * j + 1] * scale, o[4 * j + 2] * scale, o[4 * j + 3] * scale);
+          for (int j = 0; j < 8; ++j) dst[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
         }
       }
       if (direct && ok) {

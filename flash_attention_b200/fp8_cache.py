@@ -111,10 +111,10 @@ def flash_attn_fp8_cache_func(
     ``window_size`` refer to.  ``learnable_sink``, ``softcap``, ``num_splits`` (0: chosen), ``out`` and ``lse`` as in
     :func:`flash_attn_fp4_func`; a row that sees nothing gets zeros and an lse of -inf.
 
-    Not differentiable.  Softmax weights (times their value scale) keep eight bits down to 2^-14 of the largest among 128 keys and are right to 2^-22
-    of it below (more than 32 rows per kv head: eleven bits down to 2^-20 of the largest so far times the largest value scale among the keys, right to
-    2^-31 of that below).  So an output element that is made by less than that (the values of the keys that weigh are zero there, or their blocks'
-    scales are 2^-20 of another's) is right to that much of the others, not to bf16.
+    Not differentiable.  A row's softmax weights, times their value scales, keep eight bits down to 2^-14 of the largest among 128 keys and are
+    right to 2^-22 of it below (more than 32 rows per kv head: eleven bits down to 2^-20 of the largest so far, right to 2^-31 of that below).  So an
+    output element that is made by less than that (the values of the keys that weigh are zero there) is right to that much of the others, not to
+    bf16.  Value scales that a row sees lie within a factor of 2^90 of each other.
 
     A length beyond the cache's or the table's end counts as that end, a negative one as 0 (they are on the device and cannot be
     refused).  The cache behind a sequence's last token may hold anything, NaN included.  A NaN in a value that some row of a sequence sees may

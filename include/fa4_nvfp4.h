@@ -553,8 +553,9 @@ int fa4_fp8_cache_append(const fa4_fp8_cache* cache, const fa4_fp8_append* a, vo
  *   score = softmax_scale * k_scale * (q . k), soft cap, masks, sink as in fa4_nvfp4_ext
  *   out = sum of softmax weight * v_scale * v: bf16 (B, Sq, Hq, D); lse fp32 (B, Hq, Sq) or NULL
  * A row that sees no key gets zeros and an lse of -inf (of its sink).  What lies behind a sequence's last token may be anything,
- * NaN included.  Weights (times v_scale) keep eight bits down to 2^-14 of the largest of a tile of 128 keys, right to 2^-22 of it below; with
- * Sq * Hq / Hkv > 32 eleven bits down to 2^-20 of the largest so far times the largest v_scale, right to 2^-31 of that below.
+ * NaN included.  A row's weights (times v_scale) keep eight bits down to 2^-14 of the largest of a tile of 128 keys, right to 2^-22 of it below; with
+ * Sq * Hq / Hkv > 32 eleven bits down to 2^-20 of the largest so far, right to 2^-31 of that below.  Value scales that a row sees lie within
+ * 2^90 of each other.
  * `workspace`: fa4_fp8_cache_fwd_workspace_bytes of device memory, 16-byte aligned, in use until the
  * launches have run.  num_splits: 0 = chosen.
  */

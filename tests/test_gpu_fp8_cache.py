@@ -826,3 +826,59 @@ def test_bytes_that_no_row_sees_leave_the_bits(cuda_device, byte, softcap):
         got = call(bad)
         fa.check_status(cuda_device)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def attend_values(device, cache, table, lens, q, **kw):
+    """A call against 64 bits, in the room that the head of this file derives (and half a step of the smallest bf16 values, 2^-134)."""
+    n = torch.tensor(lens, dtype=torch.int32, device=device)
+    out, lse = fa.flash_attn_fp8_cache_func(q.to(device), cache, n, page_table=table, return_lse=True, **kw)
+    torch.cuda.synchronize()
+    fa.check_status(device)
+    args = dict(causal=kw.get("causal", False), window=kw.get("window_size", (None, None)), softcap=kw.get("softcap", 0.0))
+    for b, m in enumerate(lens):
+        k, v = held_of(cache, table[b].tolist(), m)
+        want, want_lse = orc.attend(q[b], k, v, q.shape[1], **args)
+        mag, _ = orc.attend(q[b], k, v.abs(), q.shape[1], **args)
+        top = float(q[b].double().norm(dim=-1).max() * k.norm(dim=-1).max()) * q.shape[-1] ** -0.5
+        off = (out[b].cpu().double() - want).abs()
+        room = 2.0 ** -8 * (mag + want.abs()) + (2.0 ** -13 + math.expm1(2.0 * min(5.0, 2.0 ** -20 * top))) * mag + 2.0 ** -134
+        assert (off <= room).all(), f"sequence {b}: {(off / room).max():.3g} of the room, first at {(~(off <= room)).nonzero()[0].tolist()}"
+        assert ((lse[b].cpu().double() - want_lse).abs() <= 2.0 ** -18 * want_lse.abs().clamp(min=1.0) + 2.0 ** -20 * top).all()
+
+
+def cache_of_scales(device, exponent, seed=2):
+    """Two sequences of 1000 tokens: values up to 200 x 2^exponent or twice that."""
+    cache, table = batch_of(device, 2, 1000)
+    g = torch.Generator().manual_seed(seed)
+    cache.v.copy_((torch.randn(cache.v.shape, generator=g) * 100).clamp(-200, 200).to(torch.float8_e4m3fn))
+    cache.v_scale.copy_(2.0 ** (exponent + torch.randint(0, 2, cache.v_scale.shape, generator=g)))
+    return cache, table
+
+
+@pytest.mark.parametrize("exponent", [-120, -110, 100, 115])
+@pytest.mark.parametrize("splits", [0, 1, 3])
+def test_many_rows_on_value_scales_at_the_ends_of_their_range(cuda_device, exponent, splits):
+    """(hundreds of keys of much the same weight, and few that outweigh the others)"""
+    cache, table = cache_of_scales(cuda_device, exponent)
+    for q_scale in (0.1, 1.0, 4.0):
+        q = (torch.randn(2, 70, 8, 128, generator=torch.Generator().manual_seed(4)) * q_scale).bfloat16()
+        attend_values(cuda_device, cache, table, [1000, 640], q, causal=True, num_splits=splits)
+
+
+@pytest.mark.parametrize("exponent", [-19, -25, -35, -60])
+@pytest.mark.parametrize("D,splits,softcap", [(128, 0, 0.0), (64, 0, 0.0), (128, 3, 0.0), (128, 1, 20.0)])
+def test_small_values_in_front_of_large_ones(cuda_device, exponent, D, splits, softcap):
+    """A causal prompt whose values grow: an early row's result is right to its own values, whatever the rows beside it see."""
+    cache = make_cache(16, 32, 2, D, 16, 1, cuda_device)
+    tables = tables_of(2, 7, 16, 1)
+    fill(cache, tables, [200, 200], 1)
+    table = torch.tensor(tables, dtype=torch.int32, device=cuda_device)
+    g = torch.Generator().manual_seed(3)
+    for b in range(2):
+        for i in range(13):
+            cache.v_scale[tables[b][i // 2], i % 2] = 2.0 ** max(-120, -8 + (2 * exponent if i == 0 else exponent if i < 3 else 0))
+    for q_scale in (1.0, 4.0):
+        attend_values(cuda_device, cache, table, [200, 197], (torch.randn(2, 197, 8, D, generator=g) * q_scale).bfloat16(), causal=True,
+                      num_splits=splits, softcap=softcap)
+        attend_values(cuda_device, cache, table, [200, 197], (torch.randn(2, 197, 8, D, generator=g) * q_scale).bfloat16(), window_size=(20, 0),
+                      num_splits=splits, softcap=softcap)
