@@ -118,15 +118,17 @@ __device__ __forceinline__ void merge_row(const Fp8Params& p, int b, int s, int 
     for (int j = 0; j < 8; ++j) {
       const float w = ex2_approx(l[j] - ref);
       sum += w;
-      acc.x = fmaf(w, v[j].x, acc.x); acc.y = fmaf(w, v[j].y, acc.y);
-      acc.z = fmaf(w, v[j].z, acc.z); acc.w = fmaf(w, v[j].w, acc.w);
+      const float w8 = w * 0x1p-8f;        // (up to 148 parts, whose values may be as large as bf16 has them)
+      acc.x = fmaf(w8, v[j].x, acc.x); acc.y = fmaf(w8, v[j].y, acc.y);
+      acc.z = fmaf(w8, v[j].z, acc.z); acc.w = fmaf(w8, v[j].w, acc.w);
     }
     m = top;
   }
   const RowEnd e = finish_row(m, sum, p.sink, h);
+  const float up = e.factor * 0x1p8f;
   if (col < p.D)
     *reinterpret_cast<uint2*>(p.out + b * p.o_b + s * p.o_s + h * p.o_h + col) =
-        make_uint2(pack_bf16x2(acc.x * e.factor, acc.y * e.factor), pack_bf16x2(acc.z * e.factor, acc.w * e.factor));
+        make_uint2(pack_bf16x2(acc.x * up, acc.y * up), pack_bf16x2(acc.z * up, acc.w * up));
   if (lane == 0 && p.lse != nullptr) p.lse[((int64_t)b * p.Hq + h) * p.Sq + s] = e.lse;
 }
 

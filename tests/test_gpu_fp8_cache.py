@@ -882,3 +882,14 @@ def test_small_values_in_front_of_large_ones(cuda_device, exponent, D, splits, s
                       num_splits=splits, softcap=softcap)
         attend_values(cuda_device, cache, table, [200, 197], (torch.randn(2, 197, 8, D, generator=g) * q_scale).bfloat16(), window_size=(20, 0),
                       num_splits=splits, softcap=softcap)
+
+
+@pytest.mark.parametrize("splits", [0, 2, 3, 16])
+def test_parts_of_the_largest_values_are_merged(cuda_device, splits):
+    """Values up to 2^127 or so: the sum of the parts of a row lies beyond fp32, their mean does not."""
+    cache, table = cache_of_scales(cuda_device, 118)
+    for q_scale in (0.1, 1.0):
+        q = (torch.randn(2, 70, 8, 128, generator=torch.Generator().manual_seed(4)) * q_scale).bfloat16()
+        attend_values(cuda_device, cache, table, [1000, 640], q, causal=True, num_splits=splits)
+    cache.v.fill_(200.0)
+    attend_values(cuda_device, cache, table, [1000, 640], q, causal=True, num_splits=splits)
