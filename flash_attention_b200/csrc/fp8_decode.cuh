@@ -13,7 +13,8 @@
 // Weights are two e4m3 rows as well, w = (w1 + w2 / 16) / 256, as neighbouring columns of one product: within 2^-9 of w down to 2^-14 and
 // 2^-22 below that.  w is softmax weight times value scale, over the largest of these that the row has in the TILE, not among all
 // keys so far (a row whose first key outweighs the rest by 2^15 would round the rest to nothing): the product of a tile is read out of
-// tensor memory and added to the row's sums in fp32 registers, two FMAs a row and thread.
+// tensor memory and added to the row's sums in fp32 registers, two FMAs a row and thread, under a reference of all tiles so far.  The sum
+// of the weights without the scales has one of its own.
 //
 // A CTA per SM works through its share of all tiles of the call: the lengths are on the device, and shares of equal size are what keeps HBM
 // busy to the end.  Up to eight kv heads go side by side through the same tokens, a CTA each: theirs lie next to each other in memory
@@ -248,8 +249,8 @@ struct Form {
       kOffFac = kOffRed + kStrands * 2 * 4 * kR * 8,                         // (keep, add): strands x 2 x rows
       kOffRow = kOffFac + kStrands * 2 * kR * 8,                             // factor of a row's scores
       kOffSum = kOffRow + kR * 4,                                            // strands x 4 warps x rows: sums
-      kOffRef = kOffSum + kStrands * 4 * kR * 4,                             // strands x rows: last references
-      kOffBar = (kOffRef + kStrands * kR * 4 + 7) / 8 * 8;
+      kOffRef = (kOffSum + kStrands * 4 * kR * 4 + 7) / 8 * 8,                             // strands x rows: last references
+      kOffBar = kOffRef + kStrands * kR * 8;
   static constexpr uint32_t kKFull = 0, kKFree = kKFull + kStages, kVFull = kKFree + kStages, kVFree = kVFull + kStages,
                             kSFull = kVFree + kStages, kSFree = kSFull + kStrands, kPFull = kSFree + kStrands,
                             kPvDone = kPFull + kStrands, kQReady = kPvDone + kStrands, kVPart = kQReady + 1, kDrain = kVPart + 1, kBars = kDrain + 2;
@@ -533,7 +534,7 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     float2* s_fac = reinterpret_cast<float2*>(gbase + F::kOffFac) + sd * 2 * kR;
     float* s_row = reinterpret_cast<float*>(gbase + F::kOffRow);
     float* s_sum = reinterpret_cast<float*>(gbase + F::kOffSum);
-    float* s_ref = reinterpret_cast<float*>(gbase + F::kOffRef);
+    float2* s_ref = reinterpret_cast<float2*>(gbase + F::kOffRef);
     float* s_acc = reinterpret_cast<float*>(gbase + F::kOffQ);       // strands x rows x kD
     auto all_strands = [] { asm volatile("bar.sync 15, %0;" ::"n"(128 * kStrands) : "memory"); };
     const int my = lane & (kR - 1), grp = lane / kR, key_in = wq * 32 + grp * kKeys;
@@ -602,7 +603,7 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       // the keys that all rows see
       const int lo_in = seq.sq > 0 ? seen_by(p, seq.sk, seq.sq, seq.sq - 1).x : 0, hi_in = seen_by(p, seq.sk, seq.sq, 0).y;
       const float factor = s_row[my];
-      float m_run = -INFINITY, l = 0.f, acc[kR];
+      float m_run = -INFINITY, v_run = -INFINITY, l = 0.f, acc[kR];    // largest score, and with its value scale
 #pragma unroll
       for (int r = 0; r < kR; ++r) acc[r] = 0.f;
       // O^T of the strand's tile before, into the sums
@@ -630,7 +631,7 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       for (int li = li0, u = u0; li < n + kStrands; li += kStrands, ++u) {
         const bool live = li < n;
         const int key0 = (t0 + li) << 7;
-        float x[kKeys], up[kKeys / 16], keep = 0.f, add_v = 0.f;
+        float x[kKeys], up[kKeys / 16], keep_v = 0.f, add_v = 0.f;
         if (live) {
         // (only barriers of this strand are waited for: a stage's barrier may be two phases behind, and a wait on parities
         // does not tell that from done)
@@ -689,9 +690,12 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           top_v = fmaxf(top_v, of.y);
         }
         const float ref = top == -INFINITY ? 0.f : top, ref_v = top_v == -INFINITY ? 0.f : top_v;
-        const float m_new = fmaxf(m_run, top), base_m = m_new == -INFINITY ? 0.f : m_new, add = ex2_approx(top - base_m);
-        keep = ex2_approx(m_run - base_m);
-        add_v = ex2_approx(top_v - base_m);
+        const float m_new = fmaxf(m_run, top), base_m = m_new == -INFINITY ? 0.f : m_new, add = ex2_approx(top - base_m), keep = ex2_approx(m_run - base_m);
+        // (the values' sums have a reference of their own: scales may be as far from 1 as fp32 reaches)
+        const float v_new = fmaxf(v_run, top_v), base_v = v_new == -INFINITY ? 0.f : v_new;
+        keep_v = ex2_approx(v_run - base_v);
+        add_v = ex2_approx(top_v - base_v);
+        v_run = v_new;
         // a weight times this is 256 at most (bounded for scales further apart than fp32 reaches)
 #pragma unroll
         for (int i = 0; i < kKeys / 16; ++i) {
@@ -714,7 +718,7 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         // the sums of the tile before, and with them its W^T, are done with
         if (u > u0) take(u - 1);
         if (!live) break;
-        if (wq == 0 && lane < kR) s_fac[(u & 1) * kR + lane] = make_float2(keep, add_v * (1.f / 256.f));
+        if (wq == 0 && lane < kR) s_fac[(u & 1) * kR + lane] = make_float2(keep_v, add_v * (1.f / 256.f));
 #pragma unroll
         for (int i = 0; i < kKeys / 16; ++i) {
           uint32_t w1[4], w2[4];
@@ -740,7 +744,7 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 #pragma unroll
       for (int o = kR; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
       if (lane < kR) s_sum[(sd * 4 + wq) * kR + lane] = l;
-      if (wq == 0 && lane < kR) s_ref[sd * kR + lane] = m_run;
+      if (wq == 0 && lane < kR) s_ref[sd * kR + lane] = make_float2(m_run, v_run);
       all_strands();                                                   // (every product of the piece is done: Q is free)
       if (t < kD) {
 #pragma unroll
@@ -767,32 +771,40 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 #pragma unroll 1
       for (int r = warp; r < R && whole; r += 4 * kStrands) {
         const int col = 4 * lane;
-        float m = -INFINITY, sum = 0.f;
+        float m = -INFINITY, v = -INFINITY, sum = 0.f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int k = 0; k < kStrands; ++k) m = fmaxf(m, s_ref[k * kR + r]);
+        for (int k = 0; k < kStrands; ++k) {
+          const float2 of = s_ref[k * kR + r];
+          m = fmaxf(m, of.x);
+          v = fmaxf(v, of.y);
+        }
 #pragma unroll
         for (int k = 0; k < kStrands; ++k) {
-          const float f = m == -INFINITY ? 1.f : ex2_approx(s_ref[k * kR + r] - m);
+          const float2 of = s_ref[k * kR + r];
+          const float f = m == -INFINITY ? 1.f : ex2_approx(of.x - m), fv = v == -INFINITY ? 1.f : ex2_approx(of.y - v);
           const float* s4 = s_sum + k * 4 * kR + r;
           sum = fmaf(f, ((s4[0] + s4[kR]) + s4[2 * kR]) + s4[3 * kR], sum);
           if (col < kD) {
             const float4 a = *reinterpret_cast<const float4*>(s_acc + (k * kR + r) * kD + col);
-            o.x = fmaf(f, a.x, o.x); o.y = fmaf(f, a.y, o.y); o.z = fmaf(f, a.z, o.z); o.w = fmaf(f, a.w, o.w);
+            o.x = fmaf(fv, a.x, o.x); o.y = fmaf(fv, a.y, o.y); o.z = fmaf(fv, a.z, o.z); o.w = fmaf(fv, a.w, o.w);
           }
         }
+        // (2^(v - m) in two steps: the values' sum may be as large as that is small)
+        const float by = v == -INFINITY ? 0.f : ex2_approx(0.5f * (v - m));
         if (direct) {
           const int s = fast_div(r, p.div_group), h = hk * p.group + r - s * p.group;
           const RowEnd e = finish_row(m, sum, p.sink, h);
+          const float f = e.factor * by;
           if (col < kD)
             *reinterpret_cast<uint2*>(p.out + b * p.o_b + s * p.o_s + h * p.o_h + col) =
-                make_uint2(pack_bf16x2(o.x * e.factor, o.y * e.factor), pack_bf16x2(o.z * e.factor, o.w * e.factor));
+                make_uint2(pack_bf16x2(o.x * f * by, o.y * f * by), pack_bf16x2(o.z * f * by, o.w * f * by));
           if (lane == 0 && p.lse != nullptr) p.lse[((int64_t)b * p.Hq + h) * p.Sq + s] = e.lse;
         } else {
           const bool none = m == -INFINITY && sum == 0.f;
-          const float f = rcp_approx(sum);
+          const float f = rcp_approx(sum) * by;
           if (col < kD && !none)
-            *reinterpret_cast<float4*>(p.o_partial + (slot * p.unit_rows + r) * kD + col) = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+            *reinterpret_cast<float4*>(p.o_partial + (slot * p.unit_rows + r) * kD + col) = make_float4(o.x * f * by, o.y * f * by, o.z * f * by, o.w * f * by);
           if (lane == 0) p.lse_partial[slot * p.unit_rows + r] = none ? -INFINITY : m + lg2_approx(sum);
         }
       }

@@ -893,3 +893,17 @@ def test_parts_of_the_largest_values_are_merged(cuda_device, splits):
         attend_values(cuda_device, cache, table, [1000, 640], q, causal=True, num_splits=splits)
     cache.v.fill_(200.0)
     attend_values(cuda_device, cache, table, [1000, 640], q, causal=True, num_splits=splits)
+
+
+@pytest.mark.parametrize("exponent", [-120, -110, 100, 115, 118])
+@pytest.mark.parametrize("Sq", [1, 6])
+@pytest.mark.parametrize("splits", [0, 1, 3])
+def test_few_rows_on_value_scales_at_the_ends_of_their_range(cuda_device, Sq, exponent, splits):
+    cache, table = cache_of_scales(cuda_device, exponent)
+    for q_scale in (0.1, 1.0, 4.0):
+        q = (torch.randn(2, Sq, 8, 128, generator=torch.Generator().manual_seed(4)) * q_scale).bfloat16()
+        attend_values(cuda_device, cache, table, [1000, 640], q, causal=True, num_splits=splits)
+    # blocks of values 2^80 from the others, whose keys weigh as much
+    for b in range(2):
+        cache.v_scale[table[b, 2:4].long()] = 2.0 ** (exponent + (80 if exponent < 0 else -80))
+    attend_values(cuda_device, cache, table, [1000, 640], torch.randn(2, Sq, 8, 128, generator=torch.Generator().manual_seed(5)).bfloat16(), num_splits=splits)
