@@ -116,8 +116,10 @@ struct Feeder {
   FeederSites site;
   Ring<kStages> st;                 // (of the issuing thread)
   bool first = true;                // round of the ring
-  int g = 0, slot = 0;              // tiles so far; place of the next among the scales
+  int issued = 0;                   // tiles so far (of the issuing thread)
+  int slot = 0;                     // place of the next tile among the scales
   uint32_t parts = 0u;
+  bool part_on_way = false;         // a tile that lands on `part` (of the issuing thread)
 
   // Tiles t0 .. t0 + n - 1 of kv head hk of sequence b, in which keys [lo, hi) are seen.  False: a wait ran out.
   __device__ __forceinline__ bool piece(const Fp8Params& p, const WaitCtx& wc, int n, int t0, int b, int hk, int lo, int hi) {
@@ -187,6 +189,8 @@ struct Feeder {
             last = st.at;
             const uint32_t mine = (boxes >> (8 * q)) & 0xffu;
             mbar_arrive_expect_tx(lands, __popc(mine) * (uint32_t)p.box * kD);
+            part_on_way = q == q1;
+            ++issued;
             for (uint32_t m = mine; m != 0u; m &= m - 1u) {
               const int i = __ffs(m) - 1;
               const int2 from = box[8 * q + i];
@@ -199,6 +203,8 @@ struct Feeder {
         ok = __all_sync(0xffffffffu, ok);
         if (is_part && ok) {
           ok = __all_sync(0xffffffffu, mbar_wait(part, parts, wc, site.lands));
+          if (!ok) return false;
+          part_on_way = false;
           parts ^= 1u;
           last = __shfl_sync(0xffffffffu, last, __ffs(__ballot_sync(0xffffffffu, lead)) - 1);
           const int key0 = (t0 + l0 + q1) << 7;
@@ -215,19 +221,22 @@ struct Feeder {
         q0 = q1 + is_part;
       }
       if (!ok) return false;
-      g += end;
       slot += end;
       if (slot >= kScales) slot -= kScales;
       at = at1; at1 = at2; sc = sc1;
     }
     return true;
   }
-  // After a wait that ran out: let the copies on their way land, within limits, before the CTA's memory is released.
+  // Before the CTA's memory is released: let the copies on their way land, within limits.  (Not only after a wait of this warp that ran
+  // out: where another one's did, nobody else may have waited for the last tiles.)
   __device__ __forceinline__ void drain() const {
-    if ((threadIdx.x & 31) != 0) return;
+    if (!elect_one()) return;
     const uint64_t begun = globaltimer_ns();
-    for (int i = g > kStages ? g - kStages : 0; i < g + 4; ++i)
-      while (!mbar_try_wait(full0 + 8 * (i % kStages), (i / kStages) & 1) && globaltimer_ns() - begun < 50ull * 1000 * 1000) {}
+    auto landed = [&](uint32_t bar, uint32_t parity) {
+      while (!mbar_try_wait(bar, parity) && globaltimer_ns() - begun < 50ull * 1000 * 1000) {}
+    };
+    if (part_on_way) landed(part, parts);
+    for (int i = issued > kStages ? issued - kStages : 0; i < issued; ++i) landed(full0 + 8 * (i % kStages), (i / kStages) & 1);
   }
 };
 
@@ -452,7 +461,7 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     feed.site = is_k ? FeederSites{kKFreeS, kKFullS} : FeederSites{kVFreeS, kVFullS};
     for (; ok && walk.more(); walk.next(p))
       ok = feed.piece(p, wc, walk.tiles(), walk.cur.first + walk.at, walk.b, walk.hb * p.bundle + in_bundle, walk.cur.lo, walk.cur.hi);
-    if (!ok) feed.drain();
+    feed.drain();
   } else if (warp == kIssueS) {
     // ============================================ Q . K^T ======================================
     // (An issuing thread gets an instruction every eight clocks or so, its code never stays in the scheduler's cache beside the softmax
@@ -490,11 +499,10 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           if (sd.at == 0) first = false;
         }
       }
-      if (!ok) {
-        const uint64_t begun = globaltimer_ns();
-        tc_commit(bar(F::kDrain));
-        while (!mbar_try_wait(bar(F::kDrain), 0) && globaltimer_ns() - begun < 50ull * 1000 * 1000) {}
-      }
+      // (every product is awaited before the CTA's memory is released, also where it was another role's wait that ran out)
+      const uint64_t begun = globaltimer_ns();
+      tc_commit(bar(F::kDrain));
+      while (!mbar_try_wait(bar(F::kDrain), 0) && globaltimer_ns() - begun < 50ull * 1000 * 1000) {}
     }
   } else if (warp == kIssueO) {
     // ============================================ V^T . W^T ====================================
@@ -520,11 +528,10 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           sd.next();
         }
       }
-      if (!ok) {
-        const uint64_t begun = globaltimer_ns();
-        tc_commit(bar(F::kDrain + 1));
-        while (!mbar_try_wait(bar(F::kDrain + 1), 0) && globaltimer_ns() - begun < 50ull * 1000 * 1000) {}
-      }
+      // (every product is awaited before the CTA's memory is released, also where it was another role's wait that ran out)
+      const uint64_t begun = globaltimer_ns();
+      tc_commit(bar(F::kDrain + 1));
+      while (!mbar_try_wait(bar(F::kDrain + 1), 0) && globaltimer_ns() - begun < 50ull * 1000 * 1000) {}
     }
   } else {
     // ============================================ softmax ======================================

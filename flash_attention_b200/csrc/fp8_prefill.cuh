@@ -283,7 +283,8 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       feed.scales = reinterpret_cast<float*>(gbase + L::kOffSc);
       feed.box = reinterpret_cast<int2*>(gbase + L::kOffBox);
       feed.site = {kKFreeS, kKFullS};
-      if (!feed.piece(p, wc, n, t0, b, hk, lo_all, hi_all)) feed.drain();
+      feed.piece(p, wc, n, t0, b, hk, lo_all, hi_all);
+      feed.drain();
     } else if (warp == 14) {
       fp8d::Feeder<kD, L::kStagesV, L::kScales> feed;
       feed.tm = &tm_v;
@@ -295,7 +296,8 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       feed.scales = nullptr;
       feed.box = reinterpret_cast<int2*>(gbase + L::kOffBox) + 32;
       feed.site = {kRawFreeS, kRawFullS};
-      if (!feed.piece(p, wc, n, t0, b, hk, lo_all, hi_all)) feed.drain();
+      feed.piece(p, wc, n, t0, b, hk, lo_all, hi_all);
+      feed.drain();
     } else if (warp == 13) {
       // ============================================ products =====================================
       // (Products are ordered by issue only where they share an accumulator and a shape: what is overwritten is waited for.

@@ -73,3 +73,18 @@ def test_products_wait_for_what_they_overwrite():
     assert "true, half" in loop[first:first + 40] and "false, half" in loop[second:second + 40]
     assert re.search(waits % ("gone", "phase"), loop[:first]) and re.search(waits % (r"gone \+ 8 \* two", "phase"), loop[:first])
     assert re.search(waits % (r"bar\(L::kUFree \+ t\)", "half") + r";\s*if \(!ok\) break;\s*tc_fence_after_sync\(\);\s*$", loop[:second])
+
+
+@pytest.mark.parametrize("banner", ["Q . K^T", "V^T . W^T"])
+def test_products_over_the_8_bit_cache_are_awaited_whoever_gave_up(banner):
+    """An issuer may have nothing left to wait for when another role's wait runs out: its last products are on their way then, and
+    the CTA's memory must not be released before them."""
+    role = _role("fp8_decode.cuh", banner)
+    drain = role.rindex("tc_commit(bar(F::kDrain")
+    assert "if (!ok)" not in role and re.search(r"const uint64_t begun = globaltimer_ns\(\);\s*$", role[:drain])
+
+
+def test_copies_of_the_8_bit_cache_are_awaited_whoever_gave_up():
+    for name, calls in (("fp8_decode.cuh", 1), ("fp8_prefill.cuh", 2)):
+        text = re.sub(r"//.*", "", open(os.path.join(CSRC, name)).read())
+        assert len(re.findall(r"^ *feed\.drain\(\);$", text, re.M)) == text.count("feed.drain()") == calls
