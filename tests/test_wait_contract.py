@@ -81,7 +81,7 @@ def test_products_over_the_8_bit_cache_are_awaited_whoever_gave_up(banner):
     the CTA's memory must not be released before them."""
     role = _role("fp8_decode.cuh", banner)
     drain = role.rindex("tc_commit(bar(F::kDrain")
-    assert "if (!ok)" not in role and re.search(r"const uint64_t begun = globaltimer_ns\(\);\s*$", role[:drain])
+    assert "if (!ok) {" not in role and re.search(r"const uint64_t begun = globaltimer_ns\(\);\s*$", role[:drain])
 
 
 def test_copies_of_the_8_bit_cache_are_awaited_whoever_gave_up():
