@@ -1045,10 +1045,18 @@ void describe_cache(Fp8Cache& f, int64_t B) {
   }
 }
 
+// e4m3 values, or their bytes
+at::Tensor e4m3_of(PyObject* o, const char* name) {
+  const at::Tensor& t = tensor_of(o, name);
+  const auto st = t.scalar_type();
+  FA4_ASSERT(st == at::kByte || st == at::ScalarType::Float8_e4m3fn, "%s must be uint8 / float8_e4m3fn, got %s", name, c10::toString(st));
+  return st == at::kByte ? t : t.view(at::kByte);
+}
+
 Fp8Cache cache_of(PyObject* const* a) {
   Fp8Cache f;
-  f.k = as_u8(a[0], "k of the cache");
-  f.v = as_u8(a[1], "v of the cache");
+  f.k = e4m3_of(a[0], "k of the cache");
+  f.v = e4m3_of(a[1], "v of the cache");
   f.k_scale = tensor_of(a[2], "k_scale");
   f.v_scale = tensor_of(a[3], "v_scale");
   f.table = optional_tensor(a[4], "page_table");

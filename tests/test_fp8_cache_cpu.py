@@ -172,3 +172,17 @@ def test_oracle_scale():
     for top in (448.0, 448.1, 224.0, 1e-40, 3.5, 3.4999, 1e38):
         s = orc.scale_for(top)
         assert top <= 448 * s and (s == 2.0 ** -120 or top > 448 * s / 2) and math.log2(s).is_integer()
+
+
+def test_a_cache_of_another_type_is_refused():
+    """Two 4-bit values a byte are no e4m3 values, though they come as bytes as well."""
+    c = fa.FP8KVCache.empty(4, 64, 2, 128, device="cpu")
+    k = torch.zeros(1, 1, 2, 128, dtype=torch.bfloat16)
+    n = torch.zeros(1, dtype=torch.int32)
+    for dtype in (torch.float4_e2m1fn_x2, torch.float8_e5m2, torch.int8):
+        other = c.k.view(torch.uint8).view(dtype)
+        for bad, name in ((fa.FP8KVCache(other, c.v, c.k_scale, c.v_scale), "k"), (fa.FP8KVCache(c.k, other, c.k_scale, c.v_scale), "v")):
+            with pytest.raises(AssertionError, match=f"{name} of the cache must be uint8 / float8_e4m3fn"):
+                fa.append_kv_fp8(bad, k, k, n)
+            with pytest.raises(AssertionError, match=f"{name} of the cache must be uint8 / float8_e4m3fn"):
+                fa.flash_attn_fp8_cache_func(k, bad, n)
