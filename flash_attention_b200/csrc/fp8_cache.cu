@@ -4,6 +4,7 @@
 #include "launch.cuh"
 
 #include <algorithm>
+#include <cmath>
 #include <numeric>
 #include <type_traits>
 
@@ -118,6 +119,15 @@ extern "C" int fa4_fp8_cache_append(const fa4_fp8_cache* c, const fa4_fp8_append
 
 namespace {
 
+// Factors of the scores: in log2 units softmax_scale * log2 e, or with a soft cap cap * log2 e tanh((q . k) * softmax_scale / cap).
+struct ScoreFactors {
+  float sl2, cap_in, cap_out;
+};
+ScoreFactors factors_of(const fa4_fp8_fwd* f) {
+  constexpr float kLog2e = 1.4426950408889634f;
+  return {f->softmax_scale * kLog2e, f->softcap > 0.f ? f->softmax_scale / f->softcap : 0.f, f->softcap * kLog2e};
+}
+
 int validate_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f) {
   if (int e = validate_cache(c)) return e;
   if (f == nullptr) return -FA4_E_NULL;
@@ -126,6 +136,8 @@ int validate_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f) {
   if (f->B <= 0 || f->Sq <= 0 || f->Hq <= 0 || f->Hq % c->Hkv != 0) return -FA4_E_SHAPE;
   if (c->page_table == nullptr && f->B > c->num_pages) return -FA4_E_SHAPE;
   if (!(f->softmax_scale > 0.f) || !(f->softcap >= 0.f) || f->num_splits < 0 || f->num_splits > 128) return -FA4_E_SHAPE;
+  const ScoreFactors by = factors_of(f);
+  if (!std::isfinite(by.sl2) || !std::isfinite(by.cap_out) || (f->softcap > 0.f && !std::isnormal(by.cap_in))) return -FA4_E_SHAPE;
   // (tiles of all sequences and heads are counted in 32 bits)
   if ((int64_t)f->B * c->Hkv * ((int64_t)c->pages_per_seq * c->page_size / 128 + 1) > 0x3fffffffll) return -FA4_E_TOO_LARGE;
   if ((int64_t)f->B * f->Sq * f->Hq > 0x0fffffffll || f->B > 65535) return -FA4_E_TOO_LARGE;
@@ -266,10 +278,10 @@ extern "C" int fa4_fp8_cache_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, v
   p.div_group = make_fastdiv((uint32_t)p.group);
   p.div_hq = make_fastdiv((uint32_t)f->Hq);
   p.div_sq = make_fastdiv((uint32_t)f->Sq);
-  constexpr float kLog2e = 1.4426950408889634f;
-  p.sl2 = f->softmax_scale * kLog2e;
-  p.cap_in = f->softcap > 0.f ? f->softmax_scale / f->softcap : 0.f;
-  p.cap_out = f->softcap * kLog2e;
+  const ScoreFactors by = factors_of(f);
+  p.sl2 = by.sl2;
+  p.cap_in = by.cap_in;
+  p.cap_out = by.cap_out;
   p.win_left = f->window_left;
   p.win_right = f->causal && f->window_right < 0 ? 0 : f->window_right;
   p.status = f->status;

@@ -1174,6 +1174,11 @@ void run_fp8(Fp8Call& c) {
   if (!(c.softcap >= 0.0) || !std::isfinite(c.softcap)) fail(PyExc_ValueError, "softcap must be a finite number >= 0");
   const double softmax_scale = c.default_softmax_scale ? 1.0 / std::sqrt((double)D) : c.softmax_scale;
   if (!(softmax_scale > 0.0) || !std::isfinite(softmax_scale)) fail(PyExc_ValueError, "softmax_scale must be a finite number > 0");
+  // (the kernels have both, their products with log2 e and the one over the other in fp32)
+  const double cap_in = c.softcap > 0.0 ? softmax_scale / c.softcap : 1.0;
+  if (!(softmax_scale >= 1e-37 && softmax_scale <= 1e37)) fail(PyExc_ValueError, "softmax_scale must be in 1e-37..1e37");
+  if (c.softcap > 0.0 && !(c.softcap >= 1e-37 && c.softcap <= 1e37 && cap_in >= 1e-37 && cap_in <= 1e37))
+    fail(PyExc_ValueError, "softcap must be 0 or in 1e-37..1e37, and softmax_scale / softcap too");
   c10::cuda::OptionalCUDAGuard guard;
   if (device.index() != c10::cuda::current_device()) guard.set_device(device);
   void* stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();

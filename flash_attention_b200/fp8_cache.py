@@ -109,7 +109,8 @@ def flash_attn_fp8_cache_func(
     written among them).  ``seqused_q`` (B,) int32: how many of the Sq rows are there; the others are not written (in a new ``out`` and
     ``lse`` they are zeros).  Row i stands at position ``seqused_k[b] - seqused_q[b] + i``, which ``causal`` and
     ``window_size`` refer to.  ``learnable_sink``, ``softcap``, ``num_splits`` (0: chosen), ``out`` and ``lse`` as in
-    :func:`flash_attn_fp4_func`; a row that sees nothing gets zeros and an lse of -inf.
+    :func:`flash_attn_fp4_func` (a soft cap lies in 1e-37 .. 1e37, and so does softmax_scale / softcap); a row that sees nothing gets zeros and an
+    lse of -inf, or its head's sink.
 
     Not differentiable.  A row's softmax weights, times their value scales, keep eight bits down to 2^-14 of the largest among 128 keys and are
     right to 2^-22 of it below (more than 32 rows per kv head: eleven bits down to 2^-20 of the largest so far, right to 2^-31 of that below).  So an

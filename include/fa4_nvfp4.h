@@ -570,7 +570,7 @@ typedef struct fa4_fp8_fwd {
   const int32_t* seqused_k;
   const int32_t* seqused_q;  /* or NULL */
   const float* sink;         /* Hq logits or NULL */
-  float softmax_scale, softcap;
+  float softmax_scale, softcap;   /* > 0, >= 0 (0: none); finite, their products with log2 e too, and softmax_scale / softcap a normal number */
   int32_t causal, window_left, window_right;   /* -1: unlimited */
   int32_t num_splits;
   void* workspace;

@@ -186,3 +186,16 @@ def test_a_cache_of_another_type_is_refused():
                 fa.append_kv_fp8(bad, k, k, n)
             with pytest.raises(AssertionError, match=f"{name} of the cache must be uint8 / float8_e4m3fn"):
                 fa.flash_attn_fp8_cache_func(k, bad, n)
+
+
+@pytest.mark.parametrize("kw", [dict(softcap=math.inf), dict(softcap=3e38), dict(softcap=1e-41), dict(softmax_scale=math.inf), dict(softmax_scale=3e38),
+                                dict(softcap=math.nan), dict(softmax_scale=1e-30, softcap=1e20), dict(softmax_scale=1e20, softcap=1e-30)])
+def test_scales_and_soft_caps_beyond_fp32_are_refused(kw):
+    """(0.1 over a cap of 1e-41 is infinite, 1e-30 over 1e20 is 0: every score would be NaN or 0)"""
+    L = fa.lib()
+    L.fa4_fp8_cache_fwd_workspace_bytes.restype = ctypes.c_int64
+    f = fwd(**kw)
+    assert L.fa4_fp8_cache_fwd(ctypes.byref(cache()), ctypes.byref(f), None) == SHAPE
+    assert L.fa4_fp8_cache_fwd_workspace_bytes(ctypes.byref(cache()), ctypes.byref(f)) == SHAPE
+    for ok in (dict(softcap=1e30), dict(softcap=1e-30), dict(softmax_scale=1e-30), dict(softmax_scale=1e30)):
+        assert L.fa4_fp8_cache_fwd_workspace_bytes(ctypes.byref(cache()), ctypes.byref(fwd(**ok))) >= 0

@@ -907,3 +907,25 @@ def test_few_rows_on_value_scales_at_the_ends_of_their_range(cuda_device, Sq, ex
     for b in range(2):
         cache.v_scale[table[b, 2:4].long()] = 2.0 ** (exponent + (80 if exponent < 0 else -80))
     attend_values(cuda_device, cache, table, [1000, 640], torch.randn(2, Sq, 8, 128, generator=torch.Generator().manual_seed(5)).bfloat16(), num_splits=splits)
+
+
+def test_scales_and_soft_caps_at_the_ends_of_fp32(cuda_device):
+    """Beyond them refused (a cap that fp32 rounds to 0 would be no cap); inside a cap far from the scores is none, or cuts all of them."""
+    cache, table = batch_of(cuda_device, 1, 200)
+    lens = torch.tensor([200], dtype=torch.int32, device=cuda_device)
+    largest = float(held_of(cache, table[0].tolist(), 200)[1].abs().max())
+    for Sq in (1, 40):
+        q = torch.randn(1, Sq, 8, 128, generator=torch.Generator().manual_seed(1)).bfloat16().to(cuda_device)
+        call = lambda **kw: fa.flash_attn_fp8_cache_func(q, cache, lens, page_table=table, return_lse=True, **kw)
+        for kw in (dict(softcap=1e300), dict(softcap=1e-300), dict(softmax_scale=1e300), dict(softmax_scale=1e-300), dict(softmax_scale=1e-20, softcap=1e20)):
+            with pytest.raises(ValueError, match="must be"):
+                call(**kw)
+        plain, even = call(), call(softmax_scale=1e-30)
+        far, near = call(softcap=1e30), call(softcap=1e-30)
+        fa.check_status(cuda_device)
+        # scores of a few units, 2^-20 of them and the weights' own 2^-8 apart
+        assert ((far[1] - plain[1]).abs() <= 2.0 ** -18 * plain[1].abs().clamp(min=1.0)).all()
+        assert ((far[0].float() - plain[0].float()).abs() <= 2.0 ** -6 * largest).all()
+        # every weight alike
+        assert ((near[1] - math.log(200)).abs() <= 2.0 ** -18 * math.log(200)).all() and torch.equal(near[1], even[1])
+        assert ((near[0].float() - even[0].float()).abs() <= 2.0 ** -6 * largest).all()
