@@ -1191,6 +1191,7 @@ void run_fp8(Fp8Call& c) {
     FA4_ASSERT(c.out.stride(3) == 1 && (reinterpret_cast<uintptr_t>(c.out.data_ptr()) & 15u) == 0 && c.out.stride(0) % 8 == 0 &&
                    c.out.stride(1) % 8 == 0 && c.out.stride(2) % 8 == 0,
                "out must be 16-byte aligned, its last dimension contiguous, its strides multiples of 8");
+    for (int i = 0; i < 3; ++i) FA4_ASSERT(c.out.size(i) <= 1 || c.out.stride(i) != 0, "out must not be expanded: its rows are written side by side");
   }
   if (c.lse.defined()) {
     validate(c.lse, "lse", {B, Hq, Sq}, at::kFloat, device);

@@ -929,3 +929,14 @@ def test_scales_and_soft_caps_at_the_ends_of_fp32(cuda_device):
         # every weight alike
         assert ((near[1] - math.log(200)).abs() <= 2.0 ** -18 * math.log(200)).all() and torch.equal(near[1], even[1])
         assert ((near[0].float() - even[0].float()).abs() <= 2.0 ** -6 * largest).all()
+
+
+def test_an_expanded_output_is_refused(cuda_device):
+    cache, table = batch_of(cuda_device, 2, 100)
+    lens = torch.tensor([90, 80], dtype=torch.int32, device=cuda_device)
+    for Sq in (2, 40):
+        q = torch.zeros(2, Sq, 8, 128, dtype=torch.bfloat16, device=cuda_device)
+        for i in range(3):
+            shape = [1 if j == i else n for j, n in enumerate(q.shape)]
+            with pytest.raises(AssertionError, match="out must not be expanded"):
+                fa.flash_attn_fp8_cache_func(q, cache, lens, page_table=table, out=torch.zeros(shape, dtype=q.dtype, device=cuda_device).expand(q.shape))
