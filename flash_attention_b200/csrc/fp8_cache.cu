@@ -174,8 +174,9 @@ struct Fp8Plan {
 // Rows of a CTA and splits of the kernel for many rows.  Chosen splits: 256 rows, whatever the batch.  CTAs that are more than the SMs: 256 rows, one
 // split.  Else what takes the least time by these figures (us): a CTA 10 with 128 rows and 13 with 256, a step of 128 keys 2.0 and 1.85 (the softmax of one tile
 // wait for the products more often), a merge 5 and the partial results, written and read once at 4 TB/s.  Measured, 128 rows / 256 rows / 256 in two
-// splits, D = 128: 333 rows of 16 heads on as many keys 13.7 / 17.0 / 21.9, 512 of 32 heads on 1024 keys 21.9 / 26.9 / 32.6, on 4096 keys
-// 57.5 / 70.9 / 55.5, three sequences of up to 333 rows of 16 heads on up to 2048 keys 41.0 / 47.4 / 40.4.
+// splits, D = 128: 333 rows of 16 heads on as many keys 13.3 / 16.6 / 21.3, 512 of 32 heads on 1024 keys 21.2 / 25.4 / 31.7, on 4096 keys
+// 56.4 / 68.2 / 54.0, three sequences of 333 rows of 16 heads on up to 2048 keys 39.3 / 40.6 / 40.2.
+// The steps are those of a table that is full: the lengths are on the device.  In front of a table for 16 times its keys the first call takes 21.2, as if split.
 void plan_many(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, Fp8Plan* plan) {
   const int group = f->Hq / c->Hkv, chosen = f->num_splits;
   const int64_t rows = (int64_t)f->Sq * group, units = (int64_t)c->Hkv * f->B, values = (int64_t)f->B * f->Sq * f->Hq * c->D;
@@ -200,7 +201,9 @@ void plan_many(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, Fp8Plan* plan) {
 Fp8Plan plan_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f) {
   Fp8Plan plan = {};
   const int64_t rows = (int64_t)f->Sq * (f->Hq / c->Hkv), units = (int64_t)c->Hkv * f->B;
-  // us, decode kernel / kernel for many rows: 8 sequences of five rows of 32 heads over up to 4099 keys 21 / 44, 32 of eight over up to 8192 75 / 225
+  // us, decode kernel / kernel for many rows: 8 sequences of five rows of 32 heads over up to 4099 keys 21 / 44, 32 of eight over up to 8192 75 / 225.
+  // So the change is a step: the decode kernel's tensor memory and registers end at 32 rows, and 36 to 64 rows take 227 (128 rows 168, 256 rows 210), 44 on
+  // the shorter ones.
   plan.decode = rows <= 32;
   if (plan.decode) {
     plan.rows = rows <= 16 ? 16 : 32;

@@ -21,10 +21,11 @@
 // (every head at its own place in the list: 4 x 65536 keys of 8 heads at 3.9 TB/s, HBM pages and translations missed).  A unit (sequence, kv head) that ends up in several CTAs is
 // merged by fp8_merge_kernel.  With a split count of the caller's a CTA has one split of one unit.
 //
-// What bounds it: HBM in its steady part, 4 x 65536 keys of 8 heads 91 us (88 the kernel: 6.1 TB/s, 94 % of a measured copy; 82 at that rate).  Short calls pay
+// What bounds it (calls back to back): HBM in its steady part, 4 x 65536 keys of 8 heads 92 us (88 the kernel: 6.1 TB/s, 94 % of a measured copy; 82 at that
+// rate; 112 in turn with other work).  Short calls pay
 // about 14 us in front and behind: dealing 1.3, a chain of table, scales and copies, the products of the first and the last tile, the merge of
-// pieces 3 to 4; 32 sequences of up to 8192 keys 55 us (38), 8 of five rows over up to 4099 keys with pages of 16 23 us (6).  A unit alone (one token over 777
-// keys: eight CTAs of seven tiles) takes 9.2 us.
+// pieces 3 to 4; 32 sequences of up to 8192 keys 55 us (38), 8 of five rows over up to 4099 keys with pages of 16 22 us (6).  A unit alone (one token over 777
+// keys: eight CTAs of seven tiles) takes 9.6 us.
 //
 // Warps: kStrands softmax warpgroups, to which the tiles are dealt in turn, then the loaders of K and V and the issuers of the two products.  The
 // loaders run ahead through the pieces of a CTA.  Every wait is bounded.  A warp whose wait ran out goes through the rest of its loops

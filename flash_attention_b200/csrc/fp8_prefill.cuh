@@ -14,13 +14,13 @@
 // its next scores waiting (with one product of 128 columns it waited 1500 of 4000 clocks for W V and Q K^T: 294 us for the first call below), and no product
 // overwrites weights that another one may still read (Q K^T behind W V by issue alone 236 us, upper scores always in the same half and W V waited for 254-267).
 //
-// What bounds it: no unit alone.  A step of 256 rows x 128 keys takes about 3300 clocks: the exponentials 2048, the products 2560 (Q K^T in halves of 64
-// columns 48 clocks an instruction, bound by shared memory), 1700 issue slots a scheduler, in chains between two warps of a scheduler.  D = 128, B = 1:
-// 1024 rows of 32 heads on 16384 keys 238 us (162 at the measured rate of bf16 products), tensor pipe 62 %, exponential unit 62 %, issue slots 53 %
-// busy; 8192 rows of 64 heads on as many keys, causal, 940 us at first and 1080 under the power cap
+// What bounds it: no unit alone.  A step of 256 rows x 128 keys takes about 3400 clocks: the exponentials 2048, the products 2560 (Q K^T in halves of 64
+// columns 48 clocks an instruction, bound by shared memory), 1800 issue slots a scheduler, in chains between two warps of a scheduler.  D = 128, B = 1:
+// 1024 rows of 32 heads on 16384 keys 245 us back to back (162 at the measured rate of bf16 products), tensor pipe 60 %, exponential unit 60 %, issue slots
+// 53 % busy; 8192 rows of 64 heads on as many keys, causal, 975 us at first and 1110 under the power cap
 // (669, or 793 at the sustained rate).  A CTA's start and end take 12000 clocks, 8000 of them Q.
-// Exponentials by polynomials: one in eight 253, one in four 261 (more instructions between the others); the logarithm of a value scale in the
-// exponents where a half has one: 248; the lower scores loaded in front of the upper exponentials or between them: 282, 247.
+// Tried on a form of 238 us: exponentials by polynomials, one in eight 253, one in four 261 (more instructions between the others); the logarithm of a value
+// scale in the exponents where a half has one 248; the lower scores loaded in front of the upper exponentials or between them 282, 247.
 //
 // Warps: 0-3 and 4-7 softmax, 8-11 widen the tiles of V (cvt.f16x2.e4m3x2 runs at 64 a clock beside the exponentials), 12 and 14 load, 13 issues
 // the products.  Every wait is bounded (those of the softmax warps, which leave no registers for a call, by the issuer's: see mbar_wait_flag); a warp
@@ -124,8 +124,8 @@ __device__ __forceinline__ void widen_tile(const uint8_t* raw, uint8_t* to, int 
 
 // x to cap * tanh(x).  While no score of the warp's 64 keys is beyond 0.5 (a cap lies well above what scores mostly are), tanh x / x is a polynomial in
 // x^2 through its values at the four Chebyshev nodes of [0, 0.5^2]: off by 6e-7 of the value, and
-// without the two special functions of tanh_of, which with the weight's own would bound the kernel.  Three sequences of up to 333 rows on up to 2048 keys:
-// tanh_of alone 56 us, six nodes of [0, 0.75^2] 49.1, four 46.7.
+// without the two special functions of tanh_of, which with the weight's own would bound the kernel.  Three sequences of up to 333 rows on up to 2048 keys,
+// in a kernel that takes 49.6 now: tanh_of alone 56 us, six nodes of [0, 0.75^2] 49.1, four 46.7.
 __device__ __forceinline__ void cap_scores(float (&x)[64], float cap) {
   float far = fabsf(x[0]);
 #pragma unroll

@@ -112,7 +112,7 @@ def flash_attn_fp8_cache_func(
     :func:`flash_attn_fp4_func` (a soft cap lies in 1e-37 .. 1e37, and so does softmax_scale / softcap); a row that sees nothing gets zeros and an
     lse of -inf, or its head's sink.
 
-    Not differentiable.  A row's softmax weights, times their value scales, keep eight bits down to 2^-14 of the largest among 128 keys and are
+    Not differentiable.  Scores take a query's elements as they are down to 2^-10 of the row's largest, smaller ones to 2^-18 of it.  A row's softmax weights, times their value scales, keep eight bits down to 2^-14 of the largest among 128 keys and are
     right to 2^-22 of it below (more than 32 rows per kv head: eleven bits down to 2^-20 of the largest so far, right to 2^-31 of that below).  So an
     output element that is made by less than that (the values of the keys that weigh are zero there) is right to that much of the others, not to
     bf16.  Value scales that a row sees lie within a factor of 2^90 of each other.

@@ -486,7 +486,8 @@ int fa4_nvfp4_fwd_linear_sf_noalloc(const fa4_nvfp4_params* p, void* cuda_stream
  *
  *   k, v     (num_pages, page_size, Hkv, D) bytes, D = 64 or 128; the last dimension is contiguous, the strides of the others
  *            are multiples of 16 bytes (so pools of (page, head, token) order are views), base 16-byte aligned
- *   k_scale, v_scale  (num_pages, page_size / block, Hkv) fp32, contiguous: value = byte * scale
+ *   k_scale, v_scale  (num_pages, page_size / block, Hkv) fp32, contiguous: value = byte * scale.  No scale of a block in use is below 0
+ *            (the maxima are taken before the scales: a negative one gives wrong results or NaN)
  *   block    16, 32, 64 or 128; page_size a multiple of it
  *   page_table (B, pages_per_seq) int32 on the device: token t of sequence b lies in page page_table[b][t / page_size].
  *            NULL: contiguous caches, page b is sequence b's (num_pages = B at least, pages_per_seq = 1)
@@ -520,7 +521,8 @@ typedef struct fa4_fp8_cache {
  *   Scale of a block: the smallest power of two (2^-120 at least) by which the largest new value is at most 448; where
  *   the block holds tokens already (its first position is in front of seqlens[b]) no less than the scale it
  *   has.  If the scale grows the tokens it holds are rounded again: e4m3(byte * (old scale / new scale)).
- *   A value that is not finite becomes the NaN code and does not count for the scale.  Bytes past the last new token are
+ *   A byte is the e4m3 value nearest to value / scale in fp32 (a quotient within 2^-25 of a tie counts as the tie; with scales of an append, powers
+ *   of two, there is no such).  A value that is not finite becomes the NaN code and does not count for the scale.  Bytes past the last new token are
  *   not touched.
  * bf16 k, v (B, S, Hkv, D), q: last dimension contiguous, strides in ELEMENTS and multiples of 8, 16-byte aligned.  A block must not
  * belong to two sequences that append to it in one call.
@@ -552,6 +554,7 @@ int fa4_fp8_cache_append(const fa4_fp8_cache* cache, const fa4_fp8_append* a, vo
  * causal and window limits refer to; rows from seqused_q[b] on are neither computed nor written.
  *   score = softmax_scale * k_scale * (q . k), soft cap, masks, sink as in fa4_nvfp4_ext
  *   out = sum of softmax weight * v_scale * v: bf16 (B, Sq, Hq, D); lse fp32 (B, Hq, Sq) or NULL
+ * The scores take a query's elements as they are down to 2^-10 of the row's largest, smaller ones to 2^-18 of it, and are fp32 sums.
  * A row that sees no key gets zeros and an lse of -inf (of its sink).  What lies behind a sequence's last token may be anything,
  * NaN included.  A row's weights (times v_scale) keep eight bits down to 2^-14 of the largest of a tile of 128 keys, right to 2^-22 of it below; with
  * Sq * Hq / Hkv > 32 eleven bits down to 2^-20 of the largest so far, right to 2^-31 of that below.  Value scales that a row sees lie within
