@@ -25,6 +25,12 @@ struct Fp8Params {
   // scores in log2 units: (q . k8) * ks * sl2, or cap_out * tanh((q . k8) * ks * cap_in) with a soft cap
   float sl2, cap_in, cap_out;
   int win_left, win_right;           // -1: unlimited
+  // Chosen blocks: (B, query blocks, Hkv, chosen) ascending.  A unit's sequence is then a query block of a sequence, its keys are those of
+  // its list one behind the other.
+  const int32_t* blocks;
+  int chosen, query_block, query_blocks;
+  int seqs;                          // B * query_blocks (dense: B)
+  FastDiv div_query_blocks, div_query_block;
   uint32_t* status;
   uint32_t epoch;
   uint64_t budget_ns;
@@ -62,6 +68,67 @@ __device__ __forceinline__ SeqLens lens_of(const Fp8Params& p, int b) {
   n.sq = p.fresh != nullptr ? p.fresh[b] : p.Sq;
   n.sq = n.sq < 0 ? 0 : (n.sq < p.Sq ? n.sq : p.Sq);
   return n;
+}
+
+// ---- chosen blocks ----
+// Query block `v` of a call: its sequence and first row.
+struct QueryBlock {
+  int b, q0;
+};
+template <bool kBlocks>
+__device__ __forceinline__ QueryBlock query_block_of(const Fp8Params& p, int v) {
+  if constexpr (!kBlocks) return {v, 0};
+  const int b = fast_div(v, p.div_query_blocks);
+  return {b, (v - b * p.query_blocks) * p.query_block};
+}
+// Valid keys and rows of a unit's sequence; with chosen blocks the position of its first row (which may be negative) and its rows.
+template <bool kBlocks>
+__device__ __forceinline__ SeqLens unit_lens(const Fp8Params& p, int v) {
+  const QueryBlock at = query_block_of<kBlocks>(p, v);
+  SeqLens n = lens_of(p, at.b);
+  if constexpr (kBlocks) {
+    n.sk = n.sk - n.sq + at.q0;
+    n.sq = n.sq - at.q0;
+    n.sq = n.sq < 0 ? 0 : (n.sq < p.query_block ? n.sq : p.query_block);
+  }
+  return n;
+}
+// A list of chosen blocks, by a whole warp: it ends at the first entry that is not above the one in front of it.
+struct BlockList {
+  const int32_t* at;
+  int n;
+};
+__device__ __forceinline__ BlockList list_of(const Fp8Params& p, int v, int hk) {
+  BlockList l;
+  l.at = p.blocks + ((int64_t)v * p.Hkv + hk) * p.chosen;
+  l.n = p.chosen;
+  const int lane = threadIdx.x & 31;
+  int last = -1;
+#pragma unroll 1
+  for (int i0 = 0; i0 < p.chosen; i0 += 32) {
+    const int e = i0 + lane < p.chosen ? l.at[i0 + lane] : -1, up = __shfl_up_sync(0xffffffffu, e, 1);
+    const uint32_t ends = __ballot_sync(0xffffffffu, e <= (lane == 0 ? last : up));
+    if (ends != 0u) {
+      l.n = min(p.chosen, i0 + __ffs(ends) - 1);
+      break;
+    }
+    last = __shfl_sync(0xffffffffu, e, 31);
+  }
+  return l;
+}
+// How many of its keys lie in front of position `end`, by a whole warp.
+__device__ __forceinline__ int keys_in_front(const Fp8Params& p, BlockList l, int end) {
+  const int lane = threadIdx.x & 31, block = end >> p.log_block;
+  int whole = 0;
+  bool part = false;
+  if (end <= 0) return 0;
+#pragma unroll 1
+  for (int i0 = 0; i0 < l.n; i0 += 32) {
+    const int e = i0 + lane < l.n ? l.at[i0 + lane] : 0x7fffffff;
+    whole += __popc(__ballot_sync(0xffffffffu, e < block));
+    part = part || __any_sync(0xffffffffu, e == block);
+  }
+  return (whole << p.log_block) + (part ? end & ((1 << p.log_block) - 1) : 0);
 }
 
 // A row's result from its sum `l` under the reference `m` (log2 units) and the sink of its head: the factor of the

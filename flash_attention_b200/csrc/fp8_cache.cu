@@ -1,43 +1,14 @@
 // C ABI of the 8-bit KV cache (see include/fa4_nvfp4.h): argument validation and launches of the append and
 // of the attention over it.  Host code only; the kernels live in the .cuh files.
 #include "fp8_prefill.cuh"
-#include "launch.cuh"
+#include "fp8_host.cuh"
 
 #include <algorithm>
 #include <cmath>
 #include <numeric>
 #include <type_traits>
 
-namespace {
-
 using namespace fa4;
-
-// Shape, strides and alignment of a cache.  Touches no CUDA API.
-int validate_cache(const fa4_fp8_cache* c) {
-  if (c == nullptr) return -FA4_E_NULL;
-  if (c->struct_size != sizeof(fa4_fp8_cache)) return -FA4_E_STRUCT;
-  if (!c->k || !c->v || !c->k_scale || !c->v_scale) return -FA4_E_NULL;
-  if (c->block != 16 && c->block != 32 && c->block != 64 && c->block != 128) return -FA4_E_SHAPE;
-  if (c->num_pages <= 0 || c->page_size <= 0 || c->page_size % c->block != 0 || c->Hkv <= 0) return -FA4_E_SHAPE;
-  if (c->D != 64 && c->D != 128) return -FA4_E_SHAPE;
-  if (c->pages_per_seq <= 0 || (c->page_table == nullptr && c->pages_per_seq != 1)) return -FA4_E_SHAPE;
-  // positions are 32-bit
-  if ((int64_t)c->pages_per_seq * c->page_size > 0x7ffffc00ll) return -FA4_E_TOO_LARGE;
-  const int64_t strides[] = {c->k_stride_page, c->k_stride_token, c->k_stride_head,
-                             c->v_stride_page, c->v_stride_token, c->v_stride_head};
-  for (int64_t s : strides)
-    if (s <= 0 || (s & 15) != 0) return -FA4_E_STRIDE;
-  if (!aligned16(c->k) || !aligned16(c->v)) return -FA4_E_ALIGN;
-  return 0;
-}
-
-int log2_of(int n) {
-  int l = 0;
-  while ((1 << l) < n) ++l;
-  return l;
-}
-
-}  // namespace
 
 extern "C" int fa4_fp8_cache_append(const fa4_fp8_cache* c, const fa4_fp8_append* a, void* cuda_stream) {
   if (int e = validate_cache(c)) return e;
@@ -153,6 +124,15 @@ int validate_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f) {
 
 namespace {
 
+// Query blocks of a call (sequences, where no blocks are chosen), rows of one, and the most tiles of 128 keys that a list has.
+int64_t seqs_of(const fa4_fp8_fwd* f, const fa4_fp8_blocks* x) {
+  return x == nullptr ? f->B : (int64_t)f->B * ((f->Sq + (int64_t)x->query_block - 1) / x->query_block);
+}
+int rows_of(const fa4_fp8_fwd* f, const fa4_fp8_blocks* x) { return x == nullptr ? f->Sq : std::min(f->Sq, x->query_block); }
+int64_t list_tiles(const fa4_fp8_cache* c, const fa4_fp8_blocks* x) {
+  return (std::min((int64_t)x->num_blocks * c->block, (int64_t)c->pages_per_seq * c->page_size) + 127) / 128;
+}
+
 // The most tiles of 128 keys that `tokens` rows of a sequence one behind the other may see.
 int64_t most_tiles(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, int64_t tokens) {
   const int64_t all = ((int64_t)c->pages_per_seq * c->page_size + 127) / 128;
@@ -161,7 +141,7 @@ int64_t most_tiles(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, int64_t tokens)
   return open ? all : std::min(all, ((int64_t)f->window_left + std::max(0, f->window_right) + tokens + 126) / 128 + 1);
 }
 
-// How a call is run.
+// How a call is run.  With chosen blocks (`x`) a query block of a sequence takes the place of a sequence, and the tiles are at most those of a full list.
 struct Fp8Plan {
   bool decode;
   int rows;          // decode: rows that the kernel is built for
@@ -177,13 +157,13 @@ struct Fp8Plan {
 // splits, D = 128: 333 rows of 16 heads on as many keys 13.3 / 16.6 / 21.3, 512 of 32 heads on 1024 keys 21.2 / 25.4 / 31.7, on 4096 keys
 // 56.4 / 68.2 / 54.0, three sequences of 333 rows of 16 heads on up to 2048 keys 39.3 / 40.6 / 40.2.
 // The steps are those of a table that is full: the lengths are on the device.  In front of a table for 16 times its keys the first call takes 21.2, as if split.
-void plan_many(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, Fp8Plan* plan) {
+void plan_many(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, const fa4_fp8_blocks* x, Fp8Plan* plan) {
   const int group = f->Hq / c->Hkv, chosen = f->num_splits;
-  const int64_t rows = (int64_t)f->Sq * group, units = (int64_t)c->Hkv * f->B, values = (int64_t)f->B * f->Sq * f->Hq * c->D;
+  const int64_t rows = (int64_t)rows_of(f, x) * group, units = (int64_t)c->Hkv * seqs_of(f, x), values = (int64_t)f->B * f->Sq * f->Hq * c->D;
   double least = 0;
   for (const int cta_rows : {256, 128}) {
     const int64_t row_tiles = (rows + cta_rows - 1) / cta_rows, room = kSms / (units * row_tiles),
-                  tiles = most_tiles(c, f, std::min<int64_t>(f->Sq, (cta_rows - 1) / group + 2));
+                  tiles = x != nullptr ? list_tiles(c, x) : most_tiles(c, f, std::min<int64_t>(f->Sq, (cta_rows - 1) / group + 2));
     if (cta_rows == 128 && (room == 0 || chosen > 0)) break;
     const int64_t most = std::max<int64_t>(1, std::min<int64_t>({128, room, tiles / 2}));
     for (int64_t splits = chosen > 0 ? chosen : 1; splits <= (chosen > 0 ? chosen : most); ++splits) {
@@ -198,9 +178,9 @@ void plan_many(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, Fp8Plan* plan) {
     }
   }
 }
-Fp8Plan plan_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f) {
+Fp8Plan plan_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, const fa4_fp8_blocks* x) {
   Fp8Plan plan = {};
-  const int64_t rows = (int64_t)f->Sq * (f->Hq / c->Hkv), units = (int64_t)c->Hkv * f->B;
+  const int64_t rows = (int64_t)rows_of(f, x) * (f->Hq / c->Hkv), units = (int64_t)c->Hkv * seqs_of(f, x);
   // us, decode kernel / kernel for many rows: 8 sequences of five rows of 32 heads over up to 4099 keys 21 / 44, 32 of eight over up to 8192 75 / 225.
   // So the change is a step: the decode kernel's tensor memory and registers end at 32 rows, and 36 to 64 rows take 227 (128 rows 168, 256 rows 210), 44 on
   // the shorter ones.
@@ -210,22 +190,25 @@ Fp8Plan plan_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f) {
     plan.splits = f->num_splits;
     // Dealing the shares and merging the pieces costs about as much as ten tiles.  us, dealt / a CTA a unit: 128 units of a window of nine
     // tiles, head dim 64 19.0 / 12.6, 8 units of seven tiles 10.5 / 9.2; but 256 units of up to 64 tiles 57.6 / 71.1.
-    if (plan.splits == 0 && units <= kSms && most_tiles(c, f, f->Sq) <= 10) plan.splits = 1;
+    if (plan.splits == 0 && units <= kSms && (x != nullptr ? list_tiles(c, x) : most_tiles(c, f, f->Sq)) <= 10) plan.splits = 1;
+    // Many lists are about as long as each other: whole units, without a look at all lengths by every CTA and without a merge.
+    if (x != nullptr && plan.splits == 0 && units >= 4 * kSms) plan.splits = -1;
     // (us, up to 8 / 4 heads side by side, which are 144 / 148 CTAs: 32 sequences of up to 8192 keys 55 / 60, drafted tokens on pages of 16 29 / 32.5)
-    for (plan.bundle = std::min(8, c->Hkv); c->Hkv % plan.bundle != 0;) --plan.bundle;
-    plan.slots = plan.splits == 0 ? 2 * kSms : plan.splits == 1 ? 0 : units * plan.splits;
+    // (heads choose blocks of their own: nothing lies side by side)
+    for (plan.bundle = x != nullptr ? 1 : std::min(8, c->Hkv); c->Hkv % plan.bundle != 0;) --plan.bundle;
+    plan.slots = plan.splits == 0 ? 2 * kSms : plan.splits == 1 || plan.splits < 0 ? 0 : units * plan.splits;
     plan.slot_rows = rows;
   } else {
-    plan_many(c, f, &plan);
+    plan_many(c, f, x, &plan);
     plan.slots = plan.splits == 1 ? 0 : plan.splits;
     plan.slot_rows = (int64_t)f->B * f->Sq * f->Hq;
   }
   return plan;
 }
 // Values, then sums, then (dealt) the pieces of the units.
-int64_t workspace_of(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, const Fp8Plan& plan) {
+int64_t workspace_of(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, const fa4_fp8_blocks* x, const Fp8Plan& plan) {
   const int64_t values = plan.slots * plan.slot_rows;
-  return values * (c->D + 1) * 4 + (plan.decode && plan.splits == 0 ? (values % 2) * 4 + (int64_t)f->B * c->Hkv * 8 : 0);
+  return values * (c->D + 1) * 4 + (plan.decode && plan.splits == 0 ? (values % 2) * 4 + seqs_of(f, x) * c->Hkv * 8 : 0);
 }
 
 // The pool as (D, token of a page, head, page) bytes.
@@ -238,15 +221,25 @@ bool encode_pool(CUtensorMap* m, const fa4_fp8_cache* c, const void* base, int64
 
 }  // namespace
 
-extern "C" int64_t fa4_fp8_cache_fwd_workspace_bytes(const fa4_fp8_cache* c, const fa4_fp8_fwd* f) {
+namespace {
+
+int validate_blocks(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, const fa4_fp8_blocks* x) {
   if (int e = validate_fwd(c, f)) return e;
-  return workspace_of(c, f, plan_fwd(c, f));
+  if (x == nullptr) return -FA4_E_NULL;
+  if (x->struct_size != sizeof(fa4_fp8_blocks)) return -FA4_E_STRUCT;
+  if (!x->blocks) return -FA4_E_NULL;
+  // (rows see what is in front of them, and nothing is split by hand)
+  if (x->num_blocks <= 0 || x->query_block <= 0 || !f->causal || f->window_left >= 0 || f->window_right > 0 || f->num_splits != 0) return -FA4_E_SHAPE;
+  const int64_t units = seqs_of(f, x) * c->Hkv;
+  if ((int64_t)x->num_blocks * c->block > 0x3fffffffll || units > 0x0fffffffll || units * (list_tiles(c, x) + 1) > 0x3fffffffll) return -FA4_E_TOO_LARGE;
+  return 0;
 }
 
-extern "C" int fa4_fp8_cache_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, void* cuda_stream) {
-  if (int e = validate_fwd(c, f)) return e;
-  const Fp8Plan plan = plan_fwd(c, f);
-  const int64_t bytes = workspace_of(c, f, plan);
+// The attention; x: over chosen blocks.
+template <bool kBlocks>
+int run_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, const fa4_fp8_blocks* x, void* cuda_stream) {
+  const Fp8Plan plan = plan_fwd(c, f, x);
+  const int64_t bytes = workspace_of(c, f, x, plan);
   if (bytes > 0 && f->workspace == nullptr) return -FA4_E_NULL;
   if (bytes > 0 && !aligned16(f->workspace)) return -FA4_E_ALIGN;
   if (bytes > 0 && f->workspace_bytes < (uint64_t)bytes) return -FA4_E_TOO_LARGE;
@@ -266,13 +259,22 @@ extern "C" int fa4_fp8_cache_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, v
   p.o_partial = static_cast<float*>(f->workspace);
   p.lse_partial = bytes > 0 ? p.o_partial + plan.slots * plan.slot_rows * c->D : nullptr;
   p.pieces = bytes > 0 ? reinterpret_cast<int2*>(p.lse_partial + (plan.slots * plan.slot_rows + 1) / 2 * 2) : nullptr;
-  p.unit_rows = f->Sq * (f->Hq / c->Hkv);
+  p.unit_rows = rows_of(f, x) * (f->Hq / c->Hkv);
   p.bundle = plan.decode ? plan.bundle : 1;
   p.bundles = c->Hkv / p.bundle;
   p.row_tiles = plan.row_tiles;
   p.cta_rows = plan.cta_rows;
   // (a contiguous cache has no page borders: what lies behind its end is read as zeros)
-  p.box = c->page_table == nullptr ? 128 : std::gcd(c->page_size, 128);
+  p.box = kBlocks ? c->block : c->page_table == nullptr ? 128 : std::gcd(c->page_size, 128);
+  p.seqs = (int)seqs_of(f, x);
+  if (kBlocks) {
+    p.blocks = x->blocks;
+    p.chosen = x->num_blocks;
+    p.query_block = rows_of(f, x);
+    p.query_blocks = p.seqs / f->B;
+    p.div_query_block = make_fastdiv((uint32_t)p.query_block);
+    p.div_query_blocks = make_fastdiv((uint32_t)p.query_blocks);
+  }
   p.B = f->B; p.Sq = f->Sq; p.Hq = f->Hq; p.Hkv = c->Hkv; p.group = f->Hq / c->Hkv; p.D = c->D;
   p.log_block = log2_of(c->block);
   p.num_pages = c->num_pages; p.page_size = c->page_size; p.pages_per_seq = c->pages_per_seq;
@@ -299,7 +301,7 @@ extern "C" int fa4_fp8_cache_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, v
   const int64_t rows = (int64_t)f->B * f->Sq * f->Hq;
   const unsigned merge_grid = (unsigned)((rows + kFp8CombineWarps - 1) / kFp8CombineWarps);
   if (plan.decode) {
-    const int64_t grid = plan.splits == 0 ? kSms / plan.bundle * plan.bundle : (int64_t)plan.splits * c->Hkv * f->B;
+    const int64_t grid = plan.splits == 0 ? kSms / plan.bundle * plan.bundle : plan.splits < 0 ? kSms : (int64_t)plan.splits * c->Hkv * p.seqs;
     p.div_groups = make_fastdiv((uint32_t)(kSms / plan.bundle));
     auto launch = [&](auto form) -> int {
       using F = decltype(form);
@@ -308,22 +310,41 @@ extern "C" int fa4_fp8_cache_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, v
     using fp8d::Form;
     auto launch_rows = [&](auto capped) -> int {
       constexpr bool kCap = decltype(capped)::value;
-      if (c->D == 128) return plan.rows == 16 ? launch(Form<128, 16, kCap>{}) : launch(Form<128, 32, kCap>{});
-      return plan.rows == 16 ? launch(Form<64, 16, kCap>{}) : launch(Form<64, 32, kCap>{});
+      if (c->D == 128) return plan.rows == 16 ? launch(Form<128, 16, kCap, kBlocks>{}) : launch(Form<128, 32, kCap, kBlocks>{});
+      return plan.rows == 16 ? launch(Form<64, 16, kCap, kBlocks>{}) : launch(Form<64, 32, kCap, kBlocks>{});
     };
     const int rc = cap ? launch_rows(std::true_type{}) : launch_rows(std::false_type{});
-    if (rc != 0 || plan.splits == 1) return rc;
-    return launch_pdl(fp8_merge_kernel, dim3(merge_grid), kFp8CombineWarps * 32, 0, stream, p);
+    if (rc != 0 || plan.splits == 1 || plan.splits < 0) return rc;
+    return launch_pdl(fp8_merge_kernel<kBlocks>, dim3(merge_grid), kFp8CombineWarps * 32, 0, stream, p);
   }
   // (a launch needs the registers that the kernel's budget counts on: see ensure_kernel)
   auto launch_many = [&](auto kernel, uint32_t smem) -> int {
     if (int e = ensure_kernel(kernel, smem, fp8p::kRegsLaunch)) return e;
-    return launch_pdl(kernel, dim3((unsigned)((int64_t)plan.row_tiles * c->Hkv * f->B * plan.splits)), fp8p::kThreads, smem, stream, tm_k, tm_v, p);
+    return launch_pdl(kernel, dim3((unsigned)((int64_t)plan.row_tiles * c->Hkv * p.seqs * plan.splits)), fp8p::kThreads, smem, stream, tm_k, tm_v, p);
   };
-  const int rc = c->D == 128 ? (cap ? launch_many(fp8_prefill_kernel<128, true>, fp8p::Layout<128>::kRequest)
-                                    : launch_many(fp8_prefill_kernel<128, false>, fp8p::Layout<128>::kRequest))
-                             : (cap ? launch_many(fp8_prefill_kernel<64, true>, fp8p::Layout<64>::kRequest)
-                                    : launch_many(fp8_prefill_kernel<64, false>, fp8p::Layout<64>::kRequest));
+  const int rc = c->D == 128 ? (cap ? launch_many(fp8_prefill_kernel<128, true, kBlocks>, fp8p::Layout<128>::kRequest)
+                                    : launch_many(fp8_prefill_kernel<128, false, kBlocks>, fp8p::Layout<128>::kRequest))
+                             : (cap ? launch_many(fp8_prefill_kernel<64, true, kBlocks>, fp8p::Layout<64>::kRequest)
+                                    : launch_many(fp8_prefill_kernel<64, false, kBlocks>, fp8p::Layout<64>::kRequest));
   if (rc != 0 || plan.splits == 1) return rc;
   return launch_pdl(fp8_combine_kernel, dim3(merge_grid), kFp8CombineWarps * 32, 0, stream, p);
+}
+
+}  // namespace
+
+extern "C" int64_t fa4_fp8_cache_fwd_workspace_bytes(const fa4_fp8_cache* c, const fa4_fp8_fwd* f) {
+  if (int e = validate_fwd(c, f)) return e;
+  return workspace_of(c, f, nullptr, plan_fwd(c, f, nullptr));
+}
+extern "C" int fa4_fp8_cache_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, void* cuda_stream) {
+  if (int e = validate_fwd(c, f)) return e;
+  return run_fwd<false>(c, f, nullptr, cuda_stream);
+}
+extern "C" int64_t fa4_fp8_cache_fwd_blocks_workspace_bytes(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, const fa4_fp8_blocks* x) {
+  if (int e = validate_blocks(c, f, x)) return e;
+  return workspace_of(c, f, x, plan_fwd(c, f, x));
+}
+extern "C" int fa4_fp8_cache_fwd_blocks(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, const fa4_fp8_blocks* x, void* cuda_stream) {
+  if (int e = validate_blocks(c, f, x)) return e;
+  return run_fwd<true>(c, f, x, cuda_stream);
 }

@@ -104,7 +104,8 @@ struct FeederSites {
   uint32_t free, lands;      // where a wait may run out
 };
 // kLogs: behind the scales the logarithms of the values', to base 2.
-template <int kD, int kStages, int kScales, bool kLogs = false>
+// kBlocks: the keys are those of a list of blocks, one behind the other.
+template <int kD, int kStages, int kScales, bool kLogs = false, bool kBlocks = false>
 struct Feeder {
   static constexpr uint32_t kTile = 128 * kD;
   static constexpr int kWords = kLogs ? 24 : 16;
@@ -123,14 +124,17 @@ struct Feeder {
   bool part_on_way = false;         // a tile that lands on `part` (of the issuing thread)
 
   // Tiles t0 .. t0 + n - 1 of kv head hk of sequence b, in which keys [lo, hi) are seen.  False: a wait ran out.
-  __device__ __forceinline__ bool piece(const Fp8Params& p, const WaitCtx& wc, int n, int t0, int b, int hk, int lo, int hi) {
+  __device__ __forceinline__ bool piece(const Fp8Params& p, const WaitCtx& wc, int n, int t0, int b, int hk, int lo, int hi,
+                                        const int32_t* list = nullptr) {
     const int lane = threadIdx.x & 31, per_box = p.box >> 4, gr = lane & 7;
     bool ok = true;
     // (page, first key of these 16 in it) for the batch from tile `li` on; key -1: no row sees them
     auto look_up = [&](int li) -> int2 {
       int2 at = make_int2(0, -1);
-      const int mine = li + (lane >> 3), key = ((t0 + mine) << 7) + 16 * gr;
+      const int mine = li + (lane >> 3);
+      int key = ((t0 + mine) << 7) + 16 * gr;
       if (mine < n && key < hi && key + 16 > lo) {
+        if constexpr (kBlocks) key = (list[key >> p.log_block] << p.log_block) + (key & ((1 << p.log_block) - 1));
         const int pg = fast_div(key, p.div_page);
         at = make_int2(p.table != nullptr ? p.table[(int64_t)b * p.pages_per_seq + pg] : b, key - pg * p.page_size);
       }
@@ -241,11 +245,11 @@ struct Feeder {
   }
 };
 
-// kR: rows (16 or 32).
-template <int kD_, int kR_, bool kCap_>
+// kR: rows (16 or 32).  kBlocks: over chosen blocks.
+template <int kD_, int kR_, bool kCap_, bool kBlocks_ = false>
 struct Form {
   static constexpr int kD = kD_, kR = kR_, kStrands = kR == 16 ? 3 : 2, kStages = kD == 128 ? 5 : 10, kThreads = 128 * kStrands + 128;
-  static constexpr bool kCap = kCap_;
+  static constexpr bool kCap = kCap_, kBlocks = kBlocks_;
   static constexpr int kN = 2 * kR, kKeys = kR;       // keys of a thread: 128 lanes hold 128 / kR copies of the rows
   static constexpr uint32_t kTile = 128 * kD;
   // Scales of K and V come with K.  Its stage is free when the product is done, which is before the softmax has read them:
@@ -278,10 +282,19 @@ struct Form {
 struct Seq {
   int sk, sq, lo, hi, first, tiles;
 };
+template <bool kBlocks>
 __device__ __forceinline__ Seq seq_of(const Fp8Params& p, int sk, int sq) {
   Seq q;
   q.sk = sk;
   q.sq = sq;
+  if constexpr (kBlocks) {
+    // (as many as the list has room for, or are in front of the last row: the list itself may have fewer)
+    const int there = sq > 0 ? (max(sk + sq, 0) + (1 << p.log_block) - 1) >> p.log_block : 0;
+    q.lo = q.first = 0;
+    q.hi = min(there, p.chosen) << p.log_block;
+    q.tiles = (q.hi + 127) >> 7;
+    return q;
+  }
   q.lo = seen_by(p, sk, sq, 0).x;
   q.hi = sq > 0 ? seen_by(p, sk, sq, sq - 1).y : 0;
   q.first = q.lo >> 7;
@@ -292,53 +305,57 @@ __device__ __forceinline__ Seq seq_of(const Fp8Params& p, int sk, int sq) {
 __device__ __forceinline__ int cost_of(const Seq& q) { return q.sq == 0 ? 0 : max(q.tiles, 1); }
 
 // The CTA's walk through its pieces: `bundle` heads of a sequence are worked on side by side by as many CTAs, so units of the walk are
-// (sequence, bundle).  One warp finds the start and leaves it in shared memory; every warp walks on by itself, with the lengths of the next
+// (sequence, bundle), sequences being query blocks where the keys are chosen.  One warp finds the start and leaves it in shared memory; every warp walks on by itself, with the lengths of the next
 // sequence on their way while a piece is worked on.
+template <bool kBlocks>
 struct alignas(16) Walk {
   Seq cur;
   int b, hb, at, left;       // unit, first place of the piece in it, places of this CTA from there on
   int share;                 // places of a CTA
   int next_sk, next_sq;
+  int units;                 // whole units alone: how many are left; else 0
 
   __device__ __forceinline__ bool more() const { return left > 0; }
   __device__ __forceinline__ int places() const { return min(left, cost_of(cur) - at); }
   __device__ __forceinline__ int tiles() const { return min(places(), cur.tiles - at); }
   __device__ __forceinline__ void fetch(const Fp8Params& p) {
     if (left <= cost_of(cur) - at) return;                     // (the last piece)
-    const SeqLens n = b + 1 < p.B ? lens_of(p, b + 1) : SeqLens{0, 0};
+    const SeqLens n = b + 1 < p.seqs ? unit_lens<kBlocks>(p, b + 1) : SeqLens{0, 0};
     next_sk = n.sk;
     next_sq = n.sq;
   }
   __device__ __forceinline__ void next(const Fp8Params& p) {
-    left -= places();
+    if (!kBlocks || units == 0) left -= places();
+    else if (--units == 0) left = 0;
     if (left <= 0) return;
     at = 0;
     if (++hb == p.bundles) {
       hb = 0;
       do {
-        if (++b >= p.B) {
+        if (++b >= p.seqs) {
           left = 0;
           return;
         }
-        cur = seq_of(p, next_sk, next_sq);
+        cur = seq_of<kBlocks>(p, next_sk, next_sq);
         fetch(p);
-      } while (cost_of(cur) == 0);
+      } while ((!kBlocks || units == 0) && cost_of(cur) == 0);
     }
   }
 };
 
 // Where group `group` of CTAs (of as many as p.div_groups divides by) starts, by one warp.
-__device__ __forceinline__ Walk deal_shares(const Fp8Params& p, int group, int lane) {
-  Walk w = {};
-  w.b = p.B;
+template <bool kBlocks>
+__device__ __forceinline__ Walk<kBlocks> deal_shares(const Fp8Params& p, int group, int lane) {
+  Walk<kBlocks> w = {};
+  w.b = p.seqs;
   auto read = [&](int b0) {
-    const SeqLens n = b0 + lane < p.B ? lens_of(p, b0 + lane) : SeqLens{0, 0};
-    return seq_of(p, n.sk, n.sq);
+    const SeqLens n = b0 + lane < p.seqs ? unit_lens<kBlocks>(p, b0 + lane) : SeqLens{0, 0};
+    return seq_of<kBlocks>(p, n.sk, n.sq);
   };
   const Seq first = read(0);
   int total = cost_of(first);
 #pragma unroll 1
-  for (int b0 = 32; b0 < p.B; b0 += 32) total += cost_of(read(b0));
+  for (int b0 = 32; b0 < p.seqs; b0 += 32) total += cost_of(read(b0));
   total = __reduce_add_sync(0xffffffffu, total) * p.bundles;
   const int groups = gridDim.x / p.bundle;
   w.share = max(fast_div(total + groups - 1, p.div_groups), kMinShare);
@@ -346,7 +363,7 @@ __device__ __forceinline__ Walk deal_shares(const Fp8Params& p, int group, int l
   if (from >= total) return w;
   int before = 0;
 #pragma unroll 1
-  for (int b0 = 0; b0 < p.B; b0 += 32) {
+  for (int b0 = 0; b0 < p.seqs; b0 += 32) {
     const Seq q = b0 == 0 ? first : read(b0);
     int upto = cost_of(q) * p.bundles;
 #pragma unroll
@@ -359,7 +376,7 @@ __device__ __forceinline__ Walk deal_shares(const Fp8Params& p, int group, int l
     if (hit != 0u) {
       const int l = __ffs(hit) - 1;
       w.b = b0 + l;
-      w.cur = seq_of(p, __shfl_sync(0xffffffffu, q.sk, l), __shfl_sync(0xffffffffu, q.sq, l));
+      w.cur = seq_of<kBlocks>(p, __shfl_sync(0xffffffffu, q.sk, l), __shfl_sync(0xffffffffu, q.sq, l));
       const int c = cost_of(w.cur), into = from - (__shfl_sync(0xffffffffu, upto, l) - c * p.bundles);
       w.hb = p.bundles > 1 ? into / c : 0;
       w.at = into - w.hb * c;
@@ -380,6 +397,7 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   using namespace fp8d;
   using dec::tmem_ld_cols;
   constexpr int kD = F::kD, kR = F::kR, kN = F::kN, kStages = F::kStages, kStrands = F::kStrands, kKeys = F::kKeys;
+  constexpr bool kBlocks = F::kBlocks;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gbase = smem_raw + (base - smem_u32(smem_raw));
@@ -387,7 +405,8 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gbase + F::kOffMisc);
   volatile uint32_t* s_abort = reinterpret_cast<volatile uint32_t*>(gbase + F::kOffMisc + 4);
   WaitCtx& wc = *reinterpret_cast<WaitCtx*>(gbase + F::kOffMisc + 16);
-  Walk& s_walk = *reinterpret_cast<Walk*>(gbase + F::kOffDeal);
+  Walk<kBlocks>& s_walk = *reinterpret_cast<Walk<kBlocks>*>(gbase + F::kOffDeal);
+  static_assert(sizeof(Walk<kBlocks>) <= 64, "the start of a walk in shared memory");
   const int tid = threadIdx.x, warp = warp_index(), lane = tid & 31;
   constexpr int kLoadK = 4 * kStrands, kLoadV = kLoadK + 1, kIssueS = kLoadK + 2, kIssueO = kLoadK + 3;
 
@@ -423,19 +442,29 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   // CTA = group * bundle + head in the bundle; with a split count of the caller's, a group is one split of one unit
   const int group = blockIdx.x / p.bundle, in_bundle = blockIdx.x - group * p.bundle;
   if (warp == 0) {
-    Walk w = {};
-    if (p.num_splits > 0) {
+    Walk<kBlocks> w = {};
+    if (kBlocks && p.num_splits < 0) {
+      // whole units, as many a CTA
+      const int64_t units = (int64_t)p.seqs * p.bundles;
+      const int from = (int)(group * units / gridDim.x);
+      w.units = (int)((group + 1) * units / gridDim.x) - from;
+      w.b = from / p.bundles;
+      w.hb = from - w.b * p.bundles;
+      const SeqLens len = unit_lens<kBlocks>(p, w.units > 0 ? w.b : 0);
+      w.cur = seq_of<kBlocks>(p, len.sk, len.sq);
+      w.left = w.units > 0 ? 0x40000000 : 0;
+    } else if (p.num_splits > 0) {
       const int unit = group / p.num_splits, split = group - unit * p.num_splits;
       w.b = unit / p.bundles;
       w.hb = unit - w.b * p.bundles;
-      const SeqLens len = lens_of(p, w.b);
-      w.cur = seq_of(p, len.sk, len.sq);
+      const SeqLens len = unit_lens<kBlocks>(p, w.b);
+      w.cur = seq_of<kBlocks>(p, len.sk, len.sq);
       const int places = cost_of(w.cur);
       w.share = p.num_splits == 1 ? places : (places + p.num_splits - 1) / p.num_splits;
       w.at = split * w.share;
       w.left = max(0, min(w.share, places - w.at));
     } else {
-      w = deal_shares(p, group, lane);
+      w = deal_shares<kBlocks>(p, group, lane);
     }
     if (lane == 0) s_walk = w;
   }
@@ -444,13 +473,13 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   pdl_trigger();
   const uint32_t tmem = *tmem_slot;
   bool ok = true;
-  Walk walk = s_walk;
+  Walk<kBlocks> walk = s_walk;
   walk.fetch(p);
 
   if (warp == kLoadK || warp == kLoadV) {
     // ============================================ loaders ======================================
     const bool is_k = warp == kLoadK;
-    Feeder<kD, kStages, F::kScales> feed;
+    Feeder<kD, kStages, F::kScales, false, kBlocks> feed;
     feed.tm = is_k ? &tm_k : &tm_v;
     feed.full0 = bar(is_k ? F::kKFull : F::kVFull);
     feed.free0 = bar(is_k ? F::kKFree : F::kVFree);
@@ -460,8 +489,14 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     feed.scales = is_k ? reinterpret_cast<float*>(gbase + F::kOffSc) : nullptr;
     feed.box = reinterpret_cast<int2*>(gbase + F::kOffBox) + (is_k ? 0 : 32);
     feed.site = is_k ? FeederSites{kKFreeS, kKFullS} : FeederSites{kVFreeS, kVFullS};
-    for (; ok && walk.more(); walk.next(p))
-      ok = feed.piece(p, wc, walk.tiles(), walk.cur.first + walk.at, walk.b, walk.hb * p.bundle + in_bundle, walk.cur.lo, walk.cur.hi);
+    for (; ok && walk.more(); walk.next(p)) {
+      if constexpr (kBlocks) {
+        const BlockList list = list_of(p, walk.b, walk.hb);
+        ok = feed.piece(p, wc, walk.tiles(), walk.at, query_block_of<true>(p, walk.b).b, walk.hb, 0, keys_in_front(p, list, walk.cur.sk + walk.cur.sq), list.at);
+      } else {
+        ok = feed.piece(p, wc, walk.tiles(), walk.cur.first + walk.at, walk.b, walk.hb * p.bundle + in_bundle, walk.cur.lo, walk.cur.hi);
+      }
+    }
     feed.drain();
   } else if (warp == kIssueS) {
     // ============================================ Q . K^T ======================================
@@ -552,7 +587,9 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       if (again) all_strands();                                        // (the sums of the last piece are read: Q may be written)
       again = true;
       const Seq seq = walk.cur;
-      const int n = walk.tiles(), t0 = seq.first + walk.at, b = walk.b, hk = walk.hb * p.bundle + in_bundle, R = seq.sq * p.group;
+      const int n = walk.tiles(), t0 = seq.first + walk.at, hk = walk.hb * p.bundle + in_bundle, R = seq.sq * p.group;
+      const QueryBlock place = query_block_of<kBlocks>(p, walk.b);
+      const int b = place.b, q0 = place.q0;          // sequence, and row of the call that the unit's first one is
       // ---- Q: a row's pieces of eight elements by neighbouring lanes, to all copies of the row
       if (n > 0) {
         constexpr int kPieces = kD / 8;
@@ -561,7 +598,7 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           uint4 u = make_uint4(0u, 0u, 0u, 0u);
           if (r < R) {
             const int s = fast_div(r, p.div_group), h = hk * p.group + r - s * p.group;
-            u = *reinterpret_cast<const uint4*>(p.q + b * p.q_b + s * p.q_s + h * p.q_h + 8 * ch);
+            u = *reinterpret_cast<const uint4*>(p.q + b * p.q_b + (q0 + s) * p.q_s + h * p.q_h + 8 * ch);
           }
           float x[8];
           unpack8(u, x);
@@ -602,14 +639,26 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         if (ok) ok = mbar_wait(bar(F::kQReady), piece++ & 1, wc, kQReadyS);
         ok = __all_sync(0xffffffffu, ok);
       }
-      int lo = 0, hi = 0;
-      if (my < R) {
-        const int2 see = seen_by(p, seq.sk, seq.sq, fast_div(my, p.div_group));
-        lo = see.x;
-        hi = see.y;
+      int lo = 0, hi = 0, lo_in = 0, hi_in = 0;      // seen by the thread's row; by all rows
+      if constexpr (kBlocks) {
+        if (n > 0) {
+          const BlockList list = list_of(p, walk.b, hk);
+          const int mine = fast_div(my, p.div_group);
+          for (int s = 0; s < seq.sq; ++s) {
+            const int keys = keys_in_front(p, list, seq.sk + s + 1);
+            if (s == 0) hi_in = keys;
+            if (s == mine) hi = keys;
+          }
+        }
+      } else {
+        if (my < R) {
+          const int2 see = seen_by(p, seq.sk, seq.sq, fast_div(my, p.div_group));
+          lo = see.x;
+          hi = see.y;
+        }
+        lo_in = seq.sq > 0 ? seen_by(p, seq.sk, seq.sq, seq.sq - 1).x : 0;
+        hi_in = seen_by(p, seq.sk, seq.sq, 0).y;
       }
-      // the keys that all rows see
-      const int lo_in = seq.sq > 0 ? seen_by(p, seq.sk, seq.sq, seq.sq - 1).x : 0, hi_in = seen_by(p, seq.sk, seq.sq, 0).y;
       const float factor = s_row[my];
       float m_run = -INFINITY, v_run = -INFINITY, l = 0.f, acc[kR];    // largest score, and with its value scale
 #pragma unroll
@@ -760,12 +809,15 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       }
       all_strands();
       // where the result goes: the output if the whole unit was this piece, else a slot of partial results
-      const int places = cost_of(seq), unit = b * p.Hkv + hk;
+      const int places = cost_of(seq), unit = walk.b * p.Hkv + hk;
       bool direct;
       int64_t slot;
       if (p.num_splits > 0) {
         direct = p.num_splits == 1;
         slot = (int64_t)unit * p.num_splits + group % p.num_splits;
+      } else if (kBlocks && p.num_splits < 0) {
+        direct = true;
+        slot = 0;
       } else {
         direct = walk.places() == places;
         slot = 2 * (int64_t)blockIdx.x + (walk.at == 0 ? 1 : 0);
@@ -805,9 +857,9 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           const RowEnd e = finish_row(m, sum, p.sink, h);
           const float f = e.factor * by;
           if (col < kD)
-            *reinterpret_cast<uint2*>(p.out + b * p.o_b + s * p.o_s + h * p.o_h + col) =
+            *reinterpret_cast<uint2*>(p.out + b * p.o_b + (q0 + s) * p.o_s + h * p.o_h + col) =
                 make_uint2(pack_bf16x2(o.x * f * by, o.y * f * by), pack_bf16x2(o.z * f * by, o.w * f * by));
-          if (lane == 0 && p.lse != nullptr) p.lse[((int64_t)b * p.Hq + h) * p.Sq + s] = e.lse;
+          if (lane == 0 && p.lse != nullptr) p.lse[((int64_t)b * p.Hq + h) * p.Sq + q0 + s] = e.lse;
         } else {
           const bool none = m == -INFINITY && sum == 0.f;
           const float f = rcp_approx(sum) * by;
@@ -827,13 +879,20 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 }
 
 // The units that several CTAs had a piece of: a warp a row.
+template <bool kBlocks>
 __global__ void __launch_bounds__(kFp8CombineWarps * 32) fp8_merge_kernel(const __grid_constant__ Fp8Params p) {
   const int lane = threadIdx.x & 31;
   const uint32_t r = blockIdx.x * kFp8CombineWarps + (threadIdx.x >> 5), rows = (uint32_t)p.B * p.Sq * p.Hq;
   pdl_wait();
   if (r >= rows) return;
   const int bs = fast_div((int)r, p.div_hq), h = (int)r - bs * p.Hq, b = fast_div(bs, p.div_sq), s = bs - b * p.Sq;
-  const int hk = fast_div(h, p.div_group), row = s * p.group + h - hk * p.group, unit = b * p.Hkv + hk;
+  int v = b, in = s;                          // the unit's sequence, and row in it
+  if constexpr (kBlocks) {
+    const int qb = fast_div(s, p.div_query_block);
+    v = b * p.query_blocks + qb;
+    in = s - qb * p.query_block;
+  }
+  const int hk = fast_div(h, p.div_group), row = in * p.group + h - hk * p.group, unit = v * p.Hkv + hk;
   // (asked for together; a sequence without rows has no pieces noted)
   const int rows_here = p.fresh != nullptr ? p.fresh[b] : p.Sq;
   const int2 at = p.num_splits == 0 ? p.pieces[unit] : make_int2(0, 0);
@@ -844,8 +903,8 @@ __global__ void __launch_bounds__(kFp8CombineWarps * 32) fp8_merge_kernel(const 
     // (the splits that have a part of the unit)
     first = (int64_t)unit * pieces;
     step = 1;
-    const SeqLens len = lens_of(p, b);
-    const int places = fp8d::cost_of(fp8d::seq_of(p, len.sk, len.sq)), per = (places + pieces - 1) / pieces;
+    const SeqLens len = unit_lens<kBlocks>(p, v);
+    const int places = fp8d::cost_of(fp8d::seq_of<kBlocks>(p, len.sk, len.sq)), per = (places + pieces - 1) / pieces;
     pieces = (places + per - 1) / per;
   } else {
     pieces = at.y;

@@ -154,7 +154,8 @@ __device__ __forceinline__ void cap_scores(float (&x)[64], float cap) {
 
 }  // namespace fp8p
 
-template <int kD, bool kCap>
+// kBlocks: over the blocks that the row tile's query block has chosen.
+template <int kD, bool kCap, bool kBlocks = false>
 __global__ void __launch_bounds__(fp8p::kThreads, 1)
 fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                    const __grid_constant__ Fp8Params p) {
@@ -176,13 +177,23 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   w /= p.num_splits;
   const int hk = w % p.Hkv;
   w /= p.Hkv;
-  const int b = w % p.B, r_first = (p.row_tiles - 1 - w / p.B) * p.cta_rows;
+  const int v = w % p.seqs, r_first = (p.row_tiles - 1 - w / p.seqs) * p.cta_rows;
+  const QueryBlock place = query_block_of<kBlocks>(p, v);
+  const int b = place.b, q0 = place.q0;                 // sequence, and row of the call that the unit's first one is
   pdl_wait();
-  const SeqLens len = lens_of(p, b);
+  const SeqLens len = unit_lens<kBlocks>(p, v);
   const int R = min(p.cta_rows, len.sq * p.group - r_first);
   if (R <= 0) return;
-  const int lo_all = seen_by(p, len.sk, len.sq, fast_div(r_first, p.div_group)).x,
-            hi_all = seen_by(p, len.sk, len.sq, fast_div(r_first + R - 1, p.div_group)).y;
+  const int s_first = fast_div(r_first, p.div_group), s_last = fast_div(r_first + R - 1, p.div_group);
+  int lo_all = 0, hi_all;
+  BlockList list = {nullptr, 0};
+  if constexpr (kBlocks) {
+    list = list_of(p, v, hk);
+    hi_all = keys_in_front(p, list, len.sk + s_last + 1);
+  } else {
+    lo_all = seen_by(p, len.sk, len.sq, s_first).x;
+    hi_all = seen_by(p, len.sk, len.sq, s_last).y;
+  }
   const int t_first = lo_all >> 7, t_total = hi_all > lo_all ? ((hi_all + 127) >> 7) - t_first : 0;
   const int per = (t_total + p.num_splits - 1) / p.num_splits;
   const int t0 = t_first + min(split * per, t_total), n = min(t_first + t_total - t0, per);
@@ -233,7 +244,7 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
 #pragma unroll 4
     for (int i = tid; i < p.cta_rows * kPieces; i += 384) {
       const int r = i / kPieces, ch = i % kPieces, s = fast_div(r_first + r, p.div_group), h = hk * p.group + r_first + r - s * p.group;
-      const __nv_bfloat16* src = r < R ? p.q + b * p.q_b + (int64_t)s * p.q_s + h * p.q_h + 8 * ch : p.q;
+      const __nv_bfloat16* src = r < R ? p.q + b * p.q_b + (int64_t)(q0 + s) * p.q_s + h * p.q_h + 8 * ch : p.q;
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(base + L::kOffV + 16 * i), "l"(src), "r"(r < R ? 16 : 0) : "memory");
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
@@ -273,7 +284,7 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   if (warp >= 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsService));
     if (warp == 12) {
-      fp8d::Feeder<kD, L::kStagesK, L::kScales, true> feed;
+      fp8d::Feeder<kD, L::kStagesK, L::kScales, true, kBlocks> feed;
       feed.tm = &tm_k;
       feed.full0 = bar(L::kKFull);
       feed.free0 = bar(L::kKFree);
@@ -283,10 +294,10 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       feed.scales = reinterpret_cast<float*>(gbase + L::kOffSc);
       feed.box = reinterpret_cast<int2*>(gbase + L::kOffBox);
       feed.site = {kKFreeS, kKFullS};
-      feed.piece(p, wc, n, t0, b, hk, lo_all, hi_all);
+      feed.piece(p, wc, n, t0, b, hk, lo_all, hi_all, list.at);
       feed.drain();
     } else if (warp == 14) {
-      fp8d::Feeder<kD, L::kStagesV, L::kScales> feed;
+      fp8d::Feeder<kD, L::kStagesV, L::kScales, false, kBlocks> feed;
       feed.tm = &tm_v;
       feed.full0 = bar(L::kRawFull);
       feed.free0 = bar(L::kRawFree);
@@ -296,7 +307,7 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       feed.scales = nullptr;
       feed.box = reinterpret_cast<int2*>(gbase + L::kOffBox) + 32;
       feed.site = {kRawFreeS, kRawFullS};
-      feed.piece(p, wc, n, t0, b, hk, lo_all, hi_all);
+      feed.piece(p, wc, n, t0, b, hk, lo_all, hi_all, list.at);
       feed.drain();
     } else if (warp == 13) {
       // ============================================ products =====================================
@@ -415,7 +426,15 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     const int s = fast_div(r_first + row, p.div_group), h = hk * p.group + r_first + row - s * p.group;
     const float factor = reinterpret_cast<const float*>(gbase + L::kOffRow)[row];
     int lo = 0, hi = 0;
-    if (row < R) {
+    if constexpr (kBlocks) {
+      // (the tokens of the warp's rows, one after the other)
+      const int s0 = fast_div(r_first + (row & ~31), p.div_group), s1 = min(fast_div(r_first + (row | 31), p.div_group), s_last);
+#pragma unroll 1
+      for (int at = s0; at <= s1; ++at) {
+        const int keys = keys_in_front(p, list, len.sk + at + 1);
+        if (at == s && row < R) hi = keys;
+      }
+    } else if (row < R) {
       const int2 see = seen_by(p, len.sk, len.sq, s);
       lo = see.x;
       hi = see.y;
@@ -562,7 +581,7 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         tc_fence_after_sync();
       }
       const float l = (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
-      const int64_t l_idx = ((int64_t)b * p.Hq + h) * p.Sq + s;
+      const int64_t l_idx = ((int64_t)b * p.Hq + h) * p.Sq + q0 + s;
       const bool none = m_ref == -INFINITY && l == 0.f;
       const RowEnd end = finish_row(m_ref, l, p.sink, h);
       const bool direct = p.num_splits == 1;
@@ -571,7 +590,7 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       const float down = m_ref == -INFINITY ? 0.f : ex2_approx(0.5f * (v_ref - m_ref - 6.f)), scale = (direct ? end.factor : rcp_approx(l)) * down;
       if (ok && row < R) {
         if (direct && p.lse != nullptr) p.lse[l_idx] = end.lse;
-        if (!direct) p.lse_partial[part + ((int64_t)b * p.Sq + s) * p.Hq + h] = none ? -INFINITY : m_ref + lg2_approx(l);
+        if (!direct) p.lse_partial[part + ((int64_t)b * p.Sq + q0 + s) * p.Hq + h] = none ? -INFINITY : m_ref + lg2_approx(l);
       }
       // Output rows go through the memory of the tile's Q (a warp's own 32 rows; every product is done), to be written by lanes side by side.
       uint8_t* stage = gbase + L::kOffQ + 2 * tile * L::kTile8 + (t & ~31) * (2 * kD);
@@ -595,7 +614,7 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
                 make_uint4(pack_bf16x2(o[8 * j], o[8 * j + 1]), pack_bf16x2(o[8 * j + 2], o[8 * j + 3]), pack_bf16x2(o[8 * j + 4], o[8 * j + 5]),
                            pack_bf16x2(o[8 * j + 6], o[8 * j + 7]));
         } else if (ok && row < R && !none) {
-          float4* dst = reinterpret_cast<float4*>(p.o_partial + (part + ((int64_t)b * p.Sq + s) * p.Hq + h) * kD + 32 * c);
+          float4* dst = reinterpret_cast<float4*>(p.o_partial + (part + ((int64_t)b * p.Sq + q0 + s) * p.Hq + h) * kD + 32 * c);
 #pragma unroll
           for (int j = 0; j < 8; ++j) dst[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
         }
@@ -607,7 +626,7 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
           const int rr = i * (32 / kChunks) + lane / kChunks, c = lane % kChunks, at = r_first + (row & ~31) + rr;
           const int ss = fast_div(at, p.div_group), hh = hk * p.group + at - ss * p.group;
           if ((row & ~31) + rr < R)
-            *reinterpret_cast<uint4*>(p.out + b * p.o_b + (int64_t)ss * p.o_s + hh * p.o_h + 8 * c) =
+            *reinterpret_cast<uint4*>(p.out + b * p.o_b + (int64_t)(q0 + ss) * p.o_s + hh * p.o_h + 8 * c) =
                 *reinterpret_cast<const uint4*>(stage + rr * (2 * kD) + ((c ^ (rr & 7)) << 4));
         }
       }

@@ -1063,10 +1063,35 @@ Fp8Cache cache_of(PyObject* const* a) {
   return f;
 }
 
-// k_cache v_cache k_scale v_scale page_table k v cache_seqlens seqused_new rotary_cos rotary_sin rotary_interleaved q
+// The index of a cache that has been described.
+fa4_fp8_index index_of(const Fp8Cache& f, const at::Tensor& bounds, const at::Tensor& scale) {
+  FA4_ASSERT(bounds.defined() && scale.defined(), "the cache has no index: key_bounds and bound_scale (FP8KVCache.empty(..., indexed=True))");
+  const fa4_fp8_cache& c = f.c;
+  const int64_t per = c.page_size / c.block;
+  validate(bounds, "key_bounds", {c.num_pages, per, c.Hkv, 2, c.D}, at::kChar, f.k.device());
+  validate(scale, "bound_scale", {c.num_pages, per, c.Hkv}, at::kFloat, f.k.device());
+  FA4_ASSERT(bounds.is_contiguous() && scale.is_contiguous() && (reinterpret_cast<uintptr_t>(bounds.data_ptr()) & 15u) == 0,
+             "the index of the cache must be contiguous, key_bounds 16-byte aligned");
+  fa4_fp8_index x = {};
+  x.struct_size = sizeof x;
+  x.bounds = bounds.data_ptr();
+  x.scale = scale.data_ptr<float>();
+  return x;
+}
+void run_index(const Fp8Cache& f, const fa4_fp8_index& x, const at::Tensor& held, const at::Tensor& fresh, int64_t B, int64_t S, uint32_t* status, void* stream) {
+  fa4_fp8_index_call a = {};
+  a.struct_size = sizeof a;
+  a.B = (int32_t)B; a.S = (int32_t)S;
+  a.seqlens = held.data_ptr<int32_t>();
+  a.seqused_new = fresh.defined() ? fresh.data_ptr<int32_t>() : nullptr;
+  a.status = status;
+  check_rc(fa4_fp8_cache_index(&f.c, &x, &a, stream), "fa4_fp8_cache_index");
+}
+
+// k_cache v_cache k_scale v_scale page_table k v cache_seqlens seqused_new rotary_cos rotary_sin rotary_interleaved q key_bounds bound_scale
 struct AppendCall {
   Fp8Cache f;
-  at::Tensor k, v, held, fresh, cos, sin, q, q_out;
+  at::Tensor k, v, held, fresh, cos, sin, q, q_out, bounds, bound_scale;
   bool interleaved = false;
   uint32_t* status = nullptr;
 };
@@ -1081,6 +1106,8 @@ void run_append(AppendCall& c) {
   validate(c.k, "k", {B, S, c.f.c.Hkv, c.f.c.D}, at::kBFloat16, device);
   validate(c.v, "v", {B, S, H, D}, at::kBFloat16, device);
   const at::Tensor held = counts_of(c.held, "cache_seqlens", B, device), fresh = counts_of(c.fresh, "seqused_new", B, device);
+  fa4_fp8_index index = {};
+  if (c.bounds.defined() || c.bound_scale.defined()) index = index_of(c.f, c.bounds, c.bound_scale);
   FA4_ASSERT(c.cos.defined() == c.sin.defined(), "rotary_cos and rotary_sin come together");
   FA4_ASSERT(!c.q.defined() || c.cos.defined(), "q is for the rotation: pass rotary_cos and rotary_sin too");
   at::Tensor cos = c.cos, sin = c.sin;
@@ -1126,6 +1153,7 @@ void run_append(AppendCall& c) {
   a.interleaved = c.interleaved;
   a.status = c.status;
   check_rc(fa4_fp8_cache_append(&c.f.c, &a, stream), "fa4_fp8_cache_append");
+  if (c.bounds.defined()) run_index(c.f, index, held, fresh, B, S, c.status, stream);
 }
 
 PyObject* append_fp8(PyObject* const* a) {
@@ -1139,6 +1167,8 @@ PyObject* append_fp8(PyObject* const* a) {
   c.sin = optional_tensor(a[10], "rotary_sin");
   c.interleaved = truth_of(a[11]);
   c.q = optional_tensor(a[12], "q");
+  c.bounds = optional_tensor(a[13], "key_bounds");
+  c.bound_scale = optional_tensor(a[14], "bound_scale");
   if (c.f.k.is_cuda()) c.status = status_word(c.f.k.device());
   {
     NoGil nogil;
@@ -1149,10 +1179,11 @@ PyObject* append_fp8(PyObject* const* a) {
 }
 
 // k_cache v_cache k_scale v_scale page_table q seqused_k seqused_q softmax_scale causal window_left window_right
-// learnable_sink softcap num_splits return_lse out lse
+// learnable_sink softcap num_splits return_lse out lse blocks query_block
 struct Fp8Call {
   Fp8Cache f;
-  at::Tensor q, used, fresh, sink, out, lse;
+  at::Tensor q, used, fresh, sink, out, lse, blocks;
+  long query_block = 0;
   bool default_softmax_scale = true, want_lse = false;
   double softmax_scale = 0.0, softcap = 0.0;
   long num_splits = 0;
@@ -1170,6 +1201,14 @@ void run_fp8(Fp8Call& c) {
   validate(c.q, "q", {B, Sq, Hq, D}, at::kBFloat16, device);
   FA4_ASSERT(Hq > 0 && Hq % Hkv == 0, "num_head must be divisible by num_head_kv");
   const at::Tensor used = counts_of(c.used, "seqused_k", B, device), fresh = counts_of(c.fresh, "seqused_q", B, device);
+  at::Tensor blocks;
+  if (c.blocks.defined()) {
+    if (c.query_block < 1 || c.query_block > 0x7fffffff) fail(PyExc_ValueError, "query_block must be positive");
+    FA4_ASSERT(c.blocks.dim() == 4 && c.blocks.size(3) > 0, "blocks must be (B, query blocks, heads_kv, num_blocks), got %s", dims_of(c.blocks.sizes()).c_str());
+    validate(c.blocks, "blocks", {B, cdiv(Sq, c.query_block), Hkv, c.blocks.size(3)}, at::kInt, device);
+    FA4_ASSERT(c.blocks.size(3) <= 0x7fffffff, "blocks too large");
+    blocks = c.blocks.contiguous();
+  }
   if (c.num_splits < 0 || c.num_splits > 128) fail(PyExc_ValueError, "num_splits must be in 0..128");
   if (!(c.softcap >= 0.0) || !std::isfinite(c.softcap)) fail(PyExc_ValueError, "softcap must be a finite number >= 0");
   const double softmax_scale = c.default_softmax_scale ? 1.0 / std::sqrt((double)D) : c.softmax_scale;
@@ -1218,15 +1257,23 @@ void run_fp8(Fp8Call& c) {
   p.window_left = c.win.left; p.window_right = c.win.right;
   p.num_splits = (int32_t)c.num_splits;
   p.status = c.status;
-  const int64_t bytes = fa4_fp8_cache_fwd_workspace_bytes(&c.f.c, &p);
-  if (bytes < 0) check_rc((int)bytes, "fa4_fp8_cache_fwd_workspace_bytes");
+  fa4_fp8_blocks x = {};
+  if (blocks.defined()) {
+    x.struct_size = sizeof x;
+    x.num_blocks = (int32_t)blocks.size(3);
+    x.query_block = (int32_t)c.query_block;
+    x.blocks = blocks.data_ptr<int32_t>();
+  }
+  const int64_t bytes = blocks.defined() ? fa4_fp8_cache_fwd_blocks_workspace_bytes(&c.f.c, &p, &x) : fa4_fp8_cache_fwd_workspace_bytes(&c.f.c, &p);
+  if (bytes < 0) check_rc((int)bytes, blocks.defined() ? "fa4_fp8_cache_fwd_blocks_workspace_bytes" : "fa4_fp8_cache_fwd_workspace_bytes");
   c10::DataPtr workspace;
   if (bytes > 0) {
     workspace = scratch_bytes(bytes);
     p.workspace = workspace.get();
     p.workspace_bytes = (uint64_t)bytes;
   }
-  check_rc(fa4_fp8_cache_fwd(&c.f.c, &p, stream), "fa4_fp8_cache_fwd");
+  if (blocks.defined()) check_rc(fa4_fp8_cache_fwd_blocks(&c.f.c, &p, &x, stream), "fa4_fp8_cache_fwd_blocks");
+  else check_rc(fa4_fp8_cache_fwd(&c.f.c, &p, stream), "fa4_fp8_cache_fwd");
 }
 
 PyObject* fwd_fp8(PyObject* const* a) {
@@ -1244,12 +1291,100 @@ PyObject* fwd_fp8(PyObject* const* a) {
   c.want_lse = truth_of(a[15]);
   c.out = optional_tensor(a[16], "out");
   c.lse = optional_tensor(a[17], "lse");
+  c.blocks = optional_tensor(a[18], "blocks");
+  if (c.blocks.defined()) c.query_block = integer_of(a[19]);
   if (c.f.k.is_cuda()) c.status = status_word(c.f.k.device());
   {
     NoGil nogil;
     run_fp8(c);
   }
   return pair_of(a[16], c.out, a[17], c.lse);
+}
+
+// k_cache v_cache k_scale v_scale page_table key_bounds bound_scale cache_seqlens num_tokens seqused_new
+PyObject* index_fp8(PyObject* const* a) {
+  Fp8Cache f = cache_of(a);
+  const at::Tensor bounds = optional_tensor(a[5], "key_bounds"), scale = optional_tensor(a[6], "bound_scale");
+  const at::Tensor held_in = tensor_of(a[7], "cache_seqlens"), fresh_in = optional_tensor(a[9], "seqused_new");
+  const long S = integer_of(a[8]);
+  uint32_t* status = f.k.is_cuda() ? status_word(f.k.device()) : nullptr;
+  {
+    NoGil nogil;
+    FA4_ASSERT(held_in.dim() == 1, "cache_seqlens must be (B,)");
+    const int64_t B = held_in.size(0);
+    FA4_ASSERT(B <= 0x7fffffff, "cache_seqlens too large");
+    if (S < 0 || S > 0x7fffffff) fail(PyExc_ValueError, "num_tokens must be in 0..2^31 - 1");
+    describe_cache(f, B);
+    const at::Device device = f.k.device();
+    const at::Tensor held = counts_of(held_in, "cache_seqlens", B, device), fresh = counts_of(fresh_in, "seqused_new", B, device);
+    const fa4_fp8_index x = index_of(f, bounds, scale);
+    c10::cuda::OptionalCUDAGuard guard;
+    if (device.index() != c10::cuda::current_device()) guard.set_device(device);
+    if (B > 0 && S > 0) run_index(f, x, held, fresh, B, S, status, c10::cuda::getCurrentCUDAStream(device.index()).stream());
+  }
+  Py_RETURN_NONE;
+}
+
+// k_cache v_cache k_scale v_scale page_table key_bounds bound_scale q seqused_k seqused_q num_blocks query_block front_blocks recent_blocks out
+PyObject* select_fp8(PyObject* const* a) {
+  Fp8Cache f = cache_of(a);
+  const at::Tensor bounds = optional_tensor(a[5], "key_bounds"), scale = optional_tensor(a[6], "bound_scale");
+  const at::Tensor q_in = tensor_of(a[7], "q"), used_in = tensor_of(a[8], "seqused_k"), fresh_in = optional_tensor(a[9], "seqused_q");
+  const long chosen = integer_of(a[10]), rows = integer_of(a[11]), front = integer_of(a[12]), recent = integer_of(a[13]);
+  at::Tensor out = optional_tensor(a[14], "out");
+  uint32_t* status = f.k.is_cuda() ? status_word(f.k.device()) : nullptr;
+  {
+    NoGil nogil;
+    FA4_ASSERT(q_in.dim() == 4, "q must be (B, Sq, heads, head_dim), got %s", dims_of(q_in.sizes()).c_str());
+    const int64_t B = q_in.size(0), Sq = q_in.size(1), Hq = q_in.size(2);
+    FA4_ASSERT(B <= 0x7fffffff && Sq <= 0x7fffffff && Hq <= 0x7fffffff, "q too large");
+    describe_cache(f, B);
+    const at::Device device = f.k.device();
+    const int64_t Hkv = f.c.Hkv;
+    validate(q_in, "q", {B, Sq, Hq, f.c.D}, at::kBFloat16, device);
+    FA4_ASSERT(Hq > 0 && Hq % Hkv == 0, "num_head must be divisible by num_head_kv");
+    const at::Tensor used = counts_of(used_in, "seqused_k", B, device), fresh = counts_of(fresh_in, "seqused_q", B, device);
+    const fa4_fp8_index x = index_of(f, bounds, scale);
+    constexpr long kMost = 0x7fffffff;
+    if (chosen < 1 || rows < 1 || front < 0 || recent < 1 || chosen > kMost || rows > kMost || front > kMost || recent > kMost)
+      fail(PyExc_ValueError, "num_blocks, query_block and recent_blocks must be positive, front_blocks not negative");
+    const int64_t always = front + recent + cdiv(std::min<int64_t>(rows, std::max<int64_t>(Sq, 1)) - 1, f.c.block);
+    if (always > chosen)
+      fail(PyExc_ValueError, "num_blocks %ld has no room for the %lld blocks that are always chosen (front_blocks, recent_blocks, those of the query block)", chosen, (long long)always);
+    if (cdiv((int64_t)f.c.pages_per_seq * f.c.page_size, f.c.block) > 53248)
+      fail(PyExc_NotImplementedError, "more than 53248 blocks a sequence are not built");
+    if (std::min<int64_t>(rows, Sq) * (Hq / Hkv) > 32768)
+      fail(PyExc_NotImplementedError, "more than 32768 rows and heads of a kv head that choose together are not built");
+    c10::cuda::OptionalCUDAGuard guard;
+    if (device.index() != c10::cuda::current_device()) guard.set_device(device);
+    void* stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
+    const int64_t query_blocks = cdiv(Sq, rows);
+    if (!out.defined()) {
+      out = new_tensor({B, query_blocks, Hkv, chosen}, at::kInt, device);
+    } else {
+      validate(out, "out", {B, query_blocks, Hkv, chosen}, at::kInt, device);
+      FA4_ASSERT(out.is_contiguous(), "out must be contiguous");
+    }
+    if (B > 0 && Sq > 0) {
+      const at::Tensor q = in_pieces(q_in);
+      fa4_fp8_select s = {};
+      s.struct_size = sizeof s;
+      s.B = (int32_t)B; s.Sq = (int32_t)Sq; s.Hq = (int32_t)Hq;
+      s.q = q.data_ptr();
+      s.q_stride_b = q.stride(0); s.q_stride_s = q.stride(1); s.q_stride_h = q.stride(2);
+      s.seqused_k = used.data_ptr<int32_t>();
+      s.seqused_q = fresh.defined() ? fresh.data_ptr<int32_t>() : nullptr;
+      s.num_blocks = (int32_t)chosen; s.query_block = (int32_t)rows; s.front_blocks = (int32_t)front; s.recent_blocks = (int32_t)recent;
+      s.blocks = out.data_ptr<int32_t>();
+      s.status = status;
+      check_rc(fa4_fp8_cache_select(&f.c, &x, &s, stream), "fa4_fp8_cache_select");
+    }
+  }
+  if (!is_none(a[14])) {
+    Py_INCREF(a[14]);
+    return a[14];
+  }
+  return THPVariable_Wrap(out);
 }
 
 // ---- the module -----------------------------------------------------------------------------------
@@ -1314,8 +1449,10 @@ PyMethodDef methods[] = {method<fwd, 23>("fwd"),
                          method<quantize_qkv, 4>("quantize_qkv"),
                          method<host_pieces, 25>("host_pieces"),
                          method<window_of, 3>("resolve_window"),
-                         method<append_fp8, 13>("append_fp8"),
-                         method<fwd_fp8, 18>("fwd_fp8"),
+                         method<append_fp8, 15>("append_fp8"),
+                         method<fwd_fp8, 20>("fwd_fp8"),
+                         method<index_fp8, 10>("index_fp8"),
+                         method<select_fp8, 15>("select_fp8"),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_host", "Native host path of flash_attention_b200.", -1, methods,
                           nullptr, nullptr, nullptr, nullptr};

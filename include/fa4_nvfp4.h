@@ -584,6 +584,75 @@ typedef struct fa4_fp8_fwd {
 int64_t fa4_fp8_cache_fwd_workspace_bytes(const fa4_fp8_cache* cache, const fa4_fp8_fwd* p);
 int fa4_fp8_cache_fwd(const fa4_fp8_cache* cache, const fa4_fp8_fwd* p, void* cuda_stream);
 
+/*
+ * ---- chosen blocks of the 8-bit cache ----------------------------------------------------------------------
+ *
+ * For contexts that are too long to be read whole for every token: an index of the cache, a choice of blocks by it, and
+ * attention over what is chosen.  A block is that of the cache's scales.  No counterpart in the reference, whose attention
+ * over a cache reads all of it.
+ *
+ *   bounds  (num_pages, page_size / block, Hkv, 2, D) int8, contiguous, 16-byte aligned: upper, then lower bounds of the block's keys
+ *   scale   (num_pages, page_size / block, Hkv) fp32, contiguous
+ * Of a block and kv head, over the tokens that are there: u = 2^(e - 6) with e the exponent of the largest |byte value| (e = -9 if all are zero);
+ * upper = ceil(max / u), lower = floor(min / u), scale = k_scale * u.  A block that holds a NaN: bounds 0, scale NaN.
+ */
+typedef struct fa4_fp8_index {
+  uint32_t struct_size;      /* = sizeof(fa4_fp8_index) */
+  uint32_t reserved;         /* 0 */
+  void* bounds;
+  float* scale;
+} fa4_fp8_index;
+/*
+ * The bounds of all blocks that tokens seqlens[b] .. seqlens[b] + seqused_new[b] - 1 (NULL: S; at most S) lie in, made anew from the cache.
+ * Tokens behind those are not looked at.
+ */
+typedef struct fa4_fp8_index_call {
+  uint32_t struct_size;      /* = sizeof(fa4_fp8_index_call) */
+  int32_t B, S;
+  uint32_t reserved;         /* 0 */
+  const int32_t* seqlens;
+  const int32_t* seqused_new;
+  uint32_t* status;
+} fa4_fp8_index_call;
+int fa4_fp8_cache_index(const fa4_fp8_cache* cache, const fa4_fp8_index* index, const fa4_fp8_index_call* a, void* cuda_stream);
+
+/*
+ * The blocks that queries choose: query_block rows one behind the other, and the heads of a kv head, choose together.
+ *   blocks (B, ceil(Sq / query_block), Hkv, num_blocks) int32: numbers of blocks of the sequence (token / block), ascending, -1 behind the last
+ * Row i stands at position seqused_k[b] - seqused_q[b] + i and sees what is in front of it, itself included.  Chosen are always the first front_blocks blocks and, up to
+ * that of the last row, those from recent_blocks - 1 in front of the first row's on; num_blocks has room for them:
+ * front_blocks + recent_blocks + ceil((query_block - 1) / block).  The rest goes by score, ties to the lower number:
+ *   x = rint(|q| 2^(14 - e)), e the exponent of the largest finite |q| of the rows and heads (-100 at least), elements that are not finite 0;
+ *   P, N = sums of x over rows and heads where q > 0, q < 0;  s = bits of the largest sum - 7, or 0;  p, n = min(127, (P, N + 2^s / 2) >> s)
+ *   score = scale * (sum over channels of p upper - n lower), a whole number below 2^24 times an fp32: one rounding.  NaN counts as +inf.
+ * No more than 53248 blocks a sequence (pages_per_seq * page_size / block).
+ */
+typedef struct fa4_fp8_select {
+  uint32_t struct_size;      /* = sizeof(fa4_fp8_select) */
+  int32_t B, Sq, Hq;
+  const void* q;             /* bf16 as in fa4_fp8_fwd */
+  int64_t q_stride_b, q_stride_s, q_stride_h;
+  const int32_t* seqused_k;
+  const int32_t* seqused_q;  /* or NULL */
+  int32_t num_blocks, query_block, front_blocks, recent_blocks;
+  int32_t* blocks;
+  uint32_t* status;
+} fa4_fp8_select;
+int fa4_fp8_cache_select(const fa4_fp8_cache* cache, const fa4_fp8_index* index, const fa4_fp8_select* a, void* cuda_stream);
+
+/*
+ * fa4_fp8_cache_fwd over chosen blocks: rows see the keys of their list that are not behind them.  `p` as there, causal set, no window limits,
+ * num_splits 0.  A list ends at the first entry that is not above the one in front of it; blocks behind a row hold nothing for it.
+ */
+typedef struct fa4_fp8_blocks {
+  uint32_t struct_size;      /* = sizeof(fa4_fp8_blocks) */
+  int32_t num_blocks, query_block;
+  uint32_t reserved;         /* 0 */
+  const int32_t* blocks;     /* (B, ceil(Sq / query_block), Hkv, num_blocks) */
+} fa4_fp8_blocks;
+int64_t fa4_fp8_cache_fwd_blocks_workspace_bytes(const fa4_fp8_cache* cache, const fa4_fp8_fwd* p, const fa4_fp8_blocks* x);
+int fa4_fp8_cache_fwd_blocks(const fa4_fp8_cache* cache, const fa4_fp8_fwd* p, const fa4_fp8_blocks* x, void* cuda_stream);
+
 #ifdef __cplusplus
 }
 #endif
