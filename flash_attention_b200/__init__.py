@@ -10,9 +10,11 @@ from .host_pipeline import HostPipeline, flash_attn_fp4_host
 from .varlen import flash_attn_varlen_fp4_func, quantize_varlen_qkv, padded_key_offsets
 from .fp8_cache import (FP8KVCache, append_kv_fp8, flash_attn_fp8_cache_func, index_kv_fp8, select_kv_blocks,
                         flash_attn_fp8_blocks_func)
+from .kv_pages import KVPages, resize_kv_pages, fork_kv_pages, compact_kv_pages, copy_kv_pages
 from .quant import NVFP4Tensor, quantize_qkv, quantize_qkv_fused, quantize_lastdim, dequantize_lastdim, sf_to_tiled
 
 __all__ = ["flash_attn_func", "flash_attn_fp4_func", "check_status", "HostPipeline", "flash_attn_fp4_host", "flash_attn_varlen_fp4_func", "quantize_varlen_qkv", "padded_key_offsets", "measure_fp4_mma_rate", "measure_ex2_rate", "NVFP4Tensor", "quantize_qkv", "quantize_qkv_fused",
            "quantize_lastdim", "dequantize_lastdim", "sf_to_tiled", "FP8KVCache", "append_kv_fp8", "flash_attn_fp8_cache_func", "index_kv_fp8",
-           "select_kv_blocks", "flash_attn_fp8_blocks_func", "build", "lib", "LIB_PATH",
+           "select_kv_blocks", "flash_attn_fp8_blocks_func", "KVPages", "resize_kv_pages", "fork_kv_pages", "compact_kv_pages",
+           "copy_kv_pages", "build", "lib", "LIB_PATH",
            "VARIANT_AUTO", "VARIANT_WS", "VARIANT_WS64", "VARIANT_DECODE"]

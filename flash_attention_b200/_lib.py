@@ -28,7 +28,7 @@ CSRC = os.path.join(_HERE, "csrc")
 HOST_PATH = os.path.join(_HERE, "_host.so")
 HOST_ABI_PATH = HOST_PATH + ".abi"
 LOCK_PATH = os.path.join(_HERE, ".build.lock")
-SOURCES = ["api.cu", "fp8_cache.cu", "fp8_blocks.cu"]
+SOURCES = ["api.cu", "fp8_cache.cu", "fp8_blocks.cu", "kv_pages.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "--threads", "4",
               "--shared", "-Xcompiler", "-fPIC", "-Xlinker", "-soname=libfa4_nvfp4.so"]
@@ -297,6 +297,9 @@ EXPORTS = ["fa4_nvfp4_fwd", "fa4_nvfp4_sf_linear_to_tiled", "fa4_nvfp4_query",
 # (the 8-bit KV cache: called by the host extension alone)
 EXPORTS_FP8 = ["fa4_fp8_cache_append", "fa4_fp8_cache_fwd", "fa4_fp8_cache_fwd_workspace_bytes", "fa4_fp8_cache_index",
                "fa4_fp8_cache_select", "fa4_fp8_cache_fwd_blocks", "fa4_fp8_cache_fwd_blocks_workspace_bytes"]
+# (pages of a KV cache: likewise)
+EXPORTS_PAGES = ["fa4_kv_pages_resize", "fa4_kv_pages_resize_workspace_bytes", "fa4_kv_pages_fork", "fa4_kv_pages_compact",
+                 "fa4_kv_pages_compact_workspace_bytes", "fa4_kv_pages_copy"]
 
 
 def check(rc: int, what: str) -> None:

@@ -1387,6 +1387,211 @@ PyObject* select_fp8(PyObject* const* a) {
   return THPVariable_Wrap(out);
 }
 
+// ---- pages of a KV cache --------------------------------------------------------------------------------
+// table refs page_size
+struct Pages {
+  at::Tensor table, refs;
+  fa4_kv_pages p = {};
+};
+Pages pages_of(PyObject* const* a) {
+  Pages k;
+  k.table = tensor_of(a[0], "table");
+  k.refs = tensor_of(a[1], "refs");
+  const long size = integer_of(a[2]);
+  if (size < 1 || size > 0x7fffffff) fail(PyExc_ValueError, "page_size must be positive");
+  k.p.page_size = (int32_t)size;
+  if (k.refs.is_cuda()) k.p.status = status_word(k.refs.device());
+  return k;
+}
+// (both are changed in place)
+void describe_pages(Pages& k) {
+  FA4_ASSERT(k.refs.is_cuda(), "the pages must be on CUDA");
+  const at::Device device = k.refs.device();
+  FA4_ASSERT(k.refs.dim() == 1 && k.refs.scalar_type() == at::kInt && k.refs.is_contiguous() && k.refs.size(0) > 0,
+             "refs must be a contiguous (num_pages,) int32 tensor");
+  FA4_ASSERT(k.table.dim() == 2 && k.table.scalar_type() == at::kInt && k.table.device() == device && k.table.is_contiguous() && k.table.size(1) > 0,
+             "table must be a contiguous (B, pages_per_seq) int32 tensor on the device of refs");
+  FA4_ASSERT(k.refs.size(0) <= 0x3fffffff && k.table.size(0) <= 0x7fffffff && k.table.size(1) * (int64_t)k.p.page_size <= 0x7ffffc00ll, "the pages or their table are too large");
+  k.p.struct_size = sizeof k.p;
+  k.p.B = (int32_t)k.table.size(0); k.p.pages_per_seq = (int32_t)k.table.size(1); k.p.num_pages = (int32_t)k.refs.size(0);
+  k.p.table = k.table.data_ptr<int32_t>();
+  k.p.refs = k.refs.data_ptr<int32_t>();
+}
+// Runs `launch(stream)` on the device of the pages.
+template <class Launch>
+void on_device_of(const at::Tensor& t, Launch launch) {
+  const at::Device device = t.device();
+  c10::cuda::OptionalCUDAGuard guard;
+  if (device.index() != c10::cuda::current_device()) guard.set_device(device);
+  launch(c10::cuda::getCurrentCUDAStream(device.index()).stream());
+}
+
+// table refs page_size held wanted
+PyObject* resize_pages(PyObject* const* a) {
+  Pages k = pages_of(a);
+  const at::Tensor held_in = tensor_of(a[3], "held"), wanted_in = tensor_of(a[4], "wanted");
+  at::Tensor pairs;
+  {
+    NoGil nogil;
+    describe_pages(k);
+    const int64_t B = k.p.B;
+    const at::Tensor held = counts_of(held_in, "held", B, k.refs.device()), wanted = counts_of(wanted_in, "wanted", B, k.refs.device());
+    if (B > 4096) fail(PyExc_NotImplementedError, "more than 4096 rows are not built");
+    on_device_of(k.refs, [&](void* stream) {
+      pairs = new_tensor({B, 2}, at::kInt, k.refs.device());
+      if (B == 0) return;
+      const int64_t bytes = fa4_kv_pages_resize_workspace_bytes(&k.p);
+      if (bytes < 0) check_rc((int)bytes, "fa4_kv_pages_resize_workspace_bytes");
+      const c10::DataPtr work = scratch_bytes(bytes);
+      check_rc(fa4_kv_pages_resize(&k.p, held.data_ptr<int32_t>(), wanted.data_ptr<int32_t>(), pairs.data_ptr<int32_t>(), work.get(), (uint64_t)bytes, stream),
+               "fa4_kv_pages_resize");
+    });
+  }
+  return THPVariable_Wrap(pairs);
+}
+
+// table refs page_size held parents new_table new_held
+PyObject* fork_pages(PyObject* const* a) {
+  Pages k = pages_of(a);
+  const at::Tensor held_in = tensor_of(a[3], "held"), parents_in = tensor_of(a[4], "parents");
+  at::Tensor table = optional_tensor(a[5], "out table"), fresh = optional_tensor(a[6], "out held");
+  {
+    NoGil nogil;
+    describe_pages(k);
+    const at::Device device = k.refs.device();
+    FA4_ASSERT(parents_in.dim() == 1, "parents must be (rows,)");
+    const int64_t B = k.p.B, rows = parents_in.size(0);
+    FA4_ASSERT(rows <= 0x7fffffff, "parents too large");
+    const at::Tensor held = counts_of(held_in, "held", B, device), parents = counts_of(parents_in, "parents", rows, device);
+    if (rows * std::max<int64_t>(B, 1) > 0x3fffffffll) fail(PyExc_NotImplementedError, "more than 2^30 pairs of an old and a new row are not built");
+    on_device_of(k.refs, [&](void* stream) {
+      if (table.defined()) {
+        validate(table, "out table", {rows, k.p.pages_per_seq}, at::kInt, device);
+        FA4_ASSERT(table.is_contiguous(), "out table must be contiguous");
+      } else {
+        table = new_tensor({rows, k.p.pages_per_seq}, at::kInt, device);
+      }
+      if (fresh.defined()) {
+        validate(fresh, "out held", {rows}, at::kInt, device);
+        FA4_ASSERT(fresh.is_contiguous(), "out held must be contiguous");
+      } else {
+        fresh = new_tensor({rows}, at::kInt, device);
+      }
+      // (what is read is not what is written)
+      auto apart = [](const at::Tensor& x, const at::Tensor& y) {
+        const char *p = static_cast<const char*>(x.data_ptr()), *q = static_cast<const char*>(y.data_ptr());
+        return p + x.nbytes() <= q || q + y.nbytes() <= p;
+      };
+      for (const at::Tensor* read : {static_cast<const at::Tensor*>(&k.table), static_cast<const at::Tensor*>(&k.refs), &held, &parents})
+        FA4_ASSERT(apart(table, *read) && apart(fresh, *read), "the new table and held must not overlap what the call reads");
+      FA4_ASSERT(apart(table, fresh), "the new table and held must not overlap");
+      if (B == 0 && rows > 0) fail(PyExc_ValueError, "a table without rows has no parents");
+      if (B == 0) return;
+      if (rows == 0) {
+        // nothing is left: every row is dropped, by an empty row of no parent
+        const at::Tensor none = new_tensor({1 + k.p.pages_per_seq + 1}, at::kInt, device);
+        C10_CUDA_CHECK(cudaMemsetAsync(none.data_ptr(), 0xff, 4, static_cast<cudaStream_t>(stream)));
+        int32_t* w = none.data_ptr<int32_t>();
+        check_rc(fa4_kv_pages_fork(&k.p, held.data_ptr<int32_t>(), w, 1, w + 1, w + 1 + k.p.pages_per_seq, stream), "fa4_kv_pages_fork");
+        return;
+      }
+      check_rc(fa4_kv_pages_fork(&k.p, held.data_ptr<int32_t>(), parents.data_ptr<int32_t>(), (int32_t)rows, table.data_ptr<int32_t>(),
+                                 fresh.data_ptr<int32_t>(), stream),
+               "fa4_kv_pages_fork");
+    });
+  }
+  return pair_of(a[5], table, a[6], fresh);
+}
+
+// table refs page_size
+PyObject* compact_pages(PyObject* const* a) {
+  Pages k = pages_of(a);
+  at::Tensor pairs, used;
+  {
+    NoGil nogil;
+    describe_pages(k);
+    // (a table without rows names nothing; refs are all there is)
+    const at::Device device = k.refs.device();
+    FA4_ASSERT(k.p.B > 0, "the table has no rows");
+    on_device_of(k.refs, [&](void* stream) {
+      pairs = new_tensor({k.p.num_pages / 2, 2}, at::kInt, device);
+      used = new_tensor({1}, at::kInt, device);
+      const int64_t bytes = fa4_kv_pages_compact_workspace_bytes(&k.p);
+      if (bytes < 0) check_rc((int)bytes, "fa4_kv_pages_compact_workspace_bytes");
+      const c10::DataPtr work = scratch_bytes(bytes);
+      check_rc(fa4_kv_pages_compact(&k.p, pairs.data_ptr<int32_t>(), used.data_ptr<int32_t>(), work.get(), (uint64_t)bytes, stream), "fa4_kv_pages_compact");
+    });
+  }
+  return pair_of(Py_None, pairs, Py_None, used);
+}
+
+// A tensor with a page in every step of its first dimension, as rows of contiguous bytes: dimensions that lie in each other become one.
+fa4_kv_paged paged_of(const at::Tensor& t, int64_t num_pages, const at::Device& device) {
+  FA4_ASSERT(t.is_cuda() && t.device() == device, "the tensors of a cache and the pairs must be on one CUDA device");
+  FA4_ASSERT(t.dim() >= 1 && t.size(0) == num_pages, "the tensors of a cache have as many pages: %lld and %s", (long long)num_pages, dims_of(t.sizes()).c_str());
+  const int64_t unit = (int64_t)t.element_size();
+  std::vector<std::pair<int64_t, int64_t>> dims;      // (stride, size), bytes
+  for (int64_t i = 1; i < t.dim(); ++i) {
+    if (t.size(i) == 1) continue;
+    FA4_ASSERT(t.size(i) == 0 || t.stride(i) > 0, "a tensor of a cache must not be expanded");
+    dims.emplace_back(t.stride(i) * unit, t.size(i));
+  }
+  FA4_ASSERT(num_pages <= 1 || t.numel() == 0 || t.stride(0) > 0, "a tensor of a cache must not be expanded");
+  std::sort(dims.begin(), dims.end());
+  fa4_kv_paged s = {};
+  s.base = t.data_ptr();
+  s.stride_page = t.stride(0) * unit;
+  s.row_bytes = unit;
+  s.rows_inner = s.rows_outer = 1;
+  int used = 0;                                       // of the two dimensions of rows
+  for (const auto& [stride, size] : dims) {
+    if (used == 0 && stride == s.row_bytes) s.row_bytes *= size;
+    else if (used == 1 && stride == s.stride_inner * s.rows_inner) s.rows_inner *= size;
+    else if (used == 2 && stride == s.stride_outer * s.rows_outer) s.rows_outer *= size;
+    else if (used == 0) { s.stride_inner = stride; s.rows_inner = size; used = 1; }
+    else if (used == 1) { s.stride_outer = stride; s.rows_outer = size; used = 2; }
+    else fail(PyExc_NotImplementedError, "pages of more than three separate dimensions are not built: shape %s", dims_of(t.sizes()).c_str());
+  }
+  return s;
+}
+
+// pairs tensor...
+PyObject* copy_pages(PyObject* const* a) {
+  const at::Tensor pairs_in = tensor_of(a[0], "pairs");
+  if (!PyTuple_Check(a[1])) fail(PyExc_TypeError, "tensors must be a tuple");
+  std::vector<at::Tensor> tensors;
+  for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(a[1]); ++i) tensors.push_back(tensor_of(PyTuple_GET_ITEM(a[1], i), "a tensor of the cache"));
+  uint32_t* status = pairs_in.is_cuda() ? status_word(pairs_in.device()) : nullptr;
+  {
+    NoGil nogil;
+    FA4_ASSERT(pairs_in.is_cuda(), "pairs must be on CUDA");
+    FA4_ASSERT(pairs_in.dim() == 2 && pairs_in.size(1) == 2 && pairs_in.scalar_type() == at::kInt, "pairs must be (n, 2) int32, got %s", dims_of(pairs_in.sizes()).c_str());
+    FA4_ASSERT(pairs_in.size(0) <= 0x7fffffff && !tensors.empty() && tensors[0].dim() >= 1 && tensors[0].size(0) <= 0x7fffffff, "no tensors, or pairs or tensors too large");
+    const at::Device device = pairs_in.device();
+    const int64_t num_pages = tensors[0].size(0);
+    std::vector<fa4_kv_paged> paged;
+    for (const at::Tensor& t : tensors) {
+      const fa4_kv_paged s = paged_of(t, num_pages, device);
+      if (t.numel() > 0) paged.push_back(s);
+    }
+    const at::Tensor pairs = pairs_in.contiguous();
+    if (pairs.size(0) > 0 && !paged.empty())
+      on_device_of(pairs, [&](void* stream) {
+        for (size_t i = 0; i < paged.size(); i += FA4_KV_COPY_TENSORS) {
+          fa4_kv_copy c = {};
+          c.struct_size = sizeof c;
+          c.num_pairs = (int32_t)pairs.size(0); c.num_pages = (int32_t)num_pages;
+          c.num_tensors = (int32_t)std::min<size_t>(FA4_KV_COPY_TENSORS, paged.size() - i);
+          c.pairs = pairs.data_ptr<int32_t>();
+          c.status = status;
+          std::copy_n(paged.begin() + i, c.num_tensors, c.tensors);
+          check_rc(fa4_kv_pages_copy(&c, stream), "fa4_kv_pages_copy");
+        }
+      });
+  }
+  Py_RETURN_NONE;
+}
+
 // ---- the module -----------------------------------------------------------------------------------
 PyObject* choose_decode_splits(PyObject* const* a) {
   return PyLong_FromLongLong(decode_splits(integer_of(a[0]), integer_of(a[1]), integer_of(a[2]), integer_of(a[3])));
@@ -1453,6 +1658,10 @@ PyMethodDef methods[] = {method<fwd, 23>("fwd"),
                          method<fwd_fp8, 20>("fwd_fp8"),
                          method<index_fp8, 10>("index_fp8"),
                          method<select_fp8, 15>("select_fp8"),
+                         method<resize_pages, 5>("resize_pages"),
+                         method<fork_pages, 7>("fork_pages"),
+                         method<compact_pages, 3>("compact_pages"),
+                         method<copy_pages, 2>("copy_pages"),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_host", "Native host path of flash_attention_b200.", -1, methods,
                           nullptr, nullptr, nullptr, nullptr};

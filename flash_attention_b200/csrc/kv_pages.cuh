@@ -1,0 +1,415 @@
+// Pages of a KV cache: who has which (a table and reference counts, both on the device), and copying them.
+//
+// A table (sequences, pages of a sequence) names pages of a pool, -1 where there is none; refs counts the entries that name a page, 0 is
+// free.  The book-keeping is a few thousand whole numbers: one cluster of eight CTAs does it in one launch, in phases between
+// rendezvous of the cluster, so nothing waits for the host and results do not depend on the order of threads (counters are
+// only added to; what is given away is ranked by prefix sums: rows in order, free pages from the lowest on).
+#pragma once
+#include "fp8_append.cuh"
+
+namespace fa4 {
+namespace pages {
+
+constexpr int kCluster = 8, kThreads = 1024, kWarps = kThreads / 32;
+constexpr int kRows = 4096;                    // of a table: their prefix sums stay in shared memory
+
+enum Site { kTableSite = 123, kLengthSite = 124, kPoolSite = 125, kParentSite = 126, kPairSite = 127 };
+
+struct Book {
+  int32_t* table;
+  int32_t* refs;
+  int B, width, num_pages, page_size;
+  FastDiv div_page;
+  uint32_t* status;
+  uint32_t epoch;
+};
+// Pages of `tokens`.
+__device__ __forceinline__ int pages_of(const Book& p, int tokens) {
+  const int whole = fast_div(tokens, p.div_page);
+  return whole + (whole * p.page_size < tokens);
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// Rendezvous of the cluster behind which everything that was written before it, global memory included, can be read (by __ldcg).
+__device__ __forceinline__ void meet() {
+  __threadfence();
+  cluster_sync();
+}
+
+// Exclusive prefix sum over the CTA's warps of a value of each; `all`: the sum.  s: kWarps + 1 words.
+__device__ __forceinline__ int scan_warps(int mine, int* s, int* all) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __syncthreads();
+  if (lane == 0) s[warp] = mine;
+  __syncthreads();
+  if (warp == 0) {
+    const int v = s[lane];
+    int upto = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int w = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += w;
+    }
+    s[lane] = upto - v;
+    if (lane == 31) s[kWarps] = upto;
+  }
+  __syncthreads();
+  *all = s[kWarps];
+  return s[warp];
+}
+
+// The part of the pool that a warp of the cluster looks at: [from, to), multiples of 32 from the pool's start.
+struct Part {
+  int from, to;
+};
+__device__ __forceinline__ Part part_of(int num_pages) {
+  const int per = ((num_pages + kCluster * kWarps - 1) / (kCluster * kWarps) + 31) & ~31;
+  const int w = (int)cluster_rank() * kWarps + (threadIdx.x >> 5);
+  const int64_t from = (int64_t)w * per;
+  return {(int)min(from, (int64_t)num_pages), (int)min(from + per, (int64_t)num_pages)};
+}
+// Calls what(page, mask of the lanes with pages that are(refs of page)) for 32 pages at a time.
+template <class Are, class What>
+__device__ __forceinline__ void over_pages(const Book& p, Part part, Are are, What what) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll 4
+  for (int i0 = part.from; i0 < part.to; i0 += 32) {
+    const int i = i0 + lane;
+    const int r = i < part.to ? __ldcg(p.refs + i) : 1;
+    what(i, __ballot_sync(0xffffffffu, i < part.to && are(i, r)));
+  }
+}
+template <class Are>
+__device__ __forceinline__ int count_pages(const Book& p, Part part, Are are) {
+  int n = 0;
+  over_pages(p, part, are, [&](int, uint32_t mask) { n += __popc(mask); });
+  return n;
+}
+
+struct ResizeParams {
+  Book book;
+  const int32_t *held, *wanted;
+  int32_t* pairs;                    // (B, 2)
+  int32_t* work;                     // B: page written to or -1 (bit 30: is copied), B: entries that lack a page, kCluster, num_pages: the free ones, in order
+};
+__host__ __device__ constexpr int64_t resize_words(int64_t B, int64_t num_pages) { return 2 * B + kCluster + num_pages; }
+
+// A row's lengths, within the table.
+struct Lengths {
+  int held, wanted;
+};
+__device__ __forceinline__ Lengths lengths_of(const ResizeParams& p, int b, bool report) {
+  Lengths n = {p.held[b], p.wanted[b]};
+  const int most = p.book.width * p.book.page_size;
+  if (report && (n.held < 0 || n.wanted < 0 || n.wanted > most)) report_bad_index(p.book.status, p.book.epoch, kLengthSite);
+  n.held = n.held < 0 ? 0 : (n.held < most ? n.held : most);
+  n.wanted = n.wanted < 0 ? 0 : (n.wanted < most ? n.wanted : most);
+  return n;
+}
+
+// Rows keep the pages of what they hold (held, at most wanted), give back those behind, and get pages for `wanted` tokens.  A row that is about to write
+// into a page which other entries name too gets a copy of it (the last of the call's rows keeps the page, if nobody else has it).
+__global__ void __launch_bounds__(kThreads) resize_kernel(const __grid_constant__ ResizeParams p) {
+  __shared__ int s_first[kRows], s_scan[kWarps + 1];
+  const Book& k = p.book;
+  const int rank = (int)cluster_rank(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row0 = rank * kWarps + warp, step = kCluster * kWarps;
+  int32_t *writes = p.work, *lacks = writes + k.B, *free_of = lacks + k.B, *free_page = free_of + kCluster;
+  pdl_wait();
+  // ---- what is given back; what is missing
+  for (int b = row0; b < k.B; b += step) {
+    const Lengths n = lengths_of(p, b, lane == 0);
+    const int keep = pages_of(k, min(n.held, n.wanted)), want = pages_of(k, n.wanted), at = fast_div(n.held, k.div_page);
+    int32_t* row = k.table + (int64_t)b * k.width;
+    int missing = max(want - keep, 0), page = -1;
+    for (int j0 = 0; j0 < k.width; j0 += 32) {
+      const int j = j0 + lane;
+      int e = j < k.width ? row[j] : 0;
+      if (e >= k.num_pages) {
+        report_bad_index(k.status, k.epoch, kTableSite);
+        e = -1;
+        row[j] = -1;
+      }
+      if (j < k.width && j >= keep && e >= 0) {
+        atomicSub(k.refs + e, 1);
+        row[j] = -1;
+      }
+      missing += __popc(__ballot_sync(0xffffffffu, j < keep && e < 0));
+      // (a row that grows keeps the page its next token goes to)
+      if (j0 <= at && at < j0 + 32) page = __shfl_sync(0xffffffffu, e, at & 31);
+    }
+    if (lane == 0) {
+      writes[b] = n.wanted > n.held && n.held != at * k.page_size && page >= 0 ? page : -1;
+      lacks[b] = missing;
+    }
+  }
+  meet();
+  // ---- who gets a copy: all but the last of a page's entries
+  for (int b = row0; b < k.B; b += step) {
+    const int page = __ldcg(writes + b);
+    if (page < 0) continue;
+    const int others = __ldcg(k.refs + page) - 1;
+    if (others <= 0) continue;
+    int earlier = 0;
+    for (int i = lane; i < b; i += 32) earlier += (__ldcg(writes + i) & 0x3fffffff) == page && __ldcg(writes + i) >= 0;
+    earlier = __reduce_add_sync(0xffffffffu, earlier);
+    if (lane == 0 && earlier < others) {
+      writes[b] = page | 0x40000000;
+      ++lacks[b];
+    }
+  }
+  // ---- the free pages, counted
+  const Part part = part_of(k.num_pages);
+  auto is_free = [](int, int r) { return r == 0; };
+  int here, before = scan_warps(count_pages(k, part, is_free), s_scan, &here);
+  if (threadIdx.x == 0) free_of[rank] = here;
+  meet();
+  // ---- where a row's new pages lie in the list of all that are wanted
+  int total, free_pages = 0;
+  {
+    int mine[kRows / kThreads], sum = 0;
+#pragma unroll
+    for (int i = 0; i < kRows / kThreads; ++i) {
+      const int b = (int)threadIdx.x * (kRows / kThreads) + i;
+      mine[i] = b < k.B ? __ldcg(lacks + b) : 0;
+      sum += mine[i];
+    }
+    int upto = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    int at = scan_warps(__shfl_sync(0xffffffffu, upto, 31), s_scan, &total) + upto - sum;
+#pragma unroll
+    for (int i = 0; i < kRows / kThreads; ++i) {
+      s_first[(int)threadIdx.x * (kRows / kThreads) + i] = at;
+      at += mine[i];
+    }
+  }
+  for (int r = 0; r < kCluster; ++r) {
+    if (r < rank) before += __ldcg(free_of + r);
+    free_pages += __ldcg(free_of + r);
+  }
+  if (before < total)
+    over_pages(k, part, is_free, [&](int page, uint32_t mask) {
+      const int at = before + __popc(mask & ((1u << lane) - 1u));
+      if ((mask >> lane & 1u) != 0u && at < total) {
+        free_page[at] = page;
+        k.refs[page] = 1;
+      }
+      before += __popc(mask);
+    });
+  meet();
+  // ---- the rows are filled
+  for (int b = row0; b < k.B; b += step) {
+    const int copied = __ldcg(writes + b);
+    const bool copies = copied >= 0 && (copied & 0x40000000) != 0;
+    const Lengths n = lengths_of(p, b, false);
+    const int want = pages_of(k, n.wanted), at = copies ? fast_div(n.held, k.div_page) : -1;
+    int32_t* row = k.table + (int64_t)b * k.width;
+    int next = s_first[b], fresh = -1;
+    for (int j0 = 0; j0 < want; j0 += 32) {
+      const int j = j0 + lane;
+      const bool lack = j < want && (j == at || row[j] < 0);
+      const uint32_t mask = __ballot_sync(0xffffffffu, lack);
+      const int i = next + __popc(mask & ((1u << lane) - 1u));
+      int page = -1;
+      if (lack) {
+        if (i < free_pages) page = __ldcg(free_page + i);
+        else report_bad_index(k.status, k.epoch, kPoolSite);
+        row[j] = page;
+      }
+      if (j0 <= at && at < j0 + 32) fresh = __shfl_sync(0xffffffffu, page, at & 31);
+      next += __popc(mask);
+    }
+    if (lane == 0) {
+      const int from = copied & 0x3fffffff;
+      if (copies) atomicSub(k.refs + from, 1);
+      p.pairs[2 * b] = copies && fresh >= 0 ? from : -1;
+      p.pairs[2 * b + 1] = copies ? fresh : -1;
+    }
+  }
+}
+
+struct ForkParams {
+  Book book;                         // (of the old table)
+  const int32_t *held, *parents;
+  int32_t *table, *new_held;         // (rows, width), (rows,)
+  int rows;
+};
+constexpr int kForkThreads = 128;
+
+// CTAs 0 .. rows - 1: a new row each; the others: the references of an old row's pages, which change by its children but one.
+__global__ void __launch_bounds__(kForkThreads) fork_kernel(const __grid_constant__ ForkParams p) {
+  const Book& k = p.book;
+  const int tid = threadIdx.x;
+  const int64_t most = (int64_t)k.width * k.page_size;
+  pdl_wait();
+  if ((int)blockIdx.x < p.rows) {
+    const int b = blockIdx.x, a = p.parents[b];
+    const bool there = a >= 0 && a < k.B;
+    if (tid == 0 && !there && a != -1) report_bad_index(k.status, k.epoch, kParentSite);
+    int held = there ? p.held[a] : 0;
+    if (tid == 0 && (held < 0 || held > most)) report_bad_index(k.status, k.epoch, kLengthSite);
+    held = held < 0 ? 0 : (held < most ? held : (int)most);
+    const int keep = pages_of(k, held);
+    for (int j = tid; j < k.width; j += kForkThreads) {
+      const int e = j < keep ? k.table[(int64_t)a * k.width + j] : -1;
+      p.table[(int64_t)b * k.width + j] = e >= 0 && e < k.num_pages ? e : -1;
+    }
+    if (tid == 0) p.new_held[b] = held;
+    return;
+  }
+  const int a = (int)blockIdx.x - p.rows;
+  __shared__ int s_children;
+  if (tid == 0) s_children = 0;
+  __syncthreads();
+  int mine = 0;
+  for (int b = tid; b < p.rows; b += kForkThreads) mine += p.parents[b] == a;
+  mine = __reduce_add_sync(0xffffffffu, mine);
+  if ((tid & 31) == 0 && mine != 0) atomicAdd(&s_children, mine);
+  __syncthreads();
+  int held = p.held[a];
+  held = held < 0 ? 0 : (held < most ? held : (int)most);
+  const int keep = pages_of(k, held), change = s_children - 1;
+  for (int j = tid; j < k.width; j += kForkThreads) {
+    const int e = k.table[(int64_t)a * k.width + j], by = j < keep ? change : -1;
+    if (e >= k.num_pages) report_bad_index(k.status, k.epoch, kTableSite);
+    else if (e >= 0 && by != 0) atomicAdd(k.refs + e, by);
+  }
+}
+
+struct CompactParams {
+  Book book;
+  int32_t* pairs;                    // (num_pages / 2, 2)
+  int32_t* used;
+  int32_t* work;                     // 3 kCluster, num_pages: where a page went
+};
+__host__ __device__ constexpr int64_t compact_words(int64_t num_pages) { return 3 * kCluster + num_pages; }
+
+// With `used` pages in use, the i-th of those at `used` or above moves to the i-th free one below.
+__global__ void __launch_bounds__(kThreads) compact_kernel(const __grid_constant__ CompactParams p) {
+  __shared__ int s_scan[kWarps + 1];
+  const Book& k = p.book;
+  const int rank = (int)cluster_rank(), lane = threadIdx.x & 31, all = rank * kThreads + threadIdx.x;
+  int32_t *live_of = p.work, *holes_of = live_of + kCluster, *movers_of = holes_of + kCluster, *to = movers_of + kCluster;
+  pdl_wait();
+  const Part part = part_of(k.num_pages);
+  int here;
+  scan_warps(count_pages(k, part, [](int, int r) { return r > 0; }), s_scan, &here);
+  if (threadIdx.x == 0) live_of[rank] = here;
+  meet();
+  int used = 0;
+  for (int r = 0; r < kCluster; ++r) used += __ldcg(live_of + r);
+  auto is_hole = [used](int i, int r) { return r <= 0 && i < used; };
+  auto is_mover = [used](int i, int r) { return r > 0 && i >= used; };
+  int hole = scan_warps(count_pages(k, part, is_hole), s_scan, &here);
+  if (threadIdx.x == 0) holes_of[rank] = here;
+  int mover = scan_warps(count_pages(k, part, is_mover), s_scan, &here);
+  if (threadIdx.x == 0) movers_of[rank] = here;
+  meet();
+  int moved = 0;
+  for (int r = 0; r < kCluster; ++r) {
+    if (r < rank) {
+      hole += __ldcg(holes_of + r);
+      mover += __ldcg(movers_of + r);
+    }
+    moved += __ldcg(movers_of + r);
+  }
+  const uint32_t in_front = (1u << lane) - 1u;
+  over_pages(k, part, is_hole, [&](int page, uint32_t mask) {
+    if ((mask >> lane & 1u) != 0u) p.pairs[2 * (hole + __popc(mask & in_front)) + 1] = page;
+    hole += __popc(mask);
+  });
+  over_pages(k, part, is_mover, [&](int page, uint32_t mask) {
+    const bool goes = (mask >> lane & 1u) != 0u;
+    if (goes) p.pairs[2 * (mover + __popc(mask & in_front))] = page;
+    else if (page >= used && page < part.to) to[page] = page;
+    mover += __popc(mask);
+  });
+  for (int i = moved + all; i < k.num_pages / 2; i += kCluster * kThreads) p.pairs[2 * i] = p.pairs[2 * i + 1] = -1;
+  if (all == 0) *p.used = used;
+  meet();
+  for (int i = all; i < moved; i += kCluster * kThreads) {
+    const int from = __ldcg(p.pairs + 2 * i), at = __ldcg(p.pairs + 2 * i + 1);
+    k.refs[at] = __ldcg(k.refs + from);
+    k.refs[from] = 0;
+    to[from] = at;
+  }
+  meet();
+  const int64_t entries = (int64_t)k.B * k.width;
+  for (int64_t i = all; i < entries; i += kCluster * kThreads) {
+    const int e = k.table[i];
+    if (e >= k.num_pages) report_bad_index(k.status, k.epoch, kTableSite);
+    else if (e >= used) k.table[i] = __ldcg(to + e);
+  }
+}
+
+// ---- copying ------------------------------------------------------------------------------------------------------
+
+// A tensor with a page in every step of its first dimension, as rows of whole pieces (of 16, 4 or 1 bytes).
+struct PagedTensor {
+  uint8_t* base;
+  int64_t page, inner, outer;        // strides, bytes
+  int pieces, log_piece;             // of a page
+  FastDiv div_row, div_inner;        // pieces of a row; rows side by side along `inner`
+  int row, rows_inner;
+};
+constexpr int kTensors = 8, kCopyThreads = 256, kCopyPieces = 4;
+struct CopyParams {
+  const int32_t* pairs;
+  int n, num_pages;
+  int tensors;
+  PagedTensor t[kTensors];
+  int first[kTensors + 1];           // tasks of a pair that are a tensor's: kCopyThreads * kCopyPieces pieces each
+  FastDiv div_tasks;
+  int64_t tasks;                     // n * first[tensors]
+  uint32_t* status;
+  uint32_t epoch;
+};
+
+template <class T>
+__device__ __forceinline__ void copy_pieces(const PagedTensor& t, int from, int to, int i0) {
+  T v[kCopyPieces];
+  int64_t at[kCopyPieces];
+#pragma unroll
+  for (int j = 0; j < kCopyPieces; ++j) {
+    const int i = i0 + j * kCopyThreads;
+    at[j] = -1;
+    if (i < t.pieces) {
+      const int r = fast_div(i, t.div_row), o = fast_div(r, t.div_inner);
+      at[j] = o * t.outer + (r - o * t.rows_inner) * t.inner + (int64_t)(i - r * t.row) * sizeof(T);
+      v[j] = *reinterpret_cast<const T*>(t.base + from * t.page + at[j]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kCopyPieces; ++j)
+    if (at[j] >= 0) *reinterpret_cast<T*>(t.base + to * t.page + at[j]) = v[j];
+}
+
+__global__ void __launch_bounds__(kCopyThreads) copy_kernel(const __grid_constant__ CopyParams p) {
+  pdl_wait();
+  const int per = p.first[p.tensors];
+  for (int64_t task = blockIdx.x; task < p.tasks; task += gridDim.x) {
+    const int pair = fast_div((int)task, p.div_tasks), part = (int)task - pair * per;
+    const int from = p.pairs[2 * pair], to = p.pairs[2 * pair + 1];
+    if (from < 0 || to < 0) continue;
+    if (from >= p.num_pages || to >= p.num_pages) {
+      if (threadIdx.x == 0) report_bad_index(p.status, p.epoch, kPairSite);
+      continue;
+    }
+    int which = 0;
+    while (part >= p.first[which + 1]) ++which;
+    const PagedTensor& t = p.t[which];
+    const int i0 = (part - p.first[which]) * (kCopyThreads * kCopyPieces) + threadIdx.x;
+    if (t.log_piece == 4) copy_pieces<uint4>(t, from, to, i0);
+    else if (t.log_piece == 2) copy_pieces<uint32_t>(t, from, to, i0);
+    else copy_pieces<uint8_t>(t, from, to, i0);
+  }
+}
+
+}  // namespace pages
+}  // namespace fa4

@@ -653,6 +653,66 @@ typedef struct fa4_fp8_blocks {
 int64_t fa4_fp8_cache_fwd_blocks_workspace_bytes(const fa4_fp8_cache* cache, const fa4_fp8_fwd* p, const fa4_fp8_blocks* x);
 int fa4_fp8_cache_fwd_blocks(const fa4_fp8_cache* cache, const fa4_fp8_fwd* p, const fa4_fp8_blocks* x, void* cuda_stream);
 
+/*
+ * ---- pages of a KV cache -------------------------------------------------------------------------------------
+ *
+ * Which pages of a pool the sequences of a batch have, kept on the device: allocating and freeing, forking (beams, samples of one
+ * prompt), copy on write, compacting.  No counterpart in the reference, whose callers make page tables on the host.
+ *
+ *   table (B, pages_per_seq) int32: pages of a sequence, in order; -1 (any negative number) where it has none
+ *   refs  (num_pages,) int32: how many entries of tables name a page; 0: free
+ * Nothing in it is a particular cache's: caches of several layers are kept by one table, and the pages that a call wants copied come
+ * back as pairs (from, to), -1 where there is none, for fa4_kv_pages_copy of each.  Everything is given out in a fixed order (rows, then
+ * entries; free pages from the lowest number on).  Bad numbers on the device are left out and recorded in the status word as FA4_S_BAD_INDEX.
+ */
+typedef struct fa4_kv_pages {
+  uint32_t struct_size;      /* = sizeof(fa4_kv_pages) */
+  int32_t B, pages_per_seq, num_pages, page_size;
+  uint32_t reserved;         /* 0 */
+  int32_t* table;
+  int32_t* refs;
+  uint32_t* status;
+} fa4_kv_pages;
+/*
+ * Row b keeps the pages of its first min(held[b], wanted[b]) tokens, gives back those behind, and gets pages for wanted[b].  Where it grows and its
+ * next token goes into a page that holds some of it and has other entries too, it gets a copy of that page: pairs[b] = (page, copy).  Of the rows that
+ * would write to one page the last one keeps it if nobody else names it.  Pages that are given back may be given out by the same call.  Where no page is
+ * left the entry is -1, which is recorded.  At most 4096 rows.  Workspace as for the attention.
+ */
+int64_t fa4_kv_pages_resize_workspace_bytes(const fa4_kv_pages* pages);
+int fa4_kv_pages_resize(const fa4_kv_pages* pages, const int32_t* held, const int32_t* wanted, int32_t* pairs /* (B, 2) */, void* workspace,
+                        uint64_t workspace_bytes, void* cuda_stream);
+/*
+ * A new table of `rows` rows: row i is row parents[i] of the old one as far as it holds tokens (-1: an empty row), new_held[i] its held.  refs
+ * follow; the old table has no entries any more as far as they go.  new_table and new_held overlap nothing else.
+ */
+int fa4_kv_pages_fork(const fa4_kv_pages* pages, const int32_t* held, const int32_t* parents, int32_t rows, int32_t* new_table, int32_t* new_held,
+                      void* cuda_stream);
+/*
+ * With used[0] pages in use, the i-th of those at used[0] or above goes to the i-th free one below: pairs (num_pages / 2, 2), the rest of which is (-1, -1).
+ * Table and refs follow; entries in other tables than this one do not.
+ */
+int64_t fa4_kv_pages_compact_workspace_bytes(const fa4_kv_pages* pages);
+int fa4_kv_pages_compact(const fa4_kv_pages* pages, int32_t* pairs, int32_t* used, void* workspace, uint64_t workspace_bytes, void* cuda_stream);
+/*
+ * Copies page pairs[i][0] of every tensor to page pairs[i][1]; pairs with a negative number are none.  No page is written twice, or both read and written, in
+ * one call.  A page is rows_outer x rows_inner rows of row_bytes bytes.
+ */
+#define FA4_KV_COPY_TENSORS 8
+typedef struct fa4_kv_paged {
+  void* base;
+  int64_t stride_page, stride_inner, stride_outer;     /* bytes */
+  int64_t row_bytes, rows_inner, rows_outer;
+} fa4_kv_paged;
+typedef struct fa4_kv_copy {
+  uint32_t struct_size;      /* = sizeof(fa4_kv_copy) */
+  int32_t num_pairs, num_pages, num_tensors;
+  const int32_t* pairs;
+  uint32_t* status;
+  fa4_kv_paged tensors[FA4_KV_COPY_TENSORS];
+} fa4_kv_copy;
+int fa4_kv_pages_copy(const fa4_kv_copy* c, void* cuda_stream);
+
 #ifdef __cplusplus
 }
 #endif
