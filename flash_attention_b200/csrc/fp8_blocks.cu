@@ -74,7 +74,7 @@ extern "C" int fa4_fp8_cache_select(const fa4_fp8_cache* c, const fa4_fp8_index*
   const int64_t query_blocks = ((int64_t)a->Sq + a->query_block - 1) / a->query_block, units = query_blocks * a->B * c->Hkv,
                 blocks = (int64_t)c->pages_per_seq * c->page_size / c->block;
   // (sums of a query block are 32-bit; a unit's scores stay in shared memory)
-  if (units > 0x0fffffffll || rows * group > 32768 || blocks > kSelectBlocks) return -FA4_E_TOO_LARGE;
+  if (units > 0x0fffffffll || rows * group > 32768 || blocks > kSelectBlocks || (int64_t)c->num_pages * (c->page_size / c->block) > 0x7fffffffll) return -FA4_E_TOO_LARGE;
   SelectParams p = {};
   p.q = static_cast<const __nv_bfloat16*>(a->q);
   p.q_b = a->q_stride_b; p.q_s = a->q_stride_s; p.q_h = a->q_stride_h;
@@ -98,9 +98,13 @@ extern "C" int fa4_fp8_cache_select(const fa4_fp8_cache* c, const fa4_fp8_index*
   p.epoch = next_launch_epoch();
   const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
   const uint32_t smem = (uint32_t)blocks * 4;
+  // Few units of many blocks: several CTAs a unit.
+  p.parts = 1;
+  while (p.parts < 8 && units * p.parts * 2 <= kSms && blocks / (p.parts * 2) >= 256) p.parts *= 2;
   auto launch = [&](auto kernel) -> int {
     if (int e = ensure_smem(kernel, kSelectBlocks * 4)) return e;
-    return launch_pdl(kernel, dim3((unsigned)units), kSelectThreads, smem, stream, p);
+    return launch_pdl_cluster((unsigned)p.parts, kernel, dim3((unsigned)(units * p.parts)), kSelectThreads, smem, stream, p);
   };
-  return c->D == 128 ? launch(fp8_select_kernel<128>) : launch(fp8_select_kernel<64>);
+  if (p.parts > 1) return c->D == 128 ? launch(fp8_select_kernel<128, true>) : launch(fp8_select_kernel<64, true>);
+  return c->D == 128 ? launch(fp8_select_kernel<128, false>) : launch(fp8_select_kernel<64, false>);
 }

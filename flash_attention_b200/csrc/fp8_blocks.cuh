@@ -143,12 +143,13 @@ struct SelectParams {
   int32_t* blocks;                   // (B, query blocks, Hkv, chosen)
   int Sq, Hkv, group, log_block, num_pages, page_size, pages_per_seq, capacity;
   int chosen, query_block, query_blocks, front, recent;
+  int parts;                         // CTAs of a unit
   FastDiv div_hkv, div_query_blocks, div_page, div_group;
   uint32_t* status;
   uint32_t epoch;
 };
 
-constexpr int kSelectThreads = 256;
+constexpr int kSelectThreads = 512;
 constexpr int kSelectBlocks = 53248;           // of a sequence: their scores are 208 KB
 
 // Order of scores as whole numbers: the larger the score the larger the key; NaN as +inf, -0 as 0.
@@ -159,17 +160,29 @@ __device__ __forceinline__ uint32_t score_key(float s) {
 }
 constexpr uint32_t kAlways = 0xffffffffu;      // (no score has it)
 
-// A CTA a unit (sequence, query block, kv head).
-template <int kD>
-__global__ void __launch_bounds__(kSelectThreads) fp8_select_kernel(const __grid_constant__ SelectParams p) {
-  constexpr int kWarps = kSelectThreads / 32, kPieces = kD / 8;
-  extern __shared__ uint32_t s_key[];
-  __shared__ int s_sum[2 * kD], s_hist[256], s_red[kWarps], s_count[2 * kWarps];
+__device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t rank, uint32_t v) {
+  asm volatile(
+      "{\n"
+      ".reg .b32 a;\n"
+      "mapa.shared::cluster.u32 a, %0, %1;\n"
+      "st.shared::cluster.u32 [a], %2;\n"
+      "}\n" ::"r"(addr), "r"(rank), "r"(v)
+      : "memory");
+}
+
+// A unit (sequence, query block, kv head) is one CTA's, or (kParts) that of a cluster whose CTAs score a part of the blocks each and leave the keys
+// with the first one, which chooses.
+template <int kD, bool kParts>
+__global__ void __launch_bounds__(kSelectThreads, 2) fp8_select_kernel(const __grid_constant__ SelectParams p) {
+  constexpr int kWarps = kSelectThreads / 32, kPieces = kD / 8, kBins = 2048;
+  extern __shared__ uint32_t s_key[];          // of the CTA's blocks: where their bounds are; then the keys
+  __shared__ int s_sum[2 * kD], s_hist[kBins], s_red[kWarps], s_count[2 * kWarps];
   __shared__ __align__(16) int8_t s_q[2 * kD];
-  __shared__ uint32_t s_prefix;
-  __shared__ int s_left;
+  __shared__ uint32_t s_range[2 * 8];          // smallest and largest key of a CTA's blocks
+  __shared__ int s_bin[3];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int unit = blockIdx.x, rest = fast_div(unit, p.div_hkv), head = unit - rest * p.Hkv, b = fast_div(rest, p.div_query_blocks),
+  const int unit = kParts ? blockIdx.x / p.parts : blockIdx.x, part = kParts ? blockIdx.x - unit * p.parts : 0;
+  const int rest = fast_div(unit, p.div_hkv), head = unit - rest * p.Hkv, b = fast_div(rest, p.div_query_blocks),
             q0 = (rest - b * p.query_blocks) * p.query_block;
   pdl_wait();
   int sk = p.used[b], sq = p.fresh != nullptr ? p.fresh[b] : p.Sq;
@@ -179,44 +192,80 @@ __global__ void __launch_bounds__(kSelectThreads) fp8_select_kernel(const __grid
   const int bt = 1 << p.log_block, n = (end + bt - 1) >> p.log_block;
   int32_t* out = p.blocks + (int64_t)unit * p.chosen;
   if (n <= p.chosen) {
-    for (int i = tid; i < p.chosen; i += kSelectThreads) out[i] = i < n ? i : -1;
+    if (part == 0)
+      for (int i = tid; i < p.chosen; i += kSelectThreads) out[i] = i < n ? i : -1;
     return;
   }
+  const int per = kParts ? ((n + p.parts - 1) / p.parts + 31) & ~31 : n, b0 = part * per, b1 = min(n, b0 + per);
+  // ---- where the bounds are
+  for (int j = b0 + tid; j < b1; j += kSelectThreads) {
+    const int at = j << p.log_block, pg = fast_div(at, p.div_page), off = at - pg * p.page_size;
+    const int page = p.table != nullptr ? p.table[(int64_t)b * p.pages_per_seq + pg] : b;
+    const bool fine = page >= 0 && page < p.num_pages;
+    if (!fine) report_bad_index(p.status, p.epoch, kPageSite);
+    s_key[j] = fine ? (uint32_t)(page * (p.page_size >> p.log_block) + (off >> p.log_block)) : 0xffffffffu;
+  }
+  for (int i = tid; i < 2 * kD; i += kSelectThreads) s_sum[i] = 0;
+  if (tid < 2) s_range[2 * part + tid] = tid == 0 ? 0xffffffffu : 0u;
   // ---- the query: largest element, sums of whole numbers, seven bits
   const __nv_bfloat16* q = p.q + b * p.q_b + (int64_t)q0 * p.q_s + (int64_t)head * p.group * p.q_h;
-  const int R = rows * p.group;
-  auto row_piece = [&](int i, float (&x)[8]) {
+  const int pieces = rows * p.group * kPieces;
+  auto piece_of = [&](int i) -> uint4 {
     const int r = i / kPieces, s = fast_div(r, p.div_group), h = r - s * p.group;
-    unpack8(*reinterpret_cast<const uint4*>(q + (int64_t)s * p.q_s + h * p.q_h + 8 * (i % kPieces)), x);
+    return *reinterpret_cast<const uint4*>(q + (int64_t)s * p.q_s + h * p.q_h + 8 * (i % kPieces));
   };
-  for (int i = tid; i < 2 * kD; i += kSelectThreads) s_sum[i] = 0;
   uint32_t top = 0u;
-  for (int i = tid; i < R * kPieces; i += kSelectThreads) {
-    float x[8];
-    row_piece(i, x);
+#pragma unroll 4
+  for (int i = tid; i < pieces; i += kSelectThreads) {
+    const uint4 u = piece_of(i);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const uint32_t m = __float_as_uint(x[k]) & 0x7fffffffu;
-      top = max(top, m < 0x7f800000u ? m : 0u);
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t lo = w[k] << 16 & 0x7fff0000u, hi = w[k] & 0x7fff0000u;
+      top = max(top, max(lo < 0x7f800000u ? lo : 0u, hi < 0x7f800000u ? hi : 0u));
     }
   }
   top = __reduce_max_sync(0xffffffffu, top);
   if (lane == 0) s_red[warp] = (int)top;
   __syncthreads();
+  // the first bounds, on their way meanwhile: four lanes a block, which hold every fourth piece of 16 bytes of it
+  constexpr int kParcels = kD / 32, kDeep = 2, kRound = kWarps * 8;           // pieces of a lane; rounds on their way; blocks of a round
+  const int sub = lane >> 2, c = lane & 3;
+  uint4 v[kDeep][kParcels];
+  float scale[kDeep];
+  auto fetch = [&](int j0) {
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) top = max(top, (uint32_t)s_red[w]);
+    for (int k = 0; k < kDeep; ++k) {
+      const int j = j0 + k * kRound + sub;
+      const uint32_t at = j < b1 ? s_key[j] : 0xffffffffu;
+      scale[k] = -INFINITY;                        // (a page outside the pool; no index has it)
+      if (at != 0xffffffffu) {
+        const int64_t i = (int64_t)at * p.Hkv + head;
+        const uint4* from = reinterpret_cast<const uint4*>(p.bounds + i * (2 * kD)) + c;
+#pragma unroll
+        for (int r = 0; r < kParcels; ++r) v[k][r] = from[4 * r];
+        scale[k] = p.scale[i];
+      } else {
+#pragma unroll
+        for (int r = 0; r < kParcels; ++r) v[k][r] = make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
+  };
+  fetch(b0 + warp * 8);
+  top = __reduce_max_sync(0xffffffffu, (uint32_t)s_red[lane & (kWarps - 1)]);
   const int e = max((int)(top >> 23) - 127, -100);
   const float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
-  {
-    int pos[8] = {}, neg[8] = {};
-    for (int i = tid; i < R * kPieces; i += kSelectThreads) {       // (a thread stays with its eight channels)
+  if (warp * 32 < pieces) {
+    int pos[8] = {}, neg[8] = {};                  // (a thread stays with its eight channels)
+#pragma unroll 2
+    for (int i = tid; i < pieces; i += kSelectThreads) {
       float x[8];
-      row_piece(i, x);
+      unpack8(piece_of(i), x);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const int v = fabsf(x[k]) < INFINITY ? __float2int_rn(x[k] * up) : 0;
-        pos[k] += max(v, 0);
-        neg[k] += max(-v, 0);
+        const int y = fabsf(x[k]) < INFINITY ? __float2int_rn(x[k] * up) : 0;
+        pos[k] += max(y, 0);
+        neg[k] += max(-y, 0);
       }
     }
     const int ch = tid % kPieces * 8;
@@ -235,99 +284,140 @@ __global__ void __launch_bounds__(kSelectThreads) fp8_select_kernel(const __grid
   }
   __syncthreads();
   {
-    int most = tid < 2 * kD ? s_sum[tid] : 0;
     static_assert(2 * kD <= kSelectThreads, "a thread a channel");
-    most = __reduce_max_sync(0xffffffffu, most);
-    if (lane == 0) s_red[warp] = most;
-    __syncthreads();
+    int most = 0;                                  // (every warp looks at all sums)
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) most = max(most, s_red[w]);
+    for (int i = 0; i < 2 * kD; i += 32) most = max(most, s_sum[i + lane]);
+    most = __reduce_max_sync(0xffffffffu, most);
     const int shift = max(0, 32 - __clz(most) - 7), half = 1 << shift >> 1;
     if (tid < 2 * kD) {
-      const int v = min((s_sum[tid] + half) >> shift, 127);
-      s_q[tid] = (int8_t)(tid < kD ? v : -v);
+      const int y = min((s_sum[tid] + half) >> shift, 127);
+      s_q[tid] = (int8_t)(tid < kD ? y : -y);
+    }
+  }
+  // (the first CTA of the cluster is there: its memory may be written to)
+  if constexpr (kParts) cluster_sync();
+  else __syncthreads();
+  // ---- scores
+  const int front = min(p.front, n), own = max(front, (max(first, 0) >> p.log_block) - (p.recent - 1));
+  {
+    uint4 mine[kParcels];
+#pragma unroll
+    for (int r = 0; r < kParcels; ++r) mine[r] = *reinterpret_cast<const uint4*>(s_q + 16 * (4 * r + c));
+    uint32_t least = 0xffffffffu, most = 0u;
+#pragma unroll 1
+    for (int j0 = b0 + warp * 8; j0 < b1; j0 += kDeep * kRound) {
+      uint32_t key[kDeep];
+#pragma unroll
+      for (int k = 0; k < kDeep; ++k) {
+        int dot = 0;
+#pragma unroll
+        for (int r = 0; r < kParcels; ++r) {
+          dot = __dp4a((int)v[k][r].x, (int)mine[r].x, dot);
+          dot = __dp4a((int)v[k][r].y, (int)mine[r].y, dot);
+          dot = __dp4a((int)v[k][r].z, (int)mine[r].z, dot);
+          dot = __dp4a((int)v[k][r].w, (int)mine[r].w, dot);
+        }
+        dot += __shfl_xor_sync(0xffffffffu, dot, 1);
+        dot += __shfl_xor_sync(0xffffffffu, dot, 2);
+        key[k] = score_key(scale[k] == -INFINITY ? -INFINITY : __fmul_rn((float)dot, scale[k]));
+      }
+      if (j0 + kDeep * kRound < b1) fetch(j0 + kDeep * kRound);
+#pragma unroll
+      for (int k = 0; k < kDeep; ++k) {
+        const int j = j0 + k * kRound + sub;
+        if (c == 0 && j < b1) {
+          if (j >= front && j < own) {
+            least = min(least, key[k]);
+            most = max(most, key[k]);
+          } else {
+            key[k] = kAlways;
+          }
+          if (kParts && part > 0) st_cluster_u32(smem_u32(s_key + j), 0, key[k]);
+          else s_key[j] = key[k];
+        }
+      }
+    }
+    least = __reduce_min_sync(0xffffffffu, least);
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0 && least <= most) {
+      atomicMin(&s_range[2 * part], least);
+      atomicMax(&s_range[2 * part + 1], most);
     }
   }
   __syncthreads();
-  // ---- scores
-  {
-    constexpr int kLanes = kD / 8, kPer = 32 / kLanes;           // lanes of a block's 2 D bytes
-    const int sub = lane / kLanes, c = lane % kLanes;
-    const uint4 mine = *reinterpret_cast<const uint4*>(s_q + 16 * c);
-    const int own = max(0, (max(first, 0) >> p.log_block) - (p.recent - 1));
-    const int log_per = p.log_block;
-#pragma unroll 4
-    for (int j0 = warp * kPer; j0 < n; j0 += kWarps * kPer) {
-      const int j = j0 + sub;
-      int dot = 0;
-      float scale = 0.f;
-      bool fine = j < n;
-      if (fine) {
-        const int key = j << log_per, pg = fast_div(key, p.div_page), off = key - pg * p.page_size;
-        const int page = p.table != nullptr ? p.table[(int64_t)b * p.pages_per_seq + pg] : b;
-        fine = page >= 0 && page < p.num_pages;
-        if (fine) {
-          const int64_t at = ((int64_t)page * (p.page_size >> p.log_block) + (off >> p.log_block)) * p.Hkv + head;
-          const uint4 v = *reinterpret_cast<const uint4*>(p.bounds + at * (2 * kD) + 16 * c);
-          scale = p.scale[at];
-          dot = __dp4a((int)v.x, (int)mine.x, dot);
-          dot = __dp4a((int)v.y, (int)mine.y, dot);
-          dot = __dp4a((int)v.z, (int)mine.z, dot);
-          dot = __dp4a((int)v.w, (int)mine.w, dot);
-        } else if (c == 0) {
-          report_bad_index(p.status, p.epoch, kPageSite);
-        }
-      }
-#pragma unroll
-      for (int o = 1; o < kLanes; o <<= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-      if (c == 0 && j < n) s_key[j] = j < p.front || j >= own ? kAlways : score_key(fine ? __fmul_rn((float)dot, scale) : -INFINITY);
+  uint32_t lo = 0xffffffffu, hi = 0u;
+  if constexpr (kParts) {
+    if (part > 0 && tid < 2) st_cluster_u32(smem_u32(s_range + 2 * part + tid), 0, s_range[2 * part + tid]);
+    cluster_sync();
+    if (part > 0) return;
+    for (int i = 0; i < p.parts; ++i) {
+      lo = min(lo, s_range[2 * i]);
+      hi = max(hi, s_range[2 * i + 1]);
     }
+  } else {
+    lo = s_range[0];
+    hi = s_range[1];
   }
-  // ---- the chosen'th largest key, eight bits at a time
-  if (tid == 0) {
-    s_prefix = 0u;
-    s_left = p.chosen;
-  }
+  // ---- what is chosen: keys from `from` on, and of those equal to `edge` the first `ties`.  A pass deals the keys of a range to 2048 bins: scores of one
+  //      kind spread over them, and two passes do mostly (with the keys' bits, eight at a time, four, whose first counts all in a few bins).
+  uint32_t from = kAlways, edge = 0u;
+  int ties = 0, left = p.chosen - (front + n - own);
 #pragma unroll 1
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    s_hist[tid] = 0;
-    static_assert(kSelectThreads == 256, "a thread a bin");
+  while (left > 0) {
+    const int shift = max(0, 32 - __clz((int)(hi - lo)) - 11);
+    for (int i = tid; i < kBins; i += kSelectThreads) s_hist[i] = 0;
     __syncthreads();
-    const uint32_t prefix = s_prefix;
-    for (int i = tid; i < n; i += kSelectThreads) {
+    for (int i = front + tid; i < own; i += kSelectThreads) {
       const uint32_t key = s_key[i];
-      if (shift == 24 || key >> (shift + 8) == prefix) atomicAdd(&s_hist[(key >> shift) & 255u], 1);
+      if (key >= lo && key <= hi) atomicAdd(&s_hist[(key - lo) >> shift], 1);
     }
     __syncthreads();
-    if (warp == 0) {
-      // bins from the largest on: lane l has 255 - 8 l and the seven below
-      int own[8], sum = 0;
+    // bins from the largest on, four a thread
+    const int4 h = *reinterpret_cast<const int4*>(s_hist + kBins - 4 - 4 * tid);
+    static_assert(kBins == 4 * kSelectThreads, "four bins a thread");
+    const int sum = h.x + h.y + h.z + h.w;
+    int upto = sum;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) sum += own[k] = s_hist[255 - 8 * lane - k];
-      int upto = sum;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += v;
-      }
-      const int left = s_left;
-      int before = upto - sum;
-      if (before < left && upto >= left) {                         // (one lane)
-        int k = 0;
-        while (before + own[k] < left) before += own[k++];
-        s_prefix = prefix << 8 | (uint32_t)(255 - 8 * lane - k);
-        s_left = left - before;
-      }
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    if (lane == 31) s_red[warp] = upto;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) upto += s_red[w];
+    int before = upto - sum;
+    if (before < left && upto >= left) {                             // (one thread)
+      int bin = kBins - 1 - 4 * tid, here = h.w;
+      if (before + here < left) { before += here; here = h.z; --bin; }
+      if (before + here < left) { before += here; here = h.y; --bin; }
+      if (before + here < left) { before += here; here = h.x; --bin; }
+      s_bin[0] = bin;
+      s_bin[1] = left - before;
+      s_bin[2] = here;
     }
     __syncthreads();
+    const uint32_t start = lo + ((uint32_t)s_bin[0] << shift);
+    left = s_bin[1];
+    if (s_bin[2] == left) {
+      from = start;
+      break;
+    }
+    if (shift == 0) {
+      from = start + 1;
+      edge = start;
+      ties = left;
+      break;
+    }
+    lo = start;
+    hi = min(hi, start + ((1u << shift) - 1u));
   }
-  // ---- the list, by number: all above that key, and of those equal to it the first ones
-  const uint32_t edge = s_prefix;
-  const int ties = s_left, per = ((n + kWarps - 1) / kWarps + 31) & ~31, i0 = warp * per, i1 = min(n, i0 + per);
+  // ---- the list, by number
+  const int seg = ((n + kWarps - 1) / kWarps + 31) & ~31, i0 = warp * seg, i1 = min(n, i0 + seg);
   int above = 0, equal = 0;
   for (int i = i0 + lane; i < i1; i += 32) {
-    above += s_key[i] > edge;
-    equal += s_key[i] == edge;
+    above += s_key[i] >= from;
+    equal += ties > 0 && s_key[i] == edge;
   }
   above = __reduce_add_sync(0xffffffffu, above);
   equal = __reduce_add_sync(0xffffffffu, equal);
@@ -343,10 +433,10 @@ __global__ void __launch_bounds__(kSelectThreads) fp8_select_kernel(const __grid
   }
   for (int i = i0; i < i1; i += 32) {
     const uint32_t key = i + lane < i1 ? s_key[i + lane] : 0u;
-    const bool is_above = i + lane < i1 && key > edge, is_equal = i + lane < i1 && key == edge;
+    const bool is_above = i + lane < i1 && key >= from, is_equal = i + lane < i1 && ties > 0 && key == edge;
     const uint32_t am = __ballot_sync(0xffffffffu, is_above), em = __ballot_sync(0xffffffffu, is_equal), in_front = (1u << lane) - 1u;
-    const int a = a0 + __popc(am & in_front), q_at = e0 + __popc(em & in_front);
-    if (is_above || (is_equal && q_at < ties)) out[a + min(q_at, ties)] = i + lane;
+    const int a = a0 + __popc(am & in_front), tie = e0 + __popc(em & in_front);
+    if (is_above || (is_equal && tie < ties)) out[a + min(tie, ties)] = i + lane;
     a0 += __popc(am);
     e0 += __popc(em);
   }
