@@ -12,7 +12,8 @@ struct Fp8Params {
   const float *k_scale, *v_scale;
   const int32_t *used, *fresh, *table;
   const float* sink;
-  int num_splits;                    // 0: dealt by the lengths (decode kernel)
+  int num_splits;                    // 0: dealt by the lengths (decode kernel); -1: whole units (chosen blocks)
+  int meet;                          // chosen blocks: CTAs of a cluster, whose splits of a unit meet in shared memory; else 1
   float* o_partial;                  // rows of D fp32, normalised; log2 of their sums, the sink left out
   float* lse_partial;                //   many rows: (splits, B, Sq, Hq); decode: (slots, unit_rows)
   int2* pieces;                      // decode, dealt: (B, Hkv) first CTA and number of pieces of a unit
@@ -153,10 +154,10 @@ __device__ __forceinline__ RowEnd finish_row(float m, float l, const float* sink
   return e;
 }
 
-// Merge of a row's partial results by one warp; at(i): index of the i-th one's row.
+// Merge of a row's n partial results by one warp; sum_of(i), values_of(i): the log2 of the i-th one's sum, four of its values.
 constexpr int kFp8CombineWarps = 4;
-template <class At>
-__device__ __forceinline__ void merge_row(const Fp8Params& p, int b, int s, int h, int lane, int n, At at) {
+template <class SumOf, class ValuesOf>
+__device__ __forceinline__ void merge_parts(const Fp8Params& p, int b, int s, int h, int lane, int n, SumOf sum_of, ValuesOf values_of) {
   const int col = 4 * lane;
   float m = -INFINITY, sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -168,8 +169,8 @@ __device__ __forceinline__ void merge_row(const Fp8Params& p, int b, int s, int 
       l[j] = -INFINITY;
       v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (i0 + j < n) {
-        l[j] = p.lse_partial[at(i0 + j)];
-        if (col < p.D) v[j] = *reinterpret_cast<const float4*>(p.o_partial + at(i0 + j) * p.D + col);
+        l[j] = sum_of(i0 + j);
+        if (col < p.D) v[j] = values_of(i0 + j);
       }
     }
 #pragma unroll
@@ -197,6 +198,12 @@ __device__ __forceinline__ void merge_row(const Fp8Params& p, int b, int s, int 
     *reinterpret_cast<uint2*>(p.out + b * p.o_b + s * p.o_s + h * p.o_h + col) =
         make_uint2(pack_bf16x2(acc.x * up, acc.y * up), pack_bf16x2(acc.z * up, acc.w * up));
   if (lane == 0 && p.lse != nullptr) p.lse[((int64_t)b * p.Hq + h) * p.Sq + s] = e.lse;
+}
+// The same from memory; at(i): index of the i-th one's row.
+template <class At>
+__device__ __forceinline__ void merge_row(const Fp8Params& p, int b, int s, int h, int lane, int n, At at) {
+  merge_parts(p, b, s, h, lane, n, [&](int i) { return p.lse_partial[at(i)]; },
+              [&](int i) { return *reinterpret_cast<const float4*>(p.o_partial + at(i) * p.D + 4 * lane); });
 }
 
 // The splits of the kernel for many rows: a warp a row.

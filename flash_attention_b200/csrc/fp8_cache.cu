@@ -148,6 +148,7 @@ struct Fp8Plan {
   int bundle;        // decode: kv heads side by side
   int row_tiles, cta_rows;   // many rows: tiles of 128 or 256
   int splits;        // 0: shares dealt on the device
+  int meet;          // chosen blocks, few rows: splits that meet in a cluster (else 1)
   int64_t slots;     // of partial results, and their rows
   int64_t slot_rows;
 };
@@ -180,6 +181,7 @@ void plan_many(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, const fa4_fp8_block
 }
 Fp8Plan plan_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, const fa4_fp8_blocks* x) {
   Fp8Plan plan = {};
+  plan.meet = 1;
   const int64_t rows = (int64_t)rows_of(f, x) * (f->Hq / c->Hkv), units = (int64_t)c->Hkv * seqs_of(f, x);
   // us, decode kernel / kernel for many rows: 8 sequences of five rows of 32 heads over up to 4099 keys 21 / 44, 32 of eight over up to 8192 75 / 225.
   // So the change is a step: the decode kernel's tensor memory and registers end at 32 rows, and 36 to 64 rows take 227 (128 rows 168, 256 rows 210), 44 on
@@ -190,13 +192,16 @@ Fp8Plan plan_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, const fa4_fp8_blo
     plan.splits = f->num_splits;
     // Dealing the shares and merging the pieces costs about as much as ten tiles.  us, dealt / a CTA a unit: 128 units of a window of nine
     // tiles, head dim 64 19.0 / 12.6, 8 units of seven tiles 10.5 / 9.2; but 256 units of up to 64 tiles 57.6 / 71.1.
+    if (x != nullptr)
+      while (plan.meet < 8 && units * plan.meet * 2 <= kSms && list_tiles(c, x) >= plan.meet * 2) plan.meet *= 2;
+    if (plan.meet > 1) plan.splits = plan.meet;
     if (plan.splits == 0 && units <= kSms && (x != nullptr ? list_tiles(c, x) : most_tiles(c, f, f->Sq)) <= 10) plan.splits = 1;
     // Many lists are about as long as each other: whole units, without a look at all lengths by every CTA and without a merge.
     if (x != nullptr && plan.splits == 0 && units >= 4 * kSms) plan.splits = -1;
     // (us, up to 8 / 4 heads side by side, which are 144 / 148 CTAs: 32 sequences of up to 8192 keys 55 / 60, drafted tokens on pages of 16 29 / 32.5)
     // (heads choose blocks of their own: nothing lies side by side)
     for (plan.bundle = x != nullptr ? 1 : std::min(8, c->Hkv); c->Hkv % plan.bundle != 0;) --plan.bundle;
-    plan.slots = plan.splits == 0 ? 2 * kSms : plan.splits == 1 || plan.splits < 0 ? 0 : units * plan.splits;
+    plan.slots = plan.splits == 0 ? 2 * kSms : plan.splits == 1 || plan.splits < 0 || plan.meet > 1 ? 0 : units * plan.splits;
     plan.slot_rows = rows;
   } else {
     plan_many(c, f, x, &plan);
@@ -256,6 +261,7 @@ int run_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, const fa4_fp8_blocks* 
   p.table = c->page_table;
   p.sink = f->sink;
   p.num_splits = plan.splits;
+  p.meet = plan.meet;
   p.o_partial = static_cast<float*>(f->workspace);
   p.lse_partial = bytes > 0 ? p.o_partial + plan.slots * plan.slot_rows * c->D : nullptr;
   p.pieces = bytes > 0 ? reinterpret_cast<int2*>(p.lse_partial + (plan.slots * plan.slot_rows + 1) / 2 * 2) : nullptr;
@@ -305,7 +311,7 @@ int run_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, const fa4_fp8_blocks* 
     p.div_groups = make_fastdiv((uint32_t)(kSms / plan.bundle));
     auto launch = [&](auto form) -> int {
       using F = decltype(form);
-      return launch_pdl(fp8_decode_kernel<F>, dim3((unsigned)grid), F::kThreads, F::kRequest, stream, tm_k, tm_v, p);
+      return launch_pdl_cluster((unsigned)plan.meet, fp8_decode_kernel<F>, dim3((unsigned)grid), F::kThreads, F::kRequest, stream, tm_k, tm_v, p);
     };
     using fp8d::Form;
     auto launch_rows = [&](auto capped) -> int {
@@ -314,7 +320,7 @@ int run_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, const fa4_fp8_blocks* 
       return plan.rows == 16 ? launch(Form<64, 16, kCap, kBlocks>{}) : launch(Form<64, 32, kCap, kBlocks>{});
     };
     const int rc = cap ? launch_rows(std::true_type{}) : launch_rows(std::false_type{});
-    if (rc != 0 || plan.splits == 1 || plan.splits < 0) return rc;
+    if (rc != 0 || plan.splits == 1 || plan.splits < 0 || plan.meet > 1) return rc;
     return launch_pdl(fp8_merge_kernel<kBlocks>, dim3(merge_grid), kFp8CombineWarps * 32, 0, stream, p);
   }
   // (a launch needs the registers that the kernel's budget counts on: see ensure_kernel)

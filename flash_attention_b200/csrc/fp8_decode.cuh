@@ -860,6 +860,13 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
             *reinterpret_cast<uint2*>(p.out + b * p.o_b + (q0 + s) * p.o_s + h * p.o_h + col) =
                 make_uint2(pack_bf16x2(o.x * f * by, o.y * f * by), pack_bf16x2(o.z * f * by, o.w * f * by));
           if (lane == 0 && p.lse != nullptr) p.lse[((int64_t)b * p.Hq + h) * p.Sq + q0 + s] = e.lse;
+        } else if (kBlocks && p.meet > 1) {
+          // (the ring of keys is free: every product of the piece is done)
+          const bool none = m == -INFINITY && sum == 0.f;
+          const float f = none ? 0.f : rcp_approx(sum) * by;
+          if (col < kD)
+            *reinterpret_cast<float4*>(gbase + F::kOffK + (r * kD + col) * 4) = make_float4(o.x * f * by, o.y * f * by, o.z * f * by, o.w * f * by);
+          if (lane == 0) *reinterpret_cast<float*>(gbase + F::kOffK + (kR * kD + r) * 4) = none ? -INFINITY : m + lg2_approx(sum);
         } else {
           const bool none = m == -INFINITY && sum == 0.f;
           const float f = rcp_approx(sum) * by;
@@ -868,6 +875,26 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           if (lane == 0) p.lse_partial[slot * p.unit_rows + r] = none ? -INFINITY : m + lg2_approx(sum);
         }
       }
+    }
+  }
+  if constexpr (kBlocks) {
+    if (p.meet > 1) {
+      // The splits of the unit: a row a warp of one of the cluster's CTAs.  A CTA without a share wrote nothing; its rows have no sum.
+      const Seq seq = s_walk.cur;
+      const QueryBlock place = query_block_of<true>(p, s_walk.b);
+      const int R = seq.sq * p.group, rank = blockIdx.x % p.meet, hk = s_walk.hb;
+      const uint32_t part = base + F::kOffK;
+      if (s_walk.left == 0)
+        for (int r = tid; r < R; r += F::kThreads) *reinterpret_cast<float*>(gbase + F::kOffK + (kR * kD + r) * 4) = -INFINITY;
+      cluster_sync();
+      uint32_t gave_up = 0u;
+      for (int i = 0; i < p.meet; ++i) gave_up |= ld_cluster_u32(base + F::kOffMisc + 4, i);
+      for (int r = rank + p.meet * warp; r < R && gave_up == 0u; r += p.meet * (F::kThreads / 32)) {
+        const int s = fast_div(r, p.div_group), h = hk * p.group + r - s * p.group;
+        merge_parts(p, place.b, place.q0 + s, h, lane, p.meet, [&](int i) { return __uint_as_float(ld_cluster_u32(part + (kR * kD + r) * 4, i)); },
+                    [&](int i) { return ld_cluster_f4(part + (r * kD + 4 * lane) * 4, i); });
+      }
+      cluster_sync();
     }
   }
   tc_fence_before_sync();

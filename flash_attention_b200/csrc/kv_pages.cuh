@@ -390,24 +390,35 @@ __device__ __forceinline__ void copy_pieces(const PagedTensor& t, int from, int 
     if (at[j] >= 0) *reinterpret_cast<T*>(t.base + to * t.page + at[j]) = v[j];
 }
 
+// CTAs take the parts of all pairs in turn.  A warp looks up the pairs of its next 32 parts at a time, so a list that is mostly empty (one pair of many
+// rows, or a long tail) costs a memory latency for 32 of them.
 __global__ void __launch_bounds__(kCopyThreads) copy_kernel(const __grid_constant__ CopyParams p) {
+  const int lane = threadIdx.x & 31, per = p.first[p.tensors];
   pdl_wait();
-  const int per = p.first[p.tensors];
-  for (int64_t task = blockIdx.x; task < p.tasks; task += gridDim.x) {
-    const int pair = fast_div((int)task, p.div_tasks), part = (int)task - pair * per;
-    const int from = p.pairs[2 * pair], to = p.pairs[2 * pair + 1];
-    if (from < 0 || to < 0) continue;
-    if (from >= p.num_pages || to >= p.num_pages) {
-      if (threadIdx.x == 0) report_bad_index(p.status, p.epoch, kPairSite);
-      continue;
+  for (int64_t t0 = blockIdx.x; t0 < p.tasks; t0 += 32 * (int64_t)gridDim.x) {
+    const int64_t mine = t0 + lane * (int64_t)gridDim.x;
+    int2 pages = make_int2(-1, -1);
+    int part = 0;
+    if (mine < p.tasks) {
+      const int pair = fast_div((int)mine, p.div_tasks);
+      part = (int)mine - pair * per;
+      pages = make_int2(p.pairs[2 * pair], p.pairs[2 * pair + 1]);
+      if (pages.x >= 0 && pages.y >= 0 && (pages.x >= p.num_pages || pages.y >= p.num_pages)) {
+        report_bad_index(p.status, p.epoch, kPairSite);
+        pages.x = -1;
+      }
     }
-    int which = 0;
-    while (part >= p.first[which + 1]) ++which;
-    const PagedTensor& t = p.t[which];
-    const int i0 = (part - p.first[which]) * (kCopyThreads * kCopyPieces) + threadIdx.x;
-    if (t.log_piece == 4) copy_pieces<uint4>(t, from, to, i0);
-    else if (t.log_piece == 2) copy_pieces<uint32_t>(t, from, to, i0);
-    else copy_pieces<uint8_t>(t, from, to, i0);
+    for (uint32_t todo = __ballot_sync(0xffffffffu, pages.x >= 0 && pages.y >= 0); todo != 0u; todo &= todo - 1u) {
+      const int l = __ffs(todo) - 1;
+      const int from = __shfl_sync(0xffffffffu, pages.x, l), to = __shfl_sync(0xffffffffu, pages.y, l), at = __shfl_sync(0xffffffffu, part, l);
+      int which = 0;
+      while (at >= p.first[which + 1]) ++which;
+      const PagedTensor& t = p.t[which];
+      const int i0 = (at - p.first[which]) * (kCopyThreads * kCopyPieces) + threadIdx.x;
+      if (t.log_piece == 4) copy_pieces<uint4>(t, from, to, i0);
+      else if (t.log_piece == 2) copy_pieces<uint32_t>(t, from, to, i0);
+      else copy_pieces<uint8_t>(t, from, to, i0);
+    }
   }
 }
 
