@@ -196,8 +196,13 @@ Fp8Plan plan_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, const fa4_fp8_blo
       while (plan.meet < 8 && units * plan.meet * 2 <= kSms && list_tiles(c, x) >= plan.meet * 2) plan.meet *= 2;
     if (plan.meet > 1) plan.splits = plan.meet;
     if (plan.splits == 0 && units <= kSms && (x != nullptr ? list_tiles(c, x) : most_tiles(c, f, f->Sq)) <= 10) plan.splits = 1;
-    // Many lists are about as long as each other: whole units, without a look at all lengths by every CTA and without a merge.
-    if (x != nullptr && plan.splits == 0 && units >= 4 * kSms) plan.splits = -1;
+    // Lists are mostly as long as each other.  Whole units, without dealing and merging, where the CTAs that get one more than others have no more than five
+    // tiles more than an even share, or where every CTA would look at many lengths (0.35 us for 32).  us, dealt / whole: 256 units of 16 tiles (32 and 27.7 a CTA) 36.0 / 33.9, 320 of
+    // nine (27 and 19.5) 27.5 / 33.3.
+    if (x != nullptr && plan.splits == 0) {
+      const int64_t tiles = list_tiles(c, x);
+      if (seqs_of(f, x) > 512 || (units + kSms - 1) / kSms * tiles * kSms <= units * tiles + 5 * kSms) plan.splits = -1;
+    }
     // (us, up to 8 / 4 heads side by side, which are 144 / 148 CTAs: 32 sequences of up to 8192 keys 55 / 60, drafted tokens on pages of 16 29 / 32.5)
     // (heads choose blocks of their own: nothing lies side by side)
     for (plan.bundle = x != nullptr ? 1 : std::min(8, c->Hkv); c->Hkv % plan.bundle != 0;) --plan.bundle;
