@@ -27,6 +27,8 @@ Book book_of(const fa4_kv_pages* k) {
   b.div_page = make_fastdiv((uint32_t)k->page_size);
   b.status = k->status;
   b.epoch = next_launch_epoch();
+  // A few hundred numbers are one CTA's.  us, one / eight: 4 rows of 15 pages, pool of 92 6.1 / 7.4, 128 of 18, 1315 14.2 / 8.8, 256 of 66, 11761 28 / 9.9.
+  b.ctas = (int64_t)k->B * k->pages_per_seq + k->num_pages <= 1024 ? 1 : kCluster;
   return b;
 }
 int check_work(const void* work, uint64_t bytes, int64_t words) {
@@ -49,7 +51,7 @@ extern "C" int fa4_kv_pages_resize(const fa4_kv_pages* k, const int32_t* held, c
   if (!held || !wanted || !pairs) return -FA4_E_NULL;
   if (int e = check_work(workspace, workspace_bytes, need / 4)) return e;
   ResizeParams p = {book_of(k), held, wanted, pairs, static_cast<int32_t*>(workspace)};
-  return launch_pdl_cluster(kCluster, resize_kernel, dim3(kCluster), kThreads, 0, static_cast<cudaStream_t>(cuda_stream), p);
+  return launch_pdl_cluster((unsigned)p.book.ctas, resize_kernel, dim3((unsigned)p.book.ctas), kThreads, 0, static_cast<cudaStream_t>(cuda_stream), p);
 }
 
 extern "C" int fa4_kv_pages_fork(const fa4_kv_pages* k, const int32_t* held, const int32_t* parents, int32_t rows, int32_t* new_table,
@@ -72,7 +74,7 @@ extern "C" int fa4_kv_pages_compact(const fa4_kv_pages* k, int32_t* pairs, int32
   if ((!pairs && k->num_pages > 1) || !used) return -FA4_E_NULL;
   if (int e = check_work(workspace, workspace_bytes, need / 4)) return e;
   CompactParams p = {book_of(k), pairs, used, static_cast<int32_t*>(workspace)};
-  return launch_pdl_cluster(kCluster, compact_kernel, dim3(kCluster), kThreads, 0, static_cast<cudaStream_t>(cuda_stream), p);
+  return launch_pdl_cluster((unsigned)p.book.ctas, compact_kernel, dim3((unsigned)p.book.ctas), kThreads, 0, static_cast<cudaStream_t>(cuda_stream), p);
 }
 
 extern "C" int fa4_kv_pages_copy(const fa4_kv_copy* c, void* cuda_stream) {

@@ -10,7 +10,7 @@
 namespace fa4 {
 namespace pages {
 
-constexpr int kCluster = 8, kThreads = 1024, kWarps = kThreads / 32;
+constexpr int kCluster = 8, kThreads = 1024, kWarps = kThreads / 32;        // (at most so many CTAs)
 constexpr int kRows = 4096;                    // of a table: their prefix sums stay in shared memory
 
 enum Site { kTableSite = 123, kLengthSite = 124, kPoolSite = 125, kParentSite = 126, kPairSite = 127 };
@@ -19,6 +19,7 @@ struct Book {
   int32_t* table;
   int32_t* refs;
   int B, width, num_pages, page_size;
+  int ctas;                          // of the cluster
   FastDiv div_page;
   uint32_t* status;
   uint32_t epoch;
@@ -34,9 +35,10 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   return r;
 }
 // Rendezvous of the cluster behind which everything that was written before it, global memory included, can be read (by __ldcg).
-__device__ __forceinline__ void meet() {
+__device__ __forceinline__ void meet(const Book& p) {
   __threadfence();
-  cluster_sync();
+  if (p.ctas > 1) cluster_sync();
+  else __syncthreads();
 }
 
 // Exclusive prefix sum over the CTA's warps of a value of each; `all`: the sum.  s: kWarps + 1 words.
@@ -65,29 +67,31 @@ __device__ __forceinline__ int scan_warps(int mine, int* s, int* all) {
 struct Part {
   int from, to;
 };
-__device__ __forceinline__ Part part_of(int num_pages) {
-  const int per = ((num_pages + kCluster * kWarps - 1) / (kCluster * kWarps) + 31) & ~31;
+__device__ __forceinline__ Part part_of(const Book& p) {
+  const int warps = p.ctas * kWarps, per = ((p.num_pages + warps - 1) / warps + 31) & ~31;
   const int w = (int)cluster_rank() * kWarps + (threadIdx.x >> 5);
   const int64_t from = (int64_t)w * per;
-  return {(int)min(from, (int64_t)num_pages), (int)min(from + per, (int64_t)num_pages)};
+  return {(int)min(from, (int64_t)p.num_pages), (int)min(from + per, (int64_t)p.num_pages)};
 }
-// Calls what(page, mask of the lanes with pages that are(refs of page)) for 32 pages at a time.
-template <class Are, class What>
-__device__ __forceinline__ void over_pages(const Book& p, Part part, Are are, What what) {
+// Calls what(page of the lane, mask of the lanes whose page is in use) for 32 pages at a time, up to the end of the part (lanes behind it count as in
+// use).  Eight groups are on their way together.
+template <class What>
+__device__ __forceinline__ void over_pages(const Book& p, Part part, What what) {
   const int lane = threadIdx.x & 31;
-#pragma unroll 4
-  for (int i0 = part.from; i0 < part.to; i0 += 32) {
-    const int i = i0 + lane;
-    const int r = i < part.to ? __ldcg(p.refs + i) : 1;
-    what(i, __ballot_sync(0xffffffffu, i < part.to && are(i, r)));
+#pragma unroll 1
+  for (int i0 = part.from; i0 < part.to; i0 += 256) {
+    int r[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int i = i0 + 32 * k + lane;
+      r[k] = i < part.to ? __ldcg(p.refs + i) : 1;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (i0 + 32 * k < part.to) what(i0 + 32 * k + lane, __ballot_sync(0xffffffffu, r[k] > 0));
   }
 }
-template <class Are>
-__device__ __forceinline__ int count_pages(const Book& p, Part part, Are are) {
-  int n = 0;
-  over_pages(p, part, are, [&](int, uint32_t mask) { n += __popc(mask); });
-  return n;
-}
+__device__ __forceinline__ uint32_t lanes_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 
 struct ResizeParams {
   Book book;
@@ -115,7 +119,7 @@ __device__ __forceinline__ Lengths lengths_of(const ResizeParams& p, int b, bool
 __global__ void __launch_bounds__(kThreads) resize_kernel(const __grid_constant__ ResizeParams p) {
   __shared__ int s_first[kRows], s_scan[kWarps + 1];
   const Book& k = p.book;
-  const int rank = (int)cluster_rank(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row0 = rank * kWarps + warp, step = kCluster * kWarps;
+  const int rank = (int)cluster_rank(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row0 = rank * kWarps + warp, step = k.ctas * kWarps;
   int32_t *writes = p.work, *lacks = writes + k.B, *free_of = lacks + k.B, *free_page = free_of + kCluster;
   pdl_wait();
   // ---- what is given back; what is missing
@@ -124,28 +128,35 @@ __global__ void __launch_bounds__(kThreads) resize_kernel(const __grid_constant_
     const int keep = pages_of(k, min(n.held, n.wanted)), want = pages_of(k, n.wanted), at = fast_div(n.held, k.div_page);
     int32_t* row = k.table + (int64_t)b * k.width;
     int missing = max(want - keep, 0), page = -1;
-    for (int j0 = 0; j0 < k.width; j0 += 32) {
-      const int j = j0 + lane;
-      int e = j < k.width ? row[j] : 0;
-      if (e >= k.num_pages) {
-        report_bad_index(k.status, k.epoch, kTableSite);
-        e = -1;
-        row[j] = -1;
+#pragma unroll 1
+    for (int j1 = 0; j1 < k.width; j1 += 128) {
+      int entry[4];                            // (asked for together)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) entry[i] = j1 + 32 * i + lane < k.width ? row[j1 + 32 * i + lane] : 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int j0 = j1 + 32 * i, j = j0 + lane;
+        int e = entry[i];
+        if (e >= k.num_pages) {
+          report_bad_index(k.status, k.epoch, kTableSite);
+          e = -1;
+          row[j] = -1;
+        }
+        if (j < k.width && j >= keep && e >= 0) {
+          atomicSub(k.refs + e, 1);
+          row[j] = -1;
+        }
+        missing += __popc(__ballot_sync(0xffffffffu, j < keep && e < 0));
+        // (a row that grows keeps the page its next token goes to)
+        if (j0 <= at && at < j0 + 32) page = __shfl_sync(0xffffffffu, e, at & 31);
       }
-      if (j < k.width && j >= keep && e >= 0) {
-        atomicSub(k.refs + e, 1);
-        row[j] = -1;
-      }
-      missing += __popc(__ballot_sync(0xffffffffu, j < keep && e < 0));
-      // (a row that grows keeps the page its next token goes to)
-      if (j0 <= at && at < j0 + 32) page = __shfl_sync(0xffffffffu, e, at & 31);
     }
     if (lane == 0) {
       writes[b] = n.wanted > n.held && n.held != at * k.page_size && page >= 0 ? page : -1;
       lacks[b] = missing;
     }
   }
-  meet();
+  meet(k);
   // ---- who gets a copy: all but the last of a page's entries
   for (int b = row0; b < k.B; b += step) {
     const int page = __ldcg(writes + b);
@@ -161,11 +172,12 @@ __global__ void __launch_bounds__(kThreads) resize_kernel(const __grid_constant_
     }
   }
   // ---- the free pages, counted
-  const Part part = part_of(k.num_pages);
-  auto is_free = [](int, int r) { return r == 0; };
-  int here, before = scan_warps(count_pages(k, part, is_free), s_scan, &here);
+  const Part part = part_of(k);
+  int here, before = 0;
+  over_pages(k, part, [&](int, uint32_t used) { before += __popc(~used); });
+  before = scan_warps(before, s_scan, &here);
   if (threadIdx.x == 0) free_of[rank] = here;
-  meet();
+  meet(k);
   // ---- where a row's new pages lie in the list of all that are wanted
   int total, free_pages = 0;
   {
@@ -189,20 +201,20 @@ __global__ void __launch_bounds__(kThreads) resize_kernel(const __grid_constant_
       at += mine[i];
     }
   }
-  for (int r = 0; r < kCluster; ++r) {
+  for (int r = 0; r < k.ctas; ++r) {
     if (r < rank) before += __ldcg(free_of + r);
     free_pages += __ldcg(free_of + r);
   }
   if (before < total)
-    over_pages(k, part, is_free, [&](int page, uint32_t mask) {
-      const int at = before + __popc(mask & ((1u << lane) - 1u));
-      if ((mask >> lane & 1u) != 0u && at < total) {
+    over_pages(k, part, [&](int page, uint32_t used) {
+      const int at = before + __popc(~used & ((1u << lane) - 1u));
+      if ((used >> lane & 1u) == 0u && at < total) {
         free_page[at] = page;
         k.refs[page] = 1;
       }
-      before += __popc(mask);
+      before += __popc(~used);
     });
-  meet();
+  meet(k);
   // ---- the rows are filled
   for (int b = row0; b < k.B; b += step) {
     const int copied = __ldcg(writes + b);
@@ -211,7 +223,8 @@ __global__ void __launch_bounds__(kThreads) resize_kernel(const __grid_constant_
     const int want = pages_of(k, n.wanted), at = copies ? fast_div(n.held, k.div_page) : -1;
     int32_t* row = k.table + (int64_t)b * k.width;
     int next = s_first[b], fresh = -1;
-    for (int j0 = 0; j0 < want; j0 += 32) {
+    const int last = next + __ldcg(lacks + b);
+    for (int j0 = 0; j0 < want && next < last; j0 += 32) {
       const int j = j0 + lane;
       const bool lack = j < want && (j == at || row[j] < 0);
       const uint32_t mask = __ballot_sync(0xffffffffu, lack);
@@ -297,22 +310,29 @@ __global__ void __launch_bounds__(kThreads) compact_kernel(const __grid_constant
   const int rank = (int)cluster_rank(), lane = threadIdx.x & 31, all = rank * kThreads + threadIdx.x;
   int32_t *live_of = p.work, *holes_of = live_of + kCluster, *movers_of = holes_of + kCluster, *to = movers_of + kCluster;
   pdl_wait();
-  const Part part = part_of(k.num_pages);
-  int here;
-  scan_warps(count_pages(k, part, [](int, int r) { return r > 0; }), s_scan, &here);
+  const Part part = part_of(k);
+  int here, live = 0;
+  over_pages(k, part, [&](int page, uint32_t in_use) { live += __popc(in_use & lanes_below(part.to - (page - lane))); });
+  scan_warps(live, s_scan, &here);
   if (threadIdx.x == 0) live_of[rank] = here;
-  meet();
+  meet(k);
   int used = 0;
-  for (int r = 0; r < kCluster; ++r) used += __ldcg(live_of + r);
-  auto is_hole = [used](int i, int r) { return r <= 0 && i < used; };
-  auto is_mover = [used](int i, int r) { return r > 0 && i >= used; };
-  int hole = scan_warps(count_pages(k, part, is_hole), s_scan, &here);
+  for (int r = 0; r < k.ctas; ++r) used += __ldcg(live_of + r);
+  // lanes of a group whose page is free and below `used`; in use and not below
+  auto holes_in = [&](int page0, uint32_t in_use) { return ~in_use & lanes_below(used - page0); };
+  auto movers_in = [&](int page0, uint32_t in_use) { return in_use & ~lanes_below(used - page0) & lanes_below(part.to - page0); };
+  int hole = 0, mover = 0;
+  over_pages(k, part, [&](int page, uint32_t in_use) {
+    hole += __popc(holes_in(page - lane, in_use));
+    mover += __popc(movers_in(page - lane, in_use));
+  });
+  hole = scan_warps(hole, s_scan, &here);
   if (threadIdx.x == 0) holes_of[rank] = here;
-  int mover = scan_warps(count_pages(k, part, is_mover), s_scan, &here);
+  mover = scan_warps(mover, s_scan, &here);
   if (threadIdx.x == 0) movers_of[rank] = here;
-  meet();
+  meet(k);
   int moved = 0;
-  for (int r = 0; r < kCluster; ++r) {
+  for (int r = 0; r < k.ctas; ++r) {
     if (r < rank) {
       hole += __ldcg(holes_of + r);
       mover += __ldcg(movers_of + r);
@@ -320,31 +340,40 @@ __global__ void __launch_bounds__(kThreads) compact_kernel(const __grid_constant
     moved += __ldcg(movers_of + r);
   }
   const uint32_t in_front = (1u << lane) - 1u;
-  over_pages(k, part, is_hole, [&](int page, uint32_t mask) {
-    if ((mask >> lane & 1u) != 0u) p.pairs[2 * (hole + __popc(mask & in_front)) + 1] = page;
-    hole += __popc(mask);
-  });
-  over_pages(k, part, is_mover, [&](int page, uint32_t mask) {
-    const bool goes = (mask >> lane & 1u) != 0u;
-    if (goes) p.pairs[2 * (mover + __popc(mask & in_front))] = page;
+  over_pages(k, part, [&](int page, uint32_t in_use) {
+    const uint32_t holes = holes_in(page - lane, in_use), movers = movers_in(page - lane, in_use);
+    if ((holes >> lane & 1u) != 0u) p.pairs[2 * (hole + __popc(holes & in_front)) + 1] = page;
+    if ((movers >> lane & 1u) != 0u) p.pairs[2 * (mover + __popc(movers & in_front))] = page;
     else if (page >= used && page < part.to) to[page] = page;
-    mover += __popc(mask);
+    hole += __popc(holes);
+    mover += __popc(movers);
   });
-  for (int i = moved + all; i < k.num_pages / 2; i += kCluster * kThreads) p.pairs[2 * i] = p.pairs[2 * i + 1] = -1;
+  for (int i = moved + all; i < k.num_pages / 2; i += k.ctas * kThreads) p.pairs[2 * i] = p.pairs[2 * i + 1] = -1;
   if (all == 0) *p.used = used;
-  meet();
-  for (int i = all; i < moved; i += kCluster * kThreads) {
+  meet(k);
+#pragma unroll 4
+  for (int i = all; i < moved; i += k.ctas * kThreads) {
     const int from = __ldcg(p.pairs + 2 * i), at = __ldcg(p.pairs + 2 * i + 1);
     k.refs[at] = __ldcg(k.refs + from);
     k.refs[from] = 0;
     to[from] = at;
   }
-  meet();
-  const int64_t entries = (int64_t)k.B * k.width;
-  for (int64_t i = all; i < entries; i += kCluster * kThreads) {
-    const int e = k.table[i];
-    if (e >= k.num_pages) report_bad_index(k.status, k.epoch, kTableSite);
-    else if (e >= used) k.table[i] = __ldcg(to + e);
+  meet(k);
+  // the table, eight entries of a thread on their way together
+  const int64_t entries = (int64_t)k.B * k.width, step = (int64_t)k.ctas * kThreads;
+#pragma unroll 1
+  for (int64_t i0 = all; i0 < entries; i0 += 8 * step) {
+    int e[8], at[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) e[j] = i0 + j * step < entries ? k.table[i0 + j * step] : -1;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (e[j] >= k.num_pages) report_bad_index(k.status, k.epoch, kTableSite);
+      at[j] = e[j] >= used && e[j] < k.num_pages ? __ldcg(to + e[j]) : -1;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (at[j] >= 0) k.table[i0 + j * step] = at[j];
   }
 }
 
