@@ -68,26 +68,33 @@ __global__ void __launch_bounds__(kIndexWarps * 32) fp8_index_kernel(const __gri
     hi[i] = __hneg2(inf);
     lo[i] = inf;
   }
-#pragma unroll 4
-  for (int r = row0; r < there; r += kRows) {
-    const uint4 u = *reinterpret_cast<const uint4*>(src + r * p.k_tok);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll 1
+  for (int r0 = row0; r0 < there; r0 += 4 * kRows) {
+    uint4 u[4];                                  // (on their way together)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t x[2];
-      asm("{\n"
-          ".reg .b16 l, h;\n"
-          "mov.b32 {l, h}, %2;\n"
-          "cvt.rn.f16x2.e4m3x2 %0, l;\n"
-          "cvt.rn.f16x2.e4m3x2 %1, h;\n"
-          "}\n"
-          : "=r"(x[0]), "=r"(x[1])
-          : "r"(w[i]));
+    for (int q = 0; q < 4; ++q)
+      if (r0 + q * kRows < there) u[q] = *reinterpret_cast<const uint4*>(src + (r0 + q * kRows) * p.k_tok);
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const __half2 v = *reinterpret_cast<const __half2*>(&x[k]);
-        hi[2 * i + k] = __hmax2_nan(hi[2 * i + k], v);       // (NaN stays in the maximum)
-        lo[2 * i + k] = __hmin2(lo[2 * i + k], v);
+    for (int q = 0; q < 4; ++q) {
+      if (r0 + q * kRows >= there) break;
+      const uint32_t w[4] = {u[q].x, u[q].y, u[q].z, u[q].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t x[2];
+        asm("{\n"
+            ".reg .b16 l, h;\n"
+            "mov.b32 {l, h}, %2;\n"
+            "cvt.rn.f16x2.e4m3x2 %0, l;\n"
+            "cvt.rn.f16x2.e4m3x2 %1, h;\n"
+            "}\n"
+            : "=r"(x[0]), "=r"(x[1])
+            : "r"(w[i]));
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const __half2 v = *reinterpret_cast<const __half2*>(&x[k]);
+          hi[2 * i + k] = __hmax2_nan(hi[2 * i + k], v);       // (NaN stays in the maximum)
+          lo[2 * i + k] = __hmin2(lo[2 * i + k], v);
+        }
       }
     }
   }
