@@ -191,6 +191,8 @@ __global__ void __launch_bounds__(kSelectThreads, 2) fp8_select_kernel(const __g
   const int unit = kParts ? blockIdx.x / p.parts : blockIdx.x, part = kParts ? blockIdx.x - unit * p.parts : 0;
   const int rest = fast_div(unit, p.div_hkv), head = unit - rest * p.Hkv, b = fast_div(rest, p.div_query_blocks),
             q0 = (rest - b * p.query_blocks) * p.query_block;
+  // (the attention's CTAs may take an SM as soon as this one's leave it, and set themselves up; with clusters that delayed those: 13.8 -> 15.2 us)
+  if constexpr (!kParts) pdl_trigger();
   pdl_wait();
   int sk = p.used[b], sq = p.fresh != nullptr ? p.fresh[b] : p.Sq;
   sk = sk < 0 ? 0 : (sk < p.capacity ? sk : p.capacity);

@@ -82,13 +82,9 @@ extern "C" int fa4_kv_pages_copy(const fa4_kv_copy* c, void* cuda_stream) {
   if (c->struct_size != sizeof(fa4_kv_copy)) return -FA4_E_STRUCT;
   if (!c->pairs) return -FA4_E_NULL;
   if (c->num_pairs <= 0 || c->num_pages <= 0 || c->num_tensors <= 0 || c->num_tensors > kTensors) return -FA4_E_SHAPE;
-  CopyParams p = {};
-  p.pairs = c->pairs;
-  p.n = c->num_pairs; p.num_pages = c->num_pages;
-  p.tensors = c->num_tensors;
-  p.status = c->status;
-  p.epoch = next_launch_epoch();
-  int64_t tasks = 0;
+  PagedTensor all[kTensors];
+  int64_t flat_bytes = 0;                     // of a page, in tensors whose pages lie in one piece
+  auto flat = [](const PagedTensor& t) { return t.log_piece == 4 && t.row == t.pieces; };
   for (int i = 0; i < c->num_tensors; ++i) {
     const fa4_kv_paged& s = c->tensors[i];
     if (!s.base) return -FA4_E_NULL;
@@ -96,12 +92,12 @@ extern "C" int fa4_kv_pages_copy(const fa4_kv_copy* c, void* cuda_stream) {
     // strides of what there is one of are never used
     const int64_t inner = s.rows_inner > 1 ? s.stride_inner : 0, outer = s.rows_outer > 1 ? s.stride_outer : 0, page = c->num_pages > 1 ? s.stride_page : 0;
     if (inner < 0 || outer < 0 || page < 0) return -FA4_E_STRIDE;
-    const uint64_t all = (uint64_t)(uintptr_t)s.base | (uint64_t)s.row_bytes | (uint64_t)inner | (uint64_t)outer | (uint64_t)page;
-    const int log_piece = (all & 15u) == 0 ? 4 : (all & 3u) == 0 ? 2 : 0;
+    const uint64_t bits = (uint64_t)(uintptr_t)s.base | (uint64_t)s.row_bytes | (uint64_t)inner | (uint64_t)outer | (uint64_t)page;
+    const int log_piece = (bits & 15u) == 0 ? 4 : (bits & 3u) == 0 ? 2 : 0;
     if (s.row_bytes > 0x7fffffffll || s.rows_inner > 0x7fffffffll || s.rows_outer > 0x7fffffffll) return -FA4_E_TOO_LARGE;
     const int64_t rows = s.rows_inner * s.rows_outer, row = s.row_bytes >> log_piece;
     if (rows > 0x3fffffffll || rows * row > 0x3fffffffll) return -FA4_E_TOO_LARGE;
-    PagedTensor& t = p.t[i];
+    PagedTensor& t = all[i];
     t.base = static_cast<uint8_t*>(s.base);
     t.page = page; t.inner = inner; t.outer = outer;
     t.pieces = (int)(rows * row);
@@ -110,13 +106,37 @@ extern "C" int fa4_kv_pages_copy(const fa4_kv_copy* c, void* cuda_stream) {
     t.rows_inner = (int)s.rows_inner;
     t.div_row = make_fastdiv((uint32_t)row);
     t.div_inner = make_fastdiv((uint32_t)s.rows_inner);
-    p.first[i] = (int)tasks;
-    tasks += (t.pieces + kCopyThreads * kCopyPieces - 1) / (kCopyThreads * kCopyPieces);
+    if (flat(t)) flat_bytes += (int64_t)t.pieces * 16;
   }
-  p.first[c->num_tensors] = (int)tasks;
-  p.div_tasks = make_fastdiv((uint32_t)tasks);
-  p.tasks = tasks * c->num_pairs;
-  if (p.tasks > 0x3fffffffll) return -FA4_E_TOO_LARGE;
-  const unsigned grid = (unsigned)std::min<int64_t>(p.tasks, kSms * 8);
-  return launch_pdl(copy_kernel, dim3(grid), kCopyThreads, 0, static_cast<cudaStream_t>(cuda_stream), p);
+  // From 64 MB on (the pairs that are none among them, which only the device can tell) by bulk copies, the rest of the tensors by a launch of its own.
+  const bool bulk = flat_bytes * c->num_pairs >= (64ll << 20);
+  CopyParams parts[2] = {};
+  for (const bool by_bulk : {true, false}) {
+    CopyParams& p = parts[by_bulk ? 0 : 1];
+    p.pairs = c->pairs;
+    p.n = c->num_pairs; p.num_pages = c->num_pages;
+    int64_t tasks = 0;
+    for (int i = 0; i < c->num_tensors; ++i) {
+      if ((bulk && flat(all[i])) != by_bulk) continue;
+      const int64_t per = by_bulk ? kBulkBytes / 16 : kCopyThreads * kCopyPieces;
+      p.first[p.tensors] = (int)tasks;
+      p.t[p.tensors++] = all[i];
+      tasks += (all[i].pieces + per - 1) / per;
+    }
+    p.first[p.tensors] = (int)tasks;
+    p.div_tasks = make_fastdiv((uint32_t)tasks);
+    p.tasks = tasks * c->num_pairs;
+    if (p.tasks > 0x3fffffffll) return -FA4_E_TOO_LARGE;
+    p.status = c->status;
+    p.epoch = next_launch_epoch();
+    p.budget_ns = kDefaultBudgetNs;
+  }
+  const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+  if (parts[0].tensors > 0) {
+    const unsigned grid = (unsigned)std::min<int64_t>(parts[0].tasks, kSms * kBulkCtas);
+    if (int e = launch_pdl(copy_bulk_kernel, dim3(grid), 32, kBulkRequest, stream, parts[0])) return e;
+  }
+  if (parts[1].tensors == 0) return 0;
+  const unsigned grid = (unsigned)std::min<int64_t>(parts[1].tasks, kSms * 8);
+  return launch_pdl(copy_kernel, dim3(grid), kCopyThreads, 0, stream, parts[1]);
 }

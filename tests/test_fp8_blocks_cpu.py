@@ -136,13 +136,15 @@ def test_bad_attention_over_blocks_is_refused(kw, more, rc):
 
 
 def test_a_workspace_that_is_none_is_refused():
+    """80 units of 25 tiles are dealt out to the CTAs, whose pieces need one; 2 of them are split among the CTAs of a cluster and need none."""
     L = fa.lib()
     L.fa4_fp8_cache_fwd_blocks_workspace_bytes.restype = ctypes.c_int64
     c, x = cache(pages_per_seq=100), blocks(num_blocks=100)
-    need = L.fa4_fp8_cache_fwd_blocks_workspace_bytes(ctypes.byref(c), ctypes.byref(fwd(causal=1)), ctypes.byref(x))
+    assert L.fa4_fp8_cache_fwd_blocks_workspace_bytes(ctypes.byref(c), ctypes.byref(fwd(causal=1, B=1)), ctypes.byref(x)) == 0
+    need = L.fa4_fp8_cache_fwd_blocks_workspace_bytes(ctypes.byref(c), ctypes.byref(fwd(causal=1, B=40)), ctypes.byref(x))
     assert need > 0
     for kw, rc in ((dict(), NULL), (dict(workspace=4104, workspace_bytes=need), ALIGN), (dict(workspace=4096, workspace_bytes=need - 1), LARGE)):
-        assert L.fa4_fp8_cache_fwd_blocks(ctypes.byref(c), ctypes.byref(fwd(causal=1, **kw)), ctypes.byref(x), None) == rc
+        assert L.fa4_fp8_cache_fwd_blocks(ctypes.byref(c), ctypes.byref(fwd(causal=1, B=40, **kw)), ctypes.byref(x), None) == rc
 
 
 @pytest.mark.parametrize("kw,rc", [(dict(struct_size=1), STRUCT), (dict(table=None), NULL), (dict(refs=None), NULL), (dict(B=0), SHAPE), (dict(pages_per_seq=0), SHAPE),

@@ -366,6 +366,44 @@ def test_copies_of_any_tensors(cuda_device):
     fa.check_status(dev)
 
 
+@pytest.mark.parametrize("page", [65536, 40016, 16384, 131088])
+def test_large_copies(cuda_device, page):
+    """From 64 MB on pages that lie in one piece go another way; beside them tensors that do not, pairs that are none, pairs outside the pool."""
+    dev, n = cuda_device, 5000
+    g = torch.Generator(device=dev).manual_seed(page)
+    flat = torch.randint(0, 256, (n, page // 16, 16), generator=g, device=dev, dtype=torch.uint8)
+    small = torch.randn(n, 8, generator=g, device=dev)
+    odd = torch.randint(0, 256, (n, 5), generator=g, device=dev, dtype=torch.uint8)
+    apart = torch.randn(n, 6, 8, 4, generator=g, device=dev)[:, :, ::2]
+    order = torch.randperm(n, generator=g, device=dev).to(torch.int32)
+    pairs = order.view(n // 2, 2).clone()
+    pairs[torch.rand(n // 2, generator=g, device=dev) < 0.4] = -1
+    pairs[7] = i32([3, -1], dev)
+    pairs[-1] = i32([int(order[-2]), int(order[-1])], dev)
+    real = pairs.long()[(pairs >= 0).all(1)]
+    tensors = [flat, small, odd, apart]
+    want = [t.clone() for t in tensors]
+    for w, t in zip(want, tensors):
+        w[real[:, 1]] = t[real[:, 0]]
+    fa.copy_kv_pages(tensors, pairs)
+    for t, w in zip(tensors, want):
+        assert torch.equal(t, w)
+    fa.check_status(dev)
+    # the same again, and with pairs outside the pool among them
+    pairs[11] = i32([n, 0], dev)
+    pairs[13] = i32([0, 2 ** 31 - 1], dev)
+    before = flat[0].clone()
+    fa.copy_kv_pages(tensors, pairs)
+    with pytest.raises(RuntimeError, match="code 2 .*site 127,"):
+        fa.check_status(dev)
+    real = pairs.long()[((pairs >= 0) & (pairs < n)).all(1)]
+    for w in want:
+        w[real[:, 1]] = w[real[:, 0]]
+    for t, w in zip(tensors, want):
+        assert torch.equal(t, w)
+    assert torch.equal(flat[0], before) or (real[:, 1] == 0).any()
+
+
 def test_copies_that_pass_32_bits(cuda_device):
     dev = cuda_device
     if torch.cuda.mem_get_info(dev)[0] < 12 * 2 ** 30:
@@ -374,6 +412,12 @@ def test_copies_that_pass_32_bits(cuda_device):
     x[7], x[99_990] = 3, 5
     fa.copy_kv_pages(x, i32([[7, 99_999], [99_990, 1]], dev))
     assert (x[99_999] == 3).all() and (x[1] == 5).all() and int(x[99_998].sum()) + int(x[0].sum()) == 0
+    # (and by bulk copies)
+    pairs = torch.full((2000, 2), -1, dtype=torch.int32, device=dev)
+    pairs[1999] = i32([99_999, 99_997], dev)
+    pairs[5] = i32([1, 2], dev)
+    fa.copy_kv_pages(x, pairs)
+    assert (x[99_997] == 3).all() and (x[2] == 5).all() and int(x[99_998].sum()) + int(x[0].sum()) == 0
     fa.check_status(dev)
 
 
