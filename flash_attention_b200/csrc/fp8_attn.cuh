@@ -94,42 +94,23 @@ __device__ __forceinline__ SeqLens unit_lens(const Fp8Params& p, int v) {
   }
   return n;
 }
-// A list of chosen blocks, by a whole warp: it ends at the first entry that is not above the one in front of it.
-struct BlockList {
-  const int32_t* at;
-  int n;
-};
-__device__ __forceinline__ BlockList list_of(const Fp8Params& p, int v, int hk) {
-  BlockList l;
-  l.at = p.blocks + ((int64_t)v * p.Hkv + hk) * p.chosen;
-  l.n = p.chosen;
-  const int lane = threadIdx.x & 31;
-  int last = -1;
-#pragma unroll 1
-  for (int i0 = 0; i0 < p.chosen; i0 += 32) {
-    const int e = i0 + lane < p.chosen ? l.at[i0 + lane] : -1, up = __shfl_up_sync(0xffffffffu, e, 1);
-    const uint32_t ends = __ballot_sync(0xffffffffu, e <= (lane == 0 ? last : up));
-    if (ends != 0u) {
-      l.n = min(p.chosen, i0 + __ffs(ends) - 1);
-      break;
-    }
-    last = __shfl_sync(0xffffffffu, e, 31);
-  }
-  return l;
-}
+// A list of chosen blocks: it ends at the first entry that is not above the one in front of it.
+__device__ __forceinline__ const int32_t* list_of(const Fp8Params& p, int v, int hk) { return p.blocks + ((int64_t)v * p.Hkv + hk) * p.chosen; }
 // How many of its keys lie in front of position `end`, by a whole warp.
-__device__ __forceinline__ int keys_in_front(const Fp8Params& p, BlockList l, int end) {
+__device__ __forceinline__ int keys_in_front(const Fp8Params& p, const int32_t* list, int end) {
   const int lane = threadIdx.x & 31, block = end >> p.log_block;
-  int whole = 0;
-  bool part = false;
+  int keys = 0, last = -1;
   if (end <= 0) return 0;
 #pragma unroll 1
-  for (int i0 = 0; i0 < l.n; i0 += 32) {
-    const int e = i0 + lane < l.n ? l.at[i0 + lane] : 0x7fffffff;
-    whole += __popc(__ballot_sync(0xffffffffu, e < block));
-    part = part || __any_sync(0xffffffffu, e == block);
+  for (int i0 = 0; i0 < p.chosen; i0 += 32) {
+    const int e = i0 + lane < p.chosen ? list[i0 + lane] : -1, up = __shfl_up_sync(0xffffffffu, e, 1);
+    const uint32_t over = __ballot_sync(0xffffffffu, e <= (lane == 0 ? last : up)), there = over == 0u ? 0xffffffffu : (over & -over) - 1u;
+    const uint32_t whole = __ballot_sync(0xffffffffu, e < block) & there, part = __ballot_sync(0xffffffffu, e == block) & there;
+    keys += (__popc(whole) << p.log_block) + (part != 0u ? end & ((1 << p.log_block) - 1) : 0);
+    if (whole != 0xffffffffu) break;
+    last = __shfl_sync(0xffffffffu, e, 31);
   }
-  return (whole << p.log_block) + (part ? end & ((1 << p.log_block) - 1) : 0);
+  return keys;
 }
 
 // A row's result from its sum `l` under the reference `m` (log2 units) and the sink of its head: the factor of the

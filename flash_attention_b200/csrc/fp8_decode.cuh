@@ -491,8 +491,8 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     feed.site = is_k ? FeederSites{kKFreeS, kKFullS} : FeederSites{kVFreeS, kVFullS};
     for (; ok && walk.more(); walk.next(p)) {
       if constexpr (kBlocks) {
-        const BlockList list = list_of(p, walk.b, walk.hb);
-        ok = feed.piece(p, wc, walk.tiles(), walk.at, query_block_of<true>(p, walk.b).b, walk.hb, 0, keys_in_front(p, list, walk.cur.sk + walk.cur.sq), list.at);
+        const int32_t* list = list_of(p, walk.b, walk.hb);
+        ok = feed.piece(p, wc, walk.tiles(), walk.at, query_block_of<true>(p, walk.b).b, walk.hb, 0, keys_in_front(p, list, walk.cur.sk + walk.cur.sq), list);
       } else {
         ok = feed.piece(p, wc, walk.tiles(), walk.cur.first + walk.at, walk.b, walk.hb * p.bundle + in_bundle, walk.cur.lo, walk.cur.hi);
       }
@@ -642,7 +642,7 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       int lo = 0, hi = 0, lo_in = 0, hi_in = 0;      // seen by the thread's row; by all rows
       if constexpr (kBlocks) {
         if (n > 0) {
-          const BlockList list = list_of(p, walk.b, hk);
+          const int32_t* list = list_of(p, walk.b, hk);
           const int mine = fast_div(my, p.div_group);
           for (int s = 0; s < seq.sq; ++s) {
             const int keys = keys_in_front(p, list, seq.sk + s + 1);
@@ -887,9 +887,9 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       if (s_walk.left == 0)
         for (int r = tid; r < R; r += F::kThreads) *reinterpret_cast<float*>(gbase + F::kOffK + (kR * kD + r) * 4) = -INFINITY;
       cluster_sync();
-      uint32_t gave_up = 0u;
-      for (int i = 0; i < p.meet; ++i) gave_up |= ld_cluster_u32(base + F::kOffMisc + 4, i);
-      for (int r = rank + p.meet * warp; r < R && gave_up == 0u; r += p.meet * (F::kThreads / 32)) {
+      // (no result where a wait of any of them ran out)
+      const bool whole = __ballot_sync(0xffffffffu, lane < p.meet && ld_cluster_u32(base + F::kOffMisc + 4, lane < p.meet ? lane : 0) != 0u) == 0u;
+      for (int r = rank + p.meet * warp; r < R && whole; r += p.meet * (F::kThreads / 32)) {
         const int s = fast_div(r, p.div_group), h = hk * p.group + r - s * p.group;
         merge_parts(p, place.b, place.q0 + s, h, lane, p.meet, [&](int i) { return __uint_as_float(ld_cluster_u32(part + (kR * kD + r) * 4, i)); },
                     [&](int i) { return ld_cluster_f4(part + (r * kD + 4 * lane) * 4, i); });

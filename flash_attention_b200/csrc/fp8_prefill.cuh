@@ -186,7 +186,7 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   if (R <= 0) return;
   const int s_first = fast_div(r_first, p.div_group), s_last = fast_div(r_first + R - 1, p.div_group);
   int lo_all = 0, hi_all;
-  BlockList list = {nullptr, 0};
+  const int32_t* list = nullptr;
   if constexpr (kBlocks) {
     list = list_of(p, v, hk);
     hi_all = keys_in_front(p, list, len.sk + s_last + 1);
@@ -294,7 +294,7 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       feed.scales = reinterpret_cast<float*>(gbase + L::kOffSc);
       feed.box = reinterpret_cast<int2*>(gbase + L::kOffBox);
       feed.site = {kKFreeS, kKFullS};
-      feed.piece(p, wc, n, t0, b, hk, lo_all, hi_all, list.at);
+      feed.piece(p, wc, n, t0, b, hk, lo_all, hi_all, list);
       feed.drain();
     } else if (warp == 14) {
       fp8d::Feeder<kD, L::kStagesV, L::kScales, false, kBlocks> feed;
@@ -307,7 +307,7 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       feed.scales = nullptr;
       feed.box = reinterpret_cast<int2*>(gbase + L::kOffBox) + 32;
       feed.site = {kRawFreeS, kRawFullS};
-      feed.piece(p, wc, n, t0, b, hk, lo_all, hi_all, list.at);
+      feed.piece(p, wc, n, t0, b, hk, lo_all, hi_all, list);
       feed.drain();
     } else if (warp == 13) {
       // ============================================ products =====================================

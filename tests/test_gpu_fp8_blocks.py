@@ -390,11 +390,12 @@ def test_padded_batches_and_rows_that_see_nothing(cuda_device, Sq, rows):
         chosen_and_attended(cuda_device, 4, B=3, lens=[600, 40, 7], fresh=[0, Sq, 1], **kw)
 
 
-@pytest.mark.parametrize("B,Sq,Hq,H,chosen", [(3, 1, 4, 1, 60), (40, 1, 4, 4, 12), (80, 1, 16, 8, 3), (1, 150, 8, 4, 4), (2, 4, 8, 8, 40)])
-def test_calls_of_few_and_many_units(cuda_device, B, Sq, Hq, H, chosen):
-    """Fewer units than CTAs, split among them; a CTA a unit; whole units one after the other."""
-    lens = [(331 * b) % 1500 + Sq for b in range(B)]
-    chosen_and_attended(cuda_device, chosen, B=B, Sq=Sq, Hq=Hq, H=H, D=64, size=32, block=16, lens=lens)
+@pytest.mark.parametrize("B,Sq,rows,Hq,H,chosen", [(3, 1, 1, 4, 1, 60), (2, 4, 1, 8, 8, 40), (25, 1, 1, 8, 4, 20), (40, 1, 1, 4, 4, 80), (40, 6, 6, 16, 4, 80),
+                                                   (40, 1, 1, 4, 4, 12), (80, 1, 1, 16, 8, 3), (1, 150, 1, 8, 4, 4)])
+def test_calls_of_few_and_many_units(cuda_device, B, Sq, rows, Hq, H, chosen):
+    """Few units, split among the CTAs of a cluster; a CTA a unit; shares dealt by the lengths and merged; whole units one after the other."""
+    lens = [(331 * b) % (1500 if B < 60 else 300) + Sq for b in range(B)]
+    chosen_and_attended(cuda_device, chosen, B=B, Sq=Sq, rows=rows, Hq=Hq, H=H, D=64, size=32, block=16, lens=lens)
 
 
 @pytest.mark.parametrize("Sq,rows", [(1, 1), (3, 1), (70, 64)])
