@@ -30,7 +30,8 @@ struct IndexParams {
 
 constexpr int kIndexWarps = 4;
 
-// A warp a block and kv head: kD / 16 lanes a row of 16-byte pieces.
+// A warp a block and kv head: kD / 16 lanes a row of 16-byte pieces, maxima and minima as pairs of fp16 (every e4m3 value is one).  It waits for loads: 131072 tokens of 8 heads,
+// blocks of 64 (118 MB) 26.2 us, 4.5 TB/s at 31 warps an SM; eight rows of a lane on their way rather than four 28 (80 registers), warps that go on to a next block 31.5.
 template <int kD>
 __global__ void __launch_bounds__(kIndexWarps * 32) fp8_index_kernel(const __grid_constant__ IndexParams p) {
   constexpr int kChunks = kD / 16, kRows = 32 / kChunks;
@@ -179,6 +180,11 @@ __device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t rank, uin
 
 // A unit (sequence, query block, kv head) is one CTA's, or (kParts) that of a cluster whose CTAs score a part of the blocks each and leave the keys
 // with the first one, which chooses.
+//
+// Four lanes have a block, pieces of 16 bytes apart by four, so a warp's load covers eight blocks and a dot product takes two shuffles (16 lanes a block took four times the
+// instructions: 2048 rows over 1024 blocks 25.7 -> 20.8 us).  The first bounds are on their way while the query is summed.  What bounds it: scattered pieces of 256 bytes in its middle (32 sequences of
+// up to 512 blocks, 21 MB, 10.7 us back to back and 16 on a cold L2), else a chain of lengths, table, bounds, three passes over the keys and the list: 128 blocks 5.4 us.  Four sequences of 4096 blocks
+// with a CTA a unit 24, as clusters of four 13.8.
 template <int kD, bool kParts>
 __global__ void __launch_bounds__(kSelectThreads, 2) fp8_select_kernel(const __grid_constant__ SelectParams p) {
   constexpr int kWarps = kSelectThreads / 32, kPieces = kD / 8, kBins = 2048;

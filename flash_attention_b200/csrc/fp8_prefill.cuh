@@ -22,6 +22,9 @@
 // Tried on a form of 238 us: exponentials by polynomials, one in eight 253, one in four 261 (more instructions between the others); the logarithm of a value
 // scale in the exponents where a half has one 248; the lower scores loaded in front of the upper exponentials or between them 282, 247.
 //
+// Over chosen blocks (kBlocks) the CTA's rows are those of one query block, its keys the blocks of that one's list one behind the other (see the decode kernel).  2048 rows of 32 heads, 64 rows
+// choose 64 blocks of 64: 170 us, two rounds of CTAs of 32 steps; a step 4000 clocks, since chosen blocks differ in level and the references of some row move in most of them.
+//
 // Warps: 0-3 and 4-7 softmax, 8-11 widen the tiles of V (cvt.f16x2.e4m3x2 runs at 64 a clock beside the exponentials), 12 and 14 load, 13 issues
 // the products.  Every wait is bounded (those of the softmax warps, which leave no registers for a call, by the issuer's: see mbar_wait_flag); a warp
 // whose wait ran out goes on without waiting.

@@ -3,7 +3,9 @@
 // A table (sequences, pages of a sequence) names pages of a pool, -1 where there is none; refs counts the entries that name a page, 0 is
 // free.  The book-keeping is a few thousand whole numbers: one cluster of eight CTAs does it in one launch, in phases between
 // rendezvous of the cluster, so nothing waits for the host and results do not depend on the order of threads (counters are
-// only added to; what is given away is ranked by prefix sums: rows in order, free pages from the lowest on).
+// only added to; what is given away is ranked by prefix sums: rows in order, free pages from the lowest on).  What bounds it is latency: a launch, three or four rendezvous
+// and a trip to memory between each.  us back to back: resize of 128 rows of 18 pages in a pool of 1315 8.7, 256 of 66 in 11761 9.9, 256 of 512 in 70000 15.4, 1024 of 256 in 300000 34;
+// compact of the same 11, 13, 21, 51; fork of 128 rows 2.2.
 #pragma once
 #include "fp8_append.cuh"
 
