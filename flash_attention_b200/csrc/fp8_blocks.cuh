@@ -257,8 +257,10 @@ __global__ void __launch_bounds__(kSelectThreads, 2) fp8_select_kernel(const __g
       if (at != 0xffffffffu) {
         const int64_t i = (int64_t)at * p.Hkv + head;
         const uint4* from = reinterpret_cast<const uint4*>(p.bounds + i * (2 * kD)) + c;
+        // (the whole of a block at once from HBM: both in turn on a cold L2 0.8 us of 50)
 #pragma unroll
-        for (int r = 0; r < kParcels; ++r) v[k][r] = from[4 * r];
+        for (int r = 0; r < kParcels; ++r)
+          asm volatile("ld.global.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[k][r].x), "=r"(v[k][r].y), "=r"(v[k][r].z), "=r"(v[k][r].w) : "l"(from + 4 * r));
         scale[k] = p.scale[i];
       } else {
 #pragma unroll
