@@ -31,7 +31,8 @@ struct Fp8Params {
   const int32_t* blocks;
   int chosen, query_block, query_blocks;
   int seqs;                          // B * query_blocks (dense: B)
-  FastDiv div_query_blocks, div_query_block;
+  int cta_units, more_units;         // whole units: as many a CTA, and one more for the first `more_units`
+  FastDiv div_query_blocks, div_query_block, div_hkv, div_splits;
   uint32_t* status;
   uint32_t epoch;
   uint64_t budget_ns;

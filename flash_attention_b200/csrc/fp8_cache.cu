@@ -285,6 +285,10 @@ int run_fwd(const fa4_fp8_cache* c, const fa4_fp8_fwd* f, const fa4_fp8_blocks* 
     p.query_blocks = p.seqs / f->B;
     p.div_query_block = make_fastdiv((uint32_t)p.query_block);
     p.div_query_blocks = make_fastdiv((uint32_t)p.query_blocks);
+    p.div_hkv = make_fastdiv((uint32_t)c->Hkv);
+    p.div_splits = make_fastdiv((uint32_t)std::max(1, plan.splits));
+    p.cta_units = (int)(seqs_of(f, x) * c->Hkv / kSms);
+    p.more_units = (int)(seqs_of(f, x) * c->Hkv % kSms);
   }
   p.B = f->B; p.Sq = f->Sq; p.Hq = f->Hq; p.Hkv = c->Hkv; p.group = f->Hq / c->Hkv; p.D = c->D;
   p.log_block = log2_of(c->block);

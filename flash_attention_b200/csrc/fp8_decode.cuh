@@ -418,22 +418,11 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   if (tid == 0) {
     *s_abort = 0u;
     wc = WaitCtx{s_abort, p.status, p.budget_ns, p.epoch};
-    for (int s = 0; s < kStages; ++s) {
-      mbar_init(bar(F::kKFull + s), 1);    // (the scales are written in front of the copies)
-      mbar_init(bar(F::kVFull + s), 1);
-      mbar_init(bar(F::kKFree + s), 1);
-      mbar_init(bar(F::kVFree + s), 1);
-    }
-    for (int s = 0; s < kStrands; ++s) {
-      mbar_init(bar(F::kSFull + s), 1);
-      mbar_init(bar(F::kSFree + s), 4);
-      mbar_init(bar(F::kPFull + s), 4);
-      mbar_init(bar(F::kPvDone + s), 1);
-    }
-    mbar_init(bar(F::kQReady), 4 * kStrands);
-    mbar_init(bar(F::kVPart), 1);
-    mbar_init(bar(F::kDrain), 1);
-    mbar_init(bar(F::kDrain + 1), 1);
+  }
+  if (tid < F::kBars) {
+    // (one arrival, of a thread or of a copy; four, of the warps of a strand; all softmax warps'.  The scales are written in front of the copies.)
+    auto in = [&](uint32_t first) { return tid >= first && tid < first + kStrands; };
+    mbar_init(bar(tid), in(F::kSFree) || in(F::kPFull) ? 4 : tid == F::kQReady ? 4 * kStrands : 1);
     fence_barrier_init();
   }
   if (warp == kLoadK && lane == 0) tma_prefetch_desc(&tm_k);
@@ -445,22 +434,21 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   tc_fence_before_sync();
   pdl_wait();
   // CTA = group * bundle + head in the bundle; with a split count of the caller's, a group is one split of one unit
-  const int group = blockIdx.x / p.bundle, in_bundle = blockIdx.x - group * p.bundle;
+  const int group = kBlocks ? blockIdx.x : blockIdx.x / p.bundle, in_bundle = kBlocks ? 0 : blockIdx.x - group * p.bundle;
   if (warp == 0) {
     Walk<kBlocks> w = {};
     if (kBlocks && p.num_splits < 0) {
       // whole units, as many a CTA
-      const int64_t units = (int64_t)p.seqs * p.bundles;
-      const int from = (int)(group * units / gridDim.x);
-      w.units = (int)((group + 1) * units / gridDim.x) - from;
-      w.b = from / p.bundles;
+      const int from = group * p.cta_units + min(group, p.more_units);
+      w.units = p.cta_units + (group < p.more_units);
+      w.b = fast_div(from, p.div_hkv);
       w.hb = from - w.b * p.bundles;
       const SeqLens len = unit_lens<kBlocks>(p, w.units > 0 ? w.b : 0);
       w.cur = seq_of<kBlocks>(p, len.sk, len.sq);
       w.left = w.units > 0 ? 0x40000000 : 0;
     } else if (p.num_splits > 0) {
-      const int unit = group / p.num_splits, split = group - unit * p.num_splits;
-      w.b = unit / p.bundles;
+      const int unit = kBlocks ? fast_div(group, p.div_splits) : group / p.num_splits, split = group - unit * p.num_splits;
+      w.b = kBlocks ? fast_div(unit, p.div_hkv) : unit / p.bundles;
       w.hb = unit - w.b * p.bundles;
       const SeqLens len = unit_lens<kBlocks>(p, w.b);
       w.cur = seq_of<kBlocks>(p, len.sk, len.sq);
