@@ -1530,21 +1530,25 @@ fa4_kv_paged paged_of(const at::Tensor& t, int64_t num_pages, const at::Device& 
   FA4_ASSERT(t.is_cuda() && t.device() == device, "the tensors of a cache and the pairs must be on one CUDA device");
   FA4_ASSERT(t.dim() >= 1 && t.size(0) == num_pages, "the tensors of a cache have as many pages: %lld and %s", (long long)num_pages, dims_of(t.sizes()).c_str());
   const int64_t unit = (int64_t)t.element_size();
-  std::vector<std::pair<int64_t, int64_t>> dims;      // (stride, size), bytes
+  constexpr int kDims = 16;
+  FA4_ASSERT(t.dim() <= kDims, "a tensor of a cache has at most %d dimensions", kDims);
+  std::pair<int64_t, int64_t> dims[kDims];            // (stride, size), bytes
+  int n = 0;
   for (int64_t i = 1; i < t.dim(); ++i) {
     if (t.size(i) == 1) continue;
     FA4_ASSERT(t.size(i) == 0 || t.stride(i) > 0, "a tensor of a cache must not be expanded");
-    dims.emplace_back(t.stride(i) * unit, t.size(i));
+    dims[n++] = {t.stride(i) * unit, t.size(i)};
   }
   FA4_ASSERT(num_pages <= 1 || t.numel() == 0 || t.stride(0) > 0, "a tensor of a cache must not be expanded");
-  std::sort(dims.begin(), dims.end());
+  std::sort(dims, dims + n);
   fa4_kv_paged s = {};
   s.base = t.data_ptr();
   s.stride_page = t.stride(0) * unit;
   s.row_bytes = unit;
   s.rows_inner = s.rows_outer = 1;
   int used = 0;                                       // of the two dimensions of rows
-  for (const auto& [stride, size] : dims) {
+  for (int i = 0; i < n; ++i) {
+    const auto& [stride, size] = dims[i];
     if (used == 0 && stride == s.row_bytes) s.row_bytes *= size;
     else if (used == 1 && stride == s.stride_inner * s.rows_inner) s.rows_inner *= size;
     else if (used == 2 && stride == s.stride_outer * s.rows_outer) s.rows_outer *= size;
@@ -1560,6 +1564,7 @@ PyObject* copy_pages(PyObject* const* a) {
   const at::Tensor pairs_in = tensor_of(a[0], "pairs");
   if (!PyTuple_Check(a[1])) fail(PyExc_TypeError, "tensors must be a tuple");
   std::vector<at::Tensor> tensors;
+  tensors.reserve(PyTuple_GET_SIZE(a[1]));
   for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(a[1]); ++i) tensors.push_back(tensor_of(PyTuple_GET_ITEM(a[1], i), "a tensor of the cache"));
   uint32_t* status = pairs_in.is_cuda() ? status_word(pairs_in.device()) : nullptr;
   {
@@ -1570,6 +1575,7 @@ PyObject* copy_pages(PyObject* const* a) {
     const at::Device device = pairs_in.device();
     const int64_t num_pages = tensors[0].size(0);
     std::vector<fa4_kv_paged> paged;
+    paged.reserve(tensors.size());
     for (const at::Tensor& t : tensors) {
       const fa4_kv_paged s = paged_of(t, num_pages, device);
       if (t.numel() > 0) paged.push_back(s);

@@ -62,6 +62,12 @@ class FP8KVCache:
     def block(self) -> int:
         return self.k.shape[1] // self.k_scale.shape[1]
 
+    def tensors(self) -> Tuple[torch.Tensor, ...]:
+        """What a page consists of: keys, values, scales, and the index if there is one."""
+        if self.key_bounds is None:
+            return (self.k, self.v, self.k_scale, self.v_scale)
+        return (self.k, self.v, self.k_scale, self.v_scale, self.key_bounds, self.bound_scale)
+
     def dequantize(self) -> Tuple[torch.Tensor, torch.Tensor]:
         """fp32 keys and values in the layout of the pool."""
         def whole(x, scale):

@@ -95,10 +95,10 @@ def copy_kv_pages(cache: Union[FP8KVCache, torch.Tensor, Sequence], pairs: torch
 
     One launch for eight tensors, no synchronisation; can be captured in a graph.  Pairs outside the pool are left out, and :func:`check_status` raises.
     """
-    tensors = []
-    for c in ((cache,) if isinstance(cache, (FP8KVCache, torch.Tensor)) else cache):
-        if isinstance(c, FP8KVCache):
-            tensors += [t for t in (c.k, c.v, c.k_scale, c.v_scale, c.key_bounds, c.bound_scale) if t is not None]
-        else:
-            tensors.append(c)
-    _lib.host().copy_pages(pairs, tuple(tensors))
+    if isinstance(cache, FP8KVCache):
+        tensors = cache.tensors()
+    elif isinstance(cache, torch.Tensor):
+        tensors = (cache,)
+    else:
+        tensors = tuple(t for c in cache for t in (c.tensors() if isinstance(c, FP8KVCache) else (c,)))
+    _lib.host().copy_pages(pairs, tensors)
