@@ -161,6 +161,7 @@ def index_kv_fp8(
 
     Of a block and kv head: the largest and the smallest value of every channel, in steps of ``k_scale`` times a power of two that bring the largest
     magnitude to 64 .. 120, rounded outwards to int8; ``bound_scale`` is a step.  A block with a NaN has bounds of 0 and a ``bound_scale`` of NaN.
+    (Where tokens of a block are dropped again, its bounds stay those of all of them until the next call for it.)
     One launch, no synchronisation; can be captured in a graph.  Positions and page numbers outside the cache are left out, and
     :func:`check_status` raises.
     """

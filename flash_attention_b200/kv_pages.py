@@ -30,7 +30,9 @@ class KVPages:
 
     table      (B, pages_per_seq) int32, contiguous: pages of a sequence, in order; -1 where it has none
     refs       (num_pages,) int32, contiguous: how many entries name a page; 0: it is free
-    page_size  tokens of a page
+    page_size  tokens of a page, as in the caches
+
+    Calls that change the same refs or table must not overlap (one stream, or events between them).
     """
     table: torch.Tensor
     refs: torch.Tensor
