@@ -189,7 +189,8 @@ template <int kD, bool kParts>
 __global__ void __launch_bounds__(kSelectThreads, 2) fp8_select_kernel(const __grid_constant__ SelectParams p) {
   constexpr int kWarps = kSelectThreads / 32, kPieces = kD / 8, kBins = 2048;
   extern __shared__ uint32_t s_key[];          // of the CTA's blocks: where their bounds are; then the keys
-  __shared__ int s_sum[2 * kD], s_hist[kBins], s_red[kWarps], s_count[2 * kWarps];
+  __shared__ int s_sum[2 * kD], s_red[kWarps], s_count[2 * kWarps];
+  __shared__ __align__(16) int s_hist[kBins];
   __shared__ __align__(16) int8_t s_q[2 * kD];
   __shared__ uint32_t s_range[2 * 8];          // smallest and largest key of a CTA's blocks
   __shared__ int s_bin[3];
