@@ -23,7 +23,7 @@
 // scale in the exponents where a half has one 248; the lower scores loaded in front of the upper exponentials or between them 282, 247.
 //
 // Over chosen blocks (kBlocks) the CTA's rows are those of one query block, its keys the blocks of that one's list one behind the other (see the decode kernel).  2048 rows of 32 heads, 64 rows
-// choose 64 blocks of 64: 170 us, two rounds of CTAs of 32 steps; a step 4000 clocks, since chosen blocks differ in level and the references of some row move in most of them.
+// choose 64 blocks of 64: 169 us, two rounds of CTAs of 32 steps; a step 4000 clocks, since chosen blocks differ in level and the references of some row move in most of them.
 //
 // Warps: 0-3 and 4-7 softmax, 8-11 widen the tiles of V (cvt.f16x2.e4m3x2 runs at 64 a clock beside the exponentials), 12 and 14 load, 13 issues
 // the products.  Every wait is bounded (those of the softmax warps, which leave no registers for a call, by the issuer's: see mbar_wait_flag); a warp
@@ -251,7 +251,8 @@ fp8_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(base + L::kOffV + 16 * i), "l"(src), "r"(r < R ? 16 : 0) : "memory");
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-#pragma unroll 1
+    // (two pieces at a time: 2048 rows over chosen blocks 172 -> 169 us, 1024 rows on 16384 keys 244 -> 241; four 174, 242)
+#pragma unroll 2
     for (int i = tid; i < p.cta_rows * kPieces; i += 384) {
       const int r = i / kPieces, ch = i % kPieces;
       const uint4 u = *reinterpret_cast<const uint4*>(gbase + L::kOffV + 16 * i);
