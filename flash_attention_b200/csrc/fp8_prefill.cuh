@@ -16,7 +16,7 @@
 //
 // What bounds it: no unit alone.  A step of 256 rows x 128 keys takes about 3400 clocks: the exponentials 2048, the products 2560 (Q K^T in halves of 64
 // columns 48 clocks an instruction, bound by shared memory), 1800 issue slots a scheduler, in chains between two warps of a scheduler.  D = 128, B = 1:
-// 1024 rows of 32 heads on 16384 keys 245 us back to back (162 at the measured rate of bf16 products), tensor pipe 60 %, exponential unit 60 %, issue slots
+// 1024 rows of 32 heads on 16384 keys 241 us back to back (162 at the measured rate of bf16 products), tensor pipe 60 %, exponential unit 60 %, issue slots
 // 53 % busy; 8192 rows of 64 heads on as many keys, causal, 975 us at first and 1110 under the power cap
 // (669, or 793 at the sustained rate).  A CTA's start and end take 12000 clocks, 8000 of them Q.
 // Tried on a form of 238 us: exponentials by polynomials, one in eight 253, one in four 261 (more instructions between the others); the logarithm of a value
