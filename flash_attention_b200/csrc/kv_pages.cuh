@@ -117,7 +117,8 @@ __device__ __forceinline__ Lengths lengths_of(const ResizeParams& p, int b, bool
 }
 
 // Rows keep the pages of what they hold (held, at most wanted), give back those behind, and get pages for `wanted` tokens.  A row that is about to write
-// into a page which other entries name too gets a copy of it (the last of the call's rows keeps the page, if nobody else has it).
+// into a page which other entries name too gets a copy of it (the last of the call's rows keeps the page, if nobody else has it).  A row that has no page
+// for some of what it holds keeps what it has.
 __global__ void __launch_bounds__(kThreads) resize_kernel(const __grid_constant__ ResizeParams p) {
   __shared__ int s_first[kRows], s_scan[kWarps + 1];
   const Book& k = p.book;
@@ -129,7 +130,7 @@ __global__ void __launch_bounds__(kThreads) resize_kernel(const __grid_constant_
     const Lengths n = lengths_of(p, b, lane == 0);
     const int keep = pages_of(k, min(n.held, n.wanted)), want = pages_of(k, n.wanted), at = fast_div(n.held, k.div_page);
     int32_t* row = k.table + (int64_t)b * k.width;
-    int missing = max(want - keep, 0), page = -1;
+    int gap = keep, page = -1;                 // first entry without a page among those that hold tokens
 #pragma unroll 1
     for (int j1 = 0; j1 < k.width; j1 += 128) {
       int entry[4];                            // (asked for together)
@@ -148,14 +149,17 @@ __global__ void __launch_bounds__(kThreads) resize_kernel(const __grid_constant_
           atomicSub(k.refs + e, 1);
           row[j] = -1;
         }
-        missing += __popc(__ballot_sync(0xffffffffu, j < keep && e < 0));
+        const uint32_t none = __ballot_sync(0xffffffffu, j < keep && e < 0);
+        if (none != 0u && gap == keep) gap = j0 + __ffs(none) - 1;
         // (a row that grows keeps the page its next token goes to)
         if (j0 <= at && at < j0 + 32) page = __shfl_sync(0xffffffffu, e, at & 31);
       }
     }
+    // (no page that could be put in a gap has what the row holds there: such a row gets nothing, and is reported)
     if (lane == 0) {
-      writes[b] = n.wanted > n.held && n.held != at * k.page_size && page >= 0 ? page : -1;
-      lacks[b] = missing;
+      writes[b] = gap == keep && n.wanted > n.held && n.held != at * k.page_size && page >= 0 ? page : -1;
+      lacks[b] = gap == keep ? max(want - keep, 0) : 0;
+      if (gap < keep) report_bad_index(k.status, k.epoch, kPoolSite);
     }
   }
   meet(k);

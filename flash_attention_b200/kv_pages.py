@@ -56,7 +56,8 @@ def resize_kv_pages(pages: KVPages, held: torch.Tensor, wanted: torch.Tensor) ->
     be given out by the same call, and what pages behind ``held`` contained is lost.
 
     One launch, no synchronisation; can be captured in a graph.  At most 4096 sequences.  Where no page is left the entry is -1 (what is appended there is left
-    out), and where lengths or entries lie outside the table or the pool they are cut or dropped; :func:`check_status` raises then.
+    out), and where lengths or entries lie outside the table or the pool they are cut or dropped; :func:`check_status` raises then.  It raises for a sequence too that has
+    no page for some of the tokens it keeps (they were left out before): that one gets nothing until it is cut in front of them, for what they were is lost.
     """
     return _lib.host().resize_pages(pages.table, pages.refs, pages.page_size, held, wanted)
 

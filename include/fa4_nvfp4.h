@@ -677,7 +677,8 @@ typedef struct fa4_kv_pages {
  * Row b keeps the pages of its first min(held[b], wanted[b]) tokens, gives back those behind, and gets pages for wanted[b].  Where it grows and its
  * next token goes into a page that holds some of it and has other entries too, it gets a copy of that page: pairs[b] = (page, copy).  Of the rows that
  * would write to one page the last one keeps it if nobody else names it.  Pages that are given back may be given out by the same call.  Where no page is
- * left the entry is -1, which is recorded.  At most 4096 rows.  Workspace as for the attention.
+ * left the entry is -1, which is recorded.  A row without a page for some of what it keeps gets nothing, which is recorded too.  At most 4096 rows.
+ * Workspace as for the attention.
  */
 int64_t fa4_kv_pages_resize_workspace_bytes(const fa4_kv_pages* pages);
 int fa4_kv_pages_resize(const fa4_kv_pages* pages, const int32_t* held, const int32_t* wanted, int32_t* pairs /* (B, 2) */, void* workspace,
