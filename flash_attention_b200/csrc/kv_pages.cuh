@@ -110,7 +110,7 @@ struct Lengths {
 __device__ __forceinline__ Lengths lengths_of(const ResizeParams& p, int b, bool report) {
   Lengths n = {p.held[b], p.wanted[b]};
   const int most = p.book.width * p.book.page_size;
-  if (report && (n.held < 0 || n.wanted < 0 || n.wanted > most)) report_bad_index(p.book.status, p.book.epoch, kLengthSite);
+  if (report && (n.held < 0 || n.held > most || n.wanted < 0 || n.wanted > most)) report_bad_index(p.book.status, p.book.epoch, kLengthSite);
   n.held = n.held < 0 ? 0 : (n.held < most ? n.held : most);
   n.wanted = n.wanted < 0 ? 0 : (n.wanted < most ? n.wanted : most);
   return n;

@@ -25,6 +25,19 @@ def reported(device, site):
     return False
 
 
+def test_lengths_outside_the_table_are_reported(cuda_device):
+    """Cut, and never without a word: held too."""
+    dev = cuda_device
+    for held, wanted, table, refs in ((99, 32, [0, 1], [1, 1, 0]), (33, 33, [0, 1], [1, 1, 0]), (2 ** 31 - 1, 3, [0, -1], [1, 0, 0]), (32, 33, [0, 1], [1, 1, 0]),
+                                      (-1, 0, [-1, -1], [0, 0, 0]), (32, -1, [-1, -1], [0, 0, 0])):
+        pages = fa.KVPages(i32([[0, 1]], dev), i32([1, 1, 0], dev), 16)
+        fa.resize_kv_pages(pages, i32([held], dev), i32([wanted], dev))
+        assert reported(dev, 124)
+        assert pages.table.tolist() == [table] and pages.refs.tolist() == refs
+    fa.resize_kv_pages(fa.KVPages(i32([[0, 1]], dev), i32([1, 1, 0], dev), 16), i32([32], dev), i32([32], dev))
+    assert not reported(dev, 124)
+
+
 # ---- entries that are missing among what a row holds ------------------------------------------------------------
 
 def test_a_gap_is_not_filled_without_a_word(cuda_device):
