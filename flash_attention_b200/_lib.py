@@ -298,7 +298,7 @@ EXPORTS = ["fa4_nvfp4_fwd", "fa4_nvfp4_sf_linear_to_tiled", "fa4_nvfp4_query",
 EXPORTS_FP8 = ["fa4_fp8_cache_append", "fa4_fp8_cache_fwd", "fa4_fp8_cache_fwd_workspace_bytes", "fa4_fp8_cache_index",
                "fa4_fp8_cache_select", "fa4_fp8_cache_fwd_blocks", "fa4_fp8_cache_fwd_blocks_workspace_bytes"]
 # (pages of a KV cache: likewise)
-EXPORTS_PAGES = ["fa4_kv_pages_resize", "fa4_kv_pages_resize_workspace_bytes", "fa4_kv_pages_fork", "fa4_kv_pages_compact",
+EXPORTS_PAGES = ["fa4_kv_pages_resize", "fa4_kv_pages_resize_ex", "fa4_kv_pages_resize_workspace_bytes", "fa4_kv_pages_fork", "fa4_kv_pages_compact",
                  "fa4_kv_pages_compact_workspace_bytes", "fa4_kv_pages_copy"]
 
 

@@ -1426,10 +1426,16 @@ void on_device_of(const at::Tensor& t, Launch launch) {
   launch(c10::cuda::getCurrentCUDAStream(device.index()).stream());
 }
 
-// table refs page_size held wanted
+// Whether two tensors, contiguous both, have no byte in common.
+bool apart(const at::Tensor& x, const at::Tensor& y) {
+  const char *p = static_cast<const char*>(x.data_ptr()), *q = static_cast<const char*>(y.data_ptr());
+  return p + x.nbytes() <= q || q + y.nbytes() <= p;
+}
+
+// table refs page_size held wanted granted
 PyObject* resize_pages(PyObject* const* a) {
   Pages k = pages_of(a);
-  const at::Tensor held_in = tensor_of(a[3], "held"), wanted_in = tensor_of(a[4], "wanted");
+  const at::Tensor held_in = tensor_of(a[3], "held"), wanted_in = tensor_of(a[4], "wanted"), granted = optional_tensor(a[5], "granted");
   at::Tensor pairs;
   {
     NoGil nogil;
@@ -1437,14 +1443,22 @@ PyObject* resize_pages(PyObject* const* a) {
     const int64_t B = k.p.B;
     const at::Tensor held = counts_of(held_in, "held", B, k.refs.device()), wanted = counts_of(wanted_in, "wanted", B, k.refs.device());
     if (B > 4096) fail(PyExc_NotImplementedError, "more than 4096 rows are not built");
+    if (granted.defined()) {
+      validate(granted, "granted", {B}, at::kInt, k.refs.device());
+      FA4_ASSERT(granted.is_contiguous(), "granted must be contiguous");
+      // (what is read is not what is written)
+      for (const at::Tensor* read : {static_cast<const at::Tensor*>(&k.table), static_cast<const at::Tensor*>(&k.refs), &held, &wanted})
+        FA4_ASSERT(apart(granted, *read), "granted must not overlap what the call reads");
+    }
     on_device_of(k.refs, [&](void* stream) {
       pairs = new_tensor({B, 2}, at::kInt, k.refs.device());
       if (B == 0) return;
       const int64_t bytes = fa4_kv_pages_resize_workspace_bytes(&k.p);
       if (bytes < 0) check_rc((int)bytes, "fa4_kv_pages_resize_workspace_bytes");
       const c10::DataPtr work = scratch_bytes(bytes);
-      check_rc(fa4_kv_pages_resize(&k.p, held.data_ptr<int32_t>(), wanted.data_ptr<int32_t>(), pairs.data_ptr<int32_t>(), work.get(), (uint64_t)bytes, stream),
-               "fa4_kv_pages_resize");
+      check_rc(fa4_kv_pages_resize_ex(&k.p, held.data_ptr<int32_t>(), wanted.data_ptr<int32_t>(), pairs.data_ptr<int32_t>(),
+                                      granted.defined() ? granted.data_ptr<int32_t>() : nullptr, work.get(), (uint64_t)bytes, stream),
+               "fa4_kv_pages_resize_ex");
     });
   }
   return THPVariable_Wrap(pairs);
@@ -1478,10 +1492,6 @@ PyObject* fork_pages(PyObject* const* a) {
         fresh = new_tensor({rows}, at::kInt, device);
       }
       // (what is read is not what is written)
-      auto apart = [](const at::Tensor& x, const at::Tensor& y) {
-        const char *p = static_cast<const char*>(x.data_ptr()), *q = static_cast<const char*>(y.data_ptr());
-        return p + x.nbytes() <= q || q + y.nbytes() <= p;
-      };
       for (const at::Tensor* read : {static_cast<const at::Tensor*>(&k.table), static_cast<const at::Tensor*>(&k.refs), &held, &parents})
         FA4_ASSERT(apart(table, *read) && apart(fresh, *read), "the new table and held must not overlap what the call reads");
       FA4_ASSERT(apart(table, fresh), "the new table and held must not overlap");
@@ -1664,7 +1674,7 @@ PyMethodDef methods[] = {method<fwd, 23>("fwd"),
                          method<fwd_fp8, 20>("fwd_fp8"),
                          method<index_fp8, 10>("index_fp8"),
                          method<select_fp8, 15>("select_fp8"),
-                         method<resize_pages, 5>("resize_pages"),
+                         method<resize_pages, 6>("resize_pages"),
                          method<fork_pages, 7>("fork_pages"),
                          method<compact_pages, 3>("compact_pages"),
                          method<copy_pages, 2>("copy_pages"),

@@ -44,14 +44,18 @@ extern "C" int64_t fa4_kv_pages_resize_workspace_bytes(const fa4_kv_pages* k) {
   if (k->B > kRows) return -FA4_E_TOO_LARGE;
   return resize_words(k->B, k->num_pages) * 4;
 }
-extern "C" int fa4_kv_pages_resize(const fa4_kv_pages* k, const int32_t* held, const int32_t* wanted, int32_t* pairs, void* workspace,
-                                   uint64_t workspace_bytes, void* cuda_stream) {
+extern "C" int fa4_kv_pages_resize_ex(const fa4_kv_pages* k, const int32_t* held, const int32_t* wanted, int32_t* pairs, int32_t* granted, void* workspace,
+                                      uint64_t workspace_bytes, void* cuda_stream) {
   const int64_t need = fa4_kv_pages_resize_workspace_bytes(k);
   if (need < 0) return (int)need;
   if (!held || !wanted || !pairs) return -FA4_E_NULL;
   if (int e = check_work(workspace, workspace_bytes, need / 4)) return e;
-  ResizeParams p = {book_of(k), held, wanted, pairs, static_cast<int32_t*>(workspace)};
+  ResizeParams p = {book_of(k), held, wanted, pairs, granted, static_cast<int32_t*>(workspace)};
   return launch_pdl_cluster((unsigned)p.book.ctas, resize_kernel, dim3((unsigned)p.book.ctas), kThreads, 0, static_cast<cudaStream_t>(cuda_stream), p);
+}
+extern "C" int fa4_kv_pages_resize(const fa4_kv_pages* k, const int32_t* held, const int32_t* wanted, int32_t* pairs, void* workspace,
+                                   uint64_t workspace_bytes, void* cuda_stream) {
+  return fa4_kv_pages_resize_ex(k, held, wanted, pairs, nullptr, workspace, workspace_bytes, cuda_stream);
 }
 
 extern "C" int fa4_kv_pages_fork(const fa4_kv_pages* k, const int32_t* held, const int32_t* parents, int32_t rows, int32_t* new_table,

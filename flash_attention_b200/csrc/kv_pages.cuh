@@ -26,6 +26,10 @@ struct Book {
   uint32_t* status;
   uint32_t epoch;
 };
+// Marks on a page number: a row's page that is copied (inside resize); the page of an entry whose row waits for a copy of it, which was to be written to and found no page.
+// The latter is in tables: the calls that read and write caches take it for no page at all, here it is an entry like others.
+constexpr int kCopied = 0x40000000, kWaits = (int)0x80000000;
+__device__ __forceinline__ int page_in(int entry) { return entry < 0 && (entry & kCopied) == 0 ? entry & ~kWaits : entry; }
 // Pages of `tokens`.
 __device__ __forceinline__ int pages_of(const Book& p, int tokens) {
   const int whole = fast_div(tokens, p.div_page);
@@ -99,7 +103,8 @@ struct ResizeParams {
   Book book;
   const int32_t *held, *wanted;
   int32_t* pairs;                    // (B, 2)
-  int32_t* work;                     // B: page written to or -1 (bit 30: is copied), B: entries that lack a page, kCluster, num_pages: the free ones, in order
+  int32_t* granted;                  // (B,), or null
+  int32_t* work;                     // B: page written to or -1 (kCopied: is copied), B: entries that lack a page (of a row with a gap -1 - its place), kCluster, num_pages: the free ones, in order
 };
 __host__ __device__ constexpr int64_t resize_words(int64_t B, int64_t num_pages) { return 2 * B + kCluster + num_pages; }
 
@@ -118,7 +123,7 @@ __device__ __forceinline__ Lengths lengths_of(const ResizeParams& p, int b, bool
 
 // Rows keep the pages of what they hold (held, at most wanted), give back those behind, and get pages for `wanted` tokens.  A row that is about to write
 // into a page which other entries name too gets a copy of it (the last of the call's rows keeps the page, if nobody else has it).  A row that has no page
-// for some of what it holds keeps what it has.
+// for some of what it holds keeps what it has.  So does a row whose copy finds no page, and with it the one that was to keep the original: they go on sharing it and do not grow.
 __global__ void __launch_bounds__(kThreads) resize_kernel(const __grid_constant__ ResizeParams p) {
   __shared__ int s_first[kRows], s_scan[kWarps + 1];
   const Book& k = p.book;
@@ -139,12 +144,12 @@ __global__ void __launch_bounds__(kThreads) resize_kernel(const __grid_constant_
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int j0 = j1 + 32 * i, j = j0 + lane;
-        int e = entry[i];
+        int e = page_in(entry[i]);
         if (e >= k.num_pages) {
           report_bad_index(k.status, k.epoch, kTableSite);
           e = -1;
-          row[j] = -1;
         }
+        if (e != entry[i] && j < k.width) row[j] = e;
         if (j < k.width && j >= keep && e >= 0) {
           atomicSub(k.refs + e, 1);
           row[j] = -1;
@@ -158,7 +163,7 @@ __global__ void __launch_bounds__(kThreads) resize_kernel(const __grid_constant_
     // (no page that could be put in a gap has what the row holds there: such a row gets nothing, and is reported)
     if (lane == 0) {
       writes[b] = gap == keep && n.wanted > n.held && n.held != at * k.page_size && page >= 0 ? page : -1;
-      lacks[b] = gap == keep ? max(want - keep, 0) : 0;
+      lacks[b] = gap == keep ? max(want - keep, 0) : -1 - gap;
       if (gap < keep) report_bad_index(k.status, k.epoch, kPoolSite);
     }
   }
@@ -170,10 +175,10 @@ __global__ void __launch_bounds__(kThreads) resize_kernel(const __grid_constant_
     const int others = __ldcg(k.refs + page) - 1;
     if (others <= 0) continue;
     int earlier = 0;
-    for (int i = lane; i < b; i += 32) earlier += (__ldcg(writes + i) & 0x3fffffff) == page && __ldcg(writes + i) >= 0;
+    for (int i = lane; i < b; i += 32) earlier += (__ldcg(writes + i) & ~kCopied) == page && __ldcg(writes + i) >= 0;
     earlier = __reduce_add_sync(0xffffffffu, earlier);
     if (lane == 0 && earlier < others) {
-      writes[b] = page | 0x40000000;
+      writes[b] = page | kCopied;
       ++lacks[b];
     }
   }
@@ -191,7 +196,7 @@ __global__ void __launch_bounds__(kThreads) resize_kernel(const __grid_constant_
 #pragma unroll
     for (int i = 0; i < kRows / kThreads; ++i) {
       const int b = (int)threadIdx.x * (kRows / kThreads) + i;
-      mine[i] = b < k.B ? __ldcg(lacks + b) : 0;
+      mine[i] = b < k.B ? max(__ldcg(lacks + b), 0) : 0;
       sum += mine[i];
     }
     int upto = sum;
@@ -223,13 +228,30 @@ __global__ void __launch_bounds__(kThreads) resize_kernel(const __grid_constant_
   meet(k);
   // ---- the rows are filled
   for (int b = row0; b < k.B; b += step) {
-    const int copied = __ldcg(writes + b);
-    const bool copies = copied >= 0 && (copied & 0x40000000) != 0;
+    const int writes_to = __ldcg(writes + b), lack_here = __ldcg(lacks + b);
+    const bool copies = writes_to >= 0 && (writes_to & kCopied) != 0;
     const Lengths n = lengths_of(p, b, false);
     const int want = pages_of(k, n.wanted), at = copies ? fast_div(n.held, k.div_page) : -1;
     int32_t* row = k.table + (int64_t)b * k.width;
-    int next = s_first[b], fresh = -1;
-    const int last = next + __ldcg(lacks + b);
+    int next = s_first[b], fresh = -1, room = lack_here < 0 ? (-1 - lack_here) * k.page_size : n.wanted;
+    const int last = next + max(lack_here, 0);
+    // (a copy takes the first of a row's pages.  Pages run out for all rows behind one, so if a sharer's copy has none, the row that was to keep the original
+    // gets none either; what it would write there belongs to both)
+    bool refused = copies && next >= free_pages;
+    if (total > free_pages && writes_to >= 0 && !copies) {
+      bool waits = false;
+      for (int i = lane; i < b; i += 32) waits = waits || (__ldcg(writes + i) == (writes_to | kCopied) && s_first[i] >= free_pages);
+      refused = __any_sync(0xffffffffu, waits);
+    }
+    if (refused) {
+      // (whoever is not told by `granted` must not write there either)
+      if (lane == 0) {
+        report_bad_index(k.status, k.epoch, kPoolSite);
+        if (p.granted == nullptr) row[fast_div(n.held, k.div_page)] = (writes_to & ~kCopied) | kWaits;
+      }
+      room = n.held;
+      next = last;
+    }
     for (int j0 = 0; j0 < want && next < last; j0 += 32) {
       const int j = j0 + lane;
       const bool lack = j < want && (j == at || row[j] < 0);
@@ -242,13 +264,16 @@ __global__ void __launch_bounds__(kThreads) resize_kernel(const __grid_constant_
         row[j] = page;
       }
       if (j0 <= at && at < j0 + 32) fresh = __shfl_sync(0xffffffffu, page, at & 31);
+      const uint32_t none = __ballot_sync(0xffffffffu, lack && page < 0);
+      if (none != 0u) room = min(room, (j0 + __ffs(none) - 1) * k.page_size);
       next += __popc(mask);
     }
     if (lane == 0) {
-      const int from = copied & 0x3fffffff;
-      if (copies) atomicSub(k.refs + from, 1);
-      p.pairs[2 * b] = copies && fresh >= 0 ? from : -1;
-      p.pairs[2 * b + 1] = copies ? fresh : -1;
+      const int from = writes_to & ~kCopied;
+      if (fresh >= 0) atomicSub(k.refs + from, 1);
+      p.pairs[2 * b] = fresh >= 0 ? from : -1;
+      p.pairs[2 * b + 1] = fresh;
+      if (p.granted != nullptr) p.granted[b] = room;
     }
   }
 }
@@ -276,7 +301,7 @@ __global__ void __launch_bounds__(kForkThreads) fork_kernel(const __grid_constan
     held = held < 0 ? 0 : (held < most ? held : (int)most);
     const int keep = pages_of(k, held);
     for (int j = tid; j < k.width; j += kForkThreads) {
-      const int e = j < keep ? k.table[(int64_t)a * k.width + j] : -1;
+      const int e = j < keep ? page_in(k.table[(int64_t)a * k.width + j]) : -1;
       p.table[(int64_t)b * k.width + j] = e >= 0 && e < k.num_pages ? e : -1;
     }
     if (tid == 0) p.new_held[b] = held;
@@ -295,7 +320,7 @@ __global__ void __launch_bounds__(kForkThreads) fork_kernel(const __grid_constan
   held = held < 0 ? 0 : (held < most ? held : (int)most);
   const int keep = pages_of(k, held), change = s_children - 1;
   for (int j = tid; j < k.width; j += kForkThreads) {
-    const int e = k.table[(int64_t)a * k.width + j], by = j < keep ? change : -1;
+    const int e = page_in(k.table[(int64_t)a * k.width + j]), by = j < keep ? change : -1;
     if (e >= k.num_pages) report_bad_index(k.status, k.epoch, kTableSite);
     else if (e >= 0 && by != 0) atomicAdd(k.refs + e, by);
   }
@@ -374,12 +399,13 @@ __global__ void __launch_bounds__(kThreads) compact_kernel(const __grid_constant
     for (int j = 0; j < 8; ++j) e[j] = i0 + j * step < entries ? k.table[i0 + j * step] : -1;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      if (e[j] >= k.num_pages) report_bad_index(k.status, k.epoch, kTableSite);
-      at[j] = e[j] >= used && e[j] < k.num_pages ? __ldcg(to + e[j]) : -1;
+      const int page = page_in(e[j]);
+      if (page >= k.num_pages) report_bad_index(k.status, k.epoch, kTableSite);
+      at[j] = page >= used && page < k.num_pages ? __ldcg(to + page) : -1;
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (at[j] >= 0) k.table[i0 + j * step] = at[j];
+      if (at[j] >= 0) k.table[i0 + j * step] = at[j] | (e[j] & kWaits);
   }
 }
 

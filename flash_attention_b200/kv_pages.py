@@ -6,10 +6,12 @@ A page table is an argument of every call that reads or fills a paged cache (:fu
 layers share one table; what has to be copied comes back as pairs of pages for :func:`copy_kv_pages` of each.  A step of a loop:
 
     pages, held = fork_kv_pages(pages, held, parents)          # beams: rows go on from the beams they were chosen from
-    pairs = resize_kv_pages(pages, held, held + 1)             # room for a token; rows that end: wanted 0
+    pairs = resize_kv_pages(pages, held, held + 1, granted=room)           # room for a token; rows that end: wanted 0
     for cache in layers: copy_kv_pages(cache, pairs)
-    for cache in layers: append_kv_fp8(cache, k, v, held, page_table=pages.table) ...
-    held += 1
+    for cache in layers: append_kv_fp8(cache, k, v, held, page_table=pages.table, seqused_new=room - held) ...
+    held.copy_(room)
+
+Where the pool is sure to have a page for everybody ``granted`` is what was wanted, and may be left out.
 
 No counterpart in the reference, whose callers make page tables on the host.
 """
@@ -28,7 +30,7 @@ from .fp8_cache import FP8KVCache
 class KVPages:
     """Who has which page of a pool.
 
-    table      (B, pages_per_seq) int32, contiguous: pages of a sequence, in order; -1 where it has none
+    table      (B, pages_per_seq) int32, contiguous: pages of a sequence, in order; -1 where it has none (-2^31 + page: see :func:`resize_kv_pages`)
     refs       (num_pages,) int32, contiguous: how many entries name a page; 0: it is free
     page_size  tokens of a page, as in the caches
 
@@ -46,7 +48,7 @@ class KVPages:
                    torch.zeros(num_pages, dtype=torch.int32, device=device), page_size)
 
 
-def resize_kv_pages(pages: KVPages, held: torch.Tensor, wanted: torch.Tensor) -> torch.Tensor:
+def resize_kv_pages(pages: KVPages, held: torch.Tensor, wanted: torch.Tensor, granted: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Pages for ``wanted[b]`` tokens for every sequence, of which it holds ``held[b]``; returns the pages to copy, (B, 2) int32 (from, to), -1 where
     there is none (:func:`copy_kv_pages`).  ``pages`` is changed in place; held and wanted (B,) int32 are not.
 
@@ -55,11 +57,22 @@ def resize_kv_pages(pages: KVPages, held: torch.Tensor, wanted: torch.Tensor) ->
     belongs to others too, it gets a copy of that page; of the sequences that would write to it the last keeps it, if nobody else has it.  Pages given back may
     be given out by the same call, and what pages behind ``held`` contained is lost.
 
-    One launch, no synchronisation; can be captured in a graph.  At most 4096 sequences.  Where no page is left the entry is -1 (what is appended there is left
-    out), and where lengths or entries lie outside the table or the pool they are cut or dropped; :func:`check_status` raises then.  It raises for a sequence too that has
-    no page for some of the tokens it keeps (they were left out before): that one gets nothing until it is cut in front of them, for what they were is lost.
+    Where no page is left, :func:`check_status` raises, and what a sequence holds stays as it is:
+
+    * an entry that should have got a page is -1 (what is appended there is left out);
+    * a copy is not made: the sequence goes on sharing the page, and neither it nor the one that was to keep the page gets to write there.  With ``granted`` their entries stay and can be
+      read; without it they become -2^31 + page, which the calls on a cache take for no page (nothing is appended or read there, and they report it), until the next call of this function
+      that has a page or does not let them grow;
+    * a sequence that has no page for some of the tokens it keeps (they were left out before) gets nothing until it is cut in front of them: what they were is lost.
+
+    ``granted`` (B,) int32, overlapping none of the others, is written: the lengths that may be appended up to.  That is ``wanted`` if nothing was missing, else the tokens in front
+    of the first entry without a page, or ``held`` where a copy was not made; append with ``seqused_new=granted - held`` and go on with it as the next held.  The same call works once
+    there are pages again.
+
+    One launch, no synchronisation; can be captured in a graph.  At most 4096 sequences.  Where lengths or entries lie outside the table or the pool they are cut
+    or dropped, and :func:`check_status` raises.
     """
-    return _lib.host().resize_pages(pages.table, pages.refs, pages.page_size, held, wanted)
+    return _lib.host().resize_pages(pages.table, pages.refs, pages.page_size, held, wanted, granted)
 
 
 def fork_kv_pages(pages: KVPages, held: torch.Tensor, parents: torch.Tensor,

@@ -659,7 +659,8 @@ int fa4_fp8_cache_fwd_blocks(const fa4_fp8_cache* cache, const fa4_fp8_fwd* p, c
  * Which pages of a pool the sequences of a batch have, kept on the device: allocating and freeing, forking (beams, samples of one
  * prompt), copy on write, compacting.  No counterpart in the reference, whose callers make page tables on the host.
  *
- *   table (B, pages_per_seq) int32: pages of a sequence, in order; -1 (any negative number) where it has none
+ *   table (B, pages_per_seq) int32: pages of a sequence, in order; -1 (any negative number above -2^30) where it has none; -2^31 + page where it waits
+ *         for a copy of a page (see fa4_kv_pages_resize)
  *   refs  (num_pages,) int32: how many entries of tables name a page; 0: free
  * Nothing in it is a particular cache's: caches of several layers are kept by one table, and the pages that a call wants copied come
  * back as pairs (from, to), -1 where there is none, for fa4_kv_pages_copy of each.  Everything is given out in a fixed order (rows, then
@@ -679,10 +680,19 @@ typedef struct fa4_kv_pages {
  * would write to one page the last one keeps it if nobody else names it.  Pages that are given back may be given out by the same call.  Where no page is
  * left the entry is -1, which is recorded.  A row without a page for some of what it keeps gets nothing, which is recorded too.  At most 4096 rows.
  * Workspace as for the attention.
+ *
+ * A copy that finds no page is recorded; the pair is (-1, -1) and refs stay.  The row goes on sharing the page, and neither it nor the row that was to keep the page may write there:
+ * with `granted` both have the lengths they hold, and their entries stay; without it their entries become -2^31 + page, which is no page for the calls on caches
+ * and is one again behind the next call that finds a page or does not let the row grow.
+ *
+ * granted (B,), or NULL: the lengths that the rows have pages of their own for, which may be appended up to: wanted[b], or where something was missing the
+ * tokens in front of the first entry without a page; held[b] where a copy found none.
  */
 int64_t fa4_kv_pages_resize_workspace_bytes(const fa4_kv_pages* pages);
 int fa4_kv_pages_resize(const fa4_kv_pages* pages, const int32_t* held, const int32_t* wanted, int32_t* pairs /* (B, 2) */, void* workspace,
                         uint64_t workspace_bytes, void* cuda_stream);
+int fa4_kv_pages_resize_ex(const fa4_kv_pages* pages, const int32_t* held, const int32_t* wanted, int32_t* pairs /* (B, 2) */, int32_t* granted, void* workspace,
+                           uint64_t workspace_bytes, void* cuda_stream);
 /*
  * A new table of `rows` rows: row i is row parents[i] of the old one as far as it holds tokens (-1: an empty row), new_held[i] its held.  refs
  * follow; the old table has no entries any more as far as they go.  new_table and new_held overlap nothing else.

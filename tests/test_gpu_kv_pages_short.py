@@ -75,3 +75,331 @@ def test_a_gap_where_a_warp_looks_for_it(cuda_device):
         pairs = fa.resize_kv_pages(pages, i32([298 * 16 + 4, 4], dev), i32([300 * 16, 4], dev))
         assert reported(dev, 125)
         assert pages.table.tolist() == table and pages.refs.tolist() == refs and pairs.tolist() == [[-1, -1]] * 2
+
+
+# ---- copies that find no page ------------------------------------------------------------------------------------
+
+class Model:
+    """The book-keeping as lists."""
+
+    def __init__(self, table, refs, size):
+        self.table, self.refs, self.size = [list(r) for r in table], list(refs), size
+
+    def count(self, tokens):
+        return -(-tokens // self.size)
+
+    def resize(self, held, wanted):
+        """(pairs, granted lengths, whether something was missing)"""
+        rows = range(len(self.table))
+        for row, h, w in zip(self.table, held, wanted):
+            for j in range(self.count(min(h, w)), len(row)):
+                if row[j] >= 0:
+                    self.refs[row[j]] -= 1
+                    row[j] = -1
+        gaps = [next((j for j in range(self.count(min(h, w))) if row[j] < 0), None) for row, h, w in zip(self.table, held, wanted)]
+        writes = [self.table[b][held[b] // self.size] if gaps[b] is None and wanted[b] > held[b] and held[b] % self.size else -1 for b in rows]
+        copied = [p >= 0 and writes[:b].count(p) < self.refs[p] - 1 for b, p in enumerate(writes)]
+        free = [p for p, r in enumerate(self.refs) if r == 0]
+        pairs, granted, failed, missing, self.refused = [], [], [], False, []
+        for b in rows:
+            row, at = self.table[b], held[b] // self.size
+            pair, room = [-1, -1], wanted[b]
+            if gaps[b] is not None:
+                room, missing = gaps[b] * self.size, True
+            elif (copied[b] and not free) or writes[b] in failed:
+                failed.append(writes[b])
+                self.refused.append(b)
+                room, missing = held[b], True
+            else:
+                for j in range(self.count(wanted[b])):
+                    if row[j] < 0 or (copied[b] and j == at):
+                        if not free:
+                            room, missing = min(room, j * self.size), True
+                            continue
+                        page = free.pop(0)
+                        self.refs[page] = 1
+                        if copied[b] and j == at:
+                            pair = [row[j], page]
+                            self.refs[row[j]] -= 1
+                        row[j] = page
+            pairs.append(pair)
+            granted.append(room)
+        return pairs, granted, missing
+
+    def fork(self, held, parents):
+        children = Counter(parents)
+        for a, (row, h) in enumerate(zip(self.table, held)):
+            for j, p in enumerate(row):
+                if p >= 0:
+                    self.refs[p] += children[a] - 1 if j < self.count(h) else -1
+        width = len(self.table[0])
+        self.table = [[-1] * width if a < 0 else [p if j < self.count(held[a]) else -1 for j, p in enumerate(self.table[a])] for a in parents]
+        return [0 if a < 0 else held[a] for a in parents]
+
+    def check(self):
+        named = Counter(p for row in self.table for p in row if p >= 0)
+        assert self.refs == [named[p] for p in range(len(self.refs))]
+
+
+WAITS = -2 ** 31                 # on the page of an entry that waits for a copy
+
+
+def test_entries_that_wait_for_a_copy(cuda_device):
+    """Rows that were not told go through every call: what they name is counted, moved and given back like other entries."""
+    dev = cuda_device
+
+    def made():
+        pages = fa.KVPages(i32([[2, 1, -1], [2, 1, -1], [0, -1, -1]], dev), i32([1, 2, 2], dev), 16)
+        fa.resize_kv_pages(pages, i32([25, 20, 16], dev), i32([26, 21, 16], dev))
+        assert reported(dev, 125)
+        assert pages.table.tolist() == [[2, WAITS + 1, -1], [2, WAITS + 1, -1], [0, -1, -1]] and pages.refs.tolist() == [1, 2, 2]
+        return pages
+    # no growth: entries like others again, with nothing to copy
+    pages = made()
+    assert fa.resize_kv_pages(pages, i32([25, 20, 16], dev), i32([25, 18, 16], dev)).tolist() == [[-1, -1]] * 3
+    assert pages.table.tolist() == [[2, 1, -1], [2, 1, -1], [0, -1, -1]] and pages.refs.tolist() == [1, 2, 2]
+    # cut in front of it, ended
+    pages = made()
+    fa.resize_kv_pages(pages, i32([25, 20, 16], dev), i32([3, 0, 16], dev))
+    assert pages.table.tolist() == [[2, -1, -1], [-1, -1, -1], [0, -1, -1]] and pages.refs.tolist() == [1, 0, 1]
+    # alone with it: written to as it is
+    pages = made()
+    assert fa.resize_kv_pages(pages, i32([25, 20, 16], dev), i32([26, 0, 16], dev)).tolist() == [[-1, -1]] * 3
+    assert pages.table.tolist() == [[2, 1, -1], [-1, -1, -1], [0, -1, -1]] and pages.refs.tolist() == [1, 1, 1]
+    # forked: shared by one more, or one less
+    pages = made()
+    pages, held = fa.fork_kv_pages(pages, i32([25, 20, 16], dev), i32([0, 0, 1, 0], dev))
+    assert pages.table.tolist() == [[2, 1, -1]] * 4 and held.tolist() == [25, 25, 20, 25] and pages.refs.tolist() == [0, 4, 4]
+    pages, held = fa.fork_kv_pages(made(), i32([25, 20, 16], dev), i32([2], dev))
+    assert pages.table.tolist() == [[0, -1, -1]] and pages.refs.tolist() == [1, 0, 0]
+    # moved: pages 3 to 5 of six, the first waited for
+    pages = fa.KVPages(i32([[4, WAITS + 3], [4, WAITS + 3], [5, -1]], dev), i32([0, 0, 0, 2, 2, 1], dev), 16)
+    pairs, used = fa.compact_kv_pages(pages)
+    assert pairs.tolist() == [[3, 0], [4, 1], [5, 2]] and used.tolist() == [3]
+    assert pages.table.tolist() == [[1, WAITS], [1, WAITS], [2, -1]] and pages.refs.tolist() == [2, 2, 1, 0, 0, 0]
+    fa.check_status(dev)
+    # numbers that no pool has
+    pages = fa.KVPages(i32([[WAITS + 9, 0]], dev), i32([1, 0, 0], dev), 16)
+    fa.resize_kv_pages(pages, i32([0], dev), i32([0], dev))
+    assert reported(dev, 123) and pages.table.tolist() == [[-1, -1]] and pages.refs.tolist() == [0, 0, 0]
+    pages = fa.KVPages(i32([[WAITS + 9, 0]], dev), i32([1, 0, 0], dev), 16)
+    new, _ = fa.fork_kv_pages(pages, i32([32], dev), i32([0], dev))
+    assert reported(dev, 123) and new.table.tolist() == [[-1, 0]] and new.refs.tolist() == [1, 0, 0]
+
+
+def both(pages, model, held, wanted, device, told=True):
+    """The call and the model's, compared; the pairs and what was granted."""
+    granted = torch.full((len(held),), -7, dtype=torch.int32, device=device) if told else None
+    pairs = fa.resize_kv_pages(pages, i32(held, device), i32(wanted, device), granted=granted)
+    want, room, missing = model.resize(held, wanted)
+    assert pairs.tolist() == want and (not told or granted.tolist() == room)
+    table = [list(row) for row in model.table]
+    if not told:
+        for b in model.refused:
+            table[b][held[b] // model.size] += WAITS
+    assert pages.table.tolist() == table and pages.refs.tolist() == model.refs
+    assert reported(device, 125) == missing
+    model.check()
+    return pairs, room
+
+
+def test_a_copy_that_finds_no_page_can_be_asked_for_again(cuda_device):
+    """Two rows share a page that both are to write to, and there is none for the copy.  Both go on holding it and do not grow; once a third row has ended
+    the same call makes the copy."""
+    dev = cuda_device
+    pages = fa.KVPages(i32([[0, -1], [0, -1], [1, -1]], dev), i32([2, 1], dev), 16)
+    for granted in (None, i32([0] * 3, dev)):
+        pairs = fa.resize_kv_pages(pages, i32([9, 9, 4], dev), i32([10, 10, 4], dev), granted=granted)
+        assert reported(dev, 125)
+        first = 0 if granted is not None else WAITS
+        assert pages.table.tolist() == [[first, -1], [first, -1], [1, -1]] and pages.refs.tolist() == [2, 1] and pairs.tolist() == [[-1, -1]] * 3
+    fa.resize_kv_pages(pages, i32([9, 9, 4], dev), i32([10, 10, 4], dev))
+    assert reported(dev, 125)
+    pairs = fa.resize_kv_pages(pages, i32([9, 9, 4], dev), i32([10, 10, 0], dev))
+    assert pages.table.tolist() == [[1, -1], [0, -1], [-1, -1]] and pages.refs.tolist() == [1, 1] and pairs.tolist() == [[0, 1], [-1, -1], [-1, -1]]
+    assert not reported(dev, 125)
+
+
+def test_what_is_granted(cuda_device):
+    dev = cuda_device
+    for table, refs, held, wanted, granted in (
+            ([[0, -1], [0, -1], [1, -1]], [2, 1], [9, 9, 4], [10, 10, 4], [9, 9, 4]),
+            ([[0, -1], [0, -1], [1, -1]], [2, 1], [9, 9, 4], [10, 10, 0], [10, 10, 0]),
+            ([[0, -1], [0, -1], [1, -1]], [2, 1, 0], [9, 9, 4], [10, 30, 6], [10, 16, 6]),        # (the last page is the copy; the keeper gets no other)
+            ([[0, -1], [0, -1], [0, -1]], [3, 0], [9, 9, 9], [10, 10, 10], [10, 9, 9]),           # (one of two copies: the keeper waits for the other)
+            ([[0, -1], [0, -1], [0, -1]], [3, 0], [9, 12, 9], [10, 12, 10], [10, 12, 9]),         # (one that does not write has it too)
+            ([[0, -1], [0, -1], [1, -1], [1, -1]], [2, 2, 0], [9, 9, 3, 5], [10, 10, 4, 6], [10, 10, 3, 5]),
+            ([[-1, -1, -1], [0, -1, -1]], [1, 0, 0], [0, 16], [48, 20], [32, 16]),                # (fresh pages alone)
+            ([[0, -1, 2], [1, -1, -1]], [1, 1, 1, 0], [40, 16], [41, 17], [16, 17]),              # (a gap)
+            ([[0, 1, -1]], [1, 1], [20, ], [25], [25]),
+            ([[0, 1, -1]], [1, 1], [20, ], [3], [3]),
+            ([[0, 1, -1]], [1, 1], [20, ], [0], [0])):
+        model = Model(table, refs, 16)
+        _, got = both(fa.KVPages(i32(table, dev), i32(refs, dev), 16), model, held, wanted, dev)
+        assert got == granted
+    # held beyond the table is cut first
+    got = torch.zeros(1, dtype=torch.int32, device=dev)
+    fa.resize_kv_pages(fa.KVPages(i32([[0, 1]], dev), i32([1, 1], dev), 16), i32([99], dev), i32([99], dev), granted=got)
+    assert got.tolist() == [32]
+    with pytest.raises(RuntimeError, match="code 2 .*site 124,"):
+        fa.check_status(dev)
+
+
+@pytest.mark.parametrize("B,width,pool,size", [(6, 3, 6, 16), (40, 5, 45, 16), (200, 9, 260, 48), (9, 40, 80, 16), (600, 3, 600, 32), (33, 70, 300, 64)])
+@pytest.mark.parametrize("told", [True, False])
+def test_nothing_that_is_held_is_lost(cuda_device, B, width, pool, size, told):
+    """Rows that are forked, cut, grown and ended in a pool that is too small, the writers appending what was granted: every row reads back what it holds.
+    Without `granted` the entries that must not be written to are marked."""
+    dev, rng = cuda_device, random.Random(str((B, width)))
+    model = Model([[-1] * width for _ in range(B)], [0] * pool, size)
+    pages = fa.KVPages.empty(B, width, pool, size, device=dev)
+    data = torch.full((pool, size), -1, dtype=torch.int64, device=dev)
+    held, story, fresh, short, refused = [0] * B, [[] for _ in range(B)], 0, 0, 0
+    for step in range(20):
+        if step % 2 == 1:
+            parents = [rng.choice([b, rng.randrange(B)]) for b in range(B)]
+            pages, now = fa.fork_kv_pages(pages, i32(held, dev), i32(parents, dev))
+            held = model.fork(held, parents)
+            assert now.tolist() == held and pages.table.tolist() == model.table and pages.refs.tolist() == model.refs
+            story = [list(story[a]) for a in parents]
+        most = width * size
+        wanted = [rng.choice([h, min(most, h + 1), min(most, h + 1), min(most, h + rng.randint(1, most // 3)), rng.randint(0, h) if rng.random() < 0.3 else h,
+                              0 if rng.random() < 0.1 else h]) for h in held]
+        pairs, room = both(pages, model, held, wanted, dev, told)
+        fa.copy_kv_pages(data, pairs)
+        short += sum(r < w for r, w in zip(room, wanted))
+        refused += sum(r == h < w and h % size > 0 for h, r, w in zip(held, room, wanted))
+        # (what is granted is never less than what is held and wanted: no row has a gap)
+        assert all(min(h, w) <= r <= w for h, w, r in zip(held, wanted, room))
+        where, what = [], []
+        for b in range(B):
+            story[b] = story[b][:room[b]]
+            for t in range(held[b], room[b]):
+                where.append(model.table[b][t // size] * size + t % size)
+                what.append(fresh)
+                story[b].append(fresh)
+                fresh += 1
+        assert len(set(where)) == len(where)                   # (no two rows write to one place)
+        if where:
+            data.view(-1)[torch.tensor(where, device=dev)] = torch.tensor(what, device=dev)
+        held = room
+        flat = data.view(-1).tolist()
+        for b in range(B):
+            assert [flat[model.table[b][t // size] * size + t % size] for t in range(held[b])] == story[b]
+    assert short > refused > 0                                  # (the pool did run out, for copies too)
+
+
+def test_a_captured_step_in_a_pool_that_runs_out(cuda_device):
+    """Fork, resize, copy and the lengths that were granted in a graph; rows end between replays, and the others go on."""
+    dev, rng = cuda_device, random.Random(8)
+    B, width, size, pool = 12, 4, 16, 20
+    model = Model([[b // 2] + [-1] * (width - 1) for b in range(B)], [2 if p < B // 2 else 0 for p in range(pool)], size)
+    first = fa.KVPages(i32(model.table, dev), i32(model.refs, dev), size)
+    second = fa.KVPages(torch.empty_like(first.table), first.refs, size)
+    held, now, room = [9] * B, [i32([9] * B, dev), i32([0] * B, dev)], i32([0] * B, dev)
+    parents, grow = i32(list(range(B)), dev), i32([1] * B, dev)
+    data = torch.randint(0, 256, (pool, size), dtype=torch.uint8, device=dev)
+    want = data.clone()
+    kept = [t.clone() for t in (first.table, first.refs, now[0], data)]
+
+    def step():
+        fa.fork_kv_pages(first, now[0], parents, out=(second, now[1]))
+        fa.copy_kv_pages(data, fa.resize_kv_pages(second, now[1], (now[1] + grow).clamp(min=0), granted=room))
+        first.table.copy_(second.table)
+        now[0].copy_(room)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for t, x in zip((first.table, first.refs, now[0], data), kept):
+        t.copy_(x)
+    torch.cuda.synchronize()
+    reported(dev, 125)
+    short = 0
+    for i in range(20):
+        p = [rng.choice([b, b, rng.randrange(B)]) for b in range(B)]
+        by = [rng.choice([1, 1, 5, 9, -100 if rng.random() < 0.2 else 1]) for _ in range(B)]
+        held = model.fork(held, p)
+        wanted = [max(0, min(h + n, width * size)) for h, n in zip(held, by)]
+        by = [w - h for h, w in zip(held, wanted)]
+        parents.copy_(i32(p, dev))
+        grow.copy_(i32(by, dev))
+        graph.replay()
+        pairs, held, missing = model.resize(held, wanted)
+        for a, b in pairs:
+            if a >= 0:
+                want[b] = want[a]
+        assert first.table.tolist() == model.table and first.refs.tolist() == model.refs and now[0].tolist() == held and torch.equal(data, want)
+        assert reported(dev, 125) == missing
+        model.check()
+        short += missing
+    assert 0 < short < 20
+
+
+def test_attention_where_a_copy_found_no_page(cuda_device):
+    """What is held is attended to as before while there is no page, and after the copy was made; the row that keeps the page is not written to by the other."""
+    dev = cuda_device
+    H, G, D, size = 2, 4, 64, 16
+    g = torch.Generator(device=dev).manual_seed(3)
+    cache = fa.FP8KVCache.empty(2, size, H, D, device=dev, indexed=True)
+    pages = fa.KVPages.empty(2, 2, 2, size, device=dev)
+    def rows(n, s, h=H):
+        return torch.randn(n, s, h, D, generator=g, device=dev).bfloat16()
+    held, k, v, q = i32([9, 4], dev), rows(2, 9), rows(2, 9), rows(3, 1, G)
+    fa.resize_kv_pages(pages, torch.zeros_like(held), held)
+    fa.append_kv_fp8(cache, k, v, torch.zeros_like(held), page_table=pages.table, seqused_new=held)
+    pages, held = fa.fork_kv_pages(pages, held, i32([0, 0, 1], dev))
+    alone = fa.flash_attn_fp8_cache_func(q, cache, held, page_table=pages.table, causal=True)[0].clone()
+    bytes_of = [t.view(torch.uint8).clone() for t in cache.tensors()]
+    k1, v1 = rows(3, 1), rows(3, 1)
+    # a caller who is not told appends to all, which changes nothing of what is held: the step can be done again
+    pairs = fa.resize_kv_pages(pages, held, held + i32([1, 1, 0], dev))
+    assert reported(dev, 125)
+    fa.copy_kv_pages(cache, pairs)
+    fa.append_kv_fp8(cache, k1, v1, held, page_table=pages.table, seqused_new=i32([1, 1, 0], dev))
+    assert reported(dev, 121)
+    assert all(torch.equal(t.view(torch.uint8), x) for t, x in zip(cache.tensors(), bytes_of))
+    fa.flash_attn_fp8_cache_func(q, cache, held, page_table=pages.table, causal=True)
+    assert reported(dev, 121)
+    granted = torch.empty_like(held)
+    pairs = fa.resize_kv_pages(pages, held, held + i32([1, 1, 0], dev), granted=granted)
+    assert reported(dev, 125) and granted.tolist() == [9, 9, 4]
+    fa.copy_kv_pages(cache, pairs)
+    k, v = rows(3, 1), rows(3, 1)
+    fa.append_kv_fp8(cache, k, v, held, page_table=pages.table, seqused_new=granted - held)
+    assert all(torch.equal(t.view(torch.uint8), x) for t, x in zip(cache.tensors(), bytes_of))
+    assert torch.equal(fa.flash_attn_fp8_cache_func(q, cache, granted, page_table=pages.table, causal=True)[0], alone)
+    pairs = fa.resize_kv_pages(pages, held, i32([10, 10, 0], dev), granted=granted)
+    assert granted.tolist() == [10, 10, 0] and pairs.tolist() == [[0, 1], [-1, -1], [-1, -1]]
+    fa.copy_kv_pages(cache, pairs)
+    fa.append_kv_fp8(cache, k, v, held, page_table=pages.table, seqused_new=granted - held)
+    # the same tokens in caches of their own
+    own = fa.FP8KVCache.empty(2, size, H, D, device=dev, indexed=True)
+    for name, x in zip(("k", "v", "k_scale", "v_scale", "key_bounds", "bound_scale"), bytes_of):
+        getattr(own, name).view(torch.uint8).copy_(x[:1].expand_as(x))
+    fa.append_kv_fp8(own, k[:2], v[:2], held[:2])
+    want = fa.flash_attn_fp8_cache_func(q[:2], own, granted[:2], causal=True)[0]
+    assert torch.equal(fa.flash_attn_fp8_cache_func(q, cache, granted, page_table=pages.table, causal=True)[0][:2], want)
+    fa.check_status(dev)
+
+
+def test_refusals_of_granted(cuda_device):
+    dev = cuda_device
+    p, n = fa.KVPages.empty(3, 4, 10, 16, device=dev), i32([0, 0, 0], dev)
+    for bad in (n.clone().long(), n.clone()[:2], n.cpu(), n.clone()[None], torch.zeros(6, dtype=torch.int32, device=dev)[::2]):
+        with pytest.raises(AssertionError, match="granted"):
+            fa.resize_kv_pages(p, n, n + 1, granted=bad)
+    for bad in (n, p.table.view(-1)[:3], p.refs[:3]):
+        with pytest.raises(AssertionError, match="overlap"):
+            fa.resize_kv_pages(p, n, n + 1, granted=bad)
+    wanted = n + 1
+    with pytest.raises(AssertionError, match="overlap"):
+        fa.resize_kv_pages(p, n, wanted, granted=wanted)
+    none = fa.KVPages(p.table[:0], p.refs, 16)
+    assert fa.resize_kv_pages(none, n[:0], n[:0], granted=n.clone()[:0]).shape == (0, 2)
+    assert not p.refs.any() and (p.table == -1).all()
+    fa.check_status(dev)
