@@ -511,6 +511,7 @@ int launch_fwd(const fa4_nvfp4_params* p, int num_splits, void* workspace, uint6
   kp.page_table = cache.page_table;
   kp.page_size = cache.page_size;
   kp.pages_per_seq = cache.pages_per_seq;
+  kp.num_pages = cache.page_table != nullptr ? cache.num_pages : 0x7fffffff;
   kp.cu_seqlens_q = cache.cu_seqlens_q;
   kp.cu_seqlens_k = cache.cu_seqlens_k;
   kp.cu_seqlens_v = cache.cu_seqlens_v;

@@ -521,7 +521,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         const int kb = __shfl_sync(0xffffffffu, at.x, li & 31), nbl = __shfl_sync(0xffffffffu, at.y, li & 31);
         if (li < n) {
           const int left = is_k ? d.lin.k_rows - nbl * kBlockN : d.lin.v_cols - nbl * 8;   // rows, bytes of a row
-          const uint8_t* src = head + kb * (is_k ? d.lin.k_b : d.lin.v_b) + (is_k ? nbl * kBlockN * row_stride : nbl * 8) +
+          const uint8_t* src = head + page_of_scales(p, page_of_tiles(p, kb)) * (is_k ? d.lin.k_b : d.lin.v_b) + (is_k ? nbl * kBlockN * row_stride : nbl * 8) +
                                lane * row_stride;
           const uint32_t skew = (uint32_t)(reinterpret_cast<uintptr_t>(src) & 3u);
           const uint32_t end = skew + (is_k || left > 8 ? 8u : (uint32_t)left);
@@ -576,7 +576,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     for (; li < n; ++li) {
       if ((li & 31) == 0 && li > 0 && !kLinear) at = locate(li);
       const uint32_t st = li % kDepth;
-      const int kb = __shfl_sync(0xffffffffu, at.x, li & 31), nbl = __shfl_sync(0xffffffffu, at.y, li & 31);
+      const int kb = page_of_tiles(p, __shfl_sync(0xffffffffu, at.x, li & 31)), nbl = __shfl_sync(0xffffffffu, at.y, li & 31);
       const bool lead = elect_one();
       if (lead) {
         if (li >= kDepth) ok = mbar_wait(bar(free0 + st), ((li - kDepth) / kDepth) & 1, wc, is_k ? kDKFree : kDVFree);
@@ -585,7 +585,8 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
           else mbar_arrive_expect_tx(bar(full0 + st), kTileBytes + kSfBytes);
           load_tile(st, kb, nbl);
           if constexpr (!kLinear)
-            bulk_load(sf0 + st * kSfBytes, sf_src + kb * sf_stride_b + (int64_t)nbl * kSfBytes, kSfBytes, bar(full0 + st));
+            bulk_load(sf0 + st * kSfBytes, sf_src + page_of_scales(p, kb) * sf_stride_b + (int64_t)nbl * kSfBytes, kSfBytes, bar(full0 + st));
+          report_page(p, kb);
         }
       }
       ok = __all_sync(0xffffffffu, ok);

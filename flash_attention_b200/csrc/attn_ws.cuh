@@ -412,7 +412,7 @@ attn_fwd_ws_kernel(const __grid_constant__ CUtensorMap tm_q,
           if constexpr (kGeneral) {
             if (p.page_table != nullptr) {
               const int pg = fast_div(nb, p.div_page);
-              kb = p.page_table[(int64_t)t.b * p.pages_per_seq + pg];
+              kb = page_of_tiles(p, p.page_table[(int64_t)t.b * p.pages_per_seq + pg]);
               nbl = nb - pg * (p.page_size / kBlockN);
             }
           }
@@ -435,9 +435,10 @@ attn_fwd_ws_kernel(const __grid_constant__ CUtensorMap tm_q,
             tma_load_4d(base + kOffK + st * kTileBytes, &tm_k, bars.at(Bars::kKFull + st), 0, t.hk,
                         nbl * kBlockN, kb);
             bulk_load(base + kOffSFK + st * kSfBytes,
-                      p.k_sf + kb * p.ksf_stride_b + t.hk * p.ksf_stride_h + (int64_t)nbl * kQkSfBytes,
+                      p.k_sf + (kGeneral ? page_of_scales(p, kb) : kb) * p.ksf_stride_b + t.hk * p.ksf_stride_h + (int64_t)nbl * kQkSfBytes,
                       kQkSfBytes, bars.at(Bars::kKFull + st));
             issued_k = G + 1;
+            if constexpr (kGeneral) report_page(p, kb);
           }
           if (iv >= 0 && iv < n) {
             const uint32_t G = gb + iv, st = G % kStagesV;
@@ -453,7 +454,7 @@ attn_fwd_ws_kernel(const __grid_constant__ CUtensorMap tm_q,
             tma_load_4d(base + kOffV + st * kTileBytes, &tm_v, bars.at(Bars::kVFull + st),
                         nbl * (kBlockN / 2), 0, t.hk, kb);
             bulk_load(base + kOffSFV + st * kSfBytes,
-                      p.v_sf + kb * p.vsf_stride_b + t.hk * p.vsf_stride_h + (int64_t)nbl * kSfBytes,
+                      p.v_sf + (kGeneral ? page_of_scales(p, kb) : kb) * p.vsf_stride_b + t.hk * p.vsf_stride_h + (int64_t)nbl * kSfBytes,
                       kSfBytes, bars.at(Bars::kVFull + st));
             issued_v = G + 1;
           }

@@ -607,23 +607,23 @@ attn_fwd_ws64_kernel(const __grid_constant__ CUtensorMap tm_q,
           const uint32_t full = bars.at(full0 + st);
           mbar_arrive_expect_tx(full, is_k ? kQkBytes + kQkSfBytes : kVBytes + kSfBytes);
           // where logical K/V block nb of this batch entry lives: the entry itself, or (KV-cache views) a
-          // page of the pool and the block in it
+          // page of the pool and the block in it (page -1: zeros, under the scale factors of page 0)
           int kb = t.b, nbl = nb;
           if constexpr (kWindow || kCache) {
             if (p.page_table != nullptr) {
               const int pg = fast_div(nb, p.div_page);
-              kb = p.page_table[(int64_t)t.b * p.pages_per_seq + pg];
+              kb = page_checked_at_once(p, p.page_table[(int64_t)t.b * p.pages_per_seq + pg]);
               nbl = nb - pg * (p.page_size / kBlockN);
             }
           }
           if (is_k) {
             load_qk_tile(base + kOffK + st * kQkSlot, &tm_k, full, t.hk, k0 + nbl * kBlockN, packed ? 0 : kb);
             bulk_load(base + kOffSFK + st * kQkSfSlot,
-                      p.k_sf + kb * p.ksf_stride_b + t.hk * p.ksf_stride_h + (int64_t)nbl * kQkSfBytes, kQkSfBytes, full);
+                      p.k_sf + max(kb, 0) * p.ksf_stride_b + t.hk * p.ksf_stride_h + (int64_t)nbl * kQkSfBytes, kQkSfBytes, full);
           } else {
             tma_load_4d(base + kOffV + st * kTileBytes, &tm_v, full, (k0 + nbl * kBlockN) / 2, 0, t.hk, packed ? 0 : kb);
             bulk_load(base + kOffSFV + st * kSfBytes,
-                      p.v_sf + kb * p.vsf_stride_b + t.hk * p.vsf_stride_h + (int64_t)nbl * kSfBytes, kSfBytes, full);
+                      p.v_sf + max(kb, 0) * p.vsf_stride_b + t.hk * p.vsf_stride_h + (int64_t)nbl * kSfBytes, kSfBytes, full);
           }
           issued = G + 1;
         }

@@ -26,13 +26,7 @@
 
 namespace fa4 {
 
-enum Fp8Site { kPositionSite = 120, kPageSite = 121, kRotationSite = 122 };
-
-// Records an index outside its range (the first failure stays); the caller leaves out what it leads to.
-__device__ __forceinline__ void report_bad_index(uint32_t* status, uint32_t epoch, uint32_t site) {
-  if (status != nullptr)
-    atomicCAS(status, 0u, (kStatusBadIndex << 24) | (site << 16) | ((epoch & 0xffu) << 8) | (blockIdx.x & 0xffu));
-}
+enum Fp8Site { kPositionSite = 120, kRotationSite = 122 };
 
 struct AppendParams {
   const __nv_bfloat16 *k, *v, *q;

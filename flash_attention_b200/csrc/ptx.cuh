@@ -56,6 +56,13 @@ __device__ __forceinline__ void report_status(const WaitCtx& w, uint32_t code, u
   }
 }
 
+// Records an index outside its range (the first failure stays); the caller leaves out what it leads to.
+constexpr uint32_t kPageSite = 121u;       // a page number
+__device__ __forceinline__ void report_bad_index(uint32_t* status, uint32_t epoch, uint32_t site) {
+  if (status != nullptr)
+    atomicCAS(status, 0u, (kStatusBadIndex << 24) | (site << 16) | ((epoch & 0xffu) << 8) | (blockIdx.x & 0xffu));
+}
+
 // Exactly one lane of a converged warp, for the roles of one thread that issue copies and products.
 // Their operands (addresses, descriptors, coordinates, tensor-memory columns) are uniform-register operands of
 // the instructions.  Behind elect.sync the compiler knows that one thread runs the branch and keeps them

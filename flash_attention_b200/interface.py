@@ -118,7 +118,9 @@ def flash_attn_fp4_func(
     int32: k, v and their scales are then a POOL of pages, k (num_pages, page_size, Hkv, D/2),
     v (num_pages, Hkv, Dv, page_size/2), scales per page in either layout, page_size a multiple
     of 128; the logical key length is ``pages_per_seq * page_size``.  Scale bytes of unused
-    cache slots must not be NaN encodings (a zero-filled cache is fine).
+    cache slots must not be NaN encodings (a zero-filled cache is fine).  Entries behind
+    ``seqused_k`` may be anything; keys and values of a page outside the pool read as zeros,
+    and :func:`check_status` raises.
 
     Built so far: D = Dv = 128 or 64, or (D, Dv) = (192, 128) (every feature but split-KV and the
     decode kernel); any Sq and Sk, as in the reference (partial last tiles are handled by

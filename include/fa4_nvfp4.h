@@ -75,9 +75,9 @@ enum {
 enum {
   FA4_S_OK = 0,
   FA4_S_WAIT_EXPIRED = 1, /* a bounded mbarrier wait ran out; `site` names the wait */
-  FA4_S_BAD_INDEX = 2    /* 8-bit cache: an index on the device lies outside its range and what it leads to was left
-                            out; `site`: 120 a position behind the cache's end, 121 a page number, 122 a position without a row
-                            in the rotation's tables.  Stops nothing, and gives way to FA4_S_WAIT_EXPIRED */
+  FA4_S_BAD_INDEX = 2    /* caches: an index on the device lies outside its range and what it leads to was left
+                            out; `site`: 120 a position behind the cache's end, 121 a page number (its keys and values read as
+                            zeros), 122 a position without a row in the rotation's tables, 123 to 127 pages and their tables.  Stops nothing, and gives way to FA4_S_WAIT_EXPIRED */
 };
 
 /* kernel variants */
@@ -184,7 +184,8 @@ typedef struct fa4_nvfp4_ext {
                                seqused_k[b] keys (clamped to 0..Sk); causal and window limits align
                                to that length.  NULL = Sk for every entry.  Scale bytes of the
                                unused slots must not be NaN encodings (a zero-filled cache is fine) */
-  const int32_t* page_table;/* (B, pages_per_seq) page numbers on the device, or NULL.  With a table
+  const int32_t* page_table;/* (B, pages_per_seq) page numbers on the device, or NULL; one that is needed and not below
+                               num_pages is recorded as FA4_S_BAD_INDEX.  With a table
                                p->k / p->v / p->k_sf / p->v_sf describe a POOL of num_pages pages of
                                page_size keys: k (num_pages, page_size, Hkv, D/2), v (num_pages, Hkv,
                                Dv, page_size/2), tiled scales per page; k_stride_b / v_stride_b are
