@@ -162,6 +162,8 @@ def index_kv_fp8(
     Of a block and kv head: the largest and the smallest value of every channel, in steps of ``k_scale`` times a power of two that bring the largest
     magnitude to 64 .. 120, rounded outwards to int8; ``bound_scale`` is a step.  A block with a NaN has bounds of 0 and a ``bound_scale`` of NaN.
     (Where tokens of a block are dropped again, its bounds stay those of all of them until the next call for it.)
+    Sequences of a call that share a block (a page that :func:`fork_kv_pages` gave to several) must have the same tokens of it: they write the same bounds then; of different ones it is
+    not defined which are written, and whether bounds and scale are of the same.  Several calls, the one with most of the block's tokens last, give bounds for all.
     One launch, no synchronisation; can be captured in a graph.  Positions and page numbers outside the cache are left out, and
     :func:`check_status` raises.
     """

@@ -605,7 +605,7 @@ typedef struct fa4_fp8_index {
 } fa4_fp8_index;
 /*
  * The bounds of all blocks that tokens seqlens[b] .. seqlens[b] + seqused_new[b] - 1 (NULL: S; at most S) lie in, made anew from the cache.
- * Tokens behind those are not looked at.
+ * Tokens behind those are not looked at.  Sequences that share a block have the same tokens of it in one call (they write the same then).
  */
 typedef struct fa4_fp8_index_call {
   uint32_t struct_size;      /* = sizeof(fa4_fp8_index_call) */
