@@ -4,8 +4,8 @@
 // free.  The book-keeping is a few thousand whole numbers: one cluster of eight CTAs does it in one launch, in phases between
 // rendezvous of the cluster, so nothing waits for the host and results do not depend on the order of threads (counters are
 // only added to; what is given away is ranked by prefix sums: rows in order, free pages from the lowest on).  What bounds it is latency: a launch, three or four rendezvous
-// and a trip to memory between each.  us back to back: resize of 128 rows of 18 pages in a pool of 1315 8.7, 256 of 66 in 11761 9.9, 256 of 512 in 70000 15.4, 1024 of 256 in 300000 34;
-// compact of the same 11, 13, 21, 51; fork of 128 rows 2.2.
+// and a trip to memory between each.  us back to back: resize of 128 rows of 18 pages in a pool of 1315 8.6, 256 of 66 in 11761 10.4, 256 of 512 in 70000 15.4, 1024 of 256 in 300000 30;
+// compact of the same 11, 13, 21, 52; fork of 128 rows 2.2.  A row is one warp's, which reads its entries 128 at a time: 64 rows of 4096 entries in 300000 48 (compact 53, fork 11.6).
 #pragma once
 #include "fp8_append.cuh"
 
@@ -144,16 +144,15 @@ __global__ void __launch_bounds__(kThreads) resize_kernel(const __grid_constant_
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int j0 = j1 + 32 * i, j = j0 + lane;
-        int e = page_in(entry[i]);
+        if (j0 >= k.width) break;
+        int e = max(page_in(entry[i]), -1);
         if (e >= k.num_pages) {
           report_bad_index(k.status, k.epoch, kTableSite);
           e = -1;
         }
-        if (e != entry[i] && j < k.width) row[j] = e;
-        if (j < k.width && j >= keep && e >= 0) {
-          atomicSub(k.refs + e, 1);
-          row[j] = -1;
-        }
+        const bool gone = j >= keep && j < k.width && e >= 0;
+        if (gone) atomicSub(k.refs + e, 1);
+        if (gone || (e != entry[i] && j < k.width)) row[j] = gone ? -1 : e;
         const uint32_t none = __ballot_sync(0xffffffffu, j < keep && e < 0);
         if (none != 0u && gap == keep) gap = j0 + __ffs(none) - 1;
         // (a row that grows keeps the page its next token goes to)
@@ -231,13 +230,13 @@ __global__ void __launch_bounds__(kThreads) resize_kernel(const __grid_constant_
     const int writes_to = __ldcg(writes + b), lack_here = __ldcg(lacks + b);
     const bool copies = writes_to >= 0 && (writes_to & kCopied) != 0;
     const Lengths n = lengths_of(p, b, false);
-    const int want = pages_of(k, n.wanted), at = copies ? fast_div(n.held, k.div_page) : -1;
     int32_t* row = k.table + (int64_t)b * k.width;
-    int next = s_first[b], fresh = -1, room = lack_here < 0 ? (-1 - lack_here) * k.page_size : n.wanted;
-    const int last = next + max(lack_here, 0);
-    // (a copy takes the first of a row's pages.  Pages run out for all rows behind one, so if a sharer's copy has none, the row that was to keep the original
+    // Entries that lack a page lie side by side, up to that of the last token: there is no gap in front of them, and a page that is copied is the last of those that hold tokens.
+    const int lacks_here = max(lack_here, 0), from = pages_of(k, n.wanted) - lacks_here, next = s_first[b];
+    int got = min(max(free_pages - next, 0), lacks_here), room = lack_here < 0 ? (-1 - lack_here) * k.page_size : got < lacks_here ? (from + got) * k.page_size : n.wanted;
+    // (pages run out for all rows behind one, so if a sharer's copy has none, the row that was to keep the original
     // gets none either; what it would write there belongs to both)
-    bool refused = copies && next >= free_pages;
+    bool refused = copies && got == 0;
     if (total > free_pages && writes_to >= 0 && !copies) {
       bool waits = false;
       for (int i = lane; i < b; i += 32) waits = waits || (__ldcg(writes + i) == (writes_to | kCopied) && s_first[i] >= free_pages);
@@ -250,29 +249,16 @@ __global__ void __launch_bounds__(kThreads) resize_kernel(const __grid_constant_
         if (p.granted == nullptr) row[fast_div(n.held, k.div_page)] = (writes_to & ~kCopied) | kWaits;
       }
       room = n.held;
-      next = last;
+    } else if (got < lacks_here && lane == 0) {
+      report_bad_index(k.status, k.epoch, kPoolSite);
     }
-    for (int j0 = 0; j0 < want && next < last; j0 += 32) {
-      const int j = j0 + lane;
-      const bool lack = j < want && (j == at || row[j] < 0);
-      const uint32_t mask = __ballot_sync(0xffffffffu, lack);
-      const int i = next + __popc(mask & ((1u << lane) - 1u));
-      int page = -1;
-      if (lack) {
-        if (i < free_pages) page = __ldcg(free_page + i);
-        else report_bad_index(k.status, k.epoch, kPoolSite);
-        row[j] = page;
-      }
-      if (j0 <= at && at < j0 + 32) fresh = __shfl_sync(0xffffffffu, page, at & 31);
-      const uint32_t none = __ballot_sync(0xffffffffu, lack && page < 0);
-      if (none != 0u) room = min(room, (j0 + __ffs(none) - 1) * k.page_size);
-      next += __popc(mask);
-    }
+    for (int i = lane; i < got; i += 32) row[from + i] = __ldcg(free_page + next + i);
     if (lane == 0) {
-      const int from = writes_to & ~kCopied;
-      if (fresh >= 0) atomicSub(k.refs + from, 1);
-      p.pairs[2 * b] = fresh >= 0 ? from : -1;
-      p.pairs[2 * b + 1] = fresh;
+      const bool done = copies && !refused;
+      const int page = writes_to & ~kCopied;
+      if (done) atomicSub(k.refs + page, 1);
+      p.pairs[2 * b] = done ? page : -1;
+      p.pairs[2 * b + 1] = done ? __ldcg(free_page + next) : -1;
       if (p.granted != nullptr) p.granted[b] = room;
     }
   }
