@@ -667,7 +667,9 @@ int launch_fwd(const fa4_nvfp4_params* p, int num_splits, void* workspace, uint6
       // fifth of what an SM's instruction cache holds (24 packed sequences up to 2048, no cap: 174 us with the code in
       // the kernel, 168 without).
       const bool cap = softcap > 0.f;
-      if (general && local && narrow)           // window (with or without sink / cache view)
+      if (general && local && narrow && cache.page_table == nullptr)           // window (with or without sink / cache view)
+        rc = cap ? FA4_WS64(true, true, true, true, true, false) : FA4_WS64(true, true, true, true, false, false);
+      else if (general && local && narrow)
         rc = cap ? FA4_WS64(true, true, true, true, true) : FA4_WS64(true, true, true, true);
       else if (general && local)
         rc = cap ? FA4_WS64(true, true, true, false, true) : FA4_WS64(true);

@@ -102,20 +102,15 @@ struct KernelParams {
 };
 
 // Page numbers come from the device and may lie outside the pool.  Such a one becomes num_pages, where the tensor maps end, so that K and V read as
-// zeros; scale factors have no tensor map and are taken from the last page.  It is reported behind the copies, which do not wait for the comparison.
-// us, without / with: one token of 16 sequences of up to 8192 keys 28.0 / 28.1, linear scales 35.1 / 32.0, 512 rows over 16384 keys in two splits 128.3 / 130.5.
+// zeros; scale factors have no tensor map and are taken from the last page.  It is reported behind the copies, which do not wait for the comparison; by the 64-key
+// kernel at its end, from a flag in shared memory (a report in its loaders moved the compiler's code of the softmax loop: 512 rows over 16384 keys 100 -> 114 us).
+// us, without / with: one token of 16 sequences of up to 8192 keys 28.0 / 28.0, linear scales 35.1 / 32.1, 512 rows over 16384 keys 100.4 / 100.3, in two splits 128.3 / 130.5;
+// and where no table is: windows of 511 keys, D = 64 66.7 / 68.4, of 127 keys with sinks 69.6 / 70.3, with a soft cap 53.0 / 51.7.
 __device__ __forceinline__ int page_of_tiles(const KernelParams& p, int page) { return (int)min((uint32_t)page, (uint32_t)p.num_pages); }
 __device__ __forceinline__ int page_of_scales(const KernelParams& p, int page) { return min(page, p.num_pages - 1); }
 static __device__ __noinline__ void report_page_slow(uint32_t* status, uint32_t epoch) { report_bad_index(status, epoch, kPageSite); }
 __device__ __forceinline__ void report_page(const KernelParams& p, int page) {
   if (page == p.num_pages) report_page_slow(p.status, p.epoch);
-}
-// The same for the 64-key kernel, at once and with -1 in num_pages' place: any report behind the copies, inline or not, moved the compiler's code of its
-// softmax loop (512 rows over 16384 keys 100 -> 114 us; this way 100).
-__device__ __forceinline__ int page_checked_at_once(const KernelParams& p, int page) {
-  if ((uint32_t)page < (uint32_t)p.num_pages) return page;
-  report_bad_index(p.status, p.epoch, kPageSite);
-  return -1;
 }
 
 // The three numbers the scales of a call fold into.  With scales on the device every thread that needs

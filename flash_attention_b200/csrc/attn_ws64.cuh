@@ -112,6 +112,7 @@ struct Bars {
   __device__ __forceinline__ uint32_t at(uint32_t idx) const { return base + 8u * idx; }
 };
 constexpr uint32_t kOffMisc = kOffBar + 8 * Bars::kCount;
+constexpr uint32_t kOffBadPage = kOffMisc + 8;      // behind the abort flag: whether a page lay outside the pool
 constexpr uint32_t kSmemUsed = kOffMisc + 16 + sizeof(WaitCtx);
 constexpr uint32_t kSmemRequest = kSmemUsed + 1024;
 static_assert(kSmemRequest <= 227 * 1024, "shared memory");
@@ -281,8 +282,9 @@ __device__ __forceinline__ uint32_t sw32_offset(uint32_t row, uint32_t chunk) {
 // tile and costs a long one, since the branch sits in the hot loop.  us, wide form -> this one: 127-key window, D = 64
 // 83.6 -> 75.1; 1023 keys, D = 128 106.5 -> 108.5 (the line lies in api.cu).  Of the 75, by masks that pass over the
 // 32-key halves a warp sees whole and a second accumulator, 69 are left.
+// kTable: the cache may have a page table (narrow windows have a form without: 127 keys, D = 64, sinks 71.5 -> 70.3 us, D = 128 46.3 -> 45.5; wide ones gained nothing).
 template <int kD, bool kGeneral = false, bool kWindow = kGeneral, bool kCache = kWindow, bool kNarrow = false,
-          bool kCap = false>
+          bool kCap = false, bool kTable = kWindow || kCache>
 __global__ void __launch_bounds__(ws64::kThreads, 1)
 attn_fwd_ws64_kernel(const __grid_constant__ CUtensorMap tm_q,
                      const __grid_constant__ CUtensorMap tm_k,
@@ -311,6 +313,7 @@ attn_fwd_ws64_kernel(const __grid_constant__ CUtensorMap tm_q,
 
   if (tid == 0) {
     *s_abort = 0u;
+    if constexpr (kTable) s_abort[1] = 0u;
     wc = WaitCtx{s_abort, p.status, p.budget_ns, p.epoch};
     for (int b = 0; b < 2; ++b) {
       mbar_init(bars.at(Bars::kQFull + b), 1);
@@ -607,25 +610,27 @@ attn_fwd_ws64_kernel(const __grid_constant__ CUtensorMap tm_q,
           const uint32_t full = bars.at(full0 + st);
           mbar_arrive_expect_tx(full, is_k ? kQkBytes + kQkSfBytes : kVBytes + kSfBytes);
           // where logical K/V block nb of this batch entry lives: the entry itself, or (KV-cache views) a
-          // page of the pool and the block in it (page -1: zeros, under the scale factors of page 0)
+          // page of the pool and the block in it
           int kb = t.b, nbl = nb;
-          if constexpr (kWindow || kCache) {
+          if constexpr (kTable) {
             if (p.page_table != nullptr) {
               const int pg = fast_div(nb, p.div_page);
-              kb = page_checked_at_once(p, p.page_table[(int64_t)t.b * p.pages_per_seq + pg]);
+              kb = page_of_tiles(p, p.page_table[(int64_t)t.b * p.pages_per_seq + pg]);
               nbl = nb - pg * (p.page_size / kBlockN);
             }
           }
           if (is_k) {
             load_qk_tile(base + kOffK + st * kQkSlot, &tm_k, full, t.hk, k0 + nbl * kBlockN, packed ? 0 : kb);
             bulk_load(base + kOffSFK + st * kQkSfSlot,
-                      p.k_sf + max(kb, 0) * p.ksf_stride_b + t.hk * p.ksf_stride_h + (int64_t)nbl * kQkSfBytes, kQkSfBytes, full);
+                      p.k_sf + (kTable ? page_of_scales(p, kb) : kb) * p.ksf_stride_b + t.hk * p.ksf_stride_h + (int64_t)nbl * kQkSfBytes, kQkSfBytes, full);
           } else {
             tma_load_4d(base + kOffV + st * kTileBytes, &tm_v, full, (k0 + nbl * kBlockN) / 2, 0, t.hk, packed ? 0 : kb);
             bulk_load(base + kOffSFV + st * kSfBytes,
-                      p.v_sf + max(kb, 0) * p.vsf_stride_b + t.hk * p.vsf_stride_h + (int64_t)nbl * kSfBytes, kSfBytes, full);
+                      p.v_sf + (kTable ? page_of_scales(p, kb) : kb) * p.vsf_stride_b + t.hk * p.vsf_stride_h + (int64_t)nbl * kSfBytes, kSfBytes, full);
           }
           issued = G + 1;
+          if constexpr (kTable)
+            if (kb == p.num_pages) asm volatile("st.shared.u32 [%0], %1;" ::"r"(base + kOffBadPage), "r"(1) : "memory");
         }
         if (!ok) break;
         gb += n;
@@ -983,6 +988,8 @@ attn_fwd_ws64_kernel(const __grid_constant__ CUtensorMap tm_q,
   tc_fence_before_sync();
   __syncthreads();
   if (warp == kIssuerWarp) tmem_dealloc(tmem, kTmemCols);
+  if constexpr (kTable)
+    if (tid == 0 && s_abort[1] != 0u) report_bad_index(p.status, p.epoch, kPageSite);
 }
 
 }  // namespace fa4

@@ -15,6 +15,7 @@ pytestmark = pytest.mark.gpu
     (70, 4, 2, 128, 128, True, dict(variant=fa.VARIANT_WS64)), (200, 4, 4, 128, 128, False, dict(variant=fa.VARIANT_WS64)),
     (70, 4, 2, 64, 64, True, dict(variant=fa.VARIANT_WS64)), (33, 2, 1, 192, 128, True, dict(variant=fa.VARIANT_WS64)),
     (70, 4, 2, 128, 128, True, dict(variant=fa.VARIANT_WS64, window_size=(700, 0), softcap=20.0)),
+    (70, 4, 2, 128, 128, True, dict(variant=fa.VARIANT_WS64, window_size=(100, 0))), (70, 4, 2, 64, 64, True, dict(variant=fa.VARIANT_WS64, window_size=(100, 0), softcap=20.0)),
     (70, 4, 2, 128, 128, True, dict(variant=fa.VARIANT_WS)), (150, 4, 2, 128, 128, True, dict(variant=fa.VARIANT_WS, num_splits=2)),
     (40, 4, 2, 64, 64, False, dict(variant=fa.VARIANT_WS, num_splits=3))])
 def test_pages_outside_the_pool(cuda_device, layout, Sq, Hq, Hkv, D, Dv, causal, kw):
