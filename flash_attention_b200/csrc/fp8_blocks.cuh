@@ -30,8 +30,8 @@ struct IndexParams {
 
 constexpr int kIndexWarps = 4;
 
-// A warp a block and kv head: kD / 16 lanes a row of 16-byte pieces, maxima and minima as pairs of fp16 (every e4m3 value is one).  It waits for loads: 131072 tokens of 8 heads,
-// blocks of 64 (118 MB) 26.2 us, 4.5 TB/s at 31 warps an SM; eight rows of a lane on their way rather than four 28 (80 registers), warps that go on to a next block 31.5.
+// A warp a block and kv head: kD / 16 lanes a row of 16-byte pieces, maxima and minima as pairs of fp16 (every e4m3 value is one).  It waits for loads: 111700 tokens of 8 heads,
+// blocks of 64 (118 MB read and written) 26.3 us, 4.5 TB/s at 31 warps an SM, issue slots 47 % busy; eight rows of a lane on their way rather than four 28 (80 registers), warps that go on to a next block 31.5.
 template <int kD>
 __global__ void __launch_bounds__(kIndexWarps * 32) fp8_index_kernel(const __grid_constant__ IndexParams p) {
   constexpr int kChunks = kD / 16, kRows = 32 / kChunks;

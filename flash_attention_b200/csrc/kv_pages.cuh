@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(kCopyThreads) copy_kernel(const __grid_constan
 }
 
 // Through shared memory by bulk copies, for pages that lie in one piece: a warp with a ring of places, of which half are being loaded and half stored.
-// HBM bounds it: 2322 pages of 131 KB (609 MB read and written) 103 us, 5.9 TB/s, 90 % of a measured copy; the kernel above 112.  Rings of 12 places of 16 KB
+// HBM bounds it: 2322 pages of 131 KB (609 MB read and written) by itself 103 us, 5.9 TB/s, 90 % of a measured copy (the kernel above 112), behind other work 108.  Rings of 12 places of 16 KB
 // or 6 of 32 KB in one CTA an SM 103, of 24 of 8 KB 110.
 constexpr int kBulkBytes = 16384, kBulkPlaces = 6, kBulkCtas = 2;      // (CTAs of an SM)
 constexpr uint32_t kBulkRequest = kBulkPlaces * kBulkBytes + 128;

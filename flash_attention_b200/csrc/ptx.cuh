@@ -240,7 +240,7 @@ __device__ __forceinline__ int fast_div(int n, FastDiv f) {
 // descriptor prefetch) and then pdl_wait()s, which returns when that kernel has finished and its
 // writes are visible -- before the first access to global memory, inputs included.  pdl_trigger()
 // lets the next kernel do the same with this one; without it the next kernel's CTAs start as this
-// one's exit.  Only the attention kernels trigger early, and only
+// one's exit.  Only the attention kernels and the choice of blocks in front of one trigger early, the attention kernels only
 //   * behind their tensor-memory allocation: a waiting successor on the same SM may hold tensor
 //     memory, and must not be able to take it before the kernel it waits for has its own;
 //   * not so the small kernels in front of a persistent one: its CTAs then started one by one

@@ -98,7 +98,7 @@ def compact_kv_pages(pages: KVPages) -> Tuple[torch.Tensor, torch.Tensor]:
     int32.  ``pages`` is changed in place; the table must be the only one that names pages of the pool.
 
     With n pages in use the i-th of those numbered n or above goes to the i-th free one below; what lies at n and above is free afterwards (the pool may be cut there once
-    :func:`copy_kv_pages` has run).  One launch, no synchronisation; can be captured in a graph.
+    :func:`copy_kv_pages` has run).  A table without rows is refused.  One launch, no synchronisation; can be captured in a graph.
     """
     return _lib.host().compact_pages(pages.table, pages.refs, pages.page_size)
 
@@ -109,7 +109,7 @@ def copy_kv_pages(cache: Union[FP8KVCache, torch.Tensor, Sequence], pairs: torch
     ``cache``: an :class:`FP8KVCache` (its index too), a tensor whose first dimension is that of pages (any type, strided as a pool may be), or a sequence of
     such (all of one number of pages).  No page may be written twice, or both read and written, in one call: what the other calls return has no such pairs.
 
-    One launch for eight tensors, no synchronisation; can be captured in a graph.  Pairs outside the pool are left out, and :func:`check_status` raises.
+    One launch for eight tensors (from 64 MB on two, if pages of some lie in one piece and of others not), no synchronisation; can be captured in a graph.  Pairs outside the pool are left out, and :func:`check_status` raises.
     """
     if isinstance(cache, FP8KVCache):
         tensors = cache.tensors()
