@@ -159,9 +159,11 @@ __global__ void __launch_bounds__(kThreads) resize_kernel(const __grid_constant_
         if (j0 <= at && at < j0 + 32) page = __shfl_sync(0xffffffffu, e, at & 31);
       }
     }
-    // (no page that could be put in a gap has what the row holds there: such a row gets nothing, and is reported)
+    // (no page that could be put in a gap has what the row holds there: such a row gets nothing, and is reported; others may have the page its next token would go to)
+    const bool into = n.wanted > n.held && n.held != at * k.page_size && page >= 0;
+    if (gap < keep && into && p.granted == nullptr && lane == (at & 31)) row[at] = page | kWaits;
     if (lane == 0) {
-      writes[b] = gap == keep && n.wanted > n.held && n.held != at * k.page_size && page >= 0 ? page : -1;
+      writes[b] = gap == keep && into ? page : -1;
       lacks[b] = gap == keep ? max(want - keep, 0) : -1 - gap;
       if (gap < keep) report_bad_index(k.status, k.epoch, kPoolSite);
     }

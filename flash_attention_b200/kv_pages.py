@@ -63,7 +63,8 @@ def resize_kv_pages(pages: KVPages, held: torch.Tensor, wanted: torch.Tensor, gr
     * a copy is not made: the sequence goes on sharing the page, and neither it nor the one that was to keep the page gets to write there.  With ``granted`` their entries stay and can be
       read; without it they become -2^31 + page, which the calls on a cache take for no page (nothing is appended or read there, and they report it), until the next call of this function
       that has a page or does not let them grow;
-    * a sequence that has no page for some of the tokens it keeps (they were left out before) gets nothing until it is cut in front of them: what they were is lost.
+    * a sequence that has no page for some of the tokens it keeps (they were left out before) gets nothing until it is cut in front of them: what they were is lost.  Without ``granted``
+      the page that its next token would go to is marked in the same way.
 
     ``granted`` (B,) int32, overlapping none of the others, is written: the lengths that may be appended up to.  That is ``wanted`` if nothing was missing, else the tokens in front
     of the first entry without a page, or ``held`` where a copy was not made; append with ``seqused_new=granted - held`` and go on with it as the next held.  The same call works once

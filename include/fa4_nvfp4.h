@@ -684,7 +684,7 @@ typedef struct fa4_kv_pages {
  *
  * A copy that finds no page is recorded; the pair is (-1, -1) and refs stay.  The row goes on sharing the page, and neither it nor the row that was to keep the page may write there:
  * with `granted` both have the lengths they hold, and their entries stay; without it their entries become -2^31 + page, which is no page for the calls on caches
- * and is one again behind the next call that finds a page or does not let the row grow.
+ * and is one again behind the next call that finds a page or does not let the row grow.  (So does, without `granted`, the entry that the next token of a row with a gap would go to.)
  *
  * granted (B,), or NULL: the lengths that the rows have pages of their own for, which may be appended up to: wanted[b], or where something was missing the
  * tokens in front of the first entry without a page; held[b] where a copy found none.

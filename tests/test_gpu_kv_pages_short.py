@@ -15,6 +15,9 @@ def i32(x, device):
     return torch.tensor(x, dtype=torch.int32, device=device)
 
 
+WAITS = -2 ** 31                 # on the page of an entry that must not be written to
+
+
 def reported(device, site):
     """Whether calls so far have recorded a bad index, which has to be one of `site`."""
     try:
@@ -43,11 +46,14 @@ def test_lengths_outside_the_table_are_reported(cuda_device):
 def test_a_gap_is_not_filled_without_a_word(cuda_device):
     """Entry 1 of the first row has no page although it holds tokens there: nothing that could be put there is what it holds."""
     dev = cuda_device
-    for wanted, row0, refs, first in ((50, [0, -1, 2, -1], [1, 1, 1, 1, 0, 0], 3),       # (grows: gets nothing)
-                                      (40, [0, -1, 2, -1], [1, 1, 1, 1, 0, 0], 3),       # (stays)
-                                      (20, [0, -1, -1, -1], [1, 1, 1, 0, 0, 0], 2)):     # (loses what is behind)
+    told = i32([0, 0], dev)
+    for wanted, row0, refs, first, granted in ((50, [0, -1, 2, -1], [1, 1, 1, 1, 0, 0], 3, told),       # (grows: gets nothing)
+                                               (50, [0, -1, WAITS + 2, -1], [1, 1, 1, 1, 0, 0], 3, None),
+                                               (48, [0, -1, WAITS + 2, -1], [1, 1, 1, 1, 0, 0], 3, None),
+                                               (40, [0, -1, 2, -1], [1, 1, 1, 1, 0, 0], 3, None),       # (stays)
+                                               (20, [0, -1, -1, -1], [1, 1, 1, 0, 0, 0], 2, None)):     # (loses what is behind)
         pages = fa.KVPages(i32([[0, -1, 2, -1], [1, -1, -1, -1]], dev), i32([1, 1, 1, 0, 0, 0], dev), 16)
-        pairs = fa.resize_kv_pages(pages, i32([40, 5], dev), i32([wanted, 20], dev))
+        pairs = fa.resize_kv_pages(pages, i32([40, 5], dev), i32([wanted, 20], dev), granted=granted)
         assert reported(dev, 125)
         assert pages.table.tolist() == [row0, [1, first, -1, -1]] and pages.refs.tolist() == refs and pairs.tolist() == [[-1, -1]] * 2
     # cut in front of the gap, or ended, it is a row like others
@@ -72,9 +78,35 @@ def test_a_gap_where_a_warp_looks_for_it(cuda_device):
         table = [row, [298] + [-1] * 299]
         refs = [int(p in row) + int(p == 298) for p in range(310)]
         pages = fa.KVPages(i32(table, dev), i32(refs, dev), size)
-        pairs = fa.resize_kv_pages(pages, i32([298 * 16 + 4, 4], dev), i32([300 * 16, 4], dev))
-        assert reported(dev, 125)
+        for granted in (None, i32([0, 0], dev)):
+            pairs = fa.resize_kv_pages(pages, i32([298 * 16 + 4, 4], dev), i32([300 * 16, 4], dev), granted=granted)
+            assert reported(dev, 125)
+            if granted is None and gap != 298:
+                assert pages.table[0, 298] == WAITS + row[298]
+        assert granted.tolist() == [gap * 16, 4]
         assert pages.table.tolist() == table and pages.refs.tolist() == refs and pairs.tolist() == [[-1, -1]] * 2
+
+
+def test_a_row_with_a_gap_is_not_appended_to(cuda_device):
+    """It shares the page its next token would go to; whoever is not told appends all the same."""
+    dev = cuda_device
+    H, D, size = 2, 64, 16
+    g = torch.Generator(device=dev).manual_seed(4)
+    cache = fa.FP8KVCache.empty(4, size, H, D, device=dev)
+    for t in cache.tensors():
+        t.view(torch.uint8).copy_(torch.randint(0, 0x70, t.view(torch.uint8).shape, generator=g, device=dev, dtype=torch.uint8))
+    cache.k_scale.fill_(0.5)
+    cache.v_scale.fill_(0.5)
+    before = [t.view(torch.uint8).clone() for t in cache.tensors()]
+    pages = fa.KVPages(i32([[0, -1, 2], [1, 3, 2]], dev), i32([1, 1, 2, 1], dev), size)
+    held = i32([40, 44], dev)
+    pairs = fa.resize_kv_pages(pages, held, held + i32([1, 0], dev))
+    assert reported(dev, 125)
+    fa.copy_kv_pages(cache, pairs)
+    k, v = (torch.randn(2, 1, H, D, generator=g, device=dev).bfloat16() * 100 for _ in range(2))
+    fa.append_kv_fp8(cache, k, v, held, page_table=pages.table, seqused_new=i32([1, 0], dev))
+    assert reported(dev, 121)
+    assert all(torch.equal(t.view(torch.uint8), x) for t, x in zip(cache.tensors(), before))
 
 
 # ---- copies that find no page ------------------------------------------------------------------------------------
@@ -141,9 +173,6 @@ class Model:
         assert self.refs == [named[p] for p in range(len(self.refs))]
 
 
-WAITS = -2 ** 31                 # on the page of an entry that waits for a copy
-
-
 def test_entries_that_wait_for_a_copy(cuda_device):
     """Rows that were not told go through every call: what they name is counted, moved and given back like other entries."""
     dev = cuda_device
@@ -196,7 +225,7 @@ def both(pages, model, held, wanted, device, told=True):
     table = [list(row) for row in model.table]
     if not told:
         for b in model.refused:
-            table[b][held[b] // model.size] += WAITS
+            table[b][held[b] // model.size] += WAITS               # (no row has a gap)
     assert pages.table.tolist() == table and pages.refs.tolist() == model.refs
     assert reported(device, 125) == missing
     model.check()
