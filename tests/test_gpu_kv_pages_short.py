@@ -416,6 +416,63 @@ def test_attention_where_a_copy_found_no_page(cuda_device):
     fa.check_status(dev)
 
 
+def test_a_loop_in_a_pool_that_runs_out(cuda_device):
+    """The calls of a serving loop where there are too few pages: rows go on from others, end, are refused room and ask again.  Lists and results are those of caches
+    that every row has to itself."""
+    dev, rng = cuda_device, random.Random(6)
+    H, G, D, size, width, pool, W, first = 2, 8, 64, 16, 8, 9, 4, 20
+    g = torch.Generator().manual_seed(7)
+    def rows(n, heads, s=1):
+        return torch.randn(n, s, heads, D, generator=g).bfloat16().to(dev)
+    cache = fa.FP8KVCache.empty(pool, size, H, D, device=dev, indexed=True, by_head=True)
+    pages, held = fa.KVPages.empty(1, width, pool, size, device=dev), i32([0], dev)
+    k0, v0 = rows(1, H, first), rows(1, H, first)
+    fa.copy_kv_pages(cache, fa.resize_kv_pages(pages, held, held + first))
+    fa.append_kv_fp8(cache, k0, v0, held, page_table=pages.table)
+    pages, held = fa.fork_kv_pages(pages, held + first, i32([0] * W, dev))
+    story, short, ended = [[] for _ in range(W)], 0, [False] * W
+    for step in range(60):
+        q, k, v = rows(W, G), rows(W, H), rows(W, H)
+        here = held.tolist()
+        end = [not e and h > first and rng.random() < 0.06 and not all(ended) for e, h in zip(ended, here)]
+        wanted = [0 if e or now or h >= 90 else h + 1 for e, now, h in zip(ended, end, here)]
+        ended = [w == 0 for w in wanted]
+        room = torch.empty_like(held)
+        fa.copy_kv_pages(cache, fa.resize_kv_pages(pages, held, i32(wanted, dev), granted=room))
+        fa.append_kv_fp8(cache, k, v, held, page_table=pages.table, seqused_new=room - held)
+        granted = room.tolist()
+        missing = granted != wanted
+        assert reported(dev, 125) == missing
+        short += missing
+        for b in range(W):
+            assert granted[b] in (wanted[b], here[b])
+            story[b] = [] if ended[b] else story[b] + [(k[b, 0], v[b, 0])] * (granted[b] - here[b])
+            assert ended[b] or len(story[b]) + first == granted[b]
+        lists = fa.select_kv_blocks(q, cache, room, 3, page_table=pages.table)
+        out, lse = fa.flash_attn_fp8_blocks_func(q, cache, lists, room, page_table=pages.table, return_lse=True)
+        fa.check_status(dev)
+        if step % 7 == 6:
+            own = fa.FP8KVCache.empty(W, width * size, H, D, size, device=dev, indexed=True)
+            there = [0 if e else 1 for e in ended]
+            fa.append_kv_fp8(own, k0.expand(W, -1, -1, -1).contiguous(), v0.expand(W, -1, -1, -1).contiguous(), i32([0] * W, dev), seqused_new=i32([first * t for t in there], dev))
+            for i in range(max(len(s) for s in story)):
+                t = [torch.stack([s[i][j] if i < len(s) else torch.zeros_like(k[0, 0]) for s in story])[:, None] for j in (0, 1)]
+                fa.append_kv_fp8(own, *t, i32([first + i] * W, dev), seqused_new=i32([int(i < len(s)) for s in story], dev))
+            mine = fa.select_kv_blocks(q, own, room, 3)
+            want, want_lse = fa.flash_attn_fp8_blocks_func(q, own, mine, room, return_lse=True)
+            assert torch.equal(lists, mine) and torch.equal(out, want) and torch.equal(lse, want_lse)
+        held = room
+        # (rows that ended begin again as another one, some time later)
+        alive = [b for b in range(W) if not ended[b]]
+        parents = [b if not ended[b] else rng.choice(alive) if alive and rng.random() < 0.3 else -1 for b in range(W)]
+        pages, held = fa.fork_kv_pages(pages, held, i32(parents, dev))
+        story = [list(story[a]) if a >= 0 else [] for a in parents]
+        ended = [a < 0 for a in parents]
+        if all(ended):
+            break
+    assert short > 5
+
+
 def test_refusals_of_granted(cuda_device):
     dev = cuda_device
     p, n = fa.KVPages.empty(3, 4, 10, 16, device=dev), i32([0, 0, 0], dev)
